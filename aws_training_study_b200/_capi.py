@@ -1,4 +1,5 @@
-"""ctypes binding of ``libpcp_attn.so`` (the C ABI in ``include/pcp_attn.h``).
+"""ctypes binding of ``libpcp_attn.so`` (the C ABI in ``include/pcp_attn.h`` and
+``include/pcp_serve.h``).
 
 There is no fallback: if the library is missing this module raises
 ``ImportError`` with the build command, and every product entry point goes
@@ -35,7 +36,7 @@ STATUS_NAMES = {
     7: "PCP_ERR_PEER",
 }
 
-# Every function declared in include/pcp_attn.h: name -> (restype, argtypes).
+# Every function declared in include/*.h: name -> (restype, argtypes).
 _c = ctypes
 _P = _c.c_void_p
 _I32 = _c.c_int32
@@ -72,7 +73,45 @@ class PcpStats(ctypes.Structure):
     ]
 
 
+class PcpHeads(ctypes.Structure):
+    _fields_ = [
+        ("data", _P),
+        ("head_stride", _c.c_int64),
+        ("row_stride", _c.c_int64),
+        ("heads", _I32),
+        ("reserved", _I32),
+    ]
+
+
+class PcpPool(ctypes.Structure):
+    _fields_ = [
+        ("data", _P),
+        ("scales", _P),
+        ("blocks", _c.c_int64),
+        ("num_kv_heads", _I32),
+        ("head_dim", _I32),
+        ("block_size", _I32),
+        ("kv_dtype", _I32),
+    ]
+
+
+class PcpBatch(ctypes.Structure):
+    _fields_ = [
+        ("offsets", _P),
+        ("kv_len", _P),
+        ("block_tables", _P),
+        ("table_stride", _c.c_int64),
+        ("table_width", _I32),
+        ("num_seqs", _I32),
+        ("rows", _I32),
+        ("reserved", _I32),
+    ]
+
+
 _PDIMS = _c.POINTER(PcpDims)
+_PHEADS = _c.POINTER(PcpHeads)
+_PPOOL = _c.POINTER(PcpPool)
+_PBATCH = _c.POINTER(PcpBatch)
 
 SIGNATURES = {
     "pcp_last_error": (_c.c_char_p, []),
@@ -108,6 +147,11 @@ SIGNATURES = {
     "pcp_set_profiling": (_c.c_int, [_P, _I32]),
     "pcp_get_stats": (_c.c_int, [_P, _c.POINTER(PcpStats)]),
     "pcp_destroy": (_c.c_int, [_P]),
+    "pcp_qk_norm_rope": (
+        _c.c_int, [_I32, _I32, _I32, _I32, _I32, _PHEADS, _PHEADS, _PHEADS, _PHEADS, _P, _I32, _P, _c.c_float, _P, _P,
+                   _c.c_float, _P]),
+    "pcp_cache_append": (_c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _P, _P]),
+    "pcp_cache_read": (_c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _P, _P]),
 }
 
 _lock = threading.Lock()

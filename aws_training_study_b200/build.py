@@ -2,7 +2,7 @@
 
     python -m aws_training_study_b200.build [--verbose-ptxas]
 
-The library is a plain C-ABI shared object (include/pcp_attn.h) loaded with
+The library is a plain C-ABI shared object (include/pcp_attn.h, include/pcp_serve.h) loaded with
 ctypes; it links the NCCL that ships with PyTorch (nvidia-nccl wheel) so the
 process uses one NCCL build.
 """
@@ -14,12 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO / "include"
+BUILD_DIR = PKG_DIR / "_build"
 LIB_NAME = "libpcp_attn.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -44,7 +46,8 @@ def _nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "pcp_attn.h"]
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
+    return sorted(CSRC.glob("*.cu")) + headers
 
 
 def needs_build() -> bool:
@@ -58,31 +61,26 @@ def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = False)
     if not force and not needs_build():
         return LIB_PATH
     nccl_inc, nccl_lib = _nccl_dirs()
-    cmd = [
-        _nvcc(),
-        *ARCH_FLAGS,
-        "-lineinfo",
-        "-O3",
-        "-std=c++17",
-        "--shared",
-        "-Xcompiler",
-        "-fPIC,-O2,-Wall",
-        "-I",
-        str(INCLUDE),
-        "-I",
-        str(nccl_inc),
-        str(CSRC / "pcp_attn.cu"),
-        "-o",
-        str(LIB_PATH) + ".tmp",
-        f"-L{nccl_lib}",
-        "-l:libnccl.so.2",
-        f"-Xlinker=-rpath,{nccl_lib}",
-    ]
+    common = [_nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2,-Wall"]
     if verbose_ptxas:
-        cmd.insert(1, "-Xptxas=-v")
-    if not quiet:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+        common.insert(1, "-Xptxas=-v")
+
+    def run(cmd: list[str]) -> None:
+        if not quiet:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+
+    # The translation units compile side by side and link into one library.
+    BUILD_DIR.mkdir(exist_ok=True)
+    units = sorted(CSRC.glob("*.cu"))
+    objects = [BUILD_DIR / (u.stem + ".o") for u in units]
+    with ThreadPoolExecutor(max_workers=len(units)) as pool:
+        jobs = [pool.submit(run, [*common, "-I", str(INCLUDE), "-I", str(nccl_inc), "-c", str(u), "-o", str(o)])
+                for u, o in zip(units, objects)]
+        for job in jobs:
+            job.result()
+    run([*common, "--shared", *map(str, objects), "-o", str(LIB_PATH) + ".tmp", f"-L{nccl_lib}", "-l:libnccl.so.2",
+         f"-Xlinker=-rpath,{nccl_lib}"])
     os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
     return LIB_PATH
 

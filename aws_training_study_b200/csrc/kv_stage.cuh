@@ -20,6 +20,7 @@
 #include <cstdint>
 
 #include "attn_common.cuh"
+#include "e4m3.cuh"
 #include "ptx.cuh"
 
 namespace pcp {
@@ -200,16 +201,6 @@ struct CacheWriteParams {
   uint8_t* pool;               // [pool_blocks][payload]
   int* err;                    // kErrBlockTable on a missing / out-of-pool entry
 };
-
-__device__ __forceinline__ uint16_t e4m3x2_from_floats(float a, float b) {
-  uint16_t c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  // Beyond the rounding range of the largest finite value (448), and NaN/Inf:
-  // the NaN code with the input's sign.
-  if (!(fabsf(a) <= 464.f)) c = static_cast<uint16_t>((c & 0xFF00u) | 0x7Fu | ((__float_as_uint(a) >> 24) & 0x80u));
-  if (!(fabsf(b) <= 464.f))
-    c = static_cast<uint16_t>((c & 0x00FFu) | ((0x7Fu | ((__float_as_uint(b) >> 24) & 0x80u)) << 8));
-  return c;
-}
 
 // grid-stride over 8-element chunks of [2][Hkv][owned][D].
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheWriteParams p) {

@@ -24,33 +24,18 @@
 #include "attn_pair_sk.cuh"
 #include "attn_pair2.cuh"
 #include "attn_kv.cuh"
+#include "host_util.h"
 #include "kv_stage.cuh"
+
+namespace pcp {
+thread_local char g_err[kErrChars] = "";
+char* error_buffer() { return g_err; }
+}  // namespace pcp
 
 namespace {
 
-thread_local char g_err[1024] = "";
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-#define CUDA_TRY(x)                                                                                     \
-  do {                                                                                                  \
-    cudaError_t e_ = (x);                                                                               \
-    if (e_ != cudaSuccess)                                                                              \
-      return fail(e_ == cudaErrorMemoryAllocation ? PCP_ERR_OUT_OF_MEMORY : PCP_ERR_CUDA, "%s: %s (%s:%d)", \
-                  #x, cudaGetErrorString(e_), __FILE__, __LINE__);                                     \
-  } while (0)
-
-#define PCP_TRY(x)          \
-  do {                      \
-    int s_ = (x);           \
-    if (s_ != PCP_OK) return s_; \
-  } while (0)
+using pcp::fail;
+using pcp::g_err;
 
 constexpr int kMaxTotalSplits = 32;
 constexpr size_t kPartialBudget = size_t(1) << 30;  // bytes of split partials a handle may hold

@@ -14,6 +14,15 @@ tokens of each prefill without host copies and without contiguous shards.
 
 Pool layout: ``[pool_blocks, 2 * Hkv * bs * D]`` in the cache dtype (e4m3fn or
 bf16) -- the packed payload format, one block per row.
+
+A batch of whole sequences on one GPU (``cache_append``, ``cache_read``)
+shares one convention: rows ``offsets[b] .. offsets[b + 1]`` of a packed
+``[heads, rows, D]`` tensor are sequence b's tokens of the call, and they are
+the last of the ``kv_len[b]`` tokens it then has; position p lives in row
+``p % block_size`` of pool block ``block_tables[b, p // block_size]``.  An e4m3
+pool may carry ``scales`` (``make_scales``): a power of two for each token, head
+and K or V, so that rows of any size keep e4m3's relative precision and what is
+read back is exact in bf16.
 """
 
 from __future__ import annotations
@@ -24,7 +33,8 @@ import torch
 
 from .. import _capi
 from .config import PCPAttentionConfig
-from .cuda_backend import _cuda_stream_ptr, make_dims, payload_elements
+from .cuda_backend import _cuda_stream_ptr, _kv_code, make_dims, payload_elements
+from .rotary import _check_rows, _check_writable, _heads
 
 
 def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -33,6 +43,16 @@ def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtyp
     if pool_blocks <= 0:
         raise ValueError("pool_blocks must be positive")
     return torch.zeros((pool_blocks, payload_elements(config)), dtype=kv_dtype, device=device)
+
+
+def make_scales(config: PCPAttentionConfig, pool_blocks: int,
+                device: int | torch.device | str = "cuda") -> torch.Tensor:
+    """Scale bytes of an e4m3 pool, ``[pool_blocks, 2 * Hkv * bs]`` uint8: a
+    byte b stands for ``2 ** (b - 127)``; all at unit scale."""
+    if pool_blocks <= 0:
+        raise ValueError("pool_blocks must be positive")
+    shape = (pool_blocks, 2 * config.num_kv_heads * config.block_size)
+    return torch.full(shape, 127, dtype=torch.uint8, device=device)
 
 
 def local_blocks_needed(config: PCPAttentionConfig, rank: int, total_len: int) -> int:
@@ -130,3 +150,119 @@ def history_attention_paged_single(q: torch.Tensor, pool: torch.Tensor, block_ta
         )
         _capi.check(lib.pcp_history_attention_status(ctypes.c_void_p(ws.data_ptr()), _cuda_stream_ptr(stream)))
     return out
+
+
+def _pool_struct(config: PCPAttentionConfig, pool: torch.Tensor, scales: torch.Tensor | None) -> _capi.PcpPool:
+    if config.pcp_size != 1:
+        raise ValueError(f"a batch holds whole sequences: pcp_size must be 1, got {config.pcp_size}")
+    if config.block_size % 16:
+        raise ValueError(f"block_size must be a multiple of 16, got {config.block_size}")
+    code = _kv_code(pool.dtype)
+    _check_pool(config, pool, pool.dtype)
+    if scales is not None:
+        shape = (pool.shape[0], 2 * config.num_kv_heads * config.block_size)
+        if code != _capi.PCP_KV_E4M3:
+            raise ValueError("scales need an e4m3 pool")
+        if tuple(scales.shape) != shape or scales.dtype != torch.uint8 or scales.device != pool.device or \
+                not scales.is_contiguous() or scales.data_ptr() % 16:
+            raise ValueError(f"scales must be a contiguous, 16-byte aligned uint8 {shape} tensor on {pool.device}")
+    return _capi.PcpPool(pool.data_ptr(), 0 if scales is None else scales.data_ptr(), pool.shape[0],
+                         config.num_kv_heads, config.head_dim, config.block_size, code)
+
+
+def _batch_struct(offsets: torch.Tensor, kv_len: torch.Tensor, block_tables: torch.Tensor, rows: int,
+                  device: torch.device) -> _capi.PcpBatch:
+    for name, t, dims in (("offsets", offsets, 1), ("kv_len", kv_len, 1), ("block_tables", block_tables, 2)):
+        if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.numel() and t.stride(-1) != 1):
+            raise ValueError(f"{name} must be an int32 tensor of {dims} dimensions with contiguous rows on {device}")
+    seqs = kv_len.shape[0]
+    if offsets.shape[0] != seqs + 1 or block_tables.shape[0] != seqs:
+        raise ValueError(f"{seqs} sequences need {seqs + 1} offsets and {seqs} block tables, got {offsets.shape[0]} "
+                         f"and {block_tables.shape[0]}")
+    return _capi.PcpBatch(offsets.data_ptr(), kv_len.data_ptr(), block_tables.data_ptr(),
+                          block_tables.stride(0) if seqs > 1 else 0, block_tables.shape[1], seqs, rows, 0)
+
+
+class _Status:
+    """The device status word of a call: the caller's (the call stays
+    asynchronous), or an own one that is read after the call, which then
+    raises what the kernels reported."""
+
+    def __init__(self, status: torch.Tensor | None, device: torch.device, stream: torch.cuda.Stream | None):
+        self.own = status is None
+        if self.own:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("a captured call needs a status tensor: its result cannot be read while recording")
+            status = torch.empty(1, dtype=torch.int32, device=device)
+        elif status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+            raise ValueError(f"status must be an int32 tensor of one element on {device}")
+        self.word, self.stream = status, stream
+        self.ptr = ctypes.c_void_p(status.data_ptr())
+
+    def finish(self) -> None:
+        if self.own:
+            _capi.check(_capi.lib().pcp_history_attention_status(self.ptr, _cuda_stream_ptr(self.stream)))
+
+
+def cache_append(config: PCPAttentionConfig, k_src: torch.Tensor, v_src: torch.Tensor, offsets: torch.Tensor,
+                 kv_len: torch.Tensor, block_tables: torch.Tensor, pool: torch.Tensor,
+                 scales: torch.Tensor | None = None, status: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None) -> None:
+    """Write the new tokens of a batch of sequences (``k_src``/``v_src``
+    ``[Hkv, rows, D]`` bf16, heads and rows at any 16-byte aligned stride) into
+    their pages: ``offsets`` int32 ``[B + 1]``, ``kv_len`` int32 ``[B]`` (the
+    tokens of each sequence once these are in), ``block_tables`` int32
+    ``[B, width]``.  A bf16 pool takes copies, an e4m3 pool codes at unit scale
+    or, with ``scales``, codes and a scale byte for each token and head.  Rows
+    of no sequence are ignored.  With ``status`` (device int32, one element)
+    the call is asynchronous and leaves 0, 109 (a page outside the pool or the
+    table; its tokens are skipped) or 112 (a position below 0) there; without,
+    it waits and raises."""
+    ps = _pool_struct(config, pool, scales)
+    rows = k_src.shape[1] if k_src.dim() == 3 else -1
+    for name, t in (("k_src", k_src), ("v_src", v_src)):
+        _check_rows(name, t, (config.num_kv_heads, rows, config.head_dim), torch.bfloat16, pool.device)
+    batch = _batch_struct(offsets, kv_len, block_tables, rows, pool.device)
+    with torch.cuda.device(pool.device):
+        st = _Status(status, pool.device, stream)
+        _capi.check(
+            _capi.lib().pcp_cache_append(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(k_src)),
+                                         ctypes.byref(_heads(v_src)), st.ptr, _cuda_stream_ptr(stream))
+        )
+        st.finish()
+
+
+def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.Tensor, block_tables: torch.Tensor,
+               pool: torch.Tensor, rows: int | None = None, scales: torch.Tensor | None = None,
+               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None,
+               status: torch.Tensor | None = None,
+               stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Read tokens of a batch of sequences back from their pages as bf16: the
+    last ``offsets[b + 1] - offsets[b]`` tokens of each sequence's ``kv_len[b]``
+    land in rows ``offsets[b] ..`` of ``k_out``/``v_out`` ``[Hkv, rows, D]``
+    (allocated for ``rows`` when not given; rows of no sequence are left as
+    they were).  Every value is exact: codes times a power of two.  ``status``
+    as in ``cache_append``; a page that cannot be followed reads as zeros."""
+    ps = _pool_struct(config, pool, scales)
+    if rows is None:
+        if k_out is None:
+            raise ValueError("cache_read needs rows, or k_out and v_out")
+        rows = k_out.shape[1] if k_out.dim() == 3 else -1
+    shape = (config.num_kv_heads, int(rows), config.head_dim)
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty(shape, dtype=torch.bfloat16, device=pool.device)
+        else:
+            _check_rows(name, t, shape, torch.bfloat16, pool.device)
+            _check_writable(name, t)
+        outs.append(t)
+    batch = _batch_struct(offsets, kv_len, block_tables, int(rows), pool.device)
+    with torch.cuda.device(pool.device):
+        st = _Status(status, pool.device, stream)
+        _capi.check(
+            _capi.lib().pcp_cache_read(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(outs[0])),
+                                       ctypes.byref(_heads(outs[1])), st.ptr, _cuda_stream_ptr(stream))
+        )
+        st.finish()
+    return outs[0], outs[1]

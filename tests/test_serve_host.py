@@ -1,0 +1,96 @@
+"""Host side of the serving operators (no GPU needed): frequencies of the
+rotation, and the C ABI's refusals, which come before any device work."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from aws_training_study_b200 import _capi
+from aws_training_study_b200.pcp_attention import PCPAttentionConfig
+from aws_training_study_b200.pcp_attention import paged
+from aws_training_study_b200.pcp_attention.rotary import Rotary, qk_norm_rope, rotary_frequencies
+
+
+def test_frequencies():
+    plain, magnitude = rotary_frequencies(64, 10000.0)
+    assert magnitude == 1.0 and plain == [10000.0 ** (-i / 32) for i in range(32)]
+    assert rotary_frequencies(64, 10000.0, "linear", factor=4.0)[0] == [f / 4.0 for f in plain]
+    bands, _ = rotary_frequencies(64, 10000.0, "bands", factor=8.0, original_len=8192, low=1.0, high=4.0)
+    for f, b in zip(plain, bands):
+        turns = 8192 * f / (2 * math.pi)
+        assert b == f if turns >= 4 else b == pytest.approx(f / 8) if turns <= 1 else f / 8 < b < f
+    ramp, magnitude = rotary_frequencies(64, 10000.0, "ramp", factor=16.0, original_len=4096)
+    assert magnitude == pytest.approx(0.1 * math.log(16.0) + 1)
+    assert ramp[0] == plain[0] and ramp[-1] == pytest.approx(plain[-1] / 16)
+    assert all(f / 16 * (1 - 1e-12) <= r <= f for f, r in zip(plain, ramp))
+
+
+def test_turns_are_the_frequencies():
+    r = Rotary(128, 128, base=1e6)
+    for t, f in zip(r._turns_host.tolist(), r.frequencies):
+        assert (t % 2 ** 64) / 2.0 ** 64 == pytest.approx(f / (2 * math.pi), rel=1e-15, abs=2.0 ** -64)
+
+
+@pytest.mark.parametrize("args", [
+    dict(head_dim=100), dict(head_dim=528), dict(head_dim=128, rotary_dim=24), dict(head_dim=128, rotary_dim=144),
+    dict(head_dim=128, layout="other"), dict(head_dim=128, base=1.0), dict(head_dim=128, scaling="other", factor=2.0),
+    dict(head_dim=128, scaling="linear", factor=0.0), dict(head_dim=128, scaling="ramp", factor=2.0),
+    dict(head_dim=128, scaling="bands", factor=2.0, original_len=8192, low=4.0, high=4.0)])
+def test_rotary_refusals(args):
+    with pytest.raises(ValueError):
+        Rotary(**args)
+
+
+def _heads(data=16, head=128, row=128, heads=2):
+    return _capi.PcpHeads(data, head, row, heads, 0)
+
+
+def test_qk_norm_rope_refusals():
+    lib = _capi.lib()
+
+    def call(dtype=2, rows=4, D=128, r=64, layout=0, q=None, k=None, q_out=None, k_out=None, positions=16, turns=16,
+             wq=0):
+        q, k = q or _heads(), k or _heads(heads=0, data=0)
+        return lib.pcp_qk_norm_rope(dtype, rows, D, r, layout, q, k, q_out or q, k_out or k, positions, 1, turns, 1.0,
+                                    wq, 0, 1e-6, None)
+
+    for args in (dict(dtype=3), dict(rows=-1), dict(D=120), dict(D=528), dict(r=8), dict(r=144), dict(layout=2),
+                 dict(q=_heads(data=8)), dict(q=_heads(row=100)), dict(q=_heads(head=4)), dict(q=_heads(data=0)),
+                 dict(q_out=_heads(heads=3)), dict(positions=0), dict(turns=0), dict(wq=8)):
+        assert call(**args) in (1, 2), args
+        assert lib.pcp_last_error()
+    assert call(rows=0) == 0
+    with pytest.raises(ValueError, match="CUDA"):
+        qk_norm_rope(torch.zeros(1, 1, 128), None, torch.zeros(1, dtype=torch.int64), Rotary(128))
+
+
+@pytest.mark.parametrize("entry", ["pcp_cache_append", "pcp_cache_read"])
+def test_cache_refusals(entry):
+    lib = _capi.lib()
+
+    def call(pool=None, batch=None, k=None, v=None, status=16):
+        pool = {"data": 16, "scales": 16, "blocks": 4, "num_kv_heads": 2, "head_dim": 128, "block_size": 64,
+                "kv_dtype": 0, **(pool or {})}
+        batch = {"offsets": 16, "kv_len": 16, "block_tables": 16, "table_stride": 4, "table_width": 4, "num_seqs": 1,
+                 "rows": 4, **(batch or {})}
+        return getattr(lib, entry)(ctypes.byref(_capi.PcpPool(**pool)), ctypes.byref(_capi.PcpBatch(**batch)),
+                                   k or _heads(), v or _heads(), status, None)
+
+    for args in (dict(pool={"head_dim": 64}), dict(pool={"block_size": 24}), dict(pool={"kv_dtype": 2}),
+                 dict(pool={"kv_dtype": 1}), dict(pool={"blocks": 0}), dict(pool={"data": 8}),
+                 dict(pool={"scales": 8}), dict(pool={"num_kv_heads": 0}), dict(batch={"rows": -1}),
+                 dict(batch={"num_seqs": -1}), dict(batch={"offsets": 0}), dict(batch={"table_stride": -1}),
+                 dict(k=_heads(heads=1)), dict(v=_heads(row=4)), dict(k=_heads(data=0)), dict(status=0)):
+        assert call(**args) in (1, 2), args
+        assert lib.pcp_last_error()
+
+
+def test_batches_hold_whole_sequences():
+    cfg = PCPAttentionConfig(2, 64, 1024, 1024, 64, 16, 4, 2, 128)
+    pool = torch.zeros(2, 2 * 2 * 64 * 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="pcp_size"):
+        paged._pool_struct(cfg, pool, None)
