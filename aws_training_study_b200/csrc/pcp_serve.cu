@@ -2,9 +2,17 @@
 // launches of the serving operators.
 #include "pcp_serve.h"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <climits>
+#include <cmath>
+#include <mutex>
 
+#include "chunk_plan.cuh"
+#include "chunk_rows.cuh"
+#include "chunk_tiles.cuh"
 #include "host_util.h"
 #include "serve_ops.cuh"
 
@@ -101,6 +109,147 @@ int cache_rows(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads
   return PCP_OK;
 }
 
+// ------------------------------------------------------- chunk attention --
+// Grids: one CTA, or half a CTA pair, per SM.  No CTA waits for another, so
+// fewer SMs only queue them.
+constexpr int kCtas = 148;
+constexpr int kPairs = kCtas / 2;
+
+size_t align_up(size_t a) { return (a + 255) / 256 * 256; }
+
+struct ChunkLayout {
+  size_t plan, small, small_start, tile, tile_start, seq_tile, tile_prefix, small_o, small_lse, tile_o, tile_lse, bytes;
+};
+
+bool has_tiles(int32_t max_chunk, int32_t group) { return static_cast<int64_t>(max_chunk) * group > pcp::kSmallRows; }
+
+ChunkLayout chunk_layout(int32_t head_dim, int32_t kv_heads, int32_t group, int32_t seqs, int32_t rows, int32_t max_chunk) {
+  ChunkLayout w{};
+  const int64_t with_rows = std::min(seqs, rows);
+  const int64_t small = with_rows * kv_heads;
+  const bool tiles = has_tiles(max_chunk, group);
+  // Query tiles of a head: whole ones of all rows, and one rest a sequence.
+  const int64_t q_tiles = tiles ? static_cast<int64_t>(rows) * group / pcp::kUnitRows + with_rows : 0;
+  size_t at = 0;
+  auto put = [&](size_t bytes) {
+    const size_t here = at;
+    at = align_up(at + bytes);
+    return here;
+  };
+  w.plan = put(sizeof(pcp::ChunkPlan));
+  w.small = put(small * sizeof(pcp::ChunkUnit));
+  w.small_start = put((small + 1) * 8);
+  w.tile = put(q_tiles * kv_heads * sizeof(pcp::ChunkUnit));
+  w.tile_start = put((q_tiles * kv_heads + 1) * 8);
+  w.seq_tile = put((static_cast<size_t>(seqs) + 1) * 4);
+  w.tile_prefix = put((q_tiles + 1) * 8);
+  w.small_o = put(size_t(2) * kCtas * pcp::kSmallRows * head_dim * 4);
+  w.small_lse = put(size_t(2) * kCtas * pcp::kSmallRows * 4);
+  w.tile_o = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * head_dim * 4 : 0);
+  w.tile_lse = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * 4 : 0);
+  w.bytes = at;
+  return w;
+}
+
+int check_chunk(const pcp_pool_t* pool, int32_t q_heads, int32_t seqs, int32_t rows, int32_t max_chunk) {
+  PCP_TRY(check_pool(pool));
+  if (q_heads <= 0 || q_heads % pool->num_kv_heads)
+    return fail(PCP_ERR_INVALID_ARGUMENT, "%d query heads must be a positive multiple of %d KV heads", q_heads,
+                pool->num_kv_heads);
+  if (seqs < 0 || rows < 0 || max_chunk <= 0)
+    return fail(PCP_ERR_INVALID_ARGUMENT, "negative number of sequences or rows, or max_chunk not positive");
+  const int64_t group = q_heads / pool->num_kv_heads;
+  if (static_cast<int64_t>(rows) * group > INT_MAX - pcp::kUnitRows)
+    return fail(PCP_ERR_UNSUPPORTED, "%d rows of %lld query heads a KV head are too many", rows,
+                static_cast<long long>(group));
+  return PCP_OK;
+}
+
+// Cache blocks [blocks][2][Hkv][bs][D] as a 5-D tensor {D, bs, Hkv, K/V,
+// blocks}; boxes of box_x elements x box_rows rows of one head of box_kv of K
+// and V of one block.
+int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t box_rows, uint32_t box_kv, bool swizzle) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  if (!fn) return fail(PCP_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
+  const bool bf16 = p.kv_dtype == PCP_KV_BF16;
+  const uint64_t D = p.head_dim, bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1;
+  cuuint64_t dims[5] = {D, bs, H, 2, static_cast<cuuint64_t>(p.blocks)};
+  cuuint64_t strides[4] = {D * elt, bs * D * elt, H * bs * D * elt, 2 * H * bs * D * elt};
+  cuuint32_t box[5] = {box_x, box_rows, 1, box_kv, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PCP_ERR_CUDA, "cuTensorMapEncodeTiled (cache pool) failed (%d)", static_cast<int>(r));
+  return PCP_OK;
+}
+
+// A kernel's dynamic shared memory is allowed once per device.
+template <auto kKernel>
+int allow_smem(int bytes) {
+  static std::mutex mutex;
+  static bool done[64] = {};
+  int device = 0;
+  CUDA_TRY(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mutex);
+  if (device < 64 && done[device]) return PCP_OK;
+  CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (device < 64) done[device] = true;
+  return PCP_OK;
+}
+
+template <int D, bool kFp8>
+int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
+  using L = pcp::RowsSmem<D, kFp8>;
+  CUtensorMap tm;
+  PCP_TRY(make_pool_map(&tm, pool, kFp8 ? 128 : 64, 16, 2, true));
+  PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes)));
+  pcp::chunk_rows_kernel<D, kFp8><<<kCtas, pcp::kRowsThreads, L::kBytes, st>>>(tm, p);
+  CUDA_TRY(cudaGetLastError());
+  return PCP_OK;
+}
+
+template <int D, int kCache>
+int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
+  using L = pcp::TilesSmem<D, kCache>;
+  // Boxes of as many rows as a page's length and half a tile share.
+  int box_rows = 64;
+  while (pool.block_size % box_rows) box_rows /= 2;
+  CUtensorMap tk, tv;
+  PCP_TRY(make_pool_map(&tk, pool, L::kFp8 ? D : 64, box_rows, 1, !L::kFp8));
+  PCP_TRY(make_pool_map(&tv, pool, L::kFp8 ? D / 2 : 64, box_rows, 1, !L::kFp8));
+  PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes)));
+  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tk, tv, box_rows, p);
+  CUDA_TRY(cudaGetLastError());
+  return PCP_OK;
+}
+
+template <int D>
+int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, bool tiles, cudaStream_t st) {
+  pcp::chunk_plan_kernel<<<1, 1024, 0, st>>>(p);
+  CUDA_TRY(cudaGetLastError());
+  const bool bf16 = pool.kv_dtype == PCP_KV_BF16;
+  if (bf16) PCP_TRY((launch_rows<D, false>(pool, p, st)));
+  else PCP_TRY((launch_rows<D, true>(pool, p, st)));
+  if (tiles) {
+    if (bf16) PCP_TRY((launch_tiles<D, pcp::kCacheBf16>(pool, p, st)));
+    else if (pool.scales) PCP_TRY((launch_tiles<D, pcp::kCacheScaled>(pool, p, st)));
+    else PCP_TRY((launch_tiles<D, pcp::kCacheE4m3>(pool, p, st)));
+  }
+  pcp::chunk_combine_kernel<D><<<4 * kCtas, 256, 0, st>>>(p);
+  CUDA_TRY(cudaGetLastError());
+  return PCP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -167,6 +316,66 @@ int pcp_cache_append(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp
 int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* k_out,
                    const pcp_heads_t* v_out, int32_t* device_status, void* stream) {
   return cache_rows(pool, batch, k_out, v_out, device_status, stream, false);
+}
+
+int pcp_chunk_attention_workspace_size(const pcp_pool_t* pool, int32_t num_q_heads, int32_t num_seqs, int32_t rows,
+                                       int32_t max_chunk, size_t* bytes) {
+  PCP_TRY(check_chunk(pool, num_q_heads, num_seqs, rows, max_chunk));
+  if (!bytes) return fail(PCP_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  *bytes = chunk_layout(pool->head_dim, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, num_seqs, rows, max_chunk).bytes;
+  return PCP_OK;
+}
+
+int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* q, const pcp_heads_t* out,
+                        int32_t max_chunk, float softmax_scale, void* workspace, size_t workspace_bytes,
+                        int32_t* device_status, void* stream) {
+  PCP_TRY(check_batch(batch));
+  if (!q) return fail(PCP_ERR_INVALID_ARGUMENT, "q is NULL");
+  PCP_TRY(check_chunk(pool, q->heads, batch->num_seqs, batch->rows, max_chunk));
+  PCP_TRY(check_heads(q, q->heads, batch->rows, 2, "q"));
+  PCP_TRY(check_heads(out, q->heads, batch->rows, 2, "out"));
+  if (!device_status) return fail(PCP_ERR_INVALID_ARGUMENT, "device_status is NULL");
+  if (!(softmax_scale > 0) || std::isinf(softmax_scale))
+    return fail(PCP_ERR_INVALID_ARGUMENT, "softmax_scale %g must be positive and finite", softmax_scale);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (batch->num_seqs == 0 || batch->rows == 0) {
+    CUDA_TRY(cudaMemsetAsync(device_status, 0, sizeof(int32_t), st));
+    return PCP_OK;
+  }
+  const int32_t group = q->heads / pool->num_kv_heads;
+  const ChunkLayout w = chunk_layout(pool->head_dim, pool->num_kv_heads, group, batch->num_seqs, batch->rows, max_chunk);
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < w.bytes)
+    return fail(PCP_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, aligned to 256, is needed (got %zu)", w.bytes,
+                workspace_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  pcp::ChunkParams p{};
+  p.batch = batch_view(*batch);
+  p.pool = pool_view(*pool);
+  p.work.plan = reinterpret_cast<pcp::ChunkPlan*>(ws + w.plan);
+  p.work.small = reinterpret_cast<pcp::ChunkUnit*>(ws + w.small);
+  p.work.small_start = reinterpret_cast<long long*>(ws + w.small_start);
+  p.work.tile = reinterpret_cast<pcp::ChunkUnit*>(ws + w.tile);
+  p.work.tile_start = reinterpret_cast<long long*>(ws + w.tile_start);
+  p.work.seq_tile = reinterpret_cast<int*>(ws + w.seq_tile);
+  p.work.tile_prefix = reinterpret_cast<long long*>(ws + w.tile_prefix);
+  p.work.small_o = reinterpret_cast<float*>(ws + w.small_o);
+  p.work.small_lse = reinterpret_cast<float*>(ws + w.small_lse);
+  p.work.tile_o = reinterpret_cast<float*>(ws + w.tile_o);
+  p.work.tile_lse = reinterpret_cast<float*>(ws + w.tile_lse);
+  p.q = static_cast<const __nv_bfloat16*>(q->data);
+  p.out = static_cast<__nv_bfloat16*>(out->data);
+  p.q_head = q->head_stride;
+  p.q_row = q->row_stride;
+  p.out_head = out->head_stride;
+  p.out_row = out->row_stride;
+  p.group = group;
+  p.max_chunk = max_chunk;
+  p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
+  p.small_ctas = kCtas;
+  p.tile_pairs = kPairs;
+  p.err = device_status;
+  const bool tiles = has_tiles(max_chunk, group);
+  return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, tiles, st) : launch_chunk<128>(*pool, p, tiles, st);
 }
 
 }  // extern "C"

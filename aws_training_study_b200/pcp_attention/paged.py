@@ -15,8 +15,8 @@ tokens of each prefill without host copies and without contiguous shards.
 Pool layout: ``[pool_blocks, 2 * Hkv * bs * D]`` in the cache dtype (e4m3fn or
 bf16) -- the packed payload format, one block per row.
 
-A batch of whole sequences on one GPU (``cache_append``, ``cache_read``)
-shares one convention: rows ``offsets[b] .. offsets[b + 1]`` of a packed
+A batch of whole sequences on one GPU (``cache_append``, ``cache_read``,
+``chunk_attention``) shares one convention: rows ``offsets[b] .. offsets[b + 1]`` of a packed
 ``[heads, rows, D]`` tensor are sequence b's tokens of the call, and they are
 the last of the ``kv_len[b]`` tokens it then has; position p lives in row
 ``p % block_size`` of pool block ``block_tables[b, p // block_size]``.  An e4m3
@@ -266,3 +266,49 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
         )
         st.finish()
     return outs[0], outs[1]
+
+
+def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Tensor, offsets: torch.Tensor,
+                    kv_len: torch.Tensor, config: PCPAttentionConfig, scales: torch.Tensor | None = None,
+                    max_chunk: int | None = None, out: torch.Tensor | None = None, softmax_scale: float | None = None,
+                    status: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Causal attention of a batch of sequences' new tokens over their paged
+    caches, which hold those tokens too (``cache_append`` first): the query at
+    position p sees positions 0 .. p of its sequence.  ``q`` ``[Hq, rows, D]``
+    bf16 (heads and rows at any 16-byte aligned stride; so may ``out``);
+    single tokens, chunks and whole prompts may be mixed.  ``max_chunk`` (default
+    ``rows``) bounds the rows of every sequence; 1 for a decode step saves the
+    launches that longer chunks would need.  ``softmax_scale`` defaults to
+    ``config.softmax_scale``.  Rows that see nothing are zeros; rows of no
+    sequence are left as they were.  ``status`` as in ``cache_append`` (112 also
+    for a sequence of more than ``max_chunk`` rows, which is not written)."""
+    ps = _pool_struct(config, pool, scales)
+    rows = q.shape[1] if q.dim() == 3 else -1
+    shape = (config.num_q_heads, rows, config.head_dim)
+    _check_rows("q", q, shape, torch.bfloat16, pool.device)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_rows("out", out, shape, torch.bfloat16, pool.device)
+    _check_writable("out", out)
+    batch = _batch_struct(offsets, kv_len, block_tables, rows, pool.device)
+    max_chunk = max(1, rows) if max_chunk is None else int(max_chunk)
+    if max_chunk <= 0:
+        raise ValueError(f"max_chunk must be positive, got {max_chunk}")
+    scale = config.softmax_scale if softmax_scale is None else float(softmax_scale)
+    lib = _capi.lib()
+    nbytes = ctypes.c_size_t()
+    _capi.check(lib.pcp_chunk_attention_workspace_size(ctypes.byref(ps), config.num_q_heads, batch.num_seqs, rows,
+                                                       max_chunk, ctypes.byref(nbytes)))
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=pool.device)
+    with torch.cuda.device(pool.device):
+        st = _Status(status, pool.device, stream)
+        _capi.check(
+            lib.pcp_chunk_attention(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(q)),
+                                    ctypes.byref(_heads(out)), max_chunk, scale, ctypes.c_void_p(ws.data_ptr()),
+                                    nbytes.value, st.ptr, _cuda_stream_ptr(stream))
+        )
+        if stream is not None:
+            ws.record_stream(stream)
+        st.finish()
+    return out

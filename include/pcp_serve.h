@@ -21,12 +21,14 @@
  *
  * Device status word (DEVICE int32, zeroed by the call):
  *   109  a table entry outside the pool, or a position past the table's width
- *        (append skips the token, read-back writes zeros, attention reads
- *        block 0 in its place: rows of that sequence are then meaningless);
- *   112  a sequence the call does not take: a position below 0 (append and
- *        read-back skip the token), more tokens than max_chunk (attention
- *        leaves its rows unwritten), or offsets that decrease or pass the
- *        rows;
+ *        (append skips the token, read-back writes zeros; attention reads
+ *        block 0 in the entry's place and stops at the table's end: rows of
+ *        that sequence are then meaningless);
+ *   112  a sequence the call does not take.  Append and read-back: a position
+ *        below 0 (the token is skipped).  Attention: a negative kv_len (taken
+ *        as 0), more rows than max_chunk (the sequence's rows are not
+ *        written), offsets that decrease or leave the rows (nothing is
+ *        written);
  *   1xx  a wait in the attention kernel that ran out (see pcp_attn.h).
  */
 #ifndef PCP_SERVE_H
@@ -119,6 +121,25 @@ int pcp_cache_append(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp
  * bf16 rows of k_out and v_out. */
 int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* k_out,
                    const pcp_heads_t* v_out, int32_t* device_status, void* stream);
+
+/* Causal attention of every sequence's rows of q over its paged cache (the new
+ * tokens' K and V already appended): the row at position p sees positions 0 ..
+ * p of its own sequence,
+ *   out = sum_j softmax_j(softmax_scale * q . k_j) v_j,
+ * KV head h serving query heads h * G .. h * G + G - 1.  Single tokens, chunks
+ * of a prompt and whole prompts may be mixed in a batch.  Rows that see nothing
+ * (positions below 0) are zeros; rows of no sequence are left as they were.
+ *   - max_chunk bounds every sequence's rows (HOST value; it picks which
+ *     kernels are launched).  Lengths and tables are read on the device.
+ *   - q, out: bf16 [num_q_heads][rows][head_dim] at any 16-byte aligned stride.
+ *   - workspace: device memory of pcp_chunk_attention_workspace_size bytes,
+ *     aligned to 256, needed until the call's work has run; calls that may
+ *     overlap need one each. */
+int pcp_chunk_attention_workspace_size(const pcp_pool_t* pool, int32_t num_q_heads, int32_t num_seqs, int32_t rows,
+                                       int32_t max_chunk, size_t* bytes);
+int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* q, const pcp_heads_t* out,
+                        int32_t max_chunk, float softmax_scale, void* workspace, size_t workspace_bytes,
+                        int32_t* device_status, void* stream);
 
 #ifdef __cplusplus
 }
