@@ -6,14 +6,21 @@
 // hide behind it.  A 128-row tcgen05 tile would spend its time on empty rows
 // (the tile kernel reads 2.4 TB/s on such a unit); here a warp's mma.sync tile is
 // 16 rows, which one token's group of heads fills, and warps split the KEYS:
-//   * A producer warp streams stages of kStageKeys keys (K and V of one head, 8
-//     KB of e4m3 or 16 KB of bf16) through a 128 KB shared-memory ring with TMA
-//     (16-row boxes, so pages of any multiple of 16 tokens; 128-byte swizzle).
-//   * Stage c goes to warp c % 8, which scores its keys against all rows and
-//     adds P V into its own 16 x D accumulators, with its own running maximum:
-//     nothing is exchanged between warps until the unit ends.  A unit of 17 to
-//     32 rows uses warps w and w + 4 as its two row tiles on the same stage.
-//   * The warps' (m, l, O) are merged through shared memory when the unit's part
+//   * A producer warp streams 32 KB stages (K and V of one head) through a ring of
+//     four with TMA.  A copy costs its issuer some 350 cycles whatever its size,
+//     and the SM's share of HBM is 8 KB in that time: so one copy brings all of a
+//     stage's rows that share a page (16 to 128: pages of any multiple of 16
+//     tokens), K and V together, 128-byte columns swizzled for the MMAs.
+//   * Teams of D / 128 warps take 16 keys each in turn: a team scores its keys
+//     against all rows and adds P V into its own accumulators, with its own running
+//     maximum, so teams exchange nothing until the unit ends.  Within a team of
+//     two each warp has half the columns: half the terms of the scores, which
+//     are summed through shared memory, and half the output.  128 columns are
+//     what lets 12 such warps live on an SM (64 accumulators a thread): one
+//     warp with all 256 columns at two warps a scheduler spilled, and read 2.0
+//     TB/s where this reads the figures below.  17 to 32 rows are two row
+//     tiles, each with half the teams, on the same stages.
+//   * The teams' (m, l, O) are merged through shared memory when the unit's part
 //     ends, into bf16 rows or an fp32 partial.
 //
 // e4m3 codes become f16 in registers (exact) on their way into the MMA.  No
@@ -36,35 +43,41 @@
 
 namespace pcp {
 
-constexpr int kRowsWarps = 8;
-constexpr int kRowsThreads = 32 * kRowsWarps + 32;  // + the producer warp
-
 template <int D, bool kFp8>
 struct RowsSmem {
   static constexpr int kElt = kFp8 ? 1 : 2;
-  static constexpr int kStageKeys = 4096 / D;             // 16 or 32
-  static constexpr int kGroups = kStageKeys / 16;          // 16-row boxes down a stage
-  static constexpr int kBoxes = D * kElt / 128;            // 128-byte boxes across a row
-  static constexpr int kBoxPair = 2 * 16 * 128;            // a box's K rows, then its V rows
-  static constexpr int kStageBytes = kGroups * kBoxes * kBoxPair;
-  static constexpr int kStages = 131072 / kStageBytes;
-  static constexpr int kScaleBytes = kFp8 ? kStageKeys * 2 : 0;  // [group][K, V][16]
+  // Consumer warps: with the producer 13 at up to 128 registers, or (bf16, which
+  // converts nothing) 9 at up to 168.
+  static constexpr int kWarps = kFp8 ? 12 : 8;
+  static constexpr int kThreads = 32 * kWarps + 32;
+  static constexpr int kTeam = D / 128;          // warps of a team
+  static constexpr int kTeams = kWarps / kTeam;
+  static constexpr int kBoxes = D * kElt / 128;             // 128-byte columns of a row
+  static constexpr int kStageBytes = 32768;
+  static constexpr int kStageKeys = kStageBytes / (256 * kBoxes);  // 32 to 128
+  static constexpr int kStages = 4;
+  // Scale bytes of a stage: a copy's K rows, then its V rows, at 128-byte slots.
+  static constexpr int kScaleStage = kFp8 ? kStageKeys / 16 * 128 : 0;
   // O exchange: 16 rows of D floats, 4 floats of padding every 32, rows 16
   // banks apart: a lane's 16-byte stores fall on distinct banks.
   static constexpr int kRowFloats = D + D / 8 + (D == 256 ? 16 : 0);
   static constexpr int kBufBytes = 16 * kRowFloats * 4;
-  static constexpr int kBufs = 4;
+  static constexpr int kBufs = kTeams / 2;
+  static_assert(kTeams % 2 == 0, "two row tiles share the teams");
   static constexpr int kQOff = kStages * kStageBytes;
   static constexpr int kQBytes = 2 * 16 * D * 2;  // two row tiles in MMA fragment order
   static constexpr int kScaleOff = kQOff + kQBytes;
-  static constexpr int kBufOff = kScaleOff + kStages * kScaleBytes;
-  static constexpr int kRowOff = kBufOff + kBufs * kBufBytes;       // float score factor[32], int position[32]
-  static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;       // float m[8][16], l[8][16]
-  static constexpr int kBarOff = kMlOff + 2 * kRowsWarps * 16 * 4;  // full, empty
+  static constexpr int kBufOff = kScaleOff + kStages * kScaleStage;
+  // The halves of a team's scores, [2 slots][warp][2][lane][4] floats, use the
+  // buffers' space before the merge.
+  static constexpr int kRowOff = kBufOff + kBufs * kBufBytes;  // float score factor[32], int position[32]
+  static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;  // float m, l: [team][16]
+  static constexpr int kBarOff = kMlOff + 2 * kTeams * 16 * 4;  // full, empty
   static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
   static constexpr int kBytes = kMiscOff + 16;
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
-  static_assert(kBufOff % 16 == 0 && kBarOff % 8 == 0 && kScaleOff % 16 == 0, "alignment");
+  static_assert(kBufOff % 16 == 0 && kBarOff % 8 == 0 && kScaleOff % 128 == 0, "alignment");
+  static_assert(2 * kWarps * 1024 <= kBufs * kBufBytes, "the score halves fit the buffers");
 };
 
 template <bool kF16>
@@ -86,23 +99,11 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "memory");
 }
 
-// Untiled copy of `bytes` (a multiple of 16) from global memory into THIS
-// CTA's shared memory, completion on `bar`.  No multicast.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
-}
-
 template <int D, bool kFp8>
-__global__ void __launch_bounds__(kRowsThreads, 1)
-    chunk_rows_kernel(const __grid_constant__ CUtensorMap tm_kv, const ChunkParams p) {
+__global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
+    chunk_rows_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale,
+                      const int box_shift, const ChunkParams p) {
   using L = RowsSmem<D, kFp8>;
-  constexpr int NST = L::kStages;
   constexpr int kBoxElts = 128 / L::kElt;
   constexpr int kBoxSteps = kBoxElts / 16;  // MMA k steps of a box: 8 or 4
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -116,16 +117,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   float* row_factor = reinterpret_cast<float*>(smem + L::kRowOff);
   int* row_pos = reinterpret_cast<int*>(smem + L::kRowOff) + kSmallRows;
   float* s_m = reinterpret_cast<float*>(smem + L::kMlOff);
-  float* s_l = s_m + kRowsWarps * 16;
+  float* s_l = s_m + L::kTeams * 16;
   auto bar_full = [&](int s) { return sbase + L::kBarOff + 8u * s; };
-  auto bar_empty = [&](int s) { return sbase + L::kBarOff + 8u * (NST + s); };
+  auto bar_empty = [&](int s) { return sbase + L::kBarOff + 8u * (L::kStages + s); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NST; ++s) {
+    for (int s = 0; s < L::kStages; ++s) {
       mbar_init(bar_full(s), 1);
-      mbar_init(bar_empty(s), 2);  // both row tiles' warps, or one warp twice
+      // Every consumer warp sees every filling of every stage, its keys in it
+      // or not: the barrier's parity could not tell two fillings apart otherwise.
+      mbar_init(bar_empty(s), L::kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -137,67 +140,68 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   ChunkUnit un;
   int kt0, kt1, slot;
   uint32_t c = 0;  // stages of this CTA so far
+  const int box_rows = 1 << box_shift;  // rows (keys) of a copy
+  const uint32_t box_bytes = 256 * L::kBoxes * box_rows, scale_slot = max(128, 2 * box_rows);
 
-  if (warp == kRowsWarps) {
+  if (warp == L::kWarps) {
     // -------------------------------------------------------- producer --
     bool ok = true;
+    const bool scaled = kFp8 && p.pool.scales;
+    const int bs = p.pool.block_size;
     while (ok && walk.next(un, kt0, kt1, slot)) {
       const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
       const int* table = p.batch.tables + un.seq * p.batch.table_stride;
-      int page = 0;  // lane i: the page of 16-key group i of the current 32
+      int page = 0, row = 0;  // lane i: where copy i of the current 32 lies
+      int i = 32;
       for (int key = k0; key < k1; key += L::kStageKeys) {
-        const int g0 = (key - k0) / 16;
-        if (g0 % 32 == 0) {
-          const int at = key + 16 * lane;
-          if (at < k1) {
-            page = table[at / p.pool.block_size];
-            if (page < 0 || page >= p.pool.blocks) {
-              atomicCAS(p.err, 0, kErrBlockTable);
-              page = 0;
+        const int st = c % L::kStages;
+        const int boxes = (min(L::kStageKeys, k1 - key) + box_rows - 1) >> box_shift;
+        if (lane == 0) {
+          ok = mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, p.err, kErrWaitKvEmpty);
+          if (ok) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (scaled ? 2 * box_rows : 0)));
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        for (int b = 0; b < boxes; ++b, ++i) {
+          if (i == 32) {
+            i = 0;
+            const int at = key + ((b + lane) << box_shift);
+            if (at < k1) {
+              page = table[at / bs];
+              row = at % bs;
+              if (page < 0 || page >= p.pool.blocks) {
+                atomicCAS(p.err, 0, kErrBlockTable);
+                page = 0;
+              }
             }
           }
-        }
-        const int st = c % NST;
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(bar_empty(st), ((c / NST) & 1u) ^ 1u, abort_flag, p.err, kErrWaitKvEmpty));
-        if (!ok) break;
-        const int groups = min(L::kGroups, (k1 - key + 15) / 16);
-        const bool scaled = kFp8 && p.pool.scales;
-        if (lane == 0)
-          mbar_arrive_expect_tx(bar_full(st), groups * (L::kBoxes * L::kBoxPair + (scaled ? 32 : 0)));
-        __syncwarp();
-        // Lane (group, box) loads a box of K and V; the lanes behind them the scales.
-        const int g = lane / L::kBoxes;
-        const int pg = __shfl_sync(0xffffffffu, page, (g0 + min(g, L::kGroups - 1)) % 32);
-        if (g < groups)
-          tma_load_5d(sbase + st * L::kStageBytes + lane * L::kBoxPair, &tm_kv, (lane % L::kBoxes) * kBoxElts,
-                      (key + 16 * g) % p.pool.block_size, un.head, 0, pg, bar_full(st));
-        if (kFp8) {
-          const int j = lane - 16;  // group, K or V
-          const int ps = __shfl_sync(0xffffffffu, page, (g0 + min(max(j, 0) / 2, L::kGroups - 1)) % 32);
-          if (scaled && j >= 0 && j < 2 * groups) {
-            const long long row = (static_cast<long long>(ps) * 2 + (j & 1)) * p.pool.heads + un.head;
-            bulk_load(sScale + st * L::kScaleBytes + j * 16,
-                      p.pool.scales + row * p.pool.block_size + (key + 16 * (j / 2)) % p.pool.block_size, 16,
-                      bar_full(st));
+          const int pg = 2 * __shfl_sync(0xffffffffu, page, i), at = __shfl_sync(0xffffffffu, row, i);
+          if (lane == 0) {
+            tma_load_5d(sbase + st * L::kStageBytes + b * box_bytes, &tm_kv, 0, at, 0, un.head, pg, bar_full(st));
+            if (scaled)
+              tma_load_3d(sScale + st * L::kScaleStage + b * scale_slot, &tm_scale, at, un.head, pg, bar_full(st));
           }
         }
         ++c;
       }
     }
-    if (!ok)  // let the copies in flight land before the CTA ends
-      for (uint32_t i = c > NST ? c - NST : 0; i < c; ++i) mbar_wait_teardown(bar_full(i % NST), (i / NST) & 1u);
+    if (!ok && lane == 0)  // let the copies in flight land before the CTA ends
+      for (uint32_t i = c > L::kStages ? c - L::kStages : 0; i < c; ++i)
+        mbar_wait_teardown(bar_full(i % L::kStages), (i / L::kStages) & 1u);
     return;
   }
 
   // ------------------------------------------------------------ consumers --
-  const int gq = lane >> 2, i4 = lane & 3;  // MMA row (and column) group, position in it
+  constexpr int kConsumers = 32 * L::kWarps;
+  constexpr int kWarpBoxes = L::kElt;        // 128-byte boxes of a warp's 128 columns
+  const int gq = lane >> 2, i4 = lane & 3;   // MMA row (and column) group, position in it
+  const int part = warp % L::kTeam;          // this warp's 128 columns
   bool ok = true;
   while (walk.next(un, kt0, kt1, slot)) {
     const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
-    const int two = un.rows > 16;  // two row tiles
+    const bool two = un.rows > 16;  // two row tiles
     // Q into fragment order: a warp a row, eight elements a lane.
-    for (int r = warp; r < (two ? 32 : 16); r += kRowsWarps) {
+    for (int r = warp; r < (two ? 32 : 16); r += L::kWarps) {
       const int row = un.row0 + r;
       const bool live = r < un.rows, mine = lane < D / 8;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -240,90 +244,122 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
       }
     }
-    named_bar_sync(1, 32 * kRowsWarps);
-    const int tile = two ? warp >> 2 : 0;
-    const uint32_t q_frag = sQ + tile * (16 * D * 2) + lane * 16;
-    const float f0 = row_factor[tile * 16 + gq], f1 = row_factor[tile * 16 + gq + 8];
-    const int pos0 = row_pos[tile * 16 + gq], pos1 = row_pos[tile * 16 + gq + 8];
+    named_bar_sync(1, kConsumers);
+    const int teams = two ? L::kTeams / 2 : L::kTeams;  // of each row tile
+    const int team = warp / L::kTeam;
+    const int qt = team / teams, turn = team % teams;
+    const uint32_t q_frag = sQ + qt * (16 * D * 2) + (part * kWarpBoxes * kBoxSteps * 32 + lane) * 16;
+    const float f0 = row_factor[qt * 16 + gq], f1 = row_factor[qt * 16 + gq + 8];
+    const int pos0 = row_pos[qt * 16 + gq], pos1 = row_pos[qt * 16 + gq + 8];
+    // Keys that every live row of the tile sees: no comparison needed there.
+    const int all_see = un.kvlen - un.qlen + (un.row0 + qt * 16) / p.group + 1;
     const bool scaled = kFp8 && p.pool.scales;
 
-    float o[D / 8][4];
+    float o[16][4];
 #pragma unroll
-    for (int t = 0; t < D / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-    const uint32_t c0 = c;
-    c += (max(k1 - k0, 0) + L::kStageKeys - 1) / L::kStageKeys;
-    const uint32_t step = two ? 4 : 8, first = two ? (warp & 3) : warp;
-    for (uint32_t cc = c0 + ((first - c0) & (step - 1)); ok && cc < c; cc += step) {
-      const int st = cc % NST;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_full(st), (cc / NST) & 1u, abort_flag, p.err, kErrWaitKvFull));
+    uint32_t swap = 0;     // which of the two score exchange slots
+    int next = 16 * turn;  // this team's next keys, from the stage's first
+    for (int key0 = k0; key0 < k1; key0 += L::kStageKeys, ++c) {
+      const int st = c % L::kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_full(st), (c / L::kStages) & 1u, abort_flag, p.err, kErrWaitKvFull));
+      // (The warps of a team of two go on together or not at all.)
+      if (L::kTeam > 1) ok = named_bar_and(2 + team, 32 * L::kTeam, ok);
       if (!ok) break;
-      const int key0 = k0 + static_cast<int>(cc - c0) * L::kStageKeys;
-#pragma unroll 1
-      for (int gr = 0; gr < L::kGroups; ++gr) {
-        const int key = key0 + 16 * gr;
-        if (key >= k1) break;
-        const uint32_t base = sbase + st * L::kStageBytes + gr * (L::kBoxes * L::kBoxPair);
-        // S = Q K^T of 16 keys: columns 2 i4, + 1 of two 8-key tiles.
+      const int here = min(L::kStageKeys, k1 - key0);
+      for (; next < here; next += 16 * teams) {
+        const int key = key0 + next;
+        const int box = next >> box_shift, in_box = next & (box_rows - 1);
+        const uint32_t col = box_rows * 128;  // a 128-byte column of K (or V) in its copy
+        const uint32_t base = sbase + st * L::kStageBytes + box * box_bytes + in_box * 128 + part * kWarpBoxes * col;
+        const uint32_t kV = L::kBoxes * col;
+        // S = Q K^T of 16 keys: columns 2 i4, + 1 of two 8-key tiles, in two
+        // chains of MMAs each.
         float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int b = 0; b < L::kBoxes; ++b) {
-          const uint32_t kr = base + b * L::kBoxPair + gq * 128;
+        for (int b = 0; b < kWarpBoxes; ++b) {
+          const uint32_t kr = base + b * col + gq * 128;
           const uint32_t ca = ((2 * i4) ^ gq) * 16, cb = ((2 * i4 + 1) ^ gq) * 16;
-          const uint4 xa = lds128(kr + ca), xb = lds128(kr + cb);
-          const uint4 ya = lds128(kr + 1024 + ca), yb = lds128(kr + 1024 + cb);
+          const uint4 xa = lds128(kr + ca), ya = lds128(kr + 1024 + ca);
+          const uint4 xb = lds128(kr + cb), yb = lds128(kr + 1024 + cb);
           const uint32_t x[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
           const uint32_t y[8] = {ya.x, ya.y, ya.z, ya.w, yb.x, yb.y, yb.z, yb.w};
 #pragma unroll
           for (int j = 0; j < kBoxSteps; ++j) {
             const uint4 a = lds128(q_frag + (b * kBoxSteps + j) * 512);
+            float(&sa)[4] = (j & 1) ? s2[0] : s[0];
+            float(&sb)[4] = (j & 1) ? s2[1] : s[1];
             if (kFp8) {
               uint32_t b0, b1;
               e4m3x4_to_f16x4(x[j], b0, b1);
-              mma16816<true>(s[0], a, b0, b1);
+              mma16816<true>(sa, a, b0, b1);
               e4m3x4_to_f16x4(y[j], b0, b1);
-              mma16816<true>(s[1], a, b0, b1);
+              mma16816<true>(sb, a, b0, b1);
             } else {
-              mma16816<false>(s[0], a, x[2 * j], x[2 * j + 1]);
-              mma16816<false>(s[1], a, y[2 * j], y[2 * j + 1]);
+              mma16816<false>(sa, a, x[2 * j], x[2 * j + 1]);
+              mma16816<false>(sb, a, y[2 * j], y[2 * j + 1]);
             }
           }
         }
-        // Scores in log2 units, hidden keys at -inf.
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+        if (L::kTeam > 1) {  // the other warp's half of the terms
+          float4* xch = reinterpret_cast<float4*>(smem + L::kBufOff) + ((swap * L::kWarps + warp) * 2) * 32 + lane;
+          xch[0] = make_float4(s[0][0], s[0][1], s[0][2], s[0][3]);
+          xch[32] = make_float4(s[1][0], s[1][1], s[1][2], s[1][3]);
+          named_bar_sync(2 + team, 32 * L::kTeam);
+          const float4* other =
+              reinterpret_cast<const float4*>(smem + L::kBufOff) + ((swap * L::kWarps + (warp ^ 1)) * 2) * 32 + lane;
+          const float4 u = other[0], v = other[32];
+          s[0][0] += u.x, s[0][1] += u.y, s[0][2] += u.z, s[0][3] += u.w;
+          s[1][0] += v.x, s[1][1] += v.y, s[1][2] += v.z, s[1][3] += v.w;
+          swap ^= 1;
+        }
+        const int left = k1 - key;  // keys of this group that are there
+        const bool whole = left >= 16 && key + 16 <= all_see;
         float vs[4] = {1.f, 1.f, 1.f, 1.f};  // V scales of this lane's four keys
-        int vb[4] = {127, 127, 127, 127};    // their exponents, biased
+        int ev = 127;                        // their largest exponent, biased
         if (scaled) {
-          const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleBytes + gr * 32 + 2 * i4;
+          const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
+          ev = 0;
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             const uint32_t kb = *reinterpret_cast<const uint16_t*>(sc + 8 * n);
-            const uint32_t vv = *reinterpret_cast<const uint16_t*>(sc + 16 + 8 * n);
+            uint32_t vv = *reinterpret_cast<const uint16_t*>(sc + box_rows + 8 * n);
+            if (!whole) {  // keys that are not there: any byte
+              if (8 * n + 2 * i4 >= left) vv &= 0xFF00u;
+              if (8 * n + 2 * i4 + 1 >= left) vv &= 0x00FFu;
+            }
             const float ka = __uint_as_float((kb & 0xFFu) << 23), kc = __uint_as_float((kb >> 8) << 23);
             s[n][0] *= ka;
             s[n][1] *= kc;
             s[n][2] *= ka;
             s[n][3] *= kc;
-            vb[2 * n] = vv & 0xFF;
-            vb[2 * n + 1] = vv >> 8;
+            vs[2 * n] = __uint_as_float((vv & 0xFFu) << 23);
+            vs[2 * n + 1] = __uint_as_float((vv >> 8) << 23);
+            ev = max(ev, static_cast<int>(max(vv & 0xFFu, vv >> 8)));
           }
         }
-        const int left = k1 - key;  // keys of this group that are there
+        // Scores in log2 units, hidden keys at -inf.
         float mx0 = -INFINITY, mx1 = -INFINITY;
-        int ev = 0;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int kk = 8 * n + 2 * i4 + j;
-            s[n][j] = kk < left && key + kk <= pos0 ? s[n][j] * f0 : -INFINITY;
-            s[n][j + 2] = kk < left && key + kk <= pos1 ? s[n][j + 2] * f1 : -INFINITY;
+            s[n][j] *= f0;
+            s[n][j + 2] *= f1;
+            if (!whole) {
+              const int kk = 8 * n + 2 * i4 + j;
+              if (kk >= left || key + kk > pos0) s[n][j] = -INFINITY;
+              if (kk >= left || key + kk > pos1) s[n][j + 2] = -INFINITY;
+            }
             mx0 = fmaxf(mx0, s[n][j]);
             mx1 = fmaxf(mx1, s[n][j + 2]);
-            if (scaled) {
-              vs[2 * n + j] = kk < left ? __uint_as_float(static_cast<uint32_t>(vb[2 * n + j]) << 23) : 0.f;
-              ev = kk < left ? max(ev, vb[2 * n + j]) : ev;
-            }
           }
 #pragma unroll
         for (int x = 1; x <= 2; x <<= 1) {
@@ -345,7 +381,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
           l0 *= a0;
           l1 *= a1;
 #pragma unroll
-          for (int t = 0; t < D / 8; ++t) {
+          for (int t = 0; t < 16; ++t) {
             o[t][0] *= a0;
             o[t][1] *= a0;
             o[t][2] *= a1;
@@ -372,38 +408,38 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const uint4 pa = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         // O += P V; rows of keys that are not there may hold anything: zeros.
         if (kFp8) {
-          const uint32_t z0 = 2 * i4 < left ? ~0u : 0u, z1 = 2 * i4 + 1 < left ? ~0u : 0u;
-          const uint32_t z2 = 2 * i4 + 8 < left ? ~0u : 0u, z3 = 2 * i4 + 9 < left ? ~0u : 0u;
+          const uint32_t vr = base + kV + 2 * i4 * 128;
+          const uint32_t ce = (gq ^ (2 * i4)) * 16, co = (gq ^ (2 * i4 + 1)) * 16;
+          uint4 v0 = lds128(vr + ce), v1 = lds128(vr + 128 + co);
+          uint4 v2 = lds128(vr + 1024 + ce), v3 = lds128(vr + 1024 + 128 + co);
+          if (left < 16) {
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            if (2 * i4 >= left) v0 = zero;
+            if (2 * i4 + 1 >= left) v1 = zero;
+            if (2 * i4 + 8 >= left) v2 = zero;
+            if (2 * i4 + 9 >= left) v3 = zero;
+          }
+          const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+          const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
 #pragma unroll
-          for (int b = 0; b < L::kBoxes; ++b) {
-            const uint32_t vr = base + b * L::kBoxPair + 2048 + 2 * i4 * 128;
-            const uint32_t ce = (gq ^ (2 * i4)) * 16, co = (gq ^ (2 * i4 + 1)) * 16;
-            const uint4 v0 = lds128(vr + ce), v1 = lds128(vr + 128 + co);
-            const uint4 v2 = lds128(vr + 1024 + ce), v3 = lds128(vr + 1024 + 128 + co);
-            const uint32_t w0[4] = {v0.x & z0, v0.y & z0, v0.z & z0, v0.w & z0};
-            const uint32_t w1[4] = {v1.x & z1, v1.y & z1, v1.z & z1, v1.w & z1};
-            const uint32_t w2[4] = {v2.x & z2, v2.y & z2, v2.z & z2, v2.w & z2};
-            const uint32_t w3[4] = {v3.x & z3, v3.y & z3, v3.z & z3, v3.w & z3};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t a0, a1, b0, b1;
-              e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x5140), a0, a1);
-              e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x5140), b0, b1);
-              mma16816<true>(o[b * 16 + 4 * j], pa, a0, b0);
-              mma16816<true>(o[b * 16 + 4 * j + 1], pa, a1, b1);
-              e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x7362), a0, a1);
-              e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x7362), b0, b1);
-              mma16816<true>(o[b * 16 + 4 * j + 2], pa, a0, b0);
-              mma16816<true>(o[b * 16 + 4 * j + 3], pa, a1, b1);
-            }
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, b0, b1;
+            e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x5140), a0, a1);
+            e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x5140), b0, b1);
+            mma16816<true>(o[4 * j], pa, a0, b0);
+            mma16816<true>(o[4 * j + 1], pa, a1, b1);
+            e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x7362), a0, a1);
+            e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x7362), b0, b1);
+            mma16816<true>(o[4 * j + 2], pa, a0, b0);
+            mma16816<true>(o[4 * j + 3], pa, a1, b1);
           }
         } else {
           const uint32_t z0 = (2 * i4 < left ? 0xFFFFu : 0u) | (2 * i4 + 1 < left ? 0xFFFF0000u : 0u);
           const uint32_t z1 = (2 * i4 + 8 < left ? 0xFFFFu : 0u) | (2 * i4 + 9 < left ? 0xFFFF0000u : 0u);
           const int vrow = lane & 15, vc = lane >> 4;
 #pragma unroll
-          for (int b = 0; b < L::kBoxes; ++b) {
-            const uint32_t vr = base + b * L::kBoxPair + 2048 + vrow * 128;
+          for (int b = 0; b < kWarpBoxes; ++b) {
+            const uint32_t vr = base + kV + b * col + vrow * 128;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t v[4];
@@ -414,66 +450,63 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
           }
         }
       }
+      next -= L::kStageKeys;
       __syncwarp();
-      if (lane == 0) mbar_arrive_n(bar_empty(st), two ? 1 : 2);
+      if (lane == 0) mbar_arrive(bar_empty(st));
     }
 
-    // ------------------------------------ merge the warps of each row tile --
+    // ------------------------------------ merge the teams of each row tile --
 #pragma unroll
     for (int x = 1; x <= 2; x <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, x);
       l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
-    if (i4 == 0) {
-      s_m[warp * 16 + gq] = m0;
-      s_m[warp * 16 + gq + 8] = m1;
-      s_l[warp * 16 + gq] = l0;
-      s_l[warp * 16 + gq + 8] = l1;
+    if (i4 == 0 && part == 0) {  // a team's warps hold the same m and l
+      s_m[team * 16 + gq] = m0;
+      s_m[team * 16 + gq + 8] = m1;
+      s_l[team * 16 + gq] = l0;
+      s_l[team * 16 + gq + 8] = l1;
     }
-    if (!named_bar_and(1, 32 * kRowsWarps, ok && *abort_flag == 0)) return;
-    const int w0 = two ? tile * 4 : 0, wn = two ? 4 : 8;
+    if (!named_bar_and(1, kConsumers, ok && *abort_flag == 0)) return;
     float M0 = -INFINITY, M1 = -INFINITY;
-    for (int w = w0; w < w0 + wn; ++w) {
+    for (int w = qt * teams; w < (qt + 1) * teams; ++w) {
       M0 = fmaxf(M0, s_m[w * 16 + gq]);
       M1 = fmaxf(M1, s_m[w * 16 + gq + 8]);
     }
-    const float a0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - M0);
-    const float a1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - M1);
+    const float a0 = ex2_approx(m0 - M0), a1 = ex2_approx(m1 - M1);
 #pragma unroll
-    for (int t = 0; t < D / 8; ++t) {
-      // A warp that saw nothing of a row adds nothing to it.
+    for (int t = 0; t < 16; ++t) {
+      // A team that saw nothing of a row adds nothing to it.
       o[t][0] = m0 == -INFINITY ? 0.f : o[t][0] * a0;
       o[t][1] = m0 == -INFINITY ? 0.f : o[t][1] * a0;
       o[t][2] = m1 == -INFINITY ? 0.f : o[t][2] * a1;
       o[t][3] = m1 == -INFINITY ? 0.f : o[t][3] * a1;
     }
-    const int half = wn / 2, wi = warp - w0;
-    float* buf = reinterpret_cast<float*>(smem + L::kBufOff + ((two ? tile * 2 : 0) + wi % half) * L::kBufBytes);
-    // This lane's elements of a row, four (e4m3) or two (bf16) at a time.
+    // The last teams write their O to the tile's buffers, those before them add
+    // theirs, round by round.
+    const int bufs = two ? L::kBufs / 2 : L::kBufs;
+    float* buf = reinterpret_cast<float*>(smem + L::kBufOff + (qt * bufs + turn % bufs) * L::kBufBytes) + part * 144;
     auto exchange = [&](bool add) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float* row = buf + (gq + 8 * r) * L::kRowFloats;
         if (kFp8) {
 #pragma unroll
-          for (int b = 0; b < L::kBoxes; ++b)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int d = b * 128 + 32 * i4 + 16 * h + 4 * j;
-                float4* at = reinterpret_cast<float4*>(row + d + 4 * (d / 32));
-                float4 v = make_float4(o[b * 16 + 4 * j][2 * r + h], o[b * 16 + 4 * j + 1][2 * r + h],
-                                       o[b * 16 + 4 * j + 2][2 * r + h], o[b * 16 + 4 * j + 3][2 * r + h]);
-                if (add) {
-                  const float4 x = *at;
-                  v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
-                }
-                *at = v;
+            for (int j = 0; j < 4; ++j) {  // columns 32 i4 + 16 h + 4 j ..
+              float4* at = reinterpret_cast<float4*>(row + 36 * i4 + 16 * h + 4 * j);
+              float4 v = make_float4(o[4 * j][2 * r + h], o[4 * j + 1][2 * r + h], o[4 * j + 2][2 * r + h],
+                                     o[4 * j + 3][2 * r + h]);
+              if (add) {
+                const float4 x = *at;
+                v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
               }
+              *at = v;
+            }
         } else {
 #pragma unroll
-          for (int t = 0; t < D / 8; ++t) {
+          for (int t = 0; t < 16; ++t) {
             const int d = 8 * t + 2 * i4;
             float2* at = reinterpret_cast<float2*>(row + d + 4 * (d / 32));
             float2 v = make_float2(o[t][2 * r], o[t][2 * r + 1]);
@@ -486,25 +519,25 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
       }
     };
-    if (wi >= half) exchange(false);
-    named_bar_sync(1, 32 * kRowsWarps);
-    if (wi < half) exchange(true);
-    named_bar_sync(1, 32 * kRowsWarps);
+    for (int round = (teams - 1) / bufs; round >= 0; --round) {
+      if (turn / bufs == round) exchange(turn + bufs < teams);
+      named_bar_sync(1, kConsumers);
+    }
     // Every thread eight elements of a row: sum the buffers, divide, write.
-    for (int x = threadIdx.x; x < un.rows * (D / 8); x += 32 * kRowsWarps) {
+    for (int x = threadIdx.x; x < un.rows * (D / 8); x += kConsumers) {
       const int r = x / (D / 8), d = (x % (D / 8)) * 8;
-      const int t = r / 16, tw0 = two ? t * 4 : 0;
+      const int t = r / 16;
       float M = -INFINITY, lsum = 0.f;
-      for (int w = tw0; w < tw0 + wn; ++w) M = fmaxf(M, s_m[w * 16 + r % 16]);
-      for (int w = tw0; w < tw0 + wn; ++w) {
+      for (int w = t * teams; w < (t + 1) * teams; ++w) M = fmaxf(M, s_m[w * 16 + r % 16]);
+      for (int w = t * teams; w < (t + 1) * teams; ++w) {
         const float mw = s_m[w * 16 + r % 16];
         // Without a maximum the sum is 0, or NaN where every score was NaN.
         lsum += mw == -INFINITY ? s_l[w * 16 + r % 16] : s_l[w * 16 + r % 16] * ex2_approx(mw - M);
       }
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       const float* src = reinterpret_cast<const float*>(smem + L::kBufOff) + (r % 16) * L::kRowFloats + d + 4 * (d / 32);
-      for (int k = 0; k < half; ++k) {
-        const float4* at = reinterpret_cast<const float4*>(src + ((two ? t * 2 : 0) + k) * (L::kBufBytes / 4));
+      for (int k = 0; k < bufs; ++k) {
+        const float4* at = reinterpret_cast<const float4*>(src + (t * bufs + k) * (L::kBufBytes / 4));
         const float4 u = at[0], v = at[1];
         f[0] += u.x, f[1] += u.y, f[2] += u.z, f[3] += u.w, f[4] += v.x, f[5] += v.y, f[6] += v.z, f[7] += v.w;
       }

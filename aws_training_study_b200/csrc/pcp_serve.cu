@@ -165,10 +165,7 @@ int check_chunk(const pcp_pool_t* pool, int32_t q_heads, int32_t seqs, int32_t r
   return PCP_OK;
 }
 
-// Cache blocks [blocks][2][Hkv][bs][D] as a 5-D tensor {D, bs, Hkv, K/V,
-// blocks}; boxes of box_x elements x box_rows rows of one head of box_kv of K
-// and V of one block.
-int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t box_rows, uint32_t box_kv, bool swizzle) {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -178,19 +175,56 @@ int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
   });
+  return fn;
+}
+
+int encode(CUtensorMap* tm, CUtensorMapDataType type, int rank, void* base, const cuuint64_t* dims,
+           const cuuint64_t* strides, const cuuint32_t* box, bool swizzle) {
+  auto fn = encode_fn();
   if (!fn) return fail(PCP_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
-  const bool bf16 = p.kv_dtype == PCP_KV_BF16;
-  const uint64_t D = p.head_dim, bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1;
-  cuuint64_t dims[5] = {D, bs, H, 2, static_cast<cuuint64_t>(p.blocks)};
-  cuuint64_t strides[4] = {D * elt, bs * D * elt, H * bs * D * elt, 2 * H * bs * D * elt};
-  cuuint32_t box[5] = {box_x, box_rows, 1, box_kv, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims,
-                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(tm, type, rank, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PCP_ERR_CUDA, "cuTensorMapEncodeTiled (cache pool) failed (%d)", static_cast<int>(r));
   return PCP_OK;
+}
+
+// Cache blocks [blocks][2][Hkv][bs][D] as a 5-D tensor {D, bs, Hkv, K/V,
+// blocks}; boxes of box_x elements x box_rows rows of one head of K or V of one
+// block.
+int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t box_rows, bool swizzle) {
+  const bool bf16 = p.kv_dtype == PCP_KV_BF16;
+  const uint64_t D = p.head_dim, bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1;
+  const cuuint64_t dims[5] = {D, bs, H, 2, static_cast<cuuint64_t>(p.blocks)};
+  const cuuint64_t strides[4] = {D * elt, bs * D * elt, H * bs * D * elt, 2 * H * bs * D * elt};
+  const cuuint32_t box[5] = {box_x, box_rows, 1, 1, 1};
+  return encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims, strides,
+                box, swizzle);
+}
+
+// The same blocks as {128 bytes, bs, 128-byte columns, Hkv, 2 * blocks}: one
+// box is box_rows whole rows of K and of V of one head, each 128-byte column of
+// them in the 128-byte swizzle.
+int make_rows_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows) {
+  const bool bf16 = p.kv_dtype == PCP_KV_BF16;
+  const uint64_t bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1, row = p.head_dim * elt;
+  const uint32_t cols = static_cast<uint32_t>(row / 128);
+  const cuuint64_t dims[5] = {128 / elt, bs, cols, H, 2 * static_cast<cuuint64_t>(p.blocks)};
+  const cuuint64_t strides[4] = {row, 128, bs * row, H * bs * row};
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(128 / elt), box_rows, cols, 1, 2};
+  return encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims, strides,
+                box, true);
+}
+
+// Scale bytes [blocks][2][Hkv][bs] as {bs, Hkv, 2 * blocks}: boxes of box_rows
+// of K and of V of one head.
+int make_scale_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows) {
+  const uint64_t bs = p.block_size, H = p.num_kv_heads;
+  const cuuint64_t dims[3] = {bs, H, 2 * static_cast<cuuint64_t>(p.blocks)};
+  const cuuint64_t strides[2] = {bs, H * bs};
+  const cuuint32_t box[3] = {box_rows, 1, 2};
+  return encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, p.scales, dims, strides, box, false);
 }
 
 // A kernel's dynamic shared memory is allowed once per device.
@@ -210,10 +244,14 @@ int allow_smem(int bytes) {
 template <int D, bool kFp8>
 int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
   using L = pcp::RowsSmem<D, kFp8>;
-  CUtensorMap tm;
-  PCP_TRY(make_pool_map(&tm, pool, kFp8 ? 128 : 64, 16, 2, true));
+  // Rows of a copy: as many as a page's length and a stage share.
+  int shift = 4;
+  while ((2 << shift) <= L::kStageKeys && pool.block_size % (2 << shift) == 0) ++shift;
+  CUtensorMap tm, ts{};
+  PCP_TRY(make_rows_map(&tm, pool, 1 << shift));
+  if (pool.scales) PCP_TRY(make_scale_map(&ts, pool, 1 << shift));
   PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes)));
-  pcp::chunk_rows_kernel<D, kFp8><<<kCtas, pcp::kRowsThreads, L::kBytes, st>>>(tm, p);
+  pcp::chunk_rows_kernel<D, kFp8><<<kCtas, L::kThreads, L::kBytes, st>>>(tm, ts, shift, p);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
 }
@@ -225,8 +263,8 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
   int box_rows = 64;
   while (pool.block_size % box_rows) box_rows /= 2;
   CUtensorMap tk, tv;
-  PCP_TRY(make_pool_map(&tk, pool, L::kFp8 ? D : 64, box_rows, 1, !L::kFp8));
-  PCP_TRY(make_pool_map(&tv, pool, L::kFp8 ? D / 2 : 64, box_rows, 1, !L::kFp8));
+  PCP_TRY(make_pool_map(&tk, pool, L::kFp8 ? D : 64, box_rows, !L::kFp8));
+  PCP_TRY(make_pool_map(&tv, pool, L::kFp8 ? D / 2 : 64, box_rows, !L::kFp8));
   PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes)));
   pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tk, tv, box_rows, p);
   CUDA_TRY(cudaGetLastError());
