@@ -12,8 +12,11 @@
 // A unit's steps are the 128-key tiles that its last row sees (at least one, so
 // that rows without keys are written too).  Each kernel cuts the list of its
 // units' steps into equal contiguous ranges, one per CTA (or CTA pair): every
-// one gets the same work whatever the lengths.  A unit that a range boundary
-// cuts leaves fp32 partials, which chunk_combine_kernel merges.
+// one gets the same work whatever the lengths.  Every CTA finds its range by
+// itself, summing the steps of all sequences in its prologue (a first kernel
+// that listed the units took 16 to 26 us; the sums of a batch take about 2).  A
+// unit that a range boundary cuts leaves fp32 partials, which
+// chunk_combine_kernel merges; a range leaves a record of what it cut.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -37,20 +40,18 @@ struct ChunkUnit {
   int steps;
 };
 
-struct ChunkPlan {
-  int small_units, tile_units;
-  long long small_steps, tile_steps;
+// What a range cut: the unit it starts in the middle of (slot 2 g), and the one
+// it leaves unfinished (slot 2 g + 1).
+struct ChunkRecord {
+  ChunkUnit last;   // the unfinished unit, when `last_cut`
+  int last_cut;
+  int first_state;  // 0: no partial, 1: does not end its unit, 2: ends it
+  int err;          // the CTA's (pair's) device error
 };
 
-// Where a launch's scratch lies.
 struct ChunkWork {
-  ChunkPlan* plan;
-  ChunkUnit* small;
-  long long* small_start;  // first step of each unit, and the total
-  ChunkUnit* tile;
-  long long* tile_start;
-  int* seq_tile;           // [seqs + 1]: query tiles (per head) before each sequence
-  long long* tile_prefix;  // [query tiles + 1]: their steps
+  ChunkRecord* small_rec;  // [small CTAs]
+  ChunkRecord* tile_rec;   // [2 pairs] (error of each CTA; the rest by pair)
   float* small_o;          // [2 small CTAs][kSmallRows][D] partials, normalised
   float* small_lse;        // [2 small CTAs][kSmallRows], log2
   float* tile_o;           // [2 pairs][kUnitRows][D]
@@ -67,8 +68,8 @@ struct ChunkParams {
   int group;       // query heads per KV head
   int max_chunk;
   float scale_log2;
-  int small_ctas, tile_pairs;  // grids of the two kernels
-  int* err;
+  int small_ctas, tile_pairs;  // grids of the two kernels (0 pairs: not launched)
+  int* status;
 };
 
 __device__ __forceinline__ float exp2_of_int(int e) {  // 2^e, 0 below the normal range
@@ -80,30 +81,6 @@ __host__ __device__ __forceinline__ long long chunk_ranges(long long steps, int 
   return steps < grid ? (steps > 1 ? steps : 1) : grid;
 }
 
-// Exclusive block scan over 1024 threads; `total` gets the sum.
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();  // the sums of an earlier scan are read
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  long long before = 0, all = 0;
-  const long long w = warp_sums[lane];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const long long s = __shfl_sync(0xffffffffu, w, i);
-    if (i < warp) before += s;
-    all += s;
-  }
-  total = all;
-  return before + x - v;
-}
-
 // Steps of rows [row0, row0 + rows) of a sequence: tiles up to the last row's
 // position.
 __device__ __forceinline__ int unit_steps(int kvlen, int qlen, int last_row, int group) {
@@ -111,234 +88,345 @@ __device__ __forceinline__ int unit_steps(int kvlen, int qlen, int last_row, int
   return max(1, (visible + kStepKeys - 1) / kStepKeys);
 }
 
-// One block of 1024 threads: checks the batch, then lists the units and their
-// steps.  A batch whose offsets decrease or leave the packed rows is not run
-// at all (its units could overlap or pass the scratch).
-__global__ void __launch_bounds__(1024, 1) chunk_plan_kernel(const ChunkParams p) {
-  __shared__ long long sums[32];
-  const BatchView& b = p.batch;
-  const int tid = threadIdx.x;
-  const int Hkv = p.pool.heads;
-  const long long capacity = static_cast<long long>(b.table_width) * p.pool.block_size;
-  if (tid == 0) *p.err = 0;
+// A sequence as a kernel sees it; `tiles` 0 unless it has units of that kind.
+struct ChunkSeq {
+  int q0, qlen, kvlen;
+  int tiles;  // units of one KV head (small: one)
+};
+
+template <bool kTile>
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int s, int* err) {
+  ChunkSeq q;
+  q.q0 = p.batch.offsets[s];
+  q.qlen = p.batch.offsets[s + 1] - q.q0;
+  q.kvlen = p.batch.kv_len[s];
+  if (q.kvlen < 0) {
+    atomicCAS(err, 0, kErrSequence);
+    q.kvlen = 0;
+  }
+  const long long capacity = static_cast<long long>(p.batch.table_width) * p.pool.block_size;
+  if (q.kvlen > capacity) {
+    atomicCAS(err, 0, kErrBlockTable);
+    q.kvlen = static_cast<int>(capacity);
+  }
+  if (q.qlen > p.max_chunk) {
+    atomicCAS(err, 0, kErrSequence);
+    q.qlen = 0;
+  }
+  const long long rows = static_cast<long long>(q.qlen) * p.group;
+  q.tiles = q.qlen <= 0 || kTile == (rows <= kSmallRows) ? 0
+            : kTile                                      ? static_cast<int>((rows + kUnitRows - 1) / kUnitRows)
+                                                         : 1;
+  return q;
+}
+
+// Unit i of a sequence's head: the last rows first, so that long units start.
+template <bool kTile>
+__device__ __forceinline__ ChunkUnit chunk_unit(const ChunkParams& p, const ChunkSeq& q, int s, int head, int i) {
+  ChunkUnit u;
+  u.seq = s;
+  u.head = head;
+  u.row0 = kTile ? (q.tiles - 1 - i) * kUnitRows : 0;
+  const int rows = q.qlen * p.group;
+  u.rows = kTile ? min(kUnitRows, rows - u.row0) : rows;
+  u.q0 = q.q0;
+  u.qlen = q.qlen;
+  u.kvlen = q.kvlen;
+  u.steps = unit_steps(q.kvlen, q.qlen, u.row0 + u.rows - 1, p.group);
+  return u;
+}
+
+// Shared memory of a range's planning.
+struct ChunkPlanShared {
+  long long sums[16];  // steps (of one KV head) of each warp's sequences
+  long long x, end;    // this range
+  int seq, head, unit, kt;
+  int err;             // the CTA's error word
+};
+
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ long long warp_scan(long long v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+// The whole block (at most 16 warps): finds range g of `grid` in the list of
+// units, in the order sequence, KV head, unit.  Warps sum runs of sequences;
+// the one whose run holds the range's first step looks it up.  A batch whose
+// offsets decrease or leave the packed rows is not run at all: its ranges are
+// empty.  sh.err must be set before.
+template <bool kTile>
+__device__ __forceinline__ void chunk_plan(const ChunkParams& p, ChunkPlanShared& sh, int grid, int g) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int per = (p.batch.seqs + warps - 1) / warps;
+  const int s0 = min(warp * per, p.batch.seqs), s1 = min(s0 + per, p.batch.seqs);
+  // Steps of one head of sequence s; with kTile by the whole warp.
+  auto steps_of = [&](int s) {
+    const ChunkSeq q = chunk_seq<kTile>(p, s, &sh.err);
+    if (!kTile) return static_cast<long long>(q.tiles ? chunk_unit<kTile>(p, q, s, 0, 0).steps : 0);
+    long long n = 0;
+    for (int i = lane; i < q.tiles; i += 32) n += chunk_unit<kTile>(p, q, s, 0, i).steps;
+    return warp_sum(n);
+  };
   bool bad = false;
-  for (int s = tid; s < b.seqs; s += 1024) {
-    const int o0 = b.offsets[s], o1 = b.offsets[s + 1];
-    bad |= o0 < 0 || o1 < o0 || o1 > b.rows;
+  for (int s = s0 + lane; s < s1; s += 32) {
+    const int o0 = p.batch.offsets[s], o1 = p.batch.offsets[s + 1];
+    bad |= o0 < 0 || o1 < o0 || o1 > p.batch.rows;
   }
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) {
-      atomicCAS(p.err, 0, kErrSequence);
-      *p.work.plan = {0, 0, 0, 0};
+  bad = __syncthreads_or(bad);
+  long long sum = 0;
+  if (!bad) {
+    if (kTile) {
+      for (int s = s0; s < s1; ++s) sum += steps_of(s);
+    } else {
+      for (int s = s0 + lane; s < s1; s += 32) sum += steps_of(s);
+      sum = warp_sum(sum);
     }
-    return;
+  } else if (threadIdx.x == 0) {
+    atomicCAS(&sh.err, 0, kErrSequence);
   }
-  long long small0 = 0, steps0 = 0, tile0 = 0;  // totals of the sequences before this block of 1024
-  for (int base = 0; base < b.seqs; base += 1024) {
-    const int s = base + tid;
-    int qlen = 0, kvlen = 0, q0 = 0;
-    if (s < b.seqs) {
-      q0 = b.offsets[s];
-      qlen = b.offsets[s + 1] - q0;
-      kvlen = b.kv_len[s];
-      if (kvlen < 0 || qlen > p.max_chunk) {
-        atomicCAS(p.err, 0, kErrSequence);
-        if (qlen > p.max_chunk) qlen = 0;
-        kvlen = max(kvlen, 0);
-      }
-      if (kvlen > capacity) {
-        atomicCAS(p.err, 0, kErrBlockTable);
-        kvlen = static_cast<int>(capacity);
-      }
-    }
-    const long long rows = static_cast<long long>(qlen) * p.group;
-    const bool small = qlen > 0 && rows <= kSmallRows;
-    const int tiles = qlen > 0 && !small ? static_cast<int>((rows + kUnitRows - 1) / kUnitRows) : 0;
-    const int steps = small ? unit_steps(kvlen, qlen, static_cast<int>(rows) - 1, p.group) : 0;
-    long long n_small, n_steps, n_tiles;
-    const long long u = small0 + block_scan(small ? 1 : 0, sums, n_small);
-    const long long st = steps0 + block_scan(steps, sums, n_steps);
-    const long long t = tile0 + block_scan(tiles, sums, n_tiles);
-    if (small)
-      for (int h = 0; h < Hkv; ++h) {
-        p.work.small[u * Hkv + h] = {s, h, 0, static_cast<int>(rows), q0, qlen, kvlen, steps};
-        p.work.small_start[u * Hkv + h] = st * Hkv + static_cast<long long>(h) * steps;
-      }
-    if (s < b.seqs) p.work.seq_tile[s] = static_cast<int>(t);
-    small0 += n_small;
-    steps0 += n_steps;
-    tile0 += n_tiles;
-  }
-  if (tid == 0) {
-    p.work.small_start[small0 * Hkv] = steps0 * Hkv;
-    p.work.seq_tile[b.seqs] = static_cast<int>(tile0);
-    *p.work.plan = {static_cast<int>(small0 * Hkv), static_cast<int>(tile0 * Hkv), steps0 * Hkv, 0};
-  }
-  if (tile0 == 0) return;
+  if (lane == 0) sh.sums[warp] = sum;
   __syncthreads();
-  // Steps before each query tile (of one head).  Tiles of a sequence are
-  // listed last first: the longest ones start.
-  auto find = [&](int t) {
-    int lo = 0, n = b.seqs;
-    while (n > 1) {
-      const int h = n >> 1;
-      if (p.work.seq_tile[lo + h] <= t) lo += h, n -= h;
-      else n = h;
-    }
-    return lo;
-  };
-  auto unit_of = [&](int t, int s) {
-    const int tiles = p.work.seq_tile[s + 1] - p.work.seq_tile[s];
-    const int q0 = b.offsets[s], qlen = b.offsets[s + 1] - q0;
-    const int kvlen = static_cast<int>(min(static_cast<long long>(max(b.kv_len[s], 0)), capacity));
-    const int row0 = (tiles - 1 - (t - p.work.seq_tile[s])) * kUnitRows;
-    const int rows = static_cast<int>(min(static_cast<long long>(kUnitRows), static_cast<long long>(qlen) * p.group - row0));
-    return ChunkUnit{s, 0, row0, rows, q0, qlen, kvlen, unit_steps(kvlen, qlen, row0 + rows - 1, p.group)};
-  };
-  long long done = 0;
-  for (int base = 0; base < tile0; base += 1024) {
-    const int t = base + tid;
-    const int steps = t < tile0 ? unit_of(t, find(t)).steps : 0;
-    long long n;
-    const long long before = block_scan(steps, sums, n);
-    if (t < tile0) p.work.tile_prefix[t] = done + before;
-    done += n;
+  long long before = 0, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += sh.sums[w];
+    total += sh.sums[w];
   }
-  if (tid == 0) {
-    p.work.tile_prefix[tile0] = done;
-    p.work.tile_start[tile0 * Hkv] = done * Hkv;
-    p.work.plan->tile_steps = done * Hkv;
+  const int heads = p.pool.heads;
+  const long long steps = total * heads, ranges = chunk_ranges(steps, grid);
+  const bool none = total == 0 || g >= ranges;
+  const long long x = none ? 0 : steps * g / ranges, end = none ? 0 : steps * (g + 1) / ranges;
+  if (threadIdx.x == 0) {
+    sh.x = x;
+    sh.end = end;
+  }
+  if (!none && before * heads <= x && x < (before + sum) * heads) {  // this warp's run
+    int seq = -1;
+    long long at = before, in_seq = 0;
+    if (kTile) {
+      for (int s = s0; s < s1 && seq < 0; ++s) {
+        in_seq = steps_of(s);
+        if (x < (at + in_seq) * heads) seq = s;
+        else at += in_seq;
+      }
+    } else {
+      for (int b = s0; b < s1 && seq < 0; b += 32) {
+        const long long n = b + lane < s1 ? steps_of(b + lane) : 0;
+        const long long upto = at + warp_scan(n);
+        const uint32_t past = __ballot_sync(0xffffffffu, x < upto * heads);
+        if (past) {
+          const int i = __ffs(past) - 1;
+          seq = b + i;
+          in_seq = __shfl_sync(0xffffffffu, n, i);
+          at = __shfl_sync(0xffffffffu, upto, i) - in_seq;
+        } else {
+          at = __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+    }
+    const long long rest = x - at * heads;
+    const int head = static_cast<int>(rest / in_seq);
+    long long kt = rest % in_seq;
+    int unit = 0;
+    if (kTile) {
+      const ChunkSeq q = chunk_seq<kTile>(p, seq, &sh.err);
+      for (int b = 0; b < q.tiles; b += 32) {
+        const long long n = b + lane < q.tiles ? chunk_unit<kTile>(p, q, seq, 0, b + lane).steps : 0;
+        const long long upto = warp_scan(n);
+        const uint32_t past = __ballot_sync(0xffffffffu, kt < upto);
+        if (past) {
+          const int i = __ffs(past) - 1;
+          unit = b + i;
+          kt -= __shfl_sync(0xffffffffu, upto - n, i);
+          break;
+        }
+        kt -= __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      sh.seq = seq;
+      sh.head = head;
+      sh.unit = unit;
+      sh.kt = static_cast<int>(kt);
+    }
   }
   __syncthreads();
-  // Units in the order sequence, KV head, tile: a pair's neighbours share K/V.
-  for (long long i = tid; i < tile0 * Hkv; i += 1024) {
-    const int t = static_cast<int>(i / Hkv), h = static_cast<int>(i % Hkv);
-    const int s = find(t);
-    ChunkUnit u = unit_of(t, s);
-    u.head = h;
-    const int first = p.work.seq_tile[s], tiles = p.work.seq_tile[s + 1] - first;
-    const long long at0 = p.work.tile_prefix[first];
-    const long long idx = static_cast<long long>(first) * Hkv + static_cast<long long>(h) * tiles + (t - first);
-    p.work.tile[idx] = u;
-    p.work.tile_start[idx] =
-        at0 * Hkv + h * (p.work.tile_prefix[first + tiles] - at0) + (p.work.tile_prefix[t] - at0);
-  }
 }
 
 // A range's walk over its units: the part [kt0, kt1) of each one's steps.
+template <bool kTile>
 struct ChunkWalk {
-  const ChunkUnit* units;
-  const long long* start;
-  long long x, end;
-  int u;
-  int range;
+  int left;  // steps of the range still to come
+  int seq, head, unit, kt;
 
-  __device__ __forceinline__ void init(const ChunkUnit* list, const long long* starts, int n, long long steps, int grid,
-                                       int g) {
-    units = list;
-    start = starts;
-    range = g;
-    const long long ranges = chunk_ranges(steps, grid);
-    x = end = 0;
-    u = 0;
-    if (n == 0 || g >= ranges) return;
-    x = steps * g / ranges;
-    end = steps * (g + 1) / ranges;
-    int k = n;  // the unit that holds step x
-    while (k > 1) {
-      const int h = k >> 1;
-      if (start[u + h] <= x) u += h, k -= h;
-      else k = h;
-    }
+  __device__ __forceinline__ void init(const ChunkPlanShared& sh) {
+    left = static_cast<int>(sh.end - sh.x);
+    seq = sh.seq;
+    head = sh.head;
+    unit = sh.unit;
+    kt = sh.kt;
   }
-  // The next part: its unit, steps [kt0, kt1) and partial slot (-1: the whole
-  // unit).  A part that starts its unit is the range's last (slot 2 range + 1)
-  // if it does not end it; every other partial part is the range's first.
-  __device__ __forceinline__ bool next(ChunkUnit& unit, int& kt0, int& kt1, int& slot) {
-    if (x >= end) return false;
-    unit = units[u];
-    const long long s0 = start[u], s1 = s0 + unit.steps;
-    const long long to = s1 < end ? s1 : end;
-    kt0 = static_cast<int>(x - s0);
-    kt1 = static_cast<int>(to - s0);
-    slot = kt0 == 0 ? (to == s1 ? -1 : 2 * range + 1) : 2 * range;
-    x = to;
-    ++u;
+  __device__ __forceinline__ bool next(const ChunkParams& p, int* err, ChunkUnit& u, int& kt0, int& kt1) {
+    if (left <= 0) return false;
+    ChunkSeq q = chunk_seq<kTile>(p, seq, err);
+    u = chunk_unit<kTile>(p, q, seq, head, unit);
+    kt0 = kt;
+    kt1 = min(u.steps, kt + left);
+    left -= kt1 - kt0;
+    kt = 0;
+    if (left > 0 && ++unit == q.tiles) {
+      unit = 0;
+      if (++head == p.pool.heads) {
+        head = 0;
+        do {
+          q = chunk_seq<kTile>(p, ++seq, err);
+        } while (q.tiles == 0);
+      }
+    }
     return true;
   }
 };
 
-// Merges the parts of split units: O = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i
-// - M).  A block takes kSmallRows rows of a unit, a warp a row at a time; rows
-// that saw no key are zeros.  Blocks of whole units leave at once.
+// Partial slot of a part of range g (-1: the whole unit).  A part that starts
+// its unit without ending it is the range's last; every other partial part is
+// the range's first.
+__device__ __forceinline__ int part_slot(const ChunkUnit& u, int kt0, int kt1, int g) {
+  return kt0 > 0 ? 2 * g : kt1 < u.steps ? 2 * g + 1 : -1;
+}
+
+// One thread of a CTA (pair) keeps its range's record.
+__device__ __forceinline__ void clear_record(ChunkRecord& r) { r.last_cut = r.first_state = 0; }
+__device__ __forceinline__ void note_part(ChunkRecord& r, const ChunkUnit& u, int kt0, int kt1) {
+  if (kt0 > 0) {
+    r.first_state = kt1 == u.steps ? 2 : 1;
+  } else if (kt1 < u.steps) {
+    r.last = u;
+    r.last_cut = 1;
+  }
+}
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Merges the parts of cut units: O = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i -
+// M); rows that saw no key are zeros.  Block (g, y) takes 8 / kW rows of the
+// unit that range g left unfinished, if any (kW warps a row, each every kW-th
+// part: few rows of many parts, as a long cache leaves them, or many of few).
+// Block (0, 0) also writes the call's status.
+template <int D, int kW>
+__device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRecord* rec, int grid, int unit_rows,
+                                             const float* part_o, const float* part_lse, int g, int y) {
+  constexpr int kPer = D / 32;
+  __shared__ float s_acc[8][D];
+  __shared__ float s_w[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (!rec[g].last_cut) return;
+  const ChunkUnit unit = rec[g].last;
+  const int r = y * (8 / kW) + warp / kW;
+  if (y * (8 / kW) >= unit.rows) return;
+  // Parts: slot 2 g + 1, then the first parts of the ranges behind it, up to
+  // the one that ends the unit.
+  int parts = 1;
+  for (int b = g + 1; b < grid; b += 32) {
+    const uint32_t ends = __ballot_sync(0xffffffffu, b + lane < grid && rec[b + lane].first_state == 2);
+    if (ends) {
+      parts += __ffs(ends);
+      break;
+    }
+    parts += 32;
+  }
+  const bool live = r < unit.rows;
+  float m = -INFINITY, acc[kPer], wsum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  if (live) {
+    auto row_of = [&](int i) { return static_cast<long long>(i == 0 ? 2 * g + 1 : 2 * (g + i)) * unit_rows + r; };
+    for (int b = 0; b < parts; b += 32) m = fmaxf(m, b + lane < parts ? part_lse[row_of(b + lane)] : -INFINITY);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int i = warp % kW; i < parts; i += kW) {
+      const long long row = row_of(i);
+      const float lse = part_lse[row];
+      // A part whose row saw nothing weighs nothing, whatever its O holds; a
+      // NaN (a NaN score somewhere) passes on.
+      const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - ref);
+      wsum += w;
+      const float* src = part_o + row * D + lane * kPer;
+#pragma unroll
+      for (int k = 0; k < kPer; k += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + k);
+        acc[k] = w == 0.f ? acc[k] : fmaf(w, v.x, acc[k]);
+        acc[k + 1] = w == 0.f ? acc[k + 1] : fmaf(w, v.y, acc[k + 1]);
+        acc[k + 2] = w == 0.f ? acc[k + 2] : fmaf(w, v.z, acc[k + 2]);
+        acc[k + 3] = w == 0.f ? acc[k + 3] : fmaf(w, v.w, acc[k + 3]);
+      }
+    }
+  }
+  if (kW > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s_acc[warp][lane * kPer + k] = acc[k];
+    if (lane == 0) s_w[warp] = wsum;
+    __syncthreads();
+    if (warp % kW) return;
+    for (int w = 1; w < kW; ++w) {
+      wsum += s_w[warp + w];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] += s_acc[warp + w][lane * kPer + k];
+    }
+  }
+  if (!live) return;
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
+  const int row = unit.row0 + r;
+  __nv_bfloat16* dst = p.out + static_cast<long long>(unit.head * p.group + row % p.group) * p.out_head +
+                       static_cast<long long>(unit.q0 + row / p.group) * p.out_row + lane * kPer;
+#pragma unroll
+  for (int k = 0; k < kPer; k += 4)
+    *reinterpret_cast<uint2*>(dst + k) =
+        make_uint2(pack_bf16x2(acc[k] * inv, acc[k + 1] * inv), pack_bf16x2(acc[k + 2] * inv, acc[k + 3] * inv));
+}
+
+constexpr int kCombineSmallY = kSmallRows / 2;  // 4 warps a row
+constexpr int kCombineTileY = kUnitRows / 8;    // a warp a row
+
 template <int D>
 __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
-  constexpr int kPer = D / 32;
-  constexpr int kParts = kUnitRows / kSmallRows;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const ChunkPlan plan = *p.work.plan;
-  const long long items = plan.small_units + static_cast<long long>(plan.tile_units) * kParts;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const bool small = it < plan.small_units;
-    const long long u = small ? it : (it - plan.small_units) / kParts;
-    const int r0 = small ? 0 : static_cast<int>((it - plan.small_units) % kParts) * kSmallRows;
-    const long long steps = small ? plan.small_steps : plan.tile_steps;
-    const long long ranges = chunk_ranges(steps, small ? p.small_ctas : p.tile_pairs);
-    const ChunkUnit unit = (small ? p.work.small : p.work.tile)[u];
-    const long long s0 = (small ? p.work.small_start : p.work.tile_start)[u];
-    const long long g0 = stream_k_pair_of(s0, steps, ranges);
-    const long long g1 = stream_k_pair_of(s0 + unit.steps - 1, steps, ranges);
-    if (g0 == g1) continue;
-    const int unit_rows = small ? kSmallRows : kUnitRows;
-    const float* part_o = small ? p.work.small_o : p.work.tile_o;
-    const float* part_lse = small ? p.work.small_lse : p.work.tile_lse;
-    for (int r = r0 + warp; r < min(r0 + kSmallRows, unit.rows); r += 8) {
-      // Lane i follows part i of each 32.
-      float m = -INFINITY, acc[kPer], wsum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-      for (long long gb = g0; gb <= g1; gb += 32) {
-        const long long g = gb + lane;
-        const long long slot = g == g0 ? 2 * g + 1 : 2 * g;
-        const float lse = g <= g1 ? part_lse[slot * unit_rows + r] : -INFINITY;
-        float mx = lse;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float nm = fmaxf(m, mx);
-        // A NaN lse (a NaN score somewhere) passes into its weight.
-        const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - (nm == -INFINITY ? 0.f : nm));
-        const float keep = m == -INFINITY ? 0.f : ex2_approx(m - nm);
-        m = nm;
-        wsum *= keep;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] *= keep;
-        const int n = static_cast<int>(min(32LL, g1 - gb + 1));
-        for (int i = 0; i < n; ++i) {
-          const float wi = __shfl_sync(0xffffffffu, w, i);
-          if (wi == 0.f) continue;  // a part whose rows saw nothing wrote no O
-          wsum += wi;
-          const long long gi = gb + i;
-          const long long si = gi == g0 ? 2 * gi + 1 : 2 * gi;
-          const float* src = part_o + (si * unit_rows + r) * D + lane * kPer;
-#pragma unroll
-          for (int k = 0; k < kPer; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src + k);
-            acc[k] = fmaf(wi, v.x, acc[k]);
-            acc[k + 1] = fmaf(wi, v.y, acc[k + 1]);
-            acc[k + 2] = fmaf(wi, v.z, acc[k + 2]);
-            acc[k + 3] = fmaf(wi, v.w, acc[k + 3]);
-          }
-        }
-      }
-      const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
-      const int row = unit.row0 + r;
-      __nv_bfloat16* dst = p.out + static_cast<long long>(unit.head * p.group + row % p.group) * p.out_head +
-                           static_cast<long long>(unit.q0 + row / p.group) * p.out_row + lane * kPer;
-#pragma unroll
-      for (int k = 0; k < kPer; k += 4)
-        *reinterpret_cast<uint2*>(dst + k) = make_uint2(pack_bf16x2(acc[k] * inv, acc[k + 1] * inv),
-                                                        pack_bf16x2(acc[k + 2] * inv, acc[k + 3] * inv));
+  grid_dependency_wait();
+  const int small_blocks = p.small_ctas * kCombineSmallY;
+  if (blockIdx.x == 0) {
+    int err = 0;
+    for (int i = threadIdx.x; i < p.small_ctas + 2 * p.tile_pairs; i += 256) {
+      const int e = i < p.small_ctas ? p.work.small_rec[i].err : p.work.tile_rec[i - p.small_ctas].err;
+      err = max(err, e);
     }
+    for (int o = 16; o > 0; o >>= 1) err = max(err, __shfl_xor_sync(0xffffffffu, err, o));
+    __shared__ int s_err[8];
+    if ((threadIdx.x & 31) == 0) s_err[threadIdx.x >> 5] = err;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) err = max(err, s_err[w]);
+      *p.status = err;
+    }
+  }
+  if (blockIdx.x < small_blocks) {
+    combine_rows<D, 4>(p, p.work.small_rec, p.small_ctas, kSmallRows, p.work.small_o, p.work.small_lse,
+                       blockIdx.x / kCombineSmallY, blockIdx.x % kCombineSmallY);
+  } else {
+    const int b = blockIdx.x - small_blocks;
+    combine_rows<D, 1>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse, b / kCombineTileY,
+                       b % kCombineTileY);
   }
 }
 

@@ -74,7 +74,8 @@ struct RowsSmem {
   static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;  // float m, l: [team][16]
   static constexpr int kBarOff = kMlOff + 2 * kTeams * 16 * 4;  // full, empty
   static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
-  static constexpr int kBytes = kMiscOff + 16;
+  static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
+  static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
   static_assert(kBufOff % 16 == 0 && kBarOff % 8 == 0 && kScaleOff % 128 == 0, "alignment");
   static_assert(2 * kWarps * 1024 <= kBufs * kBufBytes, "the score halves fit the buffers");
@@ -108,8 +109,12 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   constexpr int kBoxSteps = kBoxElts / 16;  // MMA k steps of a box: 8 or 4
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
+  ChunkRecord& rec = p.work.small_rec[blockIdx.x];
   if (sbase & 1023u) {
-    if (threadIdx.x == 0) atomicCAS(p.err, 0, kErrSmemAlign);
+    if (threadIdx.x == 0) {
+      clear_record(rec);
+      rec.err = kErrSmemAlign;
+    }
     return;
   }
   const uint32_t sQ = sbase + L::kQOff;
@@ -121,6 +126,8 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   auto bar_full = [&](int s) { return sbase + L::kBarOff + 8u * s; };
   auto bar_empty = [&](int s) { return sbase + L::kBarOff + 8u * (L::kStages + s); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff);
+  ChunkPlanShared& plan = *reinterpret_cast<ChunkPlanShared*>(smem + L::kPlanOff);
+  int* err = &plan.err;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -131,14 +138,16 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       mbar_init(bar_empty(s), L::kWarps);
     }
     *abort_flag = 0;
+    plan.err = 0;
     fence_mbar_init();
   }
+  grid_launch_dependents();  // the merge may wait on the SMs
   __syncthreads();
-  ChunkWalk walk;
-  walk.init(p.work.small, p.work.small_start, p.work.plan->small_units, p.work.plan->small_steps, p.small_ctas,
-            blockIdx.x);
+  chunk_plan<false>(p, plan, p.small_ctas, blockIdx.x);
+  ChunkWalk<false> walk;
+  walk.init(plan);
   ChunkUnit un;
-  int kt0, kt1, slot;
+  int kt0, kt1;
   uint32_t c = 0;  // stages of this CTA so far
   const int box_rows = 1 << box_shift;  // rows (keys) of a copy
   const uint32_t box_bytes = 256 * L::kBoxes * box_rows, scale_slot = max(128, 2 * box_rows);
@@ -148,7 +157,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     bool ok = true;
     const bool scaled = kFp8 && p.pool.scales;
     const int bs = p.pool.block_size;
-    while (ok && walk.next(un, kt0, kt1, slot)) {
+    while (ok && walk.next(p, err, un, kt0, kt1)) {
       const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
       const int* table = p.batch.tables + un.seq * p.batch.table_stride;
       int page = 0, row = 0;  // lane i: where copy i of the current 32 lies
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         const int st = c % L::kStages;
         const int boxes = (min(L::kStageKeys, k1 - key) + box_rows - 1) >> box_shift;
         if (lane == 0) {
-          ok = mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, p.err, kErrWaitKvEmpty);
+          ok = mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty);
           if (ok) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (scaled ? 2 * box_rows : 0)));
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
               page = table[at / bs];
               row = at % bs;
               if (page < 0 || page >= p.pool.blocks) {
-                atomicCAS(p.err, 0, kErrBlockTable);
+                atomicCAS(err, 0, kErrBlockTable);
                 page = 0;
               }
             }
@@ -197,7 +206,9 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   const int gq = lane >> 2, i4 = lane & 3;   // MMA row (and column) group, position in it
   const int part = warp % L::kTeam;          // this warp's 128 columns
   bool ok = true;
-  while (walk.next(un, kt0, kt1, slot)) {
+  if (threadIdx.x == 0) clear_record(rec);
+  while (walk.next(p, err, un, kt0, kt1)) {
+    if (threadIdx.x == 0) note_part(rec, un, kt0, kt1);
     const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
     const bool two = un.rows > 16;  // two row tiles
     // Q into fragment order: a warp a row, eight elements a lane.
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     int next = 16 * turn;  // this team's next keys, from the stage's first
     for (int key0 = k0; key0 < k1; key0 += L::kStageKeys, ++c) {
       const int st = c % L::kStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_full(st), (c / L::kStages) & 1u, abort_flag, p.err, kErrWaitKvFull));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_full(st), (c / L::kStages) & 1u, abort_flag, err, kErrWaitKvFull));
       // (The warps of a team of two go on together or not at all.)
       if (L::kTeam > 1) ok = named_bar_and(2 + team, 32 * L::kTeam, ok);
       if (!ok) break;
@@ -467,7 +478,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       s_l[team * 16 + gq] = l0;
       s_l[team * 16 + gq + 8] = l1;
     }
-    if (!named_bar_and(1, kConsumers, ok && *abort_flag == 0)) return;
+    if (!(ok = named_bar_and(1, kConsumers, ok && *abort_flag == 0))) break;
     float M0 = -INFINITY, M1 = -INFINITY;
     for (int w = qt * teams; w < (qt + 1) * teams; ++w) {
       M0 = fmaxf(M0, s_m[w * 16 + gq]);
@@ -524,6 +535,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       named_bar_sync(1, kConsumers);
     }
     // Every thread eight elements of a row: sum the buffers, divide, write.
+    const int slot = part_slot(un, kt0, kt1, blockIdx.x);
     for (int x = threadIdx.x; x < un.rows * (D / 8); x += kConsumers) {
       const int r = x / (D / 8), d = (x % (D / 8)) * 8;
       const int t = r / 16;
@@ -555,6 +567,11 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         if (d == 0) p.work.small_lse[at] = lsum == 0.f ? -INFINITY : M + __log2f(lsum);
       }
     }
+  }
+  if (threadIdx.x == 0) {
+    // After a failure nothing is merged: the partials may be unwritten.
+    if (!ok) clear_record(rec);
+    rec.err = *static_cast<volatile int*>(err);
   }
 }
 

@@ -65,7 +65,8 @@ struct TilesSmem {
   // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, red[2], scale[NB]
   static constexpr int kNumBars = 4 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kBytes = kMiscOff + 16;
+  static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
+  static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
   static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
 };
@@ -82,7 +83,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   if (sbase & 1023u) {  // identical in both CTAs: neither starts
-    if (threadIdx.x == 0) atomicCAS(p.err, 0, kErrSmemAlign);
+    if (threadIdx.x == 0) {
+      p.work.tile_rec[blockIdx.x].err = kErrSmemAlign;
+      clear_record(p.work.tile_rec[blockIdx.x >> 1]);
+    }
     return;
   }
   const uint32_t rank = cluster_ctarank();
@@ -112,6 +116,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   float* factors = reinterpret_cast<float*>(smem + L::kFactorOff);
 
+  ChunkPlanShared& plan = *reinterpret_cast<ChunkPlanShared*>(smem + L::kPlanOff);
+  int* err = &plan.err;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
@@ -135,6 +141,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     for (int b = 0; b < NB; ++b) mbar_init(bar_scale(b), kTilesConvWarps);
     mbar_init(bar_td, 1);
     *abort_flag = 0;
+    plan.err = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -146,16 +153,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int pair = blockIdx.x >> 1;
+  grid_launch_dependents();  // the merge may wait on the SMs
+  chunk_plan<true>(p, plan, p.tile_pairs, pair);
 
-  // Calls body(unit, kt0, kt1, slot) for each part of this pair's range until
+  // Calls body(unit, kt0, kt1) for each part of this pair's range until
   // it returns false; returns false if it did.
   auto for_each_segment = [&](auto&& body) -> bool {
-    ChunkWalk walk;
-    walk.init(p.work.tile, p.work.tile_start, p.work.plan->tile_units, p.work.plan->tile_steps, p.tile_pairs, pair);
+    ChunkWalk<true> walk;
+    walk.init(plan);
     ChunkUnit un;
-    int kt0, kt1, slot;
-    while (walk.next(un, kt0, kt1, slot))
-      if (!body(un, kt0, kt1, slot)) return false;
+    int kt0, kt1;
+    while (walk.next(p, err, un, kt0, kt1))
+      if (!body(un, kt0, kt1)) return false;
     return true;
   };
   // Keys of tile kt that the sequence has (may be 0 when it has none at all).
@@ -172,7 +181,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         if (un.seq == seq && lb == cached_lb) return cached_page;
         int b = lb < p.batch.table_width ? p.batch.tables[un.seq * p.batch.table_stride + lb] : -1;
         if (b < 0 || b >= p.pool.blocks) {  // reported; block 0 keeps the load in bounds
-          atomicCAS(p.err, 0, kErrBlockTable);
+          atomicCAS(err, 0, kErrBlockTable);
           b = 0;
         }
         seq = un.seq;
@@ -202,7 +211,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       auto issue = [&](const ChunkUnit& un, bool is_v, int kt) {
         const int st = c % NL;
         const uint32_t empty = kFp8 ? bar_land_empty(st) : bar_op_empty(st);
-        if (!mbar_wait(empty, ((c / NL) & 1u) ^ 1u, abort_flag, p.err, kErrWaitKvEmpty)) return false;
+        if (!mbar_wait(empty, ((c / NL) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty)) return false;
         const uint32_t dst = kFp8 ? sRaw + st * L::kRawBytes : sOp + st * L::kOpBytes;
         const int off = is_v ? 0 : 64 * static_cast<int>(rank), most = is_v ? 128 : 64;
         const int n = min(most, max(0, tile_valid(un, kt) - off));
@@ -214,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       };
       // Item order = converter and MMA consumption order: per segment K_0,
       // then (K_{j+1}, V_j) per tile.
-      const bool ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int) -> bool {
+      const bool ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
         if (!issue(un, false, kt0)) return false;
         for (int kt = kt0; kt < kt1; ++kt) {
           if (kt + 1 < kt1 && !issue(un, false, kt + 1)) return false;
@@ -236,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     uint32_t c = 0, J = 0;
     int segs = 0;
     auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err, code));
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
     };
     auto item = [&](const ChunkUnit& un, bool is_v, int kt) -> bool {
       const int ls = c % NL, os = c % NS;
@@ -314,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       ++c;
       return true;
     };
-    for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int) -> bool {
+    for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
       // Q rows into the swizzled operand layout, once the previous segment's
       // QK^T are done with it: a row over D / 8 lanes, four rows in flight.
       if (segs > 0 && !wait_all(bar_q_empty, (segs - 1) & 1u, kErrWaitQ)) return false;
@@ -384,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       auto qk = [&](uint32_t jg) {
         const uint32_t s_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
         const int st = c % NS;
-        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, p.err, kErrWaitKvFull)) return false;
+        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, err, kErrWaitKvFull)) return false;
         tc_fence_after();
         const uint32_t kbase = sOp + st * L::kOpBytes;
 #pragma unroll
@@ -400,9 +409,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         return true;
       };
       auto pv = [&](uint32_t jg, bool first) {
-        if (!mbar_wait(bar_p_full(jg & 1), (jg >> 1) & 1u, abort_flag, p.err, kErrWaitPFull)) return false;
+        if (!mbar_wait(bar_p_full(jg & 1), (jg >> 1) & 1u, abort_flag, err, kErrWaitPFull)) return false;
         const int st = c % NS;
-        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, p.err, kErrWaitKvFull)) return false;
+        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, err, kErrWaitKvFull)) return false;
         tc_fence_after();
         const uint32_t p_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
         const uint32_t vbase = sOp + st * L::kOpBytes;
@@ -420,11 +429,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         umma_commit_pair(bar_o(jg & 1), kChunkBothCtas);
         return true;
       };
-      for_each_segment([&](const ChunkUnit&, int kt0, int kt1, int) -> bool {
+      for_each_segment([&](const ChunkUnit&, int kt0, int kt1) -> bool {
         const uint32_t n = static_cast<uint32_t>(kt1 - kt0);
         // (O of the previous segment has been read out: its softmax warps
         // release P_0 of this segment only after their epilogue.)
-        if (!mbar_wait(bar_q_ready, segs & 1u, abort_flag, p.err, kErrWaitQ)) return false;
+        if (!mbar_wait(bar_q_ready, segs & 1u, abort_flag, err, kErrWaitQ)) return false;
         tc_fence_after();
         if (!qk(J)) return false;
         if (n == 1) umma_commit_pair(bar_q_empty, kChunkBothCtas);
@@ -453,7 +462,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     uint32_t J = 0;
     int segs = 0;
-    for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int slot) -> bool {
+    // The leader keeps the pair's record.
+    ChunkRecord& rec = p.work.tile_rec[pair];
+    const bool keeps = leader && threadIdx.x == 0;
+    if (keeps) clear_record(rec);
+    const bool done = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
+      if (keeps) note_part(rec, un, kt0, kt1);
       bool ok = true;
       const int r = static_cast<int>(rank) * kTileM + row;  // row of the unit
       const bool live = r < un.rows;
@@ -462,7 +476,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int n = kt1 - kt0;
       float rf = p.scale_log2;
       if (kFp8) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(segs), (segs >> 1) & 1u, abort_flag, p.err, kErrWaitQ));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(segs), (segs >> 1) & 1u, abort_flag, err, kErrWaitQ));
         if (ok) rf = factors[(segs & 1) * kTileM + row];
       }
       ++segs;
@@ -476,12 +490,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         float ev = 0.f;
         if (kScaled) {
           ok = __all_sync(0xffffffffu, mbar_wait(bar_scale(jg % (NB ? NB : 1)), (jg / (NB ? NB : 1)) & 1u, abort_flag,
-                                                 p.err, kErrWaitKvFull));
+                                                 err, kErrWaitKvFull));
           if (!ok) break;
           const int4 vm = *reinterpret_cast<const int4*>(sf + 2 * kTileN);
           ev = static_cast<float>(max(max(vm.x, vm.y), max(vm.z, vm.w)) - 127);
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(b), (jg >> 1) & 1u, abort_flag, p.err, kErrWaitSFull));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitSFull));
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_s = t_row + kTmemS0 + b * kTileN + wg * kHalfKeys;
@@ -519,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 #pragma unroll 1
         for (int pass = j > 0 ? 0 : 1; pass < 2; ++pass) {
           if (pass == 1) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar_red(b), (jg >> 1) & 1u, abort_flag, p.err, kErrWaitRed));
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_red(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
             if (!ok) break;
             const float tmax =
                 fmaxf(pmax, red[(b * kSoftmaxWarpgroups + (wg ^ 1)) * kTileM + row]) * rf + ev;
@@ -566,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         l += tile_sum;
         if (j > 0 && redo) {
           ok = __all_sync(0xffffffffu,
-                          mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, p.err, kErrWaitODone));
+                          mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
           if (!ok) break;
           tc_fence_after();
           rescale_o<kOCols>(t_row + wg * kOCols, alpha);
@@ -577,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       }
       if (ok) {
         const uint32_t jl = J + n - 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, p.err, kErrWaitODone));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
       }
       ok = named_bar_and(1, kSoftmaxThreads, ok && (*abort_flag == 0));
       if (!ok) return false;
@@ -589,6 +603,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       // Both halves read: the next segment may reuse the exchange slots.
       named_bar_sync(2, kSoftmaxThreads);
       const float inv_l = l_tot == 0.f ? 0.f : 1.f / l_tot;  // no key seen: zeros
+      const int slot = part_slot(un, kt0, kt1, pair);
       if (slot < 0) {
         store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l,
                              p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
@@ -597,10 +612,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       } else {
         const long long pr = static_cast<long long>(slot) * kUnitRows + r;
         store_o_partial<kOCols>(t_row + wg * kOCols, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
-        if (live && wg == 0) p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (m_ref == -INFINITY ? 0.f : m_ref) + __log2f(l_tot);
+        if (live && wg == 0)
+          p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (m_ref == -INFINITY ? 0.f : m_ref) + __log2f(l_tot);
       }
       return true;
     });
+    if (keeps && !done) clear_record(rec);  // after a failure nothing is merged
   }
 
   // Both CTAs: the leader's MMAs (which read the peer's smem and TMEM) are
@@ -608,6 +625,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
+  if (threadIdx.x == 0) p.work.tile_rec[blockIdx.x].err = *static_cast<volatile int*>(err);
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, kTmemCols);

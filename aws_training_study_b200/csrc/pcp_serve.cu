@@ -118,31 +118,22 @@ constexpr int kPairs = kCtas / 2;
 size_t align_up(size_t a) { return (a + 255) / 256 * 256; }
 
 struct ChunkLayout {
-  size_t plan, small, small_start, tile, tile_start, seq_tile, tile_prefix, small_o, small_lse, tile_o, tile_lse, bytes;
+  size_t small_rec, tile_rec, small_o, small_lse, tile_o, tile_lse, bytes;
 };
 
 bool has_tiles(int32_t max_chunk, int32_t group) { return static_cast<int64_t>(max_chunk) * group > pcp::kSmallRows; }
 
-ChunkLayout chunk_layout(int32_t head_dim, int32_t kv_heads, int32_t group, int32_t seqs, int32_t rows, int32_t max_chunk) {
+ChunkLayout chunk_layout(int32_t head_dim, int32_t group, int32_t max_chunk) {
   ChunkLayout w{};
-  const int64_t with_rows = std::min(seqs, rows);
-  const int64_t small = with_rows * kv_heads;
   const bool tiles = has_tiles(max_chunk, group);
-  // Query tiles of a head: whole ones of all rows, and one rest a sequence.
-  const int64_t q_tiles = tiles ? static_cast<int64_t>(rows) * group / pcp::kUnitRows + with_rows : 0;
   size_t at = 0;
   auto put = [&](size_t bytes) {
     const size_t here = at;
     at = align_up(at + bytes);
     return here;
   };
-  w.plan = put(sizeof(pcp::ChunkPlan));
-  w.small = put(small * sizeof(pcp::ChunkUnit));
-  w.small_start = put((small + 1) * 8);
-  w.tile = put(q_tiles * kv_heads * sizeof(pcp::ChunkUnit));
-  w.tile_start = put((q_tiles * kv_heads + 1) * 8);
-  w.seq_tile = put((static_cast<size_t>(seqs) + 1) * 4);
-  w.tile_prefix = put((q_tiles + 1) * 8);
+  w.small_rec = put(kCtas * sizeof(pcp::ChunkRecord));
+  w.tile_rec = put(tiles ? 2 * kPairs * sizeof(pcp::ChunkRecord) : 0);
   w.small_o = put(size_t(2) * kCtas * pcp::kSmallRows * head_dim * 4);
   w.small_lse = put(size_t(2) * kCtas * pcp::kSmallRows * 4);
   w.tile_o = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * head_dim * 4 : 0);
@@ -272,19 +263,27 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
 }
 
 template <int D>
-int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, bool tiles, cudaStream_t st) {
-  pcp::chunk_plan_kernel<<<1, 1024, 0, st>>>(p);
-  CUDA_TRY(cudaGetLastError());
+int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
   const bool bf16 = pool.kv_dtype == PCP_KV_BF16;
   if (bf16) PCP_TRY((launch_rows<D, false>(pool, p, st)));
   else PCP_TRY((launch_rows<D, true>(pool, p, st)));
-  if (tiles) {
+  if (p.tile_pairs) {
     if (bf16) PCP_TRY((launch_tiles<D, pcp::kCacheBf16>(pool, p, st)));
     else if (pool.scales) PCP_TRY((launch_tiles<D, pcp::kCacheScaled>(pool, p, st)));
     else PCP_TRY((launch_tiles<D, pcp::kCacheE4m3>(pool, p, st)));
   }
-  pcp::chunk_combine_kernel<D><<<4 * kCtas, 256, 0, st>>>(p);
-  CUDA_TRY(cudaGetLastError());
+  // The merge's blocks may be placed while the kernel before it ends (it waits
+  // for that kernel itself).
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(p.small_ctas * pcp::kCombineSmallY + p.tile_pairs * pcp::kCombineTileY);
+  config.blockDim = dim3(256);
+  config.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  CUDA_TRY(cudaLaunchKernelEx(&config, pcp::chunk_combine_kernel<D>, p));
   return PCP_OK;
 }
 
@@ -360,7 +359,7 @@ int pcp_chunk_attention_workspace_size(const pcp_pool_t* pool, int32_t num_q_hea
                                        int32_t max_chunk, size_t* bytes) {
   PCP_TRY(check_chunk(pool, num_q_heads, num_seqs, rows, max_chunk));
   if (!bytes) return fail(PCP_ERR_INVALID_ARGUMENT, "bytes is NULL");
-  *bytes = chunk_layout(pool->head_dim, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, num_seqs, rows, max_chunk).bytes;
+  *bytes = chunk_layout(pool->head_dim, num_q_heads / pool->num_kv_heads, max_chunk).bytes;
   return PCP_OK;
 }
 
@@ -381,7 +380,7 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
     return PCP_OK;
   }
   const int32_t group = q->heads / pool->num_kv_heads;
-  const ChunkLayout w = chunk_layout(pool->head_dim, pool->num_kv_heads, group, batch->num_seqs, batch->rows, max_chunk);
+  const ChunkLayout w = chunk_layout(pool->head_dim, group, max_chunk);
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < w.bytes)
     return fail(PCP_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, aligned to 256, is needed (got %zu)", w.bytes,
                 workspace_bytes);
@@ -389,13 +388,8 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   pcp::ChunkParams p{};
   p.batch = batch_view(*batch);
   p.pool = pool_view(*pool);
-  p.work.plan = reinterpret_cast<pcp::ChunkPlan*>(ws + w.plan);
-  p.work.small = reinterpret_cast<pcp::ChunkUnit*>(ws + w.small);
-  p.work.small_start = reinterpret_cast<long long*>(ws + w.small_start);
-  p.work.tile = reinterpret_cast<pcp::ChunkUnit*>(ws + w.tile);
-  p.work.tile_start = reinterpret_cast<long long*>(ws + w.tile_start);
-  p.work.seq_tile = reinterpret_cast<int*>(ws + w.seq_tile);
-  p.work.tile_prefix = reinterpret_cast<long long*>(ws + w.tile_prefix);
+  p.work.small_rec = reinterpret_cast<pcp::ChunkRecord*>(ws + w.small_rec);
+  p.work.tile_rec = reinterpret_cast<pcp::ChunkRecord*>(ws + w.tile_rec);
   p.work.small_o = reinterpret_cast<float*>(ws + w.small_o);
   p.work.small_lse = reinterpret_cast<float*>(ws + w.small_lse);
   p.work.tile_o = reinterpret_cast<float*>(ws + w.tile_o);
@@ -410,10 +404,9 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.max_chunk = max_chunk;
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
   p.small_ctas = kCtas;
-  p.tile_pairs = kPairs;
-  p.err = device_status;
-  const bool tiles = has_tiles(max_chunk, group);
-  return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, tiles, st) : launch_chunk<128>(*pool, p, tiles, st);
+  p.tile_pairs = has_tiles(max_chunk, group) ? kPairs : 0;
+  p.status = device_status;
+  return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, st) : launch_chunk<128>(*pool, p, st);
 }
 
 }  // extern "C"
