@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int w = 1; w < 8; ++w) err = max(err, s_err[w]);
-      *p.status = err;
+      if (err) atomicCAS(p.status, 0, err);
     }
   }
   if (blockIdx.x < small_blocks) {

@@ -80,7 +80,6 @@ int cache_rows(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads
   PCP_TRY(check_heads(v, pool->num_kv_heads, batch->rows, 2, "v"));
   if (!device_status) return fail(PCP_ERR_INVALID_ARGUMENT, "device_status is NULL");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CUDA_TRY(cudaMemsetAsync(device_status, 0, sizeof(int32_t), st));
   if (batch->num_seqs == 0 || batch->rows == 0) return PCP_OK;
   pcp::CacheRowsParams p{};
   p.pool = pool_view(*pool);
@@ -375,10 +374,7 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   if (!(softmax_scale > 0) || std::isinf(softmax_scale))
     return fail(PCP_ERR_INVALID_ARGUMENT, "softmax_scale %g must be positive and finite", softmax_scale);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (batch->num_seqs == 0 || batch->rows == 0) {
-    CUDA_TRY(cudaMemsetAsync(device_status, 0, sizeof(int32_t), st));
-    return PCP_OK;
-  }
+  if (batch->num_seqs == 0 || batch->rows == 0) return PCP_OK;
   const int32_t group = q->heads / pool->num_kv_heads;
   const ChunkLayout w = chunk_layout(pool->head_dim, group, max_chunk);
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < w.bytes)

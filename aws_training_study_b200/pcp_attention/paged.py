@@ -34,7 +34,7 @@ import torch
 from .. import _capi
 from .config import PCPAttentionConfig
 from .cuda_backend import _cuda_stream_ptr, _kv_code, make_dims, payload_elements
-from .rotary import _check_rows, _check_writable, _heads
+from .rotary import _check_rows, _check_writable, _heads, _launch
 
 
 def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -163,7 +163,7 @@ def _pool_struct(config: PCPAttentionConfig, pool: torch.Tensor, scales: torch.T
         shape = (pool.shape[0], 2 * config.num_kv_heads * config.block_size)
         if code != _capi.PCP_KV_E4M3:
             raise ValueError("scales need an e4m3 pool")
-        if tuple(scales.shape) != shape or scales.dtype != torch.uint8 or scales.device != pool.device or \
+        if scales.shape != shape or scales.dtype != torch.uint8 or scales.device != pool.device or \
                 not scales.is_contiguous() or scales.data_ptr() % 16:
             raise ValueError(f"scales must be a contiguous, 16-byte aligned uint8 {shape} tensor on {pool.device}")
     return _capi.PcpPool(pool.data_ptr(), 0 if scales is None else scales.data_ptr(), pool.shape[0],
@@ -173,35 +173,35 @@ def _pool_struct(config: PCPAttentionConfig, pool: torch.Tensor, scales: torch.T
 def _batch_struct(offsets: torch.Tensor, kv_len: torch.Tensor, block_tables: torch.Tensor, rows: int,
                   device: torch.device) -> _capi.PcpBatch:
     for name, t, dims in (("offsets", offsets, 1), ("kv_len", kv_len, 1), ("block_tables", block_tables, 2)):
-        if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.numel() and t.stride(-1) != 1):
+        if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.stride(-1) != 1 and t.numel()):
             raise ValueError(f"{name} must be an int32 tensor of {dims} dimensions with contiguous rows on {device}")
-    seqs = kv_len.shape[0]
-    if offsets.shape[0] != seqs + 1 or block_tables.shape[0] != seqs:
+    seqs, (tables, width) = kv_len.shape[0], block_tables.shape
+    if offsets.shape[0] != seqs + 1 or tables != seqs:
         raise ValueError(f"{seqs} sequences need {seqs + 1} offsets and {seqs} block tables, got {offsets.shape[0]} "
-                         f"and {block_tables.shape[0]}")
+                         f"and {tables}")
     return _capi.PcpBatch(offsets.data_ptr(), kv_len.data_ptr(), block_tables.data_ptr(),
-                          block_tables.stride(0) if seqs > 1 else 0, block_tables.shape[1], seqs, rows, 0)
+                          block_tables.stride(0) if seqs > 1 else 0, width, seqs, rows, 0)
 
 
 class _Status:
     """The device status word of a call: the caller's (the call stays
-    asynchronous), or an own one that is read after the call, which then
-    raises what the kernels reported."""
+    asynchronous, and a word that is not 0 is kept), or an own one that is read
+    after the call, which then raises what the kernels reported."""
 
     def __init__(self, status: torch.Tensor | None, device: torch.device, stream: torch.cuda.Stream | None):
         self.own = status is None
         if self.own:
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError("a captured call needs a status tensor: its result cannot be read while recording")
-            status = torch.empty(1, dtype=torch.int32, device=device)
+            with torch.cuda.stream(stream):
+                status = torch.zeros(1, dtype=torch.int32, device=device)
         elif status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
             raise ValueError(f"status must be an int32 tensor of one element on {device}")
-        self.word, self.stream = status, stream
-        self.ptr = ctypes.c_void_p(status.data_ptr())
+        self.word, self.ptr = status, status.data_ptr()
 
-    def finish(self) -> None:
+    def finish(self, stream: torch.cuda.Stream | None) -> None:
         if self.own:
-            _capi.check(_capi.lib().pcp_history_attention_status(self.ptr, _cuda_stream_ptr(self.stream)))
+            _launch(self.word.device, stream, _capi.lib().pcp_history_attention_status, self.ptr)
 
 
 def cache_append(config: PCPAttentionConfig, k_src: torch.Tensor, v_src: torch.Tensor, offsets: torch.Tensor,
@@ -215,21 +215,18 @@ def cache_append(config: PCPAttentionConfig, k_src: torch.Tensor, v_src: torch.T
     ``[B, width]``.  A bf16 pool takes copies, an e4m3 pool codes at unit scale
     or, with ``scales``, codes and a scale byte for each token and head.  Rows
     of no sequence are ignored.  With ``status`` (device int32, one element)
-    the call is asynchronous and leaves 0, 109 (a page outside the pool or the
-    table; its tokens are skipped) or 112 (a position below 0) there; without,
-    it waits and raises."""
+    the call is asynchronous and stores 109 (a page outside the pool or the
+    table; its tokens are skipped) or 112 (a position below 0) there unless an
+    earlier call's code still stands (the caller clears it); without, it waits
+    and raises."""
     ps = _pool_struct(config, pool, scales)
     rows = k_src.shape[1] if k_src.dim() == 3 else -1
     for name, t in (("k_src", k_src), ("v_src", v_src)):
         _check_rows(name, t, (config.num_kv_heads, rows, config.head_dim), torch.bfloat16, pool.device)
     batch = _batch_struct(offsets, kv_len, block_tables, rows, pool.device)
-    with torch.cuda.device(pool.device):
-        st = _Status(status, pool.device, stream)
-        _capi.check(
-            _capi.lib().pcp_cache_append(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(k_src)),
-                                         ctypes.byref(_heads(v_src)), st.ptr, _cuda_stream_ptr(stream))
-        )
-        st.finish()
+    st = _Status(status, pool.device, stream)
+    _launch(pool.device, stream, _capi.lib().pcp_cache_append, ps, batch, _heads(k_src), _heads(v_src), st.ptr)
+    st.finish(stream)
 
 
 def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.Tensor, block_tables: torch.Tensor,
@@ -258,13 +255,9 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
             _check_writable(name, t)
         outs.append(t)
     batch = _batch_struct(offsets, kv_len, block_tables, int(rows), pool.device)
-    with torch.cuda.device(pool.device):
-        st = _Status(status, pool.device, stream)
-        _capi.check(
-            _capi.lib().pcp_cache_read(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(outs[0])),
-                                       ctypes.byref(_heads(outs[1])), st.ptr, _cuda_stream_ptr(stream))
-        )
-        st.finish()
+    st = _Status(status, pool.device, stream)
+    _launch(pool.device, stream, _capi.lib().pcp_cache_read, ps, batch, _heads(outs[0]), _heads(outs[1]), st.ptr)
+    st.finish(stream)
     return outs[0], outs[1]
 
 
@@ -298,17 +291,13 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     scale = config.softmax_scale if softmax_scale is None else float(softmax_scale)
     lib = _capi.lib()
     nbytes = ctypes.c_size_t()
-    _capi.check(lib.pcp_chunk_attention_workspace_size(ctypes.byref(ps), config.num_q_heads, batch.num_seqs, rows,
-                                                       max_chunk, ctypes.byref(nbytes)))
+    _capi.check(lib.pcp_chunk_attention_workspace_size(ps, config.num_q_heads, batch.num_seqs, rows, max_chunk,
+                                                       ctypes.byref(nbytes)))
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=pool.device)
-    with torch.cuda.device(pool.device):
-        st = _Status(status, pool.device, stream)
-        _capi.check(
-            lib.pcp_chunk_attention(ctypes.byref(ps), ctypes.byref(batch), ctypes.byref(_heads(q)),
-                                    ctypes.byref(_heads(out)), max_chunk, scale, ctypes.c_void_p(ws.data_ptr()),
-                                    nbytes.value, st.ptr, _cuda_stream_ptr(stream))
-        )
-        if stream is not None:
-            ws.record_stream(stream)
-        st.finish()
+    st = _Status(status, pool.device, stream)
+    _launch(pool.device, stream, lib.pcp_chunk_attention, ps, batch, _heads(q), _heads(out), max_chunk, scale,
+            ws.data_ptr(), nbytes.value, st.ptr)
+    if stream is not None:
+        ws.record_stream(stream)
+    st.finish(stream)
     return out

@@ -17,13 +17,11 @@ cos/sin table, and positions of any size are as exact as small ones.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from .. import _capi
-from .cuda_backend import _cuda_stream_ptr
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # enum pcp_float_dtype
 _LAYOUTS = {"half": 0, "interleaved": 1}                           # enum pcp_rotary_layout
@@ -117,31 +115,46 @@ class Rotary:
 def _heads(t: torch.Tensor | None) -> _capi.PcpHeads:
     if t is None:
         return _capi.PcpHeads(0, 0, 0, 0, 0)
-    strides = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(2)]  # an axis of one has no step to check
-    return _capi.PcpHeads(t.data_ptr(), strides[0], strides[1], t.shape[0], 0)
+    heads, rows, _ = t.shape
+    head, row, _ = t.stride()
+    # an axis of one has no step to check
+    return _capi.PcpHeads(t.data_ptr(), head if heads > 1 else 0, row if rows > 1 else 0, heads, 0)
 
 
 def _check_rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
     """A packed tensor ``[heads, rows, head_dim]`` whose rows are contiguous
     and 16-byte aligned; the heads and rows may lie at any stride."""
-    if tuple(t.shape) != shape or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"expected {name} {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+    head, row, one = t.stride()
     unit = 16 // t.element_size()
-    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % unit)
-                      or (t.shape[1] > 1 and t.stride(1) % unit)):
+    if t.numel() and (one != 1 or t.data_ptr() % 16 or (head % unit and shape[0] > 1) or (row % unit and shape[1] > 1)):
         raise ValueError(f"{name} needs contiguous, 16-byte aligned rows, got strides {t.stride()}")
 
 
 def _check_writable(name: str, t: torch.Tensor) -> None:
     """An output's rows may not lie on one another."""
-    live = sorted((abs(t.stride(i)), t.shape[i]) for i in range(2) if t.shape[i] > 1)
-    reach = t.shape[2]
-    for stride, n in live:
-        if stride < reach:
-            raise ValueError(f"{name} overlaps itself: strides {t.stride()}")
-        reach = stride * (n - 1) + reach
+    heads, rows, reach = t.shape
+    head, row, _ = t.stride()
+    for stride, n in ((head, heads), (row, rows)) if head < row else ((row, rows), (head, heads)):
+        if n > 1:
+            if stride < reach:
+                raise ValueError(f"{name} overlaps itself: strides {t.stride()}")
+            reach += stride * (n - 1)
+
+
+def _launch(device: torch.device, stream: torch.cuda.Stream | None, entry, *args) -> None:
+    """``entry(*args, stream)`` on ``device`` and ``stream`` (default: the
+    current one of the device); raises its error.  The device and stream are
+    read without torch.cuda's wrappers, which cost a small call more host time
+    than everything else in it."""
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _launch(device, stream, entry, *args)
+    _capi.check(entry(*args, stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary,
@@ -182,15 +195,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             _check_rows(name, o, tuple(x.shape), q.dtype, dev)
             _check_writable(name, o)
         outs.append(o)
-    with torch.cuda.device(dev):
-        _capi.check(
-            _capi.lib().pcp_qk_norm_rope(
-                _DTYPES[q.dtype], rows, D, rotary.rotary_dim, _LAYOUTS[rotary.layout], ctypes.byref(_heads(q)),
-                ctypes.byref(_heads(k)), ctypes.byref(_heads(outs[0])), ctypes.byref(_heads(outs[1])),
-                ctypes.c_void_p(positions.data_ptr()), int(positions.dtype == torch.int64),
-                ctypes.c_void_p(rotary.turns(dev).data_ptr()), rotary.magnitude,
-                ctypes.c_void_p(q_weight.data_ptr() if q_weight is not None else 0),
-                ctypes.c_void_p(k_weight.data_ptr() if k_weight is not None else 0), eps, _cuda_stream_ptr(stream)
-            )
-        )
+    _launch(dev, stream, _capi.lib().pcp_qk_norm_rope, _DTYPES[q.dtype], rows, D, rotary.rotary_dim,
+            _LAYOUTS[rotary.layout], _heads(q), _heads(k), _heads(outs[0]), _heads(outs[1]), positions.data_ptr(),
+            int(positions.dtype == torch.int64), rotary.turns(dev).data_ptr(), rotary.magnitude,
+            0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps)
     return outs[0], outs[1]

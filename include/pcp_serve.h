@@ -19,7 +19,8 @@
  * never written.  Position p lives in row p % block_size of pool block
  * block_tables[b][p / block_size].
  *
- * Device status word (DEVICE int32, zeroed by the call):
+ * Device status word (DEVICE int32; a call stores its code only over 0, so the
+ * first failure since the caller last cleared the word stands):
  *   109  a table entry outside the pool, or a position past the table's width
  *        (append skips the token, read-back writes zeros; attention reads
  *        block 0 in the entry's place and stops at the table's end: rows of
