@@ -46,10 +46,11 @@ namespace pcp {
 template <int D, bool kFp8>
 struct RowsSmem {
   static constexpr int kElt = kFp8 ? 1 : 2;
-  // Consumer warps: with the producer 13 at up to 128 registers, or (bf16, which
-  // converts nothing) 9 at up to 168.
+  // Consumer warps.  bf16, which converts nothing: 8, and the producer, at up to
+  // 168 registers.  e4m3: 12, and a warpgroup of its own for the producer, which
+  // gives registers up: 384 x 152 + 128 x 56 = 512 x 128 (at 128 they spill).
   static constexpr int kWarps = kFp8 ? 12 : 8;
-  static constexpr int kThreads = 32 * kWarps + 32;
+  static constexpr int kThreads = kFp8 ? 512 : 32 * kWarps + 32;
   static constexpr int kTeam = D / 128;          // warps of a team
   static constexpr int kTeams = kWarps / kTeam;
   static constexpr int kBoxes = D * kElt / 128;             // 128-byte columns of a row
@@ -80,6 +81,9 @@ struct RowsSmem {
   static_assert(kBufOff % 16 == 0 && kBarOff % 8 == 0 && kScaleOff % 128 == 0, "alignment");
   static_assert(2 * kWarps * 1024 <= kBufs * kBufBytes, "the score halves fit the buffers");
 };
+
+constexpr int kRowsLaunchRegs = 128, kRowsConsumerRegs = 152, kRowsProducerRegs = 56;
+static_assert(384 * kRowsConsumerRegs + 128 * kRowsProducerRegs <= 512 * kRowsLaunchRegs, "more than the launch's registers");
 
 template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -152,8 +156,10 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   const int box_rows = 1 << box_shift;  // rows (keys) of a copy
   const uint32_t box_bytes = 256 * L::kBoxes * box_rows, scale_slot = max(128, 2 * box_rows);
 
-  if (warp == L::kWarps) {
+  if (warp >= L::kWarps) {
     // -------------------------------------------------------- producer --
+    if (kFp8) setmaxnreg_dec<kRowsProducerRegs>();
+    if (warp > L::kWarps) return;
     bool ok = true;
     const bool scaled = kFp8 && p.pool.scales;
     const int bs = p.pool.block_size;
@@ -201,6 +207,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   }
 
   // ------------------------------------------------------------ consumers --
+  if (kFp8) setmaxnreg_inc<kRowsConsumerRegs>();
   constexpr int kConsumers = 32 * L::kWarps;
   constexpr int kWarpBoxes = L::kElt;        // 128-byte boxes of a warp's 128 columns
   const int gq = lane >> 2, i4 = lane & 3;   // MMA row (and column) group, position in it

@@ -218,14 +218,21 @@ int make_scale_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows) {
 }
 
 // A kernel's dynamic shared memory is allowed once per device.
+// Its compiled register count is checked there too where the kernel's register
+// split (setmaxnreg) assumes one: with another the split would wait forever.
 template <auto kKernel>
-int allow_smem(int bytes) {
+int allow_smem(int bytes, int regs = 0) {
   static std::mutex mutex;
   static bool done[64] = {};
   int device = 0;
   CUDA_TRY(cudaGetDevice(&device));
   std::lock_guard<std::mutex> lock(mutex);
   if (device < 64 && done[device]) return PCP_OK;
+  if (regs) {
+    cudaFuncAttributes a{};
+    CUDA_TRY(cudaFuncGetAttributes(&a, kKernel));
+    if (a.numRegs != regs) return fail(PCP_ERR_UNSUPPORTED, "kernel compiled to %d registers, %d assumed", a.numRegs, regs);
+  }
   CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   if (device < 64) done[device] = true;
   return PCP_OK;
@@ -240,7 +247,7 @@ int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t 
   CUtensorMap tm, ts{};
   PCP_TRY(make_rows_map(&tm, pool, 1 << shift));
   if (pool.scales) PCP_TRY(make_scale_map(&ts, pool, 1 << shift));
-  PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes)));
+  PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes, kFp8 ? pcp::kRowsLaunchRegs : 0)));
   pcp::chunk_rows_kernel<D, kFp8><<<kCtas, L::kThreads, L::kBytes, st>>>(tm, ts, shift, p);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
