@@ -40,7 +40,8 @@ int check_pool(const pcp_pool_t* p) {
   if (!p) return fail(PCP_ERR_INVALID_ARGUMENT, "pool is NULL");
   if (p->head_dim != 128 && p->head_dim != 256)
     return fail(PCP_ERR_UNSUPPORTED, "head_dim %d unsupported by the paged cache (128 or 256)", p->head_dim);
-  if (p->num_kv_heads <= 0) return fail(PCP_ERR_INVALID_ARGUMENT, "num_kv_heads must be positive");
+  if (p->num_kv_heads <= 0 || p->num_kv_heads > 1024)
+    return fail(PCP_ERR_UNSUPPORTED, "num_kv_heads %d must be positive and at most 1024", p->num_kv_heads);
   if (p->block_size <= 0 || p->block_size % 16)
     return fail(PCP_ERR_UNSUPPORTED, "block_size %d must be a multiple of 16", p->block_size);
   if (p->kv_dtype != PCP_KV_E4M3 && p->kv_dtype != PCP_KV_BF16)
@@ -96,6 +97,8 @@ int cache_rows(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads
   int tpw = 32;
   while (tpw > 1 && ceil_div(batch->rows, tpw) < 148 * 16) tpw /= 2;
   p.tokens_per_warp = tpw;
+  const uint64_t per_token = 2 * static_cast<uint64_t>(pool->num_kv_heads);
+  p.inv_per_token = static_cast<unsigned>(((uint64_t(1) << 32) + per_token - 1) / per_token);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(ceil_div(batch->rows, tpw), 8), 148 * 8));
   if (append) {
     if (pool->head_dim == 256) pcp::cache_append_kernel<256><<<grid, 256, 0, st>>>(p);

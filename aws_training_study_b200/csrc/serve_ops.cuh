@@ -264,84 +264,103 @@ struct CacheRowsParams {
   const void* k;  // append: source rows; read: destination rows
   const void* v;
   long long k_head, k_row, v_head, v_row;
-  int tokens_per_warp;  // a power of two up to 32
+  int tokens_per_warp;     // up to 32
+  unsigned inv_per_token;  // ceil(2^32 / (2 heads)): exact quotients of a warp's row numbers
   int* err;
 };
 
-// Pool row (block * block_size + slot) of a packed row; -1: no sequence's,
-// -2: a table entry that cannot be followed, -3: a position below 0.
-__device__ __forceinline__ long long pool_row(const PoolView& pool, const BatchView& b, int row) {
+// Where a packed row's token lies: its pool block (-1: no sequence's row, -2: a
+// table entry that cannot be followed, -3: a position below 0) and the row in it.
+__device__ __forceinline__ int2 pool_row(const PoolView& pool, const BatchView& b, int row) {
   const int s = sequence_of(b, row);
-  if (s < 0) return -1;
+  if (s < 0) return {-1, 0};
   const int pos = b.kv_len[s] - b.offsets[s + 1] + row;
-  if (pos < 0) return -3;
+  if (pos < 0) return {-3, 0};
   const int lb = pos / pool.block_size;
-  if (lb >= b.table_width) return -2;
-  const long long blk = b.tables[s * b.table_stride + lb];
-  if (blk < 0 || blk >= pool.blocks) return -2;
-  return blk * pool.block_size + pos % pool.block_size;
+  if (lb >= b.table_width) return {-2, 0};
+  const int blk = b.tables[s * b.table_stride + lb];
+  if (blk < 0 || blk >= pool.blocks) return {-2, 0};
+  return {blk, pos - lb * pool.block_size};
 }
 
 // Both kernels: a warp takes tokens_per_warp consecutive packed rows; lane i
 // follows row i's offsets, length and table entry (the chains of dependent
-// loads run side by side), then the warp walks its (token, K/V, head) rows, a
-// row's head_dim over head_dim / 8 lanes: 16-byte bf16 and 8-byte code
-// accesses.  Bound by HBM; up to kRowsInFlight rows' loads are in flight.
+// loads run side by side), then the warp walks its (token, K/V, head) rows, 16
+// elements a lane: 32-byte bf16 and 16-byte code accesses.  Bound by HBM; the
+// loads of kRowsInFlight rows a lane are in flight together.
 constexpr int kRowsInFlight = 4;
+
+// Row r of a warp's n (token, K/V, head) rows.
+struct CacheRow {
+  int tok, which;   // token of the warp, is_v * heads + head
+  int blk;          // as pool_row's, or -1 past the warp's rows
+  long long prow;   // row of the pool, valid when blk >= 0
+};
+
+__device__ __forceinline__ CacheRow cache_row(const CacheRowsParams& p, int r, int n, int2 mine) {
+  CacheRow c;
+  const int per_token = 2 * p.pool.heads;
+  c.tok = r < n ? static_cast<int>(__umulhi(static_cast<unsigned>(r), p.inv_per_token)) : 0;
+  c.which = r - c.tok * per_token;
+  c.blk = __shfl_sync(0xffffffffu, mine.x, c.tok);
+  const int slot = __shfl_sync(0xffffffffu, mine.y, c.tok);
+  if (r >= n) c.blk = -1;
+  c.prow = (static_cast<long long>(c.blk) * per_token + c.which) * p.pool.block_size + slot;
+  return c;
+}
+
+// Element offset of a packed row's head.
+__device__ __forceinline__ const __nv_bfloat16* packed_row(const CacheRowsParams& p, long long row, int which) {
+  const bool is_v = which >= p.pool.heads;
+  return static_cast<const __nv_bfloat16*>(is_v ? p.v : p.k) +
+         (is_v ? which - p.pool.heads : which) * (is_v ? p.v_head : p.k_head) + row * (is_v ? p.v_row : p.k_row);
+}
 
 template <int D>
 __global__ void __launch_bounds__(256) cache_append_kernel(const CacheRowsParams p) {
-  constexpr int kLanes = D / 8;          // lanes of a row: 16 or 32
-  constexpr int kSide = 32 / kLanes;     // rows side by side
+  constexpr int kLanes = D / 16;      // lanes of a row: 8 or 16
+  constexpr int kSide = 32 / kLanes;  // rows side by side
   const int lane = threadIdx.x & 31;
   const int l = lane % kLanes, side = lane / kLanes;
   const int tpw = p.tokens_per_warp;
   const PoolView& pool = p.pool;
-  const int per_token = 2 * pool.heads;
   for (long long t0 = (blockIdx.x * 8LL + (threadIdx.x >> 5)) * tpw; t0 < p.batch.rows; t0 += gridDim.x * 8LL * tpw) {
     const int tokens = static_cast<int>(min(static_cast<long long>(tpw), p.batch.rows - t0));
-    long long mine = -1;
+    int2 mine = {-1, 0};
     if (lane < tokens) {
       mine = pool_row(pool, p.batch, static_cast<int>(t0) + lane);
-      if (mine < -1) atomicCAS(p.err, 0, mine == -2 ? kErrBlockTable : kErrSequence);
+      if (mine.x < -1) atomicCAS(p.err, 0, mine.x == -2 ? kErrBlockTable : kErrSequence);
     }
-    const int n = tokens * per_token;
+    const int n = tokens * 2 * pool.heads;
     for (int r0 = 0; r0 < n; r0 += kSide * kRowsInFlight) {
-      uint4 x[kRowsInFlight];
+      uint4 x[kRowsInFlight][2];
+      CacheRow c[kRowsInFlight];
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
-        const int r = r0 + u * kSide + side;
-        x[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n) {
-          const int tok = r / per_token, which = r % per_token, is_v = which >= pool.heads;
-          const int head = is_v ? which - pool.heads : which;
-          const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_v ? p.v : p.k) +
-                                     head * (is_v ? p.v_head : p.k_head) + (t0 + tok) * (is_v ? p.v_row : p.k_row);
-          x[u] = *reinterpret_cast<const uint4*>(src + 8 * l);
+        c[u] = cache_row(p, r0 + u * kSide + side, n, mine);
+        x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (c[u].blk >= 0) {
+          const uint4* src = reinterpret_cast<const uint4*>(packed_row(p, t0 + c[u].tok, c[u].which) + 16 * l);
+          x[u][0] = src[0];
+          x[u][1] = src[1];
         }
       }
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
-        const int r = r0 + u * kSide + side;
-        const int tok = min(r / per_token, tokens - 1);
-        const long long at = __shfl_sync(0xffffffffu, mine, tok);
-        const int which = r % per_token;  // is_v * heads + head: the order within a block
-        const bool live = r < n && at >= 0;
-        // rows of this block before this one, and its own slot
-        const long long blk = live ? at / pool.block_size : 0;
-        const long long prow = (blk * per_token + which) * pool.block_size + (live ? at - blk * pool.block_size : 0);
+        const bool live = c[u].blk >= 0;
         if (pool.bf16) {
-          if (live) *reinterpret_cast<uint4*>(pool.data + (prow * D + 8 * l) * 2) = x[u];
+          uint4* dst = reinterpret_cast<uint4*>(pool.data + (c[u].prow * D + 16 * l) * 2);
+          if (live) dst[0] = x[u][0], dst[1] = x[u][1];
           continue;
         }
-        float f[8];
-        Vec8<__nv_bfloat16> v8{x[u]};
-        v8.get(f);
+        float f[16];
+        Vec8<__nv_bfloat16>{x[u][0]}.get(f);
+        Vec8<__nv_bfloat16>{x[u][1]}.get(f + 8);
         if (pool.scales) {
           // Largest finite magnitude, as bits (they order like the values).
           uint32_t m = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 16; ++i) {
             const uint32_t a = __float_as_uint(f[i]) & 0x7FFFFFFFu;
             if (a < 0x7F800000u) m = max(m, a);
           }
@@ -353,14 +372,15 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheRowsParams
           e = m == 0 ? 0 : min(max(e, -100), 120);
           const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= inv;
-          if (live && l == 0) pool.scales[prow] = static_cast<uint8_t>(e + 127);
+          for (int i = 0; i < 16; ++i) f[i] *= inv;
+          if (live && l == 0) pool.scales[c[u].prow] = static_cast<uint8_t>(e + 127);
         }
-        uint32_t c[4];
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = e4m3x2_from_floats(f[2 * i], f[2 * i + 1]);
-        if (live)
-          *reinterpret_cast<uint2*>(pool.data + prow * D + 8 * l) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+        for (int i = 0; i < 4; ++i)
+          w[i] = e4m3x2_from_floats(f[4 * i], f[4 * i + 1]) |
+                 (static_cast<uint32_t>(e4m3x2_from_floats(f[4 * i + 2], f[4 * i + 3])) << 16);
+        if (live) *reinterpret_cast<uint4*>(pool.data + c[u].prow * D + 16 * l) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -368,67 +388,63 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheRowsParams
 
 template <int D>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheRowsParams p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   constexpr int kSide = 32 / kLanes;
   const int lane = threadIdx.x & 31;
   const int l = lane % kLanes, side = lane / kLanes;
   const int tpw = p.tokens_per_warp;
   const PoolView& pool = p.pool;
-  const int per_token = 2 * pool.heads;
   for (long long t0 = (blockIdx.x * 8LL + (threadIdx.x >> 5)) * tpw; t0 < p.batch.rows; t0 += gridDim.x * 8LL * tpw) {
     const int tokens = static_cast<int>(min(static_cast<long long>(tpw), p.batch.rows - t0));
-    long long mine = -1;
+    int2 mine = {-1, 0};
     if (lane < tokens) {
       mine = pool_row(pool, p.batch, static_cast<int>(t0) + lane);
-      if (mine < -1) atomicCAS(p.err, 0, mine == -2 ? kErrBlockTable : kErrSequence);
+      if (mine.x < -1) atomicCAS(p.err, 0, mine.x == -2 ? kErrBlockTable : kErrSequence);
     }
-    const int n = tokens * per_token;
+    const int n = tokens * 2 * pool.heads;
     for (int r0 = 0; r0 < n; r0 += kSide * kRowsInFlight) {
-      uint4 x[kRowsInFlight];
+      uint4 x[kRowsInFlight][2];
       uint32_t sc[kRowsInFlight];
-      long long at[kRowsInFlight];
+      CacheRow c[kRowsInFlight];
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
-        const int r = r0 + u * kSide + side;
-        at[u] = __shfl_sync(0xffffffffu, mine, min(r / per_token, tokens - 1));
-        if (r >= n) at[u] = -1;
-        x[u] = make_uint4(0u, 0u, 0u, 0u);
+        c[u] = cache_row(p, r0 + u * kSide + side, n, mine);
+        x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
         sc[u] = 127;
-        if (at[u] >= 0) {
-          const long long blk = at[u] / pool.block_size;
-          const long long prow = (blk * per_token + r % per_token) * pool.block_size + (at[u] - blk * pool.block_size);
+        if (c[u].blk >= 0) {
           if (pool.bf16) {
-            x[u] = *reinterpret_cast<const uint4*>(pool.data + (prow * D + 8 * l) * 2);
+            const uint4* src = reinterpret_cast<const uint4*>(pool.data + (c[u].prow * D + 16 * l) * 2);
+            x[u][0] = src[0];
+            x[u][1] = src[1];
           } else {
-            const uint2 c = *reinterpret_cast<const uint2*>(pool.data + prow * D + 8 * l);
-            x[u].x = c.x;
-            x[u].y = c.y;
-            if (pool.scales) sc[u] = pool.scales[prow];
+            x[u][0] = *reinterpret_cast<const uint4*>(pool.data + c[u].prow * D + 16 * l);
+            if (pool.scales) sc[u] = pool.scales[c[u].prow];
           }
         }
       }
 #pragma unroll
       for (int u = 0; u < kRowsInFlight; ++u) {
-        const int r = r0 + u * kSide + side;
-        if (at[u] != -2 && at[u] < 0) continue;  // -2: the tokens cannot be found, zeros
-        const int tok = r / per_token, which = r % per_token, is_v = which >= pool.heads;
-        const int head = is_v ? which - pool.heads : which;
-        uint4 o = x[u];
+        if (c[u].blk != -2 && c[u].blk < 0) continue;  // -2: the token cannot be found, zeros
+        uint4 o[2] = {x[u][0], x[u][1]};
         if (!pool.bf16) {
-          uint32_t h[4], w[4];
-          e4m3x4_to_f16x4(x[u].x, h[0], h[1]);
-          e4m3x4_to_f16x4(x[u].y, h[2], h[3]);
+          uint4 h[2];
+          e4m3x16_to_f16(x[u][0], h[0], h[1]);
           const float s = __uint_as_float(sc[u] << 23);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-            w[i] = pack_bf16x2(f.x * s, f.y * s);  // four significant bits: exact
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t hw[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw[j]));
+              w[j] = pack_bf16x2(f.x * s, f.y * s);  // four significant bits: exact
+            }
+            o[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          o = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(const_cast<void*>(is_v ? p.v : p.k)) +
-                             head * (is_v ? p.v_head : p.k_head) + (t0 + tok) * (is_v ? p.v_row : p.k_row);
-        *reinterpret_cast<uint4*>(dst + 8 * l) = o;
+        uint4* dst = reinterpret_cast<uint4*>(const_cast<__nv_bfloat16*>(packed_row(p, t0 + c[u].tok, c[u].which)) + 16 * l);
+        dst[0] = o[0];
+        dst[1] = o[1];
       }
     }
   }
