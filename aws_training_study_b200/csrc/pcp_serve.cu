@@ -334,11 +334,15 @@ int pcp_qk_norm_rope(int32_t dtype, int32_t rows, int32_t head_dim, int32_t rota
   const int per_pass = 32 / p.lanes;
   p.passes_q = static_cast<int>(ceil_div(q->heads, per_pass));
   p.passes = p.passes_q + static_cast<int>(ceil_div(k->heads, per_pass));
-  // Passes a warp: all of a row's when that leaves 32 warps an SM (its angles
-  // are then made once), fewer while the GPU has idle warps.
-  p.per_warp = p.passes;
-  while (p.per_warp > 1 && rows * ceil_div(p.passes, p.per_warp) < 148 * 32) p.per_warp = (p.per_warp + 1) / 2;
-  p.interleaved = layout == PCP_ROTARY_INTERLEAVED;
+  // Passes a warp: the split of a row that takes the fewest rounds of the 16
+  // warps an SM holds, where a warp's start (its angles, its first loads) costs
+  // about four passes.
+  int64_t best = INT64_MAX;
+  for (int parts = 1; parts <= p.passes; ++parts) {
+    const int per = static_cast<int>(ceil_div(p.passes, parts));
+    const int64_t cost = ceil_div(rows * ceil_div(p.passes, per), 148 * 16) * (per + 4);
+    if (cost < best) best = cost, p.per_warp = per;
+  }
   p.positions = positions;
   p.positions_64 = positions_64;
   p.turns = reinterpret_cast<const unsigned long long*>(turns);
@@ -347,9 +351,11 @@ int pcp_qk_norm_rope(int32_t dtype, int32_t rows, int32_t head_dim, int32_t rota
   const int64_t warps = rows * ceil_div(p.passes, p.per_warp);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(warps, 8), 148 * 16));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PCP_F32) pcp::qk_norm_rope_kernel<float><<<grid, 256, 0, st>>>(p);
-  else if (dtype == PCP_F16) pcp::qk_norm_rope_kernel<__half><<<grid, 256, 0, st>>>(p);
-  else pcp::qk_norm_rope_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(p); };
+  const bool inter = layout == PCP_ROTARY_INTERLEAVED;
+  if (dtype == PCP_F32) launch(inter ? pcp::qk_norm_rope_kernel<float, true> : pcp::qk_norm_rope_kernel<float, false>);
+  else if (dtype == PCP_F16) launch(inter ? pcp::qk_norm_rope_kernel<__half, true> : pcp::qk_norm_rope_kernel<__half, false>);
+  else launch(inter ? pcp::qk_norm_rope_kernel<__nv_bfloat16, true> : pcp::qk_norm_rope_kernel<__nv_bfloat16, false>);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
 }

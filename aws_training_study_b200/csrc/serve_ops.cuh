@@ -14,6 +14,30 @@ namespace pcp {
 
 constexpr int kErrSequence = 112;  // a sequence the call does not take (include/pcp_serve.h)
 
+// ------------------------------------------------------ pairs of fp32 values --
+// Two fp32 values in a 64-bit register: sm_100 multiplies and adds both in one
+// instruction, each rounded as the scalar form would.
+typedef unsigned long long f32x2;
+
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // ------------------------------------------------- eight elements a lane --
 template <typename T>
 struct Vec8;  // raw: what is loaded and stored at once
@@ -71,6 +95,22 @@ struct Vec8<float> {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void get_pairs(const Vec8<T>& v, f32x2* f) {
+  float x[8];
+  v.get(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = pair(x[2 * i], x[2 * i + 1]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_pairs(void* p, const f32x2* f) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(f[i], x[2 * i], x[2 * i + 1]);
+  Vec8<T>::store(p, x);
+}
+
 // ------------------------------------------------------- norm and rotation --
 struct HeadRows {  // [heads][rows][head_dim] at any head and row stride (elements)
   const void* in;
@@ -88,13 +128,36 @@ struct NormRopeParams {
   int passes;         // passes of 32 / lanes heads: of q's, then of k's
   int passes_q;
   int per_warp;       // passes of one row that a warp takes
-  int interleaved;
   const void* positions;
   int positions_64;
   const unsigned long long* turns;  // turns per position of each pair, as a 64-bit fraction
   float magnitude;
   float eps;
 };
+
+// sin and cos of 2 pi t / 2^64.  The nearest quarter turn comes off in integers
+// (exactly), which leaves |x| <= pi / 4, where the Taylor series to x^9 and x^10
+// are within 2e-9 of sine and cosine: below half a step of fp32, so that what
+// is lost is x's rounding (pi / 4 * 2^-24) and the sums'.
+__device__ __forceinline__ void sincos_turns(unsigned long long t, float& sn, float& cs) {
+  const unsigned long long near = t + (1ull << 61);
+  const unsigned quarter = static_cast<unsigned>(near >> 62);
+  const int rest = static_cast<int>((t - (static_cast<unsigned long long>(quarter) << 62)) >> 32);
+  const float x = static_cast<float>(rest) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float z = x * x;
+  float s = fmaf(z, 2.7557319224e-6f, -1.9841269841e-4f);  // 1/9!, -1/7!
+  s = fmaf(z, s, 8.3333333333e-3f);                        // 1/5!
+  s = fmaf(z, s, -1.6666666667e-1f);                       // -1/3!
+  s = fmaf(z * x, s, x);
+  float c = fmaf(z, -2.7557319224e-7f, 2.4801587302e-5f);  // -1/10!, 1/8!
+  c = fmaf(z, c, -1.3888888889e-3f);                       // -1/6!
+  c = fmaf(z, c, 4.1666666667e-2f);                        // 1/4!
+  c = fmaf(z, c, -0.5f);
+  c = fmaf(z, c, 1.f);
+  const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+  sn = quarter & 2 ? -a : a;
+  cs = (quarter + 1) & 2 ? -b : b;
+}
 
 // A warp takes one row (token) and some of its heads, 16 elements of a head a
 // lane: the mean of squares is one shuffle reduction, and a rotated pair's two
@@ -103,122 +166,147 @@ struct NormRopeParams {
 // between lanes.  cos and sin are made once per row and lane, from the position
 // times the pair's turns in 64-bit integers (whole turns overflow away, so
 // there is no table to read and no error that grows with the position), and
-// used for every head of the warp.  Bound by HBM: each element is read and
-// written once; kUnroll passes' loads are in flight together.
-template <typename T>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormRopeParams p) {
-  constexpr int kUnroll = sizeof(T) == 4 ? 2 : 4;
+// used for every head of the warp.  HBM's share is one read and one write of
+// each element; instructions are near it (the first version issued 322 a pass
+// of 1 KB and reached half of HBM's rate), hence two values an instruction and
+// pointers that step.  The next kUnroll passes' loads are in flight over the work
+// on kUnroll.
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const NormRopeParams p) {
+  constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
   const int lane = threadIdx.x & 31;
   const int parts = (p.passes + p.per_warp - 1) / p.per_warp;
   const long long items = static_cast<long long>(p.rows) * parts;
   const int l = lane & (p.lanes - 1);
   const int sub = lane / p.lanes;       // which of the pass's heads
   const int per_pass = 32 / p.lanes;
-  const int half = p.rotary_dim / 2;
   const bool live_lane = 16 * l < p.head_dim;
+  const int half = p.rotary_dim / 2;
   // First elements of this lane's two runs of eight, and whether they turn.
-  bool turned = 16 * l < p.rotary_dim;
+  const bool turned = 16 * l < p.rotary_dim;
   int e0 = 16 * l, e1 = 16 * l + 8;
-  if (turned && !p.interleaved) e0 = 8 * l, e1 = 8 * l + half;
+  if (turned && !kInterleaved) e0 = 8 * l, e1 = 8 * l + half;
   const float inv_d = 1.f / static_cast<float>(p.head_dim);
 
   for (long long item = blockIdx.x * 8LL + (threadIdx.x >> 5); item < items; item += gridDim.x * 8LL) {
     const int row = static_cast<int>(item / parts);
-    const int p0 = static_cast<int>(item % parts) * p.per_warp;
+    const int p0 = static_cast<int>(item - static_cast<long long>(row) * parts) * p.per_warp;
     const int p1 = min(p0 + p.per_warp, p.passes);
-    float co[8], si[8];
+    // The rotation as factors of pairs of values: half layout, (cos, cos') and
+    // (sin, sin') of two neighbouring pairs; interleaved, (cos, cos) and
+    // (-sin, sin) of one.
+    constexpr int kPairs = kInterleaved ? 8 : 4;
+    f32x2 co[kPairs], si[kPairs];
     bool have_angles = false;
-    float w0[8], w1[8];
-    for (int pb = p0; pb < p1; pb += kUnroll) {
-      Vec8<T> x0[kUnroll], x1[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int pass = pb + u;
-        if (pass >= p1 || !live_lane) continue;
-        const bool is_k = pass >= p.passes_q;
-        const HeadRows& h = is_k ? p.k : p.q;
-        const int head = (is_k ? pass - p.passes_q : pass) * per_pass + sub;
-        if (head >= h.heads) continue;
-        const T* in = static_cast<const T*>(h.in) + head * h.in_head + row * h.in_row;
-        x0[u].load(in + e0);
-        x1[u].load(in + e1);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {  // q's passes, then k's
+      const HeadRows& h = part ? p.k : p.q;
+      const int base = part ? p.passes_q : 0;
+      int a = max(p0, base) - base;
+      const int b = (part ? p1 : min(p1, p.passes_q)) - base;
+      if (a >= b) continue;
+      const int heads = h.heads;
+      const long long in_step = per_pass * h.in_head, out_step = per_pass * h.out_head;
+      const T* in = static_cast<const T*>(h.in) + row * h.in_row + (a * per_pass + sub) * h.in_head;
+      T* out = static_cast<T*>(h.out) + row * h.out_row + (a * per_pass + sub) * h.out_head;
+      const bool norm = h.weight != nullptr;
+      f32x2 w[8];
+      if (norm && live_lane) {
+        Vec8<T> x, y;
+        x.load(static_cast<const T*>(h.weight) + e0);
+        y.load(static_cast<const T*>(h.weight) + e1);
+        get_pairs(x, w);
+        get_pairs(y, w + 4);
       }
-      if (!have_angles) {  // behind the first loads
-        have_angles = true;
-        if (turned) {
-          const long long pos = p.positions_64 ? static_cast<const long long*>(p.positions)[row]
-                                               : static_cast<const int*>(p.positions)[row];
-          const int pair0 = 8 * l;
+      Vec8<T> n0[kUnroll], n1[kUnroll];  // the next passes' loads, in flight over this one's work
+      auto load = [&](int at, const T* from) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const unsigned long long t = static_cast<unsigned long long>(pos) * p.turns[pair0 + i];
-            // the top 32 bits as half turns in [-1, 1)
-            const float a = static_cast<float>(static_cast<int>(t >> 32)) * 4.656612873077393e-10f;
-            sincospif(a, &si[i], &co[i]);
-            si[i] *= p.magnitude;
-            co[i] *= p.magnitude;
+        for (int u = 0; u < kUnroll; ++u)
+          if (live_lane && at + u < b && (at + u) * per_pass + sub < heads) {
+            n0[u].load(from + u * in_step + e0);
+            n1[u].load(from + u * in_step + e1);
           }
-        }
-      }
+      };
+      load(a, in);
+#pragma unroll 1
+      for (; a < b; a += kUnroll) {
+        Vec8<T> x0[kUnroll], x1[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int pass = pb + u;
-        if (pass >= p1) continue;  // the same for the whole warp
-        const bool is_k = pass >= p.passes_q;
-        const HeadRows& h = is_k ? p.k : p.q;
-        const int head = (is_k ? pass - p.passes_q : pass) * per_pass + sub;
-        const bool live = live_lane && head < h.heads;
-        float f0[8], f1[8];
-        if (live) {
-          x0[u].get(f0);
-          x1[u].get(f1);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f0[i] = f1[i] = 0.f;
-        }
-        if (h.weight) {
-          if ((pass == p0 || pass == p.passes_q) && live_lane) {
-            Vec8<T> a, b;
-            a.load(static_cast<const T*>(h.weight) + e0);
-            b.load(static_cast<const T*>(h.weight) + e1);
-            a.get(w0);
-            b.get(w1);
-          }
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(f0[i], f0[i], fmaf(f1[i], f1[i], ss));
-          for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float r = rsqrtf(ss * inv_d + p.eps);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            f0[i] = f0[i] * r * w0[i];
-            f1[i] = f1[i] * r * w1[i];
-          }
-        }
-        if (turned) {
-          if (p.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float a = f0[2 * i], b = f0[2 * i + 1], c = f1[2 * i], d = f1[2 * i + 1];
-              f0[2 * i] = a * co[i] - b * si[i];
-              f0[2 * i + 1] = b * co[i] + a * si[i];
-              f1[2 * i] = c * co[i + 4] - d * si[i + 4];
-              f1[2 * i + 1] = d * co[i + 4] + c * si[i + 4];
-            }
-          } else {
+        for (int u = 0; u < kUnroll; ++u) x0[u] = n0[u], x1[u] = n1[u];
+        in += kUnroll * in_step;
+        load(a + kUnroll, in);
+        if (!have_angles && p.rotary_dim) {  // behind the first loads
+          have_angles = true;
+          if (turned) {
+            const long long pos = p.positions_64 ? static_cast<const long long*>(p.positions)[row]
+                                                 : static_cast<const int*>(p.positions)[row];
+            float c[8], s[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float a = f0[i], b = f1[i];
-              f0[i] = a * co[i] - b * si[i];
-              f1[i] = b * co[i] + a * si[i];
+              sincos_turns(static_cast<unsigned long long>(pos) * p.turns[8 * l + i], s[i], c[i]);
+              s[i] *= p.magnitude;
+              c[i] *= p.magnitude;
+            }
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              co[i] = kInterleaved ? pair(c[i], c[i]) : pair(c[(2 * i) & 7], c[(2 * i + 1) & 7]);
+              si[i] = kInterleaved ? pair(-s[i], s[i]) : pair(s[(2 * i) & 7], s[(2 * i + 1) & 7]);
             }
           }
         }
-        if (live) {
-          T* out = static_cast<T*>(h.out) + head * h.out_head + row * h.out_row;
-          Vec8<T>::store(out + e0, f0);
-          Vec8<T>::store(out + e1, f1);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (a + u >= b) break;  // the same for the whole warp
+          const bool live = live_lane && (a + u) * per_pass + sub < heads;
+          f32x2 f[8];
+          if (live) {
+            get_pairs(x0[u], f);
+            get_pairs(x1[u], f + 4);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0;
+          }
+          if (norm) {
+            f32x2 sq = mul2(f[0], f[0]), sr = mul2(f[1], f[1]);
+#pragma unroll
+            for (int i = 2; i < 8; i += 2) {
+              sq = fma2(f[i], f[i], sq);
+              sr = fma2(f[i + 1], f[i + 1], sr);
+            }
+            float s0, s1, s2, s3;
+            split(sq, s0, s1);
+            split(sr, s2, s3);
+            float ss = (s0 + s1) + (s2 + s3);
+            for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
+            const f32x2 rr = pair(r, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = mul2(mul2(f[i], rr), w[i]);
+          }
+          if (turned) {
+            if (kInterleaved) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float x, y;
+                split(f[i], x, y);
+                f[i] = fma2(f[i], co[i], mul2(pair(y, x), si[i]));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const f32x2 x = f[i], y = f[4 + i];
+                f[4 + i] = fma2(y, co[i & (kPairs - 1)], mul2(x, si[i & (kPairs - 1)]));
+                const f32x2 ys = mul2(y, si[i & (kPairs - 1)]);
+                f[i] = fma2(x, co[i & (kPairs - 1)], ys ^ 0x8000000080000000ull);
+              }
+            }
+          }
+          if (live) {
+            store_pairs<T>(out + u * out_step + e0, f);
+            store_pairs<T>(out + u * out_step + e1, f + 4);
+          }
         }
+        out += kUnroll * out_step;
       }
     }
   }

@@ -3,7 +3,7 @@ in 64 bits.
 
 Tolerance: half a step of the output type, plus what fp32 arithmetic may lose
 of the terms a pair is summed from, 2e-6 * magnitude * (|a| + |b|): the angle
-in half turns is rounded once (pi * 2^-25), sincospif, the magnitude, two
+is rounded once (pi / 4 * 2^-24), sine and cosine, the magnitude, two
 products and a sum are each within about 2^-24, and the norm's sum of squares
 over at most 16 serial and 5 shuffled terms, its square root and two products
 within 1e-6."""
