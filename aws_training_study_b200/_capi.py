@@ -152,7 +152,8 @@ SIGNATURES = {
                    _c.c_float, _P]),
     "pcp_cache_append": (_c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _P, _P]),
     "pcp_cache_read": (_c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _P, _P]),
-    "pcp_chunk_attention_workspace_size": (_c.c_int, [_PPOOL, _I32, _I32, _I32, _I32, _c.POINTER(_c.c_size_t)]),
+    "pcp_chunk_attention_workspace_size": (
+        _c.c_int, [_PPOOL, _I32, _I32, _I32, _I32, _I32, _c.POINTER(_c.c_size_t)]),
     "pcp_chunk_attention": (
         _c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _I32, _c.c_float, _P, _c.c_size_t, _P, _P]),
 }

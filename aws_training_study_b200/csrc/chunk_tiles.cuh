@@ -16,6 +16,9 @@
 //   * bf16 caches land in operand layout straight from TMA; the converter warps
 //     only pass the tile on (and clear V rows past the sequence, which may hold
 //     anything: 0 * NaN would reach every row).
+//   * An e4m3 cache that many query tiles read is expanded into a bf16 copy first
+//     (chunk_expand_kernel; exact, scales included), when the copy is of moderate
+//     size: reading it in place converts every key tile again for each 256 rows.
 //   * Scaled e4m3 caches: K's 2^e multiplies the scores of its key, V's 2^e the
 //     weights, and the softmax reference is kept above score + V exponent, as in
 //     chunk_rows.cuh.
@@ -70,6 +73,64 @@ struct TilesSmem {
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
   static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
 };
+
+// The pages of sequences with tile units as bf16, page lb of sequence s at block
+// s * table_width + lb of `copy`, in the payload's layout.  Bound by HBM (1 byte
+// read, 2 written an element); a block takes the rows of one head of K or V of a
+// page at a time.
+struct ExpandParams {
+  ChunkParams c;
+  __nv_bfloat16* copy;
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p) {
+  constexpr int kPerRow = D / 16;
+  const PoolView& pool = p.c.pool;
+  const int per_page = 2 * pool.heads;
+  const long long items = static_cast<long long>(p.c.batch.seqs) * p.c.batch.table_width * per_page;
+  __shared__ int s_ignored;  // lengths the attention reports itself
+  if (threadIdx.x == 0) s_ignored = 0;
+  __syncthreads();
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    const long long page = it / per_page;
+    const int which = static_cast<int>(it - page * per_page);
+    const int s = static_cast<int>(page / p.c.batch.table_width), lb = static_cast<int>(page - static_cast<long long>(s) * p.c.batch.table_width);
+    const ChunkSeq q = chunk_seq<true>(p.c, s, &s_ignored);
+    const int n = min(pool.block_size, q.kvlen - lb * pool.block_size);
+    if (q.tiles == 0 || n <= 0) continue;
+    const int blk = p.c.batch.tables[s * p.c.batch.table_stride + lb];
+    const bool found = blk >= 0 && blk < pool.blocks;
+    if (!found && threadIdx.x == 0) atomicCAS(p.c.status, 0, kErrBlockTable);
+    const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size;
+    const uint4* codes = reinterpret_cast<const uint4*>(pool.data + src * D);
+    const uint8_t* scales = pool.scales ? pool.scales + src : nullptr;
+    uint4* dst = reinterpret_cast<uint4*>(p.copy + (page * per_page + which) * pool.block_size * D);
+    for (int e0 = threadIdx.x; e0 < n * kPerRow; e0 += 4 * 256) {
+      uint4 x[4];
+      uint32_t sc[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + u * 256;
+        x[u] = make_uint4(0u, 0u, 0u, 0u);
+        sc[u] = 127;
+        if (found && e < n * kPerRow) {
+          x[u] = codes[e];
+          if (scales) sc[u] = scales[e / kPerRow];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + u * 256;
+        if (e >= n * kPerRow) break;
+        uint4 o[2];
+        e4m3x16_to_bf16(x[u], sc[u], o);
+        dst[2 * e] = o[0];
+        dst[2 * e + 1] = o[1];
+      }
+    }
+  }
+}
 
 template <int D, int kCache>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
@@ -179,7 +240,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       int seq = -1, cached_lb = -1, cached_page = 0;
       auto page_of = [&](const ChunkUnit& un, int lb) -> int {
         if (un.seq == seq && lb == cached_lb) return cached_page;
-        int b = lb < p.batch.table_width ? p.batch.tables[un.seq * p.batch.table_stride + lb] : -1;
+        int b = lb >= p.batch.table_width ? -1
+                : p.batch.tables          ? p.batch.tables[un.seq * p.batch.table_stride + lb]
+                                          : un.seq * p.batch.table_width + lb;  // the expanded copy
         if (b < 0 || b >= p.pool.blocks) {  // reported; block 0 keeps the load in bounds
           atomicCAS(err, 0, kErrBlockTable);
           b = 0;
@@ -260,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             if (pg < 0 || pg >= p.pool.blocks) pg = 0;  // the producer reports it
             const uint8_t* sc = p.pool.scales +
                                 (static_cast<long long>(pg) * 2 * p.pool.heads + un.head) * p.pool.block_size +
-                                key % p.pool.block_size;
+                                key - lb * p.pool.block_size;
             kb = sc[0];
             vb = sc[static_cast<long long>(p.pool.heads) * p.pool.block_size];
           }
@@ -324,16 +387,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       return true;
     };
     for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
-      // Q rows into the swizzled operand layout, once the previous segment's
-      // QK^T are done with it: a row over D / 8 lanes, four rows in flight.
-      if (segs > 0 && !wait_all(bar_q_empty, (segs - 1) & 1u, kErrWaitQ)) return false;
+      // Q rows into the swizzled operand layout: a row over D / 8 lanes,
+      // kFlight loads a lane in flight, the first of them before the wait for the
+      // previous segment's QK^T to be done with the buffer.
       constexpr int kSide = 256 / D;  // rows side by side in a warp
+      constexpr int kFlight = kFp8 ? 4 : 16;  // (the conversion unrolled 16 times costs the instruction cache more)
       const int side = lane / (D / 8), ch = lane % (D / 8);
 #pragma unroll 1
-      for (int r0 = cw * 32; r0 < cw * 32 + 32; r0 += 4 * kSide) {
-        uint4 x[4];
+      for (int r0 = cw * 32; r0 < cw * 32 + 32; r0 += kFlight * kSide) {
+        uint4 x[kFlight];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kFlight; ++u) {
           const int r = static_cast<int>(rank) * kTileM + r0 + u * kSide + side;
           const int row = un.row0 + r;
           x[u] = make_uint4(0u, 0u, 0u, 0u);
@@ -342,8 +406,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
                 p.q + static_cast<long long>(un.head * p.group + row % p.group) * p.q_head +
                 static_cast<long long>(un.q0 + row / p.group) * p.q_row + 8 * ch);
         }
+        if (r0 == cw * 32 && segs > 0 && !wait_all(bar_q_empty, (segs - 1) & 1u, kErrWaitQ)) return false;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kFlight; ++u) {
           const int r = r0 + u * kSide + side;
           if (kFp8) {
             float f[8];

@@ -120,13 +120,21 @@ constexpr int kPairs = kCtas / 2;
 size_t align_up(size_t a) { return (a + 255) / 256 * 256; }
 
 struct ChunkLayout {
-  size_t small_rec, tile_rec, small_o, small_lse, tile_o, tile_lse, bytes;
+  size_t small_rec, tile_rec, small_o, small_lse, tile_o, tile_lse, copy, bytes;
+  bool expand;  // tile units read a bf16 copy of their e4m3 pages
 };
+
+// An e4m3 cache is expanded for the tile units from kExpandRows rows a KV head
+// on (8 tiles), while the copy of all sequences' tables stays within
+// kExpandBytes.  EXPAND_FIGURES
+constexpr int64_t kExpandRows = 2048;
+constexpr int64_t kExpandBytes = int64_t(1) << 30;
 
 bool has_tiles(int32_t max_chunk, int32_t group) { return static_cast<int64_t>(max_chunk) * group > pcp::kSmallRows; }
 
-ChunkLayout chunk_layout(int32_t head_dim, int32_t group, int32_t max_chunk) {
+ChunkLayout chunk_layout(const pcp_pool_t& pool, int32_t group, int32_t seqs, int32_t table_width, int32_t max_chunk) {
   ChunkLayout w{};
+  const int32_t head_dim = pool.head_dim;
   const bool tiles = has_tiles(max_chunk, group);
   size_t at = 0;
   auto put = [&](size_t bytes) {
@@ -140,6 +148,11 @@ ChunkLayout chunk_layout(int32_t head_dim, int32_t group, int32_t max_chunk) {
   w.small_lse = put(size_t(2) * kCtas * pcp::kSmallRows * 4);
   w.tile_o = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * head_dim * 4 : 0);
   w.tile_lse = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * 4 : 0);
+  const int64_t page = int64_t(2) * pool.num_kv_heads * pool.block_size * head_dim * 2;
+  const int64_t pages = static_cast<int64_t>(seqs) * table_width;
+  w.expand = tiles && pool.kv_dtype == PCP_KV_E4M3 && static_cast<int64_t>(max_chunk) * group >= kExpandRows &&
+             pages > 0 && pages <= kExpandBytes / page;
+  w.copy = put(w.expand ? static_cast<size_t>(pages * page) : 0);
   w.bytes = at;
   return w;
 }
@@ -271,13 +284,33 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
   return PCP_OK;
 }
 
+// Tile units over the bf16 copy of their pages.
 template <int D>
-int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
+int launch_expanded(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, cudaStream_t st) {
+  const pcp::ExpandParams e{p, static_cast<__nv_bfloat16*>(copy)};
+  const int64_t pages = static_cast<int64_t>(p.batch.seqs) * p.batch.table_width;
+  const int64_t items = pages * 2 * pool.num_kv_heads;
+  pcp::chunk_expand_kernel<D><<<static_cast<unsigned>(std::min<int64_t>(items, 8 * kCtas)), 256, 0, st>>>(e);
+  CUDA_TRY(cudaGetLastError());
+  pcp_pool_t dense = pool;
+  dense.data = copy;
+  dense.scales = nullptr;
+  dense.blocks = pages;
+  dense.kv_dtype = PCP_KV_BF16;
+  pcp::ChunkParams d = p;
+  d.pool = pool_view(dense);
+  d.batch.tables = nullptr;
+  return launch_tiles<D, pcp::kCacheBf16>(dense, d, st);
+}
+
+template <int D>
+int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, cudaStream_t st) {
   const bool bf16 = pool.kv_dtype == PCP_KV_BF16;
   if (bf16) PCP_TRY((launch_rows<D, false>(pool, p, st)));
   else PCP_TRY((launch_rows<D, true>(pool, p, st)));
   if (p.tile_pairs) {
-    if (bf16) PCP_TRY((launch_tiles<D, pcp::kCacheBf16>(pool, p, st)));
+    if (copy) PCP_TRY(launch_expanded<D>(pool, p, copy, st));
+    else if (bf16) PCP_TRY((launch_tiles<D, pcp::kCacheBf16>(pool, p, st)));
     else if (pool.scales) PCP_TRY((launch_tiles<D, pcp::kCacheScaled>(pool, p, st)));
     else PCP_TRY((launch_tiles<D, pcp::kCacheE4m3>(pool, p, st)));
   }
@@ -371,10 +404,10 @@ int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_h
 }
 
 int pcp_chunk_attention_workspace_size(const pcp_pool_t* pool, int32_t num_q_heads, int32_t num_seqs, int32_t rows,
-                                       int32_t max_chunk, size_t* bytes) {
+                                       int32_t table_width, int32_t max_chunk, size_t* bytes) {
   PCP_TRY(check_chunk(pool, num_q_heads, num_seqs, rows, max_chunk));
   if (!bytes) return fail(PCP_ERR_INVALID_ARGUMENT, "bytes is NULL");
-  *bytes = chunk_layout(pool->head_dim, num_q_heads / pool->num_kv_heads, max_chunk).bytes;
+  *bytes = chunk_layout(*pool, num_q_heads / pool->num_kv_heads, num_seqs, std::max(table_width, 0), max_chunk).bytes;
   return PCP_OK;
 }
 
@@ -392,7 +425,7 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (batch->num_seqs == 0 || batch->rows == 0) return PCP_OK;
   const int32_t group = q->heads / pool->num_kv_heads;
-  const ChunkLayout w = chunk_layout(pool->head_dim, group, max_chunk);
+  const ChunkLayout w = chunk_layout(*pool, group, batch->num_seqs, batch->table_width, max_chunk);
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < w.bytes)
     return fail(PCP_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, aligned to 256, is needed (got %zu)", w.bytes,
                 workspace_bytes);
@@ -418,7 +451,8 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.small_ctas = kCtas;
   p.tile_pairs = has_tiles(max_chunk, group) ? kPairs : 0;
   p.status = device_status;
-  return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, st) : launch_chunk<128>(*pool, p, st);
+  void* copy = w.expand ? ws + w.copy : nullptr;
+  return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, copy, st) : launch_chunk<128>(*pool, p, copy, st);
 }
 
 }  // extern "C"

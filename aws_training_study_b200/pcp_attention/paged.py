@@ -291,8 +291,8 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     scale = config.softmax_scale if softmax_scale is None else float(softmax_scale)
     lib = _capi.lib()
     nbytes = ctypes.c_size_t()
-    _capi.check(lib.pcp_chunk_attention_workspace_size(ps, config.num_q_heads, batch.num_seqs, rows, max_chunk,
-                                                       ctypes.byref(nbytes)))
+    _capi.check(lib.pcp_chunk_attention_workspace_size(ps, config.num_q_heads, batch.num_seqs, rows,
+                                                       batch.table_width, max_chunk, ctypes.byref(nbytes)))
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=pool.device)
     st = _Status(status, pool.device, stream)
     _launch(pool.device, stream, lib.pcp_chunk_attention, ps, batch, _heads(q), _heads(out), max_chunk, scale,

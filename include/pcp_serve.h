@@ -137,7 +137,7 @@ int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_h
  *     aligned to 256, needed until the call's work has run; calls that may
  *     overlap need one each. */
 int pcp_chunk_attention_workspace_size(const pcp_pool_t* pool, int32_t num_q_heads, int32_t num_seqs, int32_t rows,
-                                       int32_t max_chunk, size_t* bytes);
+                                       int32_t table_width, int32_t max_chunk, size_t* bytes);
 int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* q, const pcp_heads_t* out,
                         int32_t max_chunk, float softmax_scale, void* workspace, size_t workspace_bytes,
                         int32_t* device_status, void* stream);
