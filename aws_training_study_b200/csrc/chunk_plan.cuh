@@ -264,10 +264,18 @@ __device__ __forceinline__ void chunk_plan(const ChunkParams& p, ChunkPlanShared
 }
 
 // A range's walk over its units: the part [kt0, kt1) of each one's steps.
+//
+// Tile units of a sequence share its K/V, and a long cache does not fit the L2:
+// ranges should be at the same keys at the same time.  So a range that starts in
+// the middle of a unit leaves that part for last: whole units first, from key 0
+// on in every range, then the unit it leaves unfinished, likewise, then the
+// part it started with.  (Ranges are equally long, so those last parts keep a
+// constant distance in keys to the others too.)
 template <bool kTile>
 struct ChunkWalk {
-  int left;  // steps of the range still to come
+  int left;  // steps of the range still to come, but for a part left for last
   int seq, head, unit, kt;
+  int later_seq, later_head, later_unit, later_kt, later;  // that part and its steps
 
   __device__ __forceinline__ void init(const ChunkPlanShared& sh) {
     left = static_cast<int>(sh.end - sh.x);
@@ -275,24 +283,47 @@ struct ChunkWalk {
     head = sh.head;
     unit = sh.unit;
     kt = sh.kt;
+    later = 0;
+  }
+  __device__ __forceinline__ void advance(const ChunkParams& p, int* err, int tiles) {
+    kt = 0;
+    if (left > 0 && ++unit == tiles) {
+      unit = 0;
+      if (++head == p.pool.heads) {
+        head = 0;
+        while (chunk_seq<kTile>(p, ++seq, err).tiles == 0) {
+        }
+      }
+    }
   }
   __device__ __forceinline__ bool next(const ChunkParams& p, int* err, ChunkUnit& u, int& kt0, int& kt1) {
-    if (left <= 0) return false;
-    ChunkSeq q = chunk_seq<kTile>(p, seq, err);
+    if (left <= 0 && (!kTile || later == 0)) return false;
+    if (kTile && left <= 0) {
+      left = later;
+      seq = later_seq;
+      head = later_head;
+      unit = later_unit;
+      kt = later_kt;
+      later = 0;
+    } else if (kTile && kt > 0) {
+      const ChunkSeq q = chunk_seq<kTile>(p, seq, err);
+      const int rest = chunk_unit<kTile>(p, q, seq, head, unit).steps - kt;
+      if (rest < left) {
+        later = rest;
+        later_seq = seq;
+        later_head = head;
+        later_unit = unit;
+        later_kt = kt;
+        left -= rest;
+        advance(p, err, q.tiles);
+      }
+    }
+    const ChunkSeq q = chunk_seq<kTile>(p, seq, err);
     u = chunk_unit<kTile>(p, q, seq, head, unit);
     kt0 = kt;
     kt1 = min(u.steps, kt + left);
     left -= kt1 - kt0;
-    kt = 0;
-    if (left > 0 && ++unit == q.tiles) {
-      unit = 0;
-      if (++head == p.pool.heads) {
-        head = 0;
-        do {
-          q = chunk_seq<kTile>(p, ++seq, err);
-        } while (q.tiles == 0);
-      }
-    }
+    advance(p, err, q.tiles);
     return true;
   }
 };
