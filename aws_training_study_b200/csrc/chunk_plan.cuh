@@ -66,6 +66,7 @@ struct ChunkParams {
   __nv_bfloat16* out;
   long long q_head, q_row, out_head, out_row;
   int group;       // query heads per KV head
+  long long capacity;  // tokens a sequence's table holds
   int max_chunk;
   float scale_log2;
   int small_ctas, tile_pairs;  // grids of the two kernels (0 pairs: not launched)
@@ -74,6 +75,17 @@ struct ChunkParams {
 
 __device__ __forceinline__ float exp2_of_int(int e) {  // 2^e, 0 below the normal range
   return __uint_as_float(static_cast<uint32_t>(min(max(e + 127, 0), 254)) << 23);
+}
+
+// One lane of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 
 // CTAs (or pairs) that a list of `steps` is cut for: at least one step each.
@@ -104,10 +116,9 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int s, int* 
     atomicCAS(err, 0, kErrSequence);
     q.kvlen = 0;
   }
-  const long long capacity = static_cast<long long>(p.batch.table_width) * p.pool.block_size;
-  if (q.kvlen > capacity) {
+  if (q.kvlen > p.capacity) {
     atomicCAS(err, 0, kErrBlockTable);
-    q.kvlen = static_cast<int>(capacity);
+    q.kvlen = static_cast<int>(p.capacity);
   }
   if (q.qlen > p.max_chunk) {
     atomicCAS(err, 0, kErrSequence);

@@ -2,11 +2,22 @@
 // the tensor cores.
 //
 // Bound by the MMAs (4 * 256 * 128 * D flops per 128-key tile of a unit against
-// 2 * 128 * D cache elements).  The pipeline is that of attn_kv.cuh: a cluster
-// of two CTAs shares every tcgen05 MMA (cta_group::2: each CTA holds 128 query
-// rows, half of each K tile's keys and half of each V tile's columns), scores
-// and probabilities live in TMEM, two softmax warpgroups per CTA own a row half
-// each and rescale O lazily.  What differs:
+// 2 * 128 * D cache elements), with the softmax next: 128 x 128 exponentials a
+// CTA and tile take the MUFU 1024 cycles, the MMAs 1024 (D = 128) or 2048.  As in
+// attn_kv.cuh a cluster of two CTAs shares every tcgen05 MMA (cta_group::2: each
+// CTA holds 128 query rows, half of each K tile's keys and half of each V tile's
+// columns), and scores and probabilities live in TMEM.  What differs:
+//   * D = 128: the two softmax warpgroups of a CTA take turns, one with the even
+//     key tiles and one with the odd ones, a thread a whole row of 128 keys.  Each
+//     has two tiles' time for one, its loads and maxima run under the other's
+//     exponentials, and all that passes between them is each row's reference
+//     maximum, which the other published half a turn ago.  The accumulator leaves
+//     TMEM columns to keep P apart from S, so that a score buffer is free, and the
+//     next QK^T but one issued, once its scores are in registers.
+//   * D = 256: no columns are left; P overwrites S, and a tile's QK^T waits for the
+//     product before last.  That chain (softmax, PV, QK^T and about 1300 cycles of
+//     hand-over in two tiles) is the limit, and the warpgroups split each tile's
+//     keys between them, which makes its softmax shortest.
 //   * Units come from the plan (chunk_plan.cuh): any mix of sequences, each pair
 //     walking an equal range of the batch's steps.
 //   * K and V are read from pages of any multiple of 16 tokens, through the
@@ -38,8 +49,14 @@ enum : int { kCacheBf16 = 0, kCacheE4m3 = 1, kCacheScaled = 2 };
 
 constexpr int kTilesConvWarps = 4;
 constexpr int kTilesConvThreads = 32 * kTilesConvWarps;
-constexpr int kTilesConvWarp0 = kMmaWarp + 1;
-constexpr int kTilesThreads = kThreads + kTilesConvThreads;  // 448
+// Four warpgroups: softmax 0 and 1, TMA and MMA warps (two idle), converters;
+// their registers, out of the launch's 512 x 128.
+constexpr int kTilesConvWarp0 = 12;
+constexpr int kTilesThreads = 512;
+constexpr int kTilesLaunchRegs = 128, kTilesSoftmaxRegs = 176, kTilesControlRegs = 72, kTilesConvRegs = 88;
+static_assert(2 * kTilesSoftmaxRegs + kTilesControlRegs + kTilesConvRegs <= 4 * kTilesLaunchRegs,
+              "more than the launch's registers");
+constexpr int kTurnsP = 128;  // TMEM columns of P, D = 128: O 0-127, P 128-255, S 256-511
 constexpr uint16_t kChunkBothCtas = 3, kChunkLeader = 1;
 
 template <int D, int kCache>
@@ -48,25 +65,30 @@ struct TilesSmem {
   static constexpr int kQBytes = D * 2 * kTileM;
   static constexpr int kOpBytes = 128 * D;  // 16-bit K half [64, D] or V half [128, D/2], swizzled
   static constexpr int kRawBytes = 64 * D;  // e4m3 K half [64][D] or V half [128][D/2]
-  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 8) : (D == 256 ? 5 : 11);
-  static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 6) : 0;
+  static constexpr bool kTurns = D == 128;  // the softmax warpgroups take turns
+  static constexpr int kAhead = kTurns ? 2 : 1;  // QK^T issued ahead of PV, in tiles
+  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 7) : (D == 256 ? 5 : 9);
+  static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 5) : 0;
   static constexpr int kLandStages = kFp8 ? kRawStages : kOpStages;  // stages the TMA fills
   static constexpr int kKBox = 64 * 128;
   static constexpr int kVBox = 128 * 128;
-  // A tile's scales are rewritten once its P has been consumed: K of tile J + k
-  // is converted after item 2 (J + k) - 1 - kOpStages was consumed, V of tile J
-  // is item 2 J + 2.
-  static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 4) / 2 : 0;
+  // A tile's scales are rewritten once its P has been consumed: among the items
+  // in their order, V of tile J is at most 2 J + kAhead + 1, K of tile J + k at
+  // least 2 (J + k) - kAhead, and an item is converted once the one kOpStages
+  // before it was consumed.
+  static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 2 * kAhead + 2) / 2 : 0;
+  static constexpr int kOutBytes = kTurns ? 8 * 4096 : 0;  // output rows on their way out, 4 KB a softmax warp
   static constexpr int kOpOff = kQBytes;
   static constexpr int kRawOff = kOpOff + kOpStages * kOpBytes;
-  static constexpr int kScaleOff = kRawOff + kRawStages * kRawBytes;  // float k[128], v[128], int vmax[4]
+  static constexpr int kOutOff = kRawOff + kRawStages * kRawBytes;
+  static constexpr int kScaleOff = kOutOff + kOutBytes;  // float k[128], v[128], int vmax[4]
   static constexpr int kScaleBuf = 2 * kTileN * 4 + 16;
   static constexpr int kFactorOff = kScaleOff + kScaleBufs * kScaleBuf;  // float[2][128], by segment parity
   static constexpr int kRedOff = kFactorOff + (kFp8 ? 2 * kTileM * 4 : 0);
-  static constexpr int kBarOff = kRedOff + 2 * kSoftmaxWarpgroups * kTileM * 4;
-  // q_ready, q_empty, rows[2], land_full[NL], land_empty[NR], op_full[NS],
-  // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, red[2], scale[NB]
-  static constexpr int kNumBars = 4 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs;
+  static constexpr int kBarOff = kRedOff + 4 * kTileM * 4;
+  // q_ready, q_empty, rows[2], o_free, s_free[2], land_full[NL], land_empty[NR], op_full[NS],
+  // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, ref[2], scale[NB]
+  static constexpr int kNumBars = 7 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
   static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
@@ -74,13 +96,63 @@ struct TilesSmem {
   static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
 };
 
-// The pages of sequences with tile units as bf16, page lb of sequence s at block
-// s * table_width + lb of `copy`, in the payload's layout.  Bound by HBM (1 byte
-// read, 2 written an element); a block takes the rows of one head of K or V of a
-// page at a time.
+// A warp's 32 rows (a lane each), O * inv_l of kCols TMEM columns from t_o, to
+// `dst` (NULL: not written), bf16 or fp32.  128 bytes of each row at a time turn
+// in 4 KB of shared memory, so that eight lanes store 128 bytes of one row (a
+// lane storing its own row touches 32 lines with every instruction: 3700 cycles
+// a unit).
+template <int kCols, bool kBf16, typename T>
+__device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, uint8_t* turn, int lane) {
+  constexpr int kStep = kBf16 ? 64 : 32;  // columns of 128 bytes
+  const uint32_t base = smem_u32(turn);
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += kStep) {
+#pragma unroll
+    for (int h = 0; h < kStep / 32; ++h) {
+      float o[32];
+      tmem_ld32(t_o + c + 32 * h, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] *= inv_l;
+#pragma unroll
+      for (int q = 0; q < (kBf16 ? 4 : 8); ++q) {
+        const uint4 v = kBf16 ? make_uint4(pack_bf16x2(o[(8 * q) & 31], o[(8 * q + 1) & 31]),
+                                           pack_bf16x2(o[(8 * q + 2) & 31], o[(8 * q + 3) & 31]),
+                                           pack_bf16x2(o[(8 * q + 4) & 31], o[(8 * q + 5) & 31]),
+                                           pack_bf16x2(o[(8 * q + 6) & 31], o[(8 * q + 7) & 31]))
+                              : make_uint4(__float_as_uint(o[4 * q]), __float_as_uint(o[4 * q + 1]),
+                                           __float_as_uint(o[4 * q + 2]), __float_as_uint(o[4 * q + 3]));
+        sts128(base + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4), v);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + lane / 8;
+      const unsigned long long at = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r);
+      const uint4 v = lds128(base + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+      if (at) reinterpret_cast<uint4*>(at + c * sizeof(T))[lane & 7] = v;
+    }
+    __syncwarp();
+  }
+}
+
+// How K and V tiles are copied.  A copy costs its issuer some 350 cycles
+// whatever its size (eight a tile held the kernel at 2900 cycles a tile, D = 256),
+// so one brings as many rows, and as many 64-element columns, as the pages allow.
+struct TileBoxes {
+  int k_rows, v_rows;  // rows of a copy: K up to 64, V up to 128
+  int all_cols;        // bf16: all 64-element columns in a copy (pages of a multiple of 64 tokens)
+};
+
+// The pages of sequences with tile units as bf16: sequence s is one block of
+// `copy`, [2][Hkv][copy_rows][D].  Bound by HBM (1 byte read, 2 written an
+// element); a thread block takes the rows of one head of K or V of a page at a
+// time.
 struct ExpandParams {
   ChunkParams c;
   __nv_bfloat16* copy;
+  int copy_rows;  // table_width * block_size, up to a multiple of 128
 };
 
 template <int D>
@@ -105,7 +177,8 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
     const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size;
     const uint4* codes = reinterpret_cast<const uint4*>(pool.data + src * D);
     const uint8_t* scales = pool.scales ? pool.scales + src : nullptr;
-    uint4* dst = reinterpret_cast<uint4*>(p.copy + (page * per_page + which) * pool.block_size * D);
+    uint4* dst = reinterpret_cast<uint4*>(
+        p.copy + ((static_cast<long long>(s) * per_page + which) * p.copy_rows + static_cast<long long>(lb) * pool.block_size) * D);
     for (int e0 = threadIdx.x; e0 < n * kPerRow; e0 += 4 * 256) {
       uint4 x[4];
       uint32_t sc[4];
@@ -135,7 +208,7 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
 template <int D, int kCache>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     chunk_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                       const int box_rows, const ChunkParams p) {
+                       const TileBoxes box, const ChunkParams p) {
   using L = TilesSmem<D, kCache>;
   constexpr bool kFp8 = L::kFp8;
   constexpr bool kScaled = kCache == kCacheScaled;
@@ -161,16 +234,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   // This CTA's row factors written, by segment parity (two: the converters may
   // be a segment ahead of a softmax warp that has not waited yet).
   auto bar_rows = [&](int s) { return bars + 16 + 8u * (s & 1); };
-  auto bar_land_full = [&](int s) { return bars + 8u * (4 + s); };
-  auto bar_land_empty = [&](int s) { return bars + 8u * (4 + NL + s); };
-  auto bar_op_full = [&](int s) { return bars + 8u * (4 + NL + NR + s); };
-  auto bar_op_empty = [&](int s) { return bars + 8u * (4 + NL + NR + NS + s); };
-  constexpr int kB2 = 4 + NL + NR + 2 * NS;
+  const uint32_t bar_o_free = bars + 32;  // leader: O of the segment read by every softmax warp of both CTAs
+  // Leader: scores of the buffer in registers (kTurns: its next QK^T may be issued).
+  auto bar_s_free = [&](int b) { return bars + 40 + 8u * b; };
+  auto bar_land_full = [&](int s) { return bars + 8u * (7 + s); };
+  auto bar_land_empty = [&](int s) { return bars + 8u * (7 + NL + s); };
+  auto bar_op_full = [&](int s) { return bars + 8u * (7 + NL + NR + s); };
+  auto bar_op_empty = [&](int s) { return bars + 8u * (7 + NL + NR + NS + s); };
+  constexpr int kB2 = 7 + NL + NR + 2 * NS;
   auto bar_s_full = [&](int b) { return bars + 8u * (kB2 + b); };
   auto bar_p_full = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
   auto bar_o = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
   const uint32_t bar_td = bars + 8u * (kB2 + 6);
-  auto bar_red = [&](int b) { return bars + 8u * (kB2 + 7 + b); };
+  auto bar_ref = [&](int b) { return bars + 8u * (kB2 + 7 + b); };
   auto bar_scale = [&](int b) { return bars + 8u * (kB2 + 9 + b); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
@@ -195,11 +271,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_s_full(b), 1);
-      mbar_init(bar_p_full(b), 2 * kSoftmaxThreads / 32);  // one arrive per softmax warp of both CTAs
+      // One arrive per softmax warp that does the tile, of both CTAs.
+      mbar_init(bar_p_full(b), L::kTurns ? 2 * 4 : 2 * 8);
+      mbar_init(bar_s_free(b), 2 * 4);
       mbar_init(bar_o(b), 1);
-      mbar_init(bar_red(b), kSoftmaxThreads);
+      mbar_init(bar_ref(b), L::kTurns ? 128 : 256);
     }
     for (int b = 0; b < NB; ++b) mbar_init(bar_scale(b), kTilesConvWarps);
+    mbar_init(bar_o_free, 2 * 8);
     mbar_init(bar_td, 1);
     *abort_flag = 0;
     plan.err = 0;
@@ -228,78 +307,182 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       if (!body(un, kt0, kt1)) return false;
     return true;
   };
+  // The items of a segment in the order of their loads, conversions and MMAs:
+  // K of the first kAhead tiles, then (K of tile j + kAhead, V of tile j).
+  auto for_each_item = [&](int kt0, int kt1, auto&& body) -> bool {
+    for (int kt = kt0 - L::kAhead; kt < kt1; ++kt) {
+      if (kt + L::kAhead < kt1 && !body(false, kt + L::kAhead)) return false;
+      if (kt >= kt0 && !body(true, kt)) return false;
+    }
+    return true;
+  };
+  // V's 64-element columns in an operand stage: each of 128 rows, or (copied 64
+  // rows at a time) all columns of keys 0-63, then of 64-127.
+  const bool v_halves = !kFp8 && box.all_cols && box.v_rows == 64;
+  const uint32_t v_col = v_halves ? L::kVBox / 2 : L::kVBox;
+  const uint32_t v_half = v_halves ? (D / 128) * (L::kVBox / 2) - 64 * 128 : 0;  // beyond 64 rows
   // Keys of tile kt that the sequence has (may be 0 when it has none at all).
   auto tile_valid = [&](const ChunkUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
 
-  if (warp == kProducerWarp) {
-    // ------------------------------------------------------ TMA producer --
-    if (lane == 0) {
+  if (warp >= kProducerWarp && warp < kTilesConvWarp0) {
+    setmaxnreg_dec<kTilesControlRegs>();
+    // Both roles walk with the whole warp and issue from one elected lane: in
+    // code that only one lane runs, every operand of an MMA or a copy takes its
+    // way through a vector register (100 cycles an MMA; the tensor cores waited).
+    const bool elected = elect_one();
+    if (warp == kProducerWarp) {
+      // ---------------------------------------------------- TMA producer --
       uint32_t c = 0;
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
+      if (elected) {
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+      }
       int seq = -1, cached_lb = -1, cached_page = 0;
       auto page_of = [&](const ChunkUnit& un, int lb) -> int {
         if (un.seq == seq && lb == cached_lb) return cached_page;
         int b = lb >= p.batch.table_width ? -1
                 : p.batch.tables          ? p.batch.tables[un.seq * p.batch.table_stride + lb]
-                                          : un.seq * p.batch.table_width + lb;  // the expanded copy
+                                          : un.seq;  // the expanded copy
         if (b < 0 || b >= p.pool.blocks) {  // reported; block 0 keeps the load in bounds
-          atomicCAS(err, 0, kErrBlockTable);
+          if (elected) atomicCAS(err, 0, kErrBlockTable);
           b = 0;
         }
         seq = un.seq;
         cached_lb = lb;
         return cached_page = b;
       };
-      // Boxes of [key0, key0 + n) of K or V of one head; row 0 of `dst` is key0.
+      // Rows [key0, key0 + n) of K or V of one head; row 0 of `dst` is key0.
       auto load_rows = [&](const ChunkUnit& un, bool is_v, int key0, int n, uint32_t dst, uint32_t full) {
-        for (int r = 0; r < n; r += box_rows) {
+        const int step = is_v ? box.v_rows : box.k_rows;
+        for (int r = 0; r < n; r += step) {
           const int key = key0 + r;
           const int pg = page_of(un, key / p.pool.block_size), at = key % p.pool.block_size;
+          if (!elected) continue;
           if (kFp8) {
             if (is_v)
               tma_load_5d(dst + r * (D / 2), &tm_v, static_cast<int>(rank) * (D / 2), at, un.head, 1, pg, full);
             else
               tma_load_5d(dst + r * D, &tm_k, 0, at, un.head, 0, pg, full);
+          } else if (box.all_cols) {  // {64 elements, rows, columns, head, 2 page + K/V}
+            if (is_v)
+              tma_load_5d(dst + r * D, &tm_v, 0, at, static_cast<int>(rank) * (D / 128), un.head, 2 * pg + 1, full);
+            else
+              tma_load_5d(dst, &tm_k, 0, at, 0, un.head, 2 * pg, full);
           } else if (is_v) {
             for (int b = 0; b < D / 128; ++b)
-              tma_load_5d(dst + b * L::kVBox + r * 128, &tm_v, static_cast<int>(rank) * (D / 2) + b * 64, at, un.head, 1,
-                          pg, full);
+              tma_load_5d(dst + b * L::kVBox + r * 128, &tm_v, 0, at, static_cast<int>(rank) * (D / 128) + b, un.head,
+                          2 * pg + 1, full);
           } else {
             for (int b = 0; b < D / 64; ++b)
-              tma_load_5d(dst + b * L::kKBox + r * 128, &tm_k, b * 64, at, un.head, 0, pg, full);
+              tma_load_5d(dst + b * L::kKBox + r * 128, &tm_k, 0, at, b, un.head, 2 * pg, full);
           }
         }
       };
       auto issue = [&](const ChunkUnit& un, bool is_v, int kt) {
         const int st = c % NL;
         const uint32_t empty = kFp8 ? bar_land_empty(st) : bar_op_empty(st);
-        if (!mbar_wait(empty, ((c / NL) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty)) return false;
+        if (!__all_sync(0xffffffffu, mbar_wait(empty, ((c / NL) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty)))
+          return false;
         const uint32_t dst = kFp8 ? sRaw + st * L::kRawBytes : sOp + st * L::kOpBytes;
         const int off = is_v ? 0 : 64 * static_cast<int>(rank), most = is_v ? 128 : 64;
         const int n = min(most, max(0, tile_valid(un, kt) - off));
-        const int rows = (n + box_rows - 1) / box_rows * box_rows;
-        mbar_arrive_expect_tx(bar_land_full(st), rows * (is_v ? D / 2 : D) * (kFp8 ? 1 : 2));
+        const int step = is_v ? box.v_rows : box.k_rows;
+        const int rows = (n + step - 1) / step * step;
+        if (elected) mbar_arrive_expect_tx(bar_land_full(st), rows * (is_v ? D / 2 : D) * (kFp8 ? 1 : 2));
         load_rows(un, is_v, kt * kTileN + off, n, dst, bar_land_full(st));
         ++c;
         return true;
       };
-      // Item order = converter and MMA consumption order: per segment K_0,
-      // then (K_{j+1}, V_j) per tile.
       const bool ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
-        if (!issue(un, false, kt0)) return false;
-        for (int kt = kt0; kt < kt1; ++kt) {
-          if (kt + 1 < kt1 && !issue(un, false, kt + 1)) return false;
-          if (!issue(un, true, kt)) return false;
-        }
-        return true;
+        return for_each_item(kt0, kt1, [&](bool is_v, int kt) { return issue(un, is_v, kt); });
       });
-      if (!ok)  // let this CTA's copies still in flight land before it exits
+      if (!ok && elected)  // let this CTA's copies still in flight land before it exits
         for (uint32_t i = (c > (uint32_t)NL ? c - NL : 0); i < c; ++i)
           mbar_wait_teardown(bar_land_full(i % NL), (i / NL) & 1u);
     }
+    if (warp == kMmaWarp && leader) {
+      // ------------------------------------------ MMA issuer (leader only) --
+      constexpr uint32_t idesc_qk =
+          kFp8 ? make_idesc_f16(kUnitRows, kTileN, false, false) : make_idesc_bf16(kUnitRows, kTileN, false, false);
+      constexpr uint32_t idesc_pv =
+          kFp8 ? make_idesc_f16(kUnitRows, D, false, true) : make_idesc_bf16(kUnitRows, D, false, true);
+      uint32_t c = 0;
+      uint32_t J = 0;  // tiles of all earlier segments
+      int segs = 0;
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+      };
+      // Descriptors of the first k step; the others differ in the address alone.
+      const uint64_t q_desc = make_sw128_desc(sQ, 16, 1024);
+      const uint64_t k_desc = make_sw128_desc(sOp, 16, 1024);
+      const uint64_t v_desc = make_sw128_desc(sOp, v_col, 1024);
+      auto qk = [&](uint32_t jg) {
+        const uint32_t s_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
+        const int st = c % NS;
+        if (L::kTurns && jg >= 2 && !wait(bar_s_free(jg & 1), ((jg - 2) >> 1) & 1u, kErrWaitSFull)) return false;
+        if (!wait(bar_op_full(st), (c / NS) & 1u, kErrWaitKvFull)) return false;
+        tc_fence_after();
+        const uint64_t kd = k_desc + static_cast<uint32_t>(st) * (L::kOpBytes >> 4);
+        if (elected) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_ss_pair(s_tmem, q_desc + (((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4),
+                         kd + (((kk / 4) * L::kKBox + (kk % 4) * 32) >> 4), idesc_qk, kk != 0 ? 1u : 0u);
+          umma_commit_pair(bar_op_empty(st), kChunkBothCtas);
+          umma_commit_pair(bar_s_full(jg & 1), kChunkBothCtas);
+        }
+        ++c;
+        return true;
+      };
+      auto pv = [&](uint32_t jg, bool first, int seg) {
+        // O of the previous segment has been read out.
+        if (first && seg > 0 && !wait(bar_o_free, (seg - 1) & 1u, kErrWaitODone)) return false;
+        if (!wait(bar_p_full(jg & 1), (jg >> 1) & 1u, kErrWaitPFull)) return false;
+        const int st = c % NS;
+        if (!wait(bar_op_full(st), (c / NS) & 1u, kErrWaitKvFull)) return false;
+        tc_fence_after();
+        const uint32_t p_tmem = tmem + (L::kTurns ? kTurnsP + (jg & 1) * (kTileN / 2) : kTmemS0 + (jg & 1) * kTileN);
+        const uint64_t vd = v_desc + static_cast<uint32_t>(st) * (L::kOpBytes >> 4);
+        const uint64_t vd2 = vd + (v_half >> 4);
+        if (elected) {
+#pragma unroll
+          for (int kk = 0; kk < kTileN / 16; ++kk) {
+            // A = P (kTurns: its own TMEM columns; else over S, each warpgroup's
+            // in its own half), B = V half, MN-major: 64-dim chunks v_col apart,
+            // 8-key groups 1 KB apart.
+            umma_ts_pair(tmem, p_tmem + kk * 8 + (!L::kTurns && kk >= 4 ? 32 : 0), (kk >= 4 ? vd2 : vd) + kk * (2048 >> 4),
+                         idesc_pv, (!first || kk > 0) ? 1u : 0u);
+          }
+          umma_commit_pair(bar_op_empty(st), kChunkBothCtas);
+          umma_commit_pair(bar_o(jg & 1), kChunkBothCtas);
+        }
+        ++c;
+        return true;
+      };
+      for_each_segment([&](const ChunkUnit&, int kt0, int kt1) -> bool {
+        const uint32_t n = static_cast<uint32_t>(kt1 - kt0);
+        if (!wait(bar_q_ready, segs & 1u, kErrWaitQ)) return false;
+        tc_fence_after();
+        const bool ok = for_each_item(0, static_cast<int>(n), [&](bool is_v, int j) {
+          if (is_v) return pv(J + j, j == 0, segs);
+          if (!qk(J + j)) return false;
+          if (j + 1 == static_cast<int>(n) && elected) umma_commit_pair(bar_q_empty, kChunkBothCtas);  // the segment's last
+          return true;
+        });
+        if (!ok) return false;
+        J += n;
+        ++segs;
+        return true;
+      });
+      // Drain: completes when every MMA issued above has.
+      if (elected) {
+        umma_commit_pair(bar_td, kChunkLeader);
+        mbar_wait_teardown(bar_td, 0);
+      }
+    }
     __syncwarp();
   } else if (warp >= kTilesConvWarp0) {
+    setmaxnreg_dec<kTilesConvRegs>();
     // ------------------------------- Q gather, e4m3 -> f16, V past the end --
     const int ct = threadIdx.x - kTilesConvWarp0 * 32;
     const int cw = warp - kTilesConvWarp0;
@@ -377,7 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t op = sOp + os * L::kOpBytes;
           for (int i = max(0, valid) * 8 + ct; i < kTileN * 8; i += kTilesConvThreads)
-            for (int b = 0; b < D / 128; ++b) sts128(op + b * L::kVBox + i * 16, zero);
+            for (int b = 0; b < D / 128; ++b) sts128(op + b * v_col + (i >= 64 * 8 ? v_half : 0) + i * 16, zero);
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -437,94 +620,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         mbar_arrive_remote(mapa_shared(bar_q_ready, 0));
       }
       ++segs;
-      if (!item(un, false, kt0)) return false;
-      for (int kt = kt0; kt < kt1; ++kt) {
-        if (kt + 1 < kt1 && !item(un, false, kt + 1)) return false;
-        if (!item(un, true, kt)) return false;
-      }
-      return true;
+      return for_each_item(kt0, kt1, [&](bool is_v, int kt) { return item(un, is_v, kt); });
     });
     __syncwarp();
-  } else if (warp == kMmaWarp) {
-    // --------------------------------------------- MMA issuer (leader only) --
-    if (leader && lane == 0) {
-      constexpr uint32_t idesc_qk =
-          kFp8 ? make_idesc_f16(kUnitRows, kTileN, false, false) : make_idesc_bf16(kUnitRows, kTileN, false, false);
-      constexpr uint32_t idesc_pv =
-          kFp8 ? make_idesc_f16(kUnitRows, D, false, true) : make_idesc_bf16(kUnitRows, D, false, true);
-      uint32_t c = 0;
-      uint32_t J = 0;  // tiles of all earlier segments
-      int segs = 0;
-      auto qk = [&](uint32_t jg) {
-        const uint32_t s_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
-        const int st = c % NS;
-        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, err, kErrWaitKvFull)) return false;
-        tc_fence_after();
-        const uint32_t kbase = sOp + st * L::kOpBytes;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t qa = sQ + (kk / 4) * kBoxBytes + (kk % 4) * 32;
-          const uint32_t kb = kbase + (kk / 4) * L::kKBox + (kk % 4) * 32;
-          umma_ss_pair(s_tmem, make_sw128_desc(qa, 16, 1024), make_sw128_desc(kb, 16, 1024), idesc_qk,
-                       kk != 0 ? 1u : 0u);
-        }
-        umma_commit_pair(bar_op_empty(st), kChunkBothCtas);
-        ++c;
-        umma_commit_pair(bar_s_full(jg & 1), kChunkBothCtas);
-        return true;
-      };
-      auto pv = [&](uint32_t jg, bool first) {
-        if (!mbar_wait(bar_p_full(jg & 1), (jg >> 1) & 1u, abort_flag, err, kErrWaitPFull)) return false;
-        const int st = c % NS;
-        if (!mbar_wait(bar_op_full(st), (c / NS) & 1u, abort_flag, err, kErrWaitKvFull)) return false;
-        tc_fence_after();
-        const uint32_t p_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
-        const uint32_t vbase = sOp + st * L::kOpBytes;
-#pragma unroll
-        for (int kk = 0; kk < kTileN / 16; ++kk) {
-          // A = P (TMEM columns of the S buffer, each warpgroup's in its own
-          // half), B = V half, MN-major: 64-dim chunks 16 KB apart, 8-key
-          // groups 1 KB apart.
-          const uint32_t a_cols = kk * 8 + (kk >= 4 ? 32 : 0);
-          umma_ts_pair(tmem, p_tmem + a_cols, make_sw128_desc(vbase + kk * 2048, L::kVBox, 1024), idesc_pv,
-                       (!first || kk > 0) ? 1u : 0u);
-        }
-        umma_commit_pair(bar_op_empty(st), kChunkBothCtas);
-        ++c;
-        umma_commit_pair(bar_o(jg & 1), kChunkBothCtas);
-        return true;
-      };
-      for_each_segment([&](const ChunkUnit&, int kt0, int kt1) -> bool {
-        const uint32_t n = static_cast<uint32_t>(kt1 - kt0);
-        // (O of the previous segment has been read out: its softmax warps
-        // release P_0 of this segment only after their epilogue.)
-        if (!mbar_wait(bar_q_ready, segs & 1u, abort_flag, err, kErrWaitQ)) return false;
-        tc_fence_after();
-        if (!qk(J)) return false;
-        if (n == 1) umma_commit_pair(bar_q_empty, kChunkBothCtas);
-        for (uint32_t j = 0; j < n; ++j) {
-          if (j + 1 < n) {
-            if (!qk(J + j + 1)) return false;
-            if (j + 2 == n) umma_commit_pair(bar_q_empty, kChunkBothCtas);  // last QK^T of the segment
-          }
-          if (!pv(J + j, j == 0)) return false;
-        }
-        J += n;
-        ++segs;
-        return true;
-      });
-      // Drain: completes when every MMA issued above has.
-      umma_commit_pair(bar_td, kChunkLeader);
-      mbar_wait_teardown(bar_td, 0);
-    }
-    __syncwarp();
   } else {
+    setmaxnreg_inc<kTilesSoftmaxRegs>();
     // ---------------------------------------- softmax / correction / epilogue --
-    constexpr int kHalfKeys = kTileN / kSoftmaxWarpgroups;  // 64
-    constexpr int kOCols = D / kSoftmaxWarpgroups;
+    constexpr int kOCols = D / 2;
+    constexpr int kKeys = L::kTurns ? kTileN : kTileN / 2;  // a thread's keys of a tile
     const int wg = warp >> 2;
     const int row = threadIdx.x & (kTileM - 1);  // == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // kTurns: refs[2][128], each row's reference after a tile, by the tile's
+    // parity; else the halves' maxima [tile parity][2][128].  At the end refs is
+    // each warpgroup's last reference and sums its l.
+    float* refs = red;
+    float* sums = red + 2 * kTileM;
     uint32_t J = 0;
     int segs = 0;
     // The leader keeps the pair's record.
@@ -538,40 +649,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const bool live = r < un.rows;
       const int at = un.row0 + (live ? r : un.rows - 1);
       const int pos = un.kvlen - un.qlen + at / p.group;  // last key this row sees
-      const int n = kt1 - kt0;
+      const uint32_t Jend = J + (kt1 - kt0);
       float rf = p.scale_log2;
       if (kFp8) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(segs), (segs >> 1) & 1u, abort_flag, err, kErrWaitQ));
         if (ok) rf = factors[(segs & 1) * kTileM + row];
       }
       ++segs;
-      float m_ref = -INFINITY;  // log2 units, V's exponents included
-      float l = 0.f;
-      for (int j = 0; j < n && ok; ++j) {
-        const uint32_t jg = J + j;
-        const int b = jg & 1;
-        const int key0 = (kt0 + j) * kTileN + wg * kHalfKeys;
-        const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
-        float ev = 0.f;
+      float m = -INFINITY;  // (this warpgroup's last) reference: log2 units, V's exponents included
+      float l = 0.f;        // its keys' weights over 2^m
+
+      // This thread's scores of tile jg: loaded, K's scales applied, keys past
+      // the row's position at -inf.  `ev` gets the tile's largest V exponent.
+      const uint32_t first_key = L::kTurns ? 0 : wg * kKeys;
+      auto scores = [&](uint32_t jg, float (&s)[kKeys], float& ev) -> bool {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_s_full(jg & 1), (jg >> 1) & 1u, abort_flag, err, kErrWaitSFull)))
+          return false;
+        tc_fence_after();
+        const uint32_t t_s = t_row + kTmemS0 + (jg & 1) * kTileN + first_key;
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
+        tmem_wait_ld();
+        if (L::kTurns) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(mapa_shared(bar_s_free(jg & 1), 0));
+        }
+        ev = 0.f;
         if (kScaled) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_scale(jg % (NB ? NB : 1)), (jg / (NB ? NB : 1)) & 1u, abort_flag,
-                                                 err, kErrWaitKvFull));
-          if (!ok) break;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_scale(jg % (NB ? NB : 1)), (jg / (NB ? NB : 1)) & 1u, abort_flag,
+                                                 err, kErrWaitKvFull)))
+            return false;
+          const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
           const int4 vm = *reinterpret_cast<const int4*>(sf + 2 * kTileN);
           ev = static_cast<float>(max(max(vm.x, vm.y), max(vm.z, vm.w)) - 127);
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitSFull));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t t_s = t_row + kTmemS0 + b * kTileN + wg * kHalfKeys;
-        float s[kHalfKeys];
+          const float4* ks = reinterpret_cast<const float4*>(sf + first_key);
 #pragma unroll
-        for (int c = 0; c < kHalfKeys / 32; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
-        tmem_wait_ld();
-        if (kScaled) {
-          const float4* ks = reinterpret_cast<const float4*>(sf + wg * kHalfKeys);
-#pragma unroll
-          for (int i = 0; i < kHalfKeys / 4; ++i) {
+          for (int i = 0; i < kKeys / 4; ++i) {
             const float4 k4 = ks[i];
             s[4 * i] *= k4.x;
             s[4 * i + 1] *= k4.y;
@@ -579,107 +693,180 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             s[4 * i + 3] *= k4.w;
           }
         }
-        const int visible = pos + 1 - key0;
-        if (visible < kHalfKeys) {
+        const int visible = pos + 1 - (kt0 + static_cast<int>(jg - J)) * kTileN - static_cast<int>(first_key);
+        if (visible < kKeys) {
 #pragma unroll
-          for (int i = 0; i < kHalfKeys; ++i)
+          for (int i = 0; i < kKeys; ++i)
             if (i >= visible) s[i] = -INFINITY;
         }
-        const float pmax = row_max(s);
-        red[(b * kSoftmaxWarpgroups + wg) * kTileM + row] = pmax;
-        mbar_arrive(bar_red(b));
-        // Pass 0 (tiles after the first): speculative P with the current
-        // reference, before the other half's maximum is known.  Pass 1:
-        // exchange the half maxima; P is recomputed only when some row's
-        // moved past the threshold.
-        float tile_sum = 0.f;
-        float alpha = 1.f;
-        bool redo = false;
-#pragma unroll 1
-        for (int pass = j > 0 ? 0 : 1; pass < 2; ++pass) {
-          if (pass == 1) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar_red(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
-            if (!ok) break;
-            const float tmax =
-                fmaxf(pmax, red[(b * kSoftmaxWarpgroups + (wg ^ 1)) * kTileM + row]) * rf + ev;
-            const bool need = tmax > m_ref + kRescaleThreshold;  // from its start as soon as a key is seen
-            redo = __any_sync(0xffffffffu, need) || j == 0;
-            if (need) {
-              alpha = ex2_approx(m_ref - tmax);  // 0 from the start
-              m_ref = tmax;
-              l *= alpha;
-            }
-            if (!redo) break;
-          }
-          // P over this warpgroup's S columns; a row that has seen nothing yet
-          // has only -inf scores.
-          const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-          float sum0 = 0.f, sum1 = 0.f;
+        return true;
+      };
+      // P = 2^(s rf - ref), times V's scales, into TMEM columns [t_p, t_p + kKeys
+      // / 2); returns the sum of 2^(s rf - ref).  A row that has seen nothing yet
+      // has only -inf scores.
+      auto probs = [&](uint32_t jg, const float (&s)[kKeys], float ref, uint32_t t_p) -> float {
+        const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
+        const float neg = ref == -INFINITY ? 0.f : -ref;
+        float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-          for (int c2 = 0; c2 < kHalfKeys / 32; ++c2) {
-            uint32_t pk[16];
+        for (int c2 = 0; c2 < kKeys / 32; ++c2) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float q0 = ex2_approx(fmaf(s[c2 * 32 + 2 * i], rf, neg));
-              float q1 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 1], rf, neg));
-              float q2 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 2], rf, neg));
-              float q3 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 3], rf, neg));
-              sum0 += q0 + q2;
-              sum1 += q1 + q3;
-              if (kScaled) {
-                const float4 v4 = *reinterpret_cast<const float4*>(sf + kTileN + wg * kHalfKeys + c2 * 32 + 2 * i);
-                q0 *= v4.x;
-                q1 *= v4.y;
-                q2 *= v4.z;
-                q3 *= v4.w;
-              }
-              pk[i] = kFp8 ? pack_f16x2(q0, q1) : pack_bf16x2(q0, q1);
-              pk[i + 1] = kFp8 ? pack_f16x2(q2, q3) : pack_bf16x2(q2, q3);
+          for (int i = 0; i < 16; i += 2) {
+            float q0 = ex2_approx(fmaf(s[c2 * 32 + 2 * i], rf, neg));
+            float q1 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 1], rf, neg));
+            float q2 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 2], rf, neg));
+            float q3 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 3], rf, neg));
+            sum0 += q0 + q2;
+            sum1 += q1 + q3;
+            if (kScaled) {
+              const float4 v4 = *reinterpret_cast<const float4*>(sf + kTileN + first_key + c2 * 32 + 2 * i);
+              q0 *= v4.x;
+              q1 *= v4.y;
+              q2 *= v4.z;
+              q3 *= v4.w;
             }
-            tmem_st16(t_s + c2 * 16, pk);
+            pk[i] = kFp8 ? pack_f16x2(q0, q1) : pack_bf16x2(q0, q1);
+            pk[i + 1] = kFp8 ? pack_f16x2(q2, q3) : pack_bf16x2(q2, q3);
           }
-          tmem_wait_st();
-          tile_sum = sum0 + sum1;
+          tmem_st16(t_p + c2 * 16, pk);
         }
-        if (!ok) break;
-        l += tile_sum;
-        if (j > 0 && redo) {
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
-          if (!ok) break;
-          tc_fence_after();
-          rescale_o<kOCols>(t_row + wg * kOCols, alpha);
-        }
+        tmem_wait_st();
+        return sum0 + sum1;
+      };
+      auto release = [&](uint32_t jg) {  // tile jg's P is in place
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(mapa_shared(bar_p_full(b), 0));
+        if (lane == 0) mbar_arrive_remote(mapa_shared(bar_p_full(jg & 1), 0));
+      };
+      // The reference moves when a tile's largest weight would pass 2^8 (and
+      // from its start, as soon as a key is seen); O of the tiles before goes
+      // over to the new one once their last product is in it.
+      if constexpr (L::kTurns) {
+        for (uint32_t jg = J + ((J ^ wg) & 1u); jg < Jend && ok; jg += 2) {
+          float s[kKeys], ev;
+          ok = scores(jg, s, ev);
+          if (!ok) break;
+          const float tmax = row_max(s) * rf + ev;
+          float before = -INFINITY;
+          if (jg > J) {
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(bar_ref(wg ^ 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitRed));
+            if (!ok) break;
+            before = refs[(wg ^ 1) * kTileM + row];
+          }
+          const bool need = tmax > before + kRescaleThreshold;
+          const float ref = need ? tmax : before;
+          refs[wg * kTileM + row] = ref;
+          mbar_arrive(bar_ref(wg));
+          if (ref != m) {  // it moved since this warpgroup's last tile
+            l *= ex2_approx(m - ref);
+            m = ref;
+          }
+          // P's columns are free once the product before last is done.
+          if (jg >= 2) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_o(wg), ((jg - 2) >> 1) & 1u, abort_flag, err, kErrWaitODone));
+            if (!ok) break;
+            tc_fence_after();
+          }
+          l += probs(jg, s, ref, t_row + kTurnsP + wg * (kTileN / 2));
+          if (jg > J && __any_sync(0xffffffffu, need)) {
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(bar_o(wg ^ 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
+            if (!ok) break;
+            tc_fence_after();
+            rescale_o<D>(t_row, need ? ex2_approx(before - ref) : 1.f);
+          }
+          release(jg);
+        }
+      } else {
+        for (uint32_t jg = J; jg < Jend && ok; ++jg) {
+          const int b = jg & 1;
+          float s[kKeys], ev;
+          ok = scores(jg, s, ev);
+          if (!ok) break;
+          const float pmax = row_max(s);
+          red[(b * 2 + wg) * kTileM + row] = pmax;
+          mbar_arrive(bar_ref(b));
+          // Pass 0 (tiles after the first): speculative P with the current
+          // reference, before the other half's maximum is known.  Pass 1:
+          // exchange the half maxima; P is recomputed only when some row's
+          // moved past the threshold.
+          float tile_sum = 0.f;
+          float alpha = 1.f;
+          bool redo = false;
+#pragma unroll 1
+          for (int pass = jg > J ? 0 : 1; pass < 2; ++pass) {
+            if (pass == 1) {
+              ok = __all_sync(0xffffffffu, mbar_wait(bar_ref(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
+              if (!ok) break;
+              const float tmax = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]) * rf + ev;
+              const bool need = tmax > m + kRescaleThreshold;
+              redo = __any_sync(0xffffffffu, need) || jg == J;
+              if (need) {
+                alpha = ex2_approx(m - tmax);  // 0 from the start
+                m = tmax;
+                l *= alpha;
+              }
+              if (!redo) break;
+            }
+            tile_sum = probs(jg, s, m, t_row + kTmemS0 + b * kTileN + wg * kKeys);
+          }
+          if (!ok) break;
+          l += tile_sum;
+          if (jg > J && redo) {
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
+            if (!ok) break;
+            tc_fence_after();
+            rescale_o<kOCols>(t_row + wg * kOCols, alpha);
+          }
+          release(jg);
+        }
       }
       if (ok) {
-        const uint32_t jl = J + n - 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
+        // The last product.  A warpgroup that did not do its tile has not seen
+        // the one before on that barrier complete, and its parity alone could
+        // not tell the two apart: that one first.
+        const uint32_t jl = Jend - 1;
+        if (jl >= 2) ok = mbar_wait(bar_o(jl & 1), ((jl >> 1) & 1u) ^ 1u, abort_flag, err, kErrWaitODone);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
       }
+      refs[wg * kTileM + row] = m;  // (both read by the other warpgroup only below)
+      sums[wg * kTileM + row] = l;
       ok = named_bar_and(1, kSoftmaxThreads, ok && (*abort_flag == 0));
       if (!ok) return false;
-      J += n;
+      J = Jend;
       tc_fence_after();
-      red[wg * kTileM + row] = l;
-      named_bar_sync(2, kSoftmaxThreads);
-      const float l_tot = l + red[(wg ^ 1) * kTileM + row];
-      // Both halves read: the next segment may reuse the exchange slots.
+      // O carries the last reference, the larger of the two.
+      const float m_other = refs[(wg ^ 1) * kTileM + row], l_other = sums[(wg ^ 1) * kTileM + row];
+      const float top = fmaxf(m, m_other);
+      const float l_tot = (m == top ? l : l * ex2_approx(m - top)) +
+                          (m_other == top ? l_other : l_other * ex2_approx(m_other - top));
+      // Both read: the next segment may reuse the slots.
       named_bar_sync(2, kSoftmaxThreads);
       const float inv_l = l_tot == 0.f ? 0.f : 1.f / l_tot;  // no key seen: zeros
       const int slot = part_slot(un, kt0, kt1, pair);
-      if (slot < 0) {
-        store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l,
-                             p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
-                                 static_cast<long long>(un.q0 + at / p.group) * p.out_row + wg * kOCols,
-                             live);
+      __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
+                           static_cast<long long>(un.q0 + at / p.group) * p.out_row + wg * kOCols;
+      const long long pr = static_cast<long long>(slot) * kUnitRows + r;
+      if (slot >= 0 && live && wg == 0)
+        p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __log2f(l_tot);
+      if constexpr (L::kTurns) {
+        uint8_t* turn = smem + L::kOutOff + warp * 4096;
+        if (slot < 0)
+          store_rows<kOCols, true>(t_row + wg * kOCols, inv_l, live ? out : nullptr, turn, lane);
+        else
+          store_rows<kOCols, false>(t_row + wg * kOCols, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr,
+                                    turn, lane);
+      } else if (slot < 0) {
+        store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l, out, live);
       } else {
-        const long long pr = static_cast<long long>(slot) * kUnitRows + r;
         store_o_partial<kOCols>(t_row + wg * kOCols, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
-        if (live && wg == 0)
-          p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (m_ref == -INFINITY ? 0.f : m_ref) + __log2f(l_tot);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(mapa_shared(bar_o_free, 0));
       return true;
     });
     if (keeps && !done) clear_record(rec);  // after a failure nothing is merged

@@ -132,6 +132,11 @@ constexpr int64_t kExpandBytes = int64_t(1) << 30;
 
 bool has_tiles(int32_t max_chunk, int32_t group) { return static_cast<int64_t>(max_chunk) * group > pcp::kSmallRows; }
 
+// Rows of a sequence in the copy: what its table holds, in whole key tiles.
+int copy_rows(int32_t block_size, int32_t table_width) {
+  return static_cast<int>(ceil_div(static_cast<int64_t>(block_size) * table_width, 128) * 128);
+}
+
 ChunkLayout chunk_layout(const pcp_pool_t& pool, int32_t group, int32_t seqs, int32_t table_width, int32_t max_chunk) {
   ChunkLayout w{};
   const int32_t head_dim = pool.head_dim;
@@ -148,11 +153,11 @@ ChunkLayout chunk_layout(const pcp_pool_t& pool, int32_t group, int32_t seqs, in
   w.small_lse = put(size_t(2) * kCtas * pcp::kSmallRows * 4);
   w.tile_o = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * head_dim * 4 : 0);
   w.tile_lse = put(tiles ? size_t(2) * kPairs * pcp::kUnitRows * 4 : 0);
-  const int64_t page = int64_t(2) * pool.num_kv_heads * pool.block_size * head_dim * 2;
-  const int64_t pages = static_cast<int64_t>(seqs) * table_width;
+  const int64_t row = int64_t(2) * pool.num_kv_heads * head_dim * 2 * seqs;  // of every sequence
   w.expand = tiles && pool.kv_dtype == PCP_KV_E4M3 && static_cast<int64_t>(max_chunk) * group >= kExpandRows &&
-             pages > 0 && pages <= kExpandBytes / page;
-  w.copy = put(w.expand ? static_cast<size_t>(pages * page) : 0);
+             table_width > 0 && row > 0 &&
+             static_cast<int64_t>(table_width) * pool.block_size <= kExpandBytes / row - 128;
+  w.copy = put(w.expand ? static_cast<size_t>(row * copy_rows(pool.block_size, table_width)) : 0);
   w.bytes = at;
   return w;
 }
@@ -196,29 +201,27 @@ int encode(CUtensorMap* tm, CUtensorMapDataType type, int rank, void* base, cons
   return PCP_OK;
 }
 
-// Cache blocks [blocks][2][Hkv][bs][D] as a 5-D tensor {D, bs, Hkv, K/V,
-// blocks}; boxes of box_x elements x box_rows rows of one head of K or V of one
-// block.
-int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t box_rows, bool swizzle) {
-  const bool bf16 = p.kv_dtype == PCP_KV_BF16;
-  const uint64_t D = p.head_dim, bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1;
+// e4m3 cache blocks [blocks][2][Hkv][bs][D] as a 5-D tensor {D, bs, Hkv, K/V,
+// blocks}; boxes of box_x bytes x box_rows rows of one head of K or V of one
+// block, not swizzled.
+int make_pool_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_x, uint32_t box_rows) {
+  const uint64_t D = p.head_dim, bs = p.block_size, H = p.num_kv_heads;
   const cuuint64_t dims[5] = {D, bs, H, 2, static_cast<cuuint64_t>(p.blocks)};
-  const cuuint64_t strides[4] = {D * elt, bs * D * elt, H * bs * D * elt, 2 * H * bs * D * elt};
+  const cuuint64_t strides[4] = {D, bs * D, H * bs * D, 2 * H * bs * D};
   const cuuint32_t box[5] = {box_x, box_rows, 1, 1, 1};
-  return encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims, strides,
-                box, swizzle);
+  return encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims, strides, box, false);
 }
 
-// The same blocks as {128 bytes, bs, 128-byte columns, Hkv, 2 * blocks}: one
-// box is box_rows whole rows of K and of V of one head, each 128-byte column of
-// them in the 128-byte swizzle.
-int make_rows_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows) {
+// Cache blocks as {128 bytes, bs, 128-byte columns, Hkv, 2 * blocks}: a box is
+// box_cols columns of box_rows rows of one head, of K or V or (box_kv 2) both,
+// each column in the 128-byte swizzle.
+int make_rows_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows, uint32_t box_cols, uint32_t box_kv) {
   const bool bf16 = p.kv_dtype == PCP_KV_BF16;
   const uint64_t bs = p.block_size, H = p.num_kv_heads, elt = bf16 ? 2 : 1, row = p.head_dim * elt;
   const uint32_t cols = static_cast<uint32_t>(row / 128);
   const cuuint64_t dims[5] = {128 / elt, bs, cols, H, 2 * static_cast<cuuint64_t>(p.blocks)};
   const cuuint64_t strides[4] = {row, 128, bs * row, H * bs * row};
-  const cuuint32_t box[5] = {static_cast<cuuint32_t>(128 / elt), box_rows, cols, 1, 2};
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(128 / elt), box_rows, box_cols, 1, box_kv};
   return encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, p.data, dims, strides,
                 box, true);
 }
@@ -261,7 +264,7 @@ int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t 
   int shift = 4;
   while ((2 << shift) <= L::kStageKeys && pool.block_size % (2 << shift) == 0) ++shift;
   CUtensorMap tm, ts{};
-  PCP_TRY(make_rows_map(&tm, pool, 1 << shift));
+  PCP_TRY(make_rows_map(&tm, pool, 1 << shift, L::kBoxes, 2));
   if (pool.scales) PCP_TRY(make_scale_map(&ts, pool, 1 << shift));
   PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes, kFp8 ? pcp::kRowsLaunchRegs : 0)));
   pcp::chunk_rows_kernel<D, kFp8><<<kCtas, L::kThreads, L::kBytes, st>>>(tm, ts, shift, p);
@@ -272,14 +275,21 @@ int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t 
 template <int D, int kCache>
 int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
   using L = pcp::TilesSmem<D, kCache>;
-  // Boxes of as many rows as a page's length and half a tile share.
-  int box_rows = 64;
-  while (pool.block_size % box_rows) box_rows /= 2;
+  // Copies of as many rows as a page's length and a tile (K: half a tile) share.
+  pcp::TileBoxes box{64, 128, 0};
+  while (pool.block_size % box.k_rows) box.k_rows /= 2;
+  while (pool.block_size % box.v_rows) box.v_rows /= 2;
+  box.all_cols = !L::kFp8 && box.k_rows == 64;
   CUtensorMap tk, tv;
-  PCP_TRY(make_pool_map(&tk, pool, L::kFp8 ? D : 64, box_rows, !L::kFp8));
-  PCP_TRY(make_pool_map(&tv, pool, L::kFp8 ? D / 2 : 64, box_rows, !L::kFp8));
-  PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes)));
-  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tk, tv, box_rows, p);
+  if (L::kFp8) {
+    PCP_TRY(make_pool_map(&tk, pool, D, box.k_rows));
+    PCP_TRY(make_pool_map(&tv, pool, D / 2, box.v_rows));
+  } else {
+    PCP_TRY(make_rows_map(&tk, pool, box.k_rows, box.all_cols ? D / 64 : 1, 1));
+    PCP_TRY(make_rows_map(&tv, pool, box.v_rows, box.all_cols ? D / 128 : 1, 1));
+  }
+  PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes, pcp::kTilesLaunchRegs)));
+  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tk, tv, box, p);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
 }
@@ -287,19 +297,22 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
 // Tile units over the bf16 copy of their pages.
 template <int D>
 int launch_expanded(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, cudaStream_t st) {
-  const pcp::ExpandParams e{p, static_cast<__nv_bfloat16*>(copy)};
-  const int64_t pages = static_cast<int64_t>(p.batch.seqs) * p.batch.table_width;
-  const int64_t items = pages * 2 * pool.num_kv_heads;
+  const int rows = copy_rows(pool.block_size, p.batch.table_width);
+  const pcp::ExpandParams e{p, static_cast<__nv_bfloat16*>(copy), rows};
+  const int64_t items = static_cast<int64_t>(p.batch.seqs) * p.batch.table_width * 2 * pool.num_kv_heads;
   pcp::chunk_expand_kernel<D><<<static_cast<unsigned>(std::min<int64_t>(items, 8 * kCtas)), 256, 0, st>>>(e);
   CUDA_TRY(cudaGetLastError());
+  // The copy as a cache of one page a sequence.
   pcp_pool_t dense = pool;
   dense.data = copy;
   dense.scales = nullptr;
-  dense.blocks = pages;
+  dense.blocks = p.batch.seqs;
+  dense.block_size = rows;
   dense.kv_dtype = PCP_KV_BF16;
   pcp::ChunkParams d = p;
   d.pool = pool_view(dense);
   d.batch.tables = nullptr;
+  d.batch.table_width = 1;
   return launch_tiles<D, pcp::kCacheBf16>(dense, d, st);
 }
 
@@ -446,6 +459,7 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.out_head = out->head_stride;
   p.out_row = out->row_stride;
   p.group = group;
+  p.capacity = static_cast<int64_t>(batch->table_width) * pool->block_size;
   p.max_chunk = max_chunk;
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
   p.small_ctas = kCtas;
