@@ -77,6 +77,18 @@ __device__ __forceinline__ float exp2_of_int(int e) {  // 2^e, 0 below the norma
   return __uint_as_float(static_cast<uint32_t>(min(max(e + 127, 0), 254)) << 23);
 }
 
+// 5-D tiled TMA load into THIS CTA's shared memory whose bytes count on
+// `cluster_bar`, an mbarrier of either CTA of the pair.  Local-GPU memory; no
+// multicast.
+__device__ __forceinline__ void tma_load_5d_pair(uint32_t dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2,
+                                                 int32_t c3, int32_t c4, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(cluster_bar)
+      : "memory");
+}
+
 // One lane of the (converged) warp, always the same.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -286,38 +298,19 @@ template <bool kTile>
 struct ChunkWalk {
   int left;  // steps of the range still to come, but for a part left for last
   int seq, head, unit, kt;
+  ChunkSeq q;                                              // of seq
   int later_seq, later_head, later_unit, later_kt, later;  // that part and its steps
 
-  __device__ __forceinline__ void init(const ChunkPlanShared& sh) {
+  __device__ __forceinline__ void init(const ChunkParams& p, const ChunkPlanShared& sh, int* err) {
     left = static_cast<int>(sh.end - sh.x);
     seq = sh.seq;
     head = sh.head;
     unit = sh.unit;
     kt = sh.kt;
     later = 0;
-  }
-  __device__ __forceinline__ void advance(const ChunkParams& p, int* err, int tiles) {
-    kt = 0;
-    if (left > 0 && ++unit == tiles) {
-      unit = 0;
-      if (++head == p.pool.heads) {
-        head = 0;
-        while (chunk_seq<kTile>(p, ++seq, err).tiles == 0) {
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ bool next(const ChunkParams& p, int* err, ChunkUnit& u, int& kt0, int& kt1) {
-    if (left <= 0 && (!kTile || later == 0)) return false;
-    if (kTile && left <= 0) {
-      left = later;
-      seq = later_seq;
-      head = later_head;
-      unit = later_unit;
-      kt = later_kt;
-      later = 0;
-    } else if (kTile && kt > 0) {
-      const ChunkSeq q = chunk_seq<kTile>(p, seq, err);
+    if (left <= 0) return;
+    q = chunk_seq<kTile>(p, seq, err);
+    if (kTile && kt > 0) {
       const int rest = chunk_unit<kTile>(p, q, seq, head, unit).steps - kt;
       if (rest < left) {
         later = rest;
@@ -326,15 +319,38 @@ struct ChunkWalk {
         later_unit = unit;
         later_kt = kt;
         left -= rest;
-        advance(p, err, q.tiles);
+        advance(p, err);
       }
     }
-    const ChunkSeq q = chunk_seq<kTile>(p, seq, err);
+  }
+  __device__ __forceinline__ void advance(const ChunkParams& p, int* err) {
+    kt = 0;
+    if (left > 0 && ++unit == q.tiles) {
+      unit = 0;
+      if (++head == p.pool.heads) {
+        head = 0;
+        do {
+          q = chunk_seq<kTile>(p, ++seq, err);
+        } while (q.tiles == 0);
+      }
+    }
+  }
+  __device__ __forceinline__ bool next(const ChunkParams& p, int* err, ChunkUnit& u, int& kt0, int& kt1) {
+    if (left <= 0) {
+      if (!kTile || later == 0) return false;
+      left = later;
+      seq = later_seq;
+      head = later_head;
+      unit = later_unit;
+      kt = later_kt;
+      later = 0;
+      q = chunk_seq<kTile>(p, seq, err);
+    }
     u = chunk_unit<kTile>(p, q, seq, head, unit);
     kt0 = kt;
     kt1 = min(u.steps, kt + left);
     left -= kt1 - kt0;
-    advance(p, err, q.tiles);
+    advance(p, err);
     return true;
   }
 };

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   __syncthreads();
   chunk_plan<false>(p, plan, p.small_ctas, blockIdx.x);
   ChunkWalk<false> walk;
-  walk.init(plan);
+  walk.init(p, plan, err);
   ChunkUnit un;
   int kt0, kt1;
   uint32_t c = 0;  // stages of this CTA so far

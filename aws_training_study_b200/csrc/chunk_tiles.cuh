@@ -13,7 +13,9 @@
 //     exponentials, and all that passes between them is each row's reference
 //     maximum, which the other published half a turn ago.  The accumulator leaves
 //     TMEM columns to keep P apart from S, so that a score buffer is free, and the
-//     next QK^T but one issued, once its scores are in registers.
+//     next QK^T but one issued, once its scores are in registers.  The turns go on
+//     from unit to unit: Q has two buffers, and while the warpgroup that did a
+//     unit's last tile writes its output, the other is at the next unit's first.
 //   * D = 256: no columns are left; P overwrites S, and a tile's QK^T waits for the
 //     product before last.  That chain (softmax, PV, QK^T and about 1300 cycles of
 //     hand-over in two tiles) is the limit, and the warpgroups split each tile's
@@ -49,15 +51,25 @@ enum : int { kCacheBf16 = 0, kCacheE4m3 = 1, kCacheScaled = 2 };
 
 constexpr int kTilesConvWarps = 4;
 constexpr int kTilesConvThreads = 32 * kTilesConvWarps;
-// Four warpgroups: softmax 0 and 1, TMA and MMA warps (two idle), converters;
-// their registers, out of the launch's 512 x 128.
+// Four warpgroups: softmax 0 and 1, K/V copies, MMA, segment and Q warps, converters;
+// they split the launch's 512 x 128 registers (TilesSmem).
+constexpr int kSegmentWarp = 10, kQWarp = 11;
 constexpr int kTilesConvWarp0 = 12;
 constexpr int kTilesThreads = 512;
-constexpr int kTilesLaunchRegs = 128, kTilesSoftmaxRegs = 176, kTilesControlRegs = 72, kTilesConvRegs = 88;
-static_assert(2 * kTilesSoftmaxRegs + kTilesControlRegs + kTilesConvRegs <= 4 * kTilesLaunchRegs,
-              "more than the launch's registers");
+constexpr int kTilesLaunchRegs = 128;
 constexpr int kTurnsP = 128;  // TMEM columns of P, D = 128: O 0-127, P 128-255, S 256-511
 constexpr uint16_t kChunkBothCtas = 3, kChunkLeader = 1;
+
+// A segment: the part [kt0, kt1) of a unit's key tiles; kt1 = 0 after the last.
+struct __align__(16) TileSegment {
+  ChunkUnit un;
+  int kt0, kt1;
+  int pad[2];
+};
+// Segments on their way from the warp that walks the range to the others (each
+// walking by itself, the loads and divisions of a step took every role some 1500
+// to 2000 cycles a unit).
+constexpr int kTileSegments = 4;
 
 template <int D, int kCache>
 struct TilesSmem {
@@ -66,8 +78,11 @@ struct TilesSmem {
   static constexpr int kOpBytes = 128 * D;  // 16-bit K half [64, D] or V half [128, D/2], swizzled
   static constexpr int kRawBytes = 64 * D;  // e4m3 K half [64][D] or V half [128][D/2]
   static constexpr bool kTurns = D == 128;  // the softmax warpgroups take turns
+  static constexpr int kSoftmaxRegs = kTurns ? 168 : 144, kControlRegs = kTurns ? 88 : 112, kConvRegs = kControlRegs;
+  static_assert(2 * kSoftmaxRegs + kControlRegs + kConvRegs <= 4 * kTilesLaunchRegs, "more than the launch's registers");
   static constexpr int kAhead = kTurns ? 2 : 1;  // QK^T issued ahead of PV, in tiles
-  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 7) : (D == 256 ? 5 : 9);
+  static constexpr int kQBufs = kTurns ? 2 : 1;
+  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 5) : (D == 256 ? 5 : 7);
   static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 5) : 0;
   static constexpr int kLandStages = kFp8 ? kRawStages : kOpStages;  // stages the TMA fills
   static constexpr int kKBox = 64 * 128;
@@ -78,22 +93,29 @@ struct TilesSmem {
   // before it was consumed.
   static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 2 * kAhead + 2) / 2 : 0;
   static constexpr int kOutBytes = kTurns ? 8 * 4096 : 0;  // output rows on their way out, 4 KB a softmax warp
-  static constexpr int kOpOff = kQBytes;
+  static constexpr int kOpOff = kQBufs * kQBytes;
   static constexpr int kRawOff = kOpOff + kOpStages * kOpBytes;
   static constexpr int kOutOff = kRawOff + kRawStages * kRawBytes;
   static constexpr int kScaleOff = kOutOff + kOutBytes;  // float k[128], v[128], int vmax[4]
   static constexpr int kScaleBuf = 2 * kTileN * 4 + 16;
-  static constexpr int kFactorOff = kScaleOff + kScaleBufs * kScaleBuf;  // float[2][128], by segment parity
-  static constexpr int kRedOff = kFactorOff + (kFp8 ? 2 * kTileM * 4 : 0);
-  static constexpr int kBarOff = kRedOff + 4 * kTileM * 4;
-  // q_ready, q_empty, rows[2], o_free, s_free[2], land_full[NL], land_empty[NR], op_full[NS],
-  // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, ref[2], scale[NB]
-  static constexpr int kNumBars = 7 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs;
-  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
+  // Row factors of a segment, float[128] each.  Q of a segment is written once
+  // QK^T of the one kQBufs before it is done, and QK^T of a tile once the scores
+  // two tiles back were read: so a softmax warpgroup may be three segments behind
+  // (of one tile each) with kTurns, one without.
+  static constexpr int kFactorBufs = kTurns ? 4 : 2;
+  static constexpr int kFactorOff = kScaleOff + kScaleBufs * kScaleBuf;
+  static constexpr int kRedOff = kFactorOff + (kFp8 ? kFactorBufs * kTileM * 4 : 0);
+  static constexpr int kBarOff = kRedOff + (kTurns ? 6 : 4) * kTileM * 4;
+  // q_ready[2], q_empty[2], rows[4], o_free, s_free[2], part[2], land_full[NL], land_empty[NR], op_full[NS],
+  // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, ref[2], scale[NB],
+  // seg_full[], seg_empty[]
+  static constexpr int kNumBars = 13 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs + 2 * kTileSegments;
+  static constexpr int kMiscOff = (kBarOff + kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kSegOff = kMiscOff + 16;  // TileSegment[kTileSegments]
+  static constexpr int kPlanOff = kSegOff + kTileSegments * sizeof(TileSegment);  // ChunkPlanShared
   static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
-  static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
+  static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kSegOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
 };
 
 // A warp's 32 rows (a lane each), O * inv_l of kCols TMEM columns from t_o, to
@@ -141,6 +163,7 @@ __device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, ui
 // whatever its size (eight a tile held the kernel at 2900 cycles a tile, D = 256),
 // so one brings as many rows, and as many 64-element columns, as the pages allow.
 struct TileBoxes {
+  int q_copy;          // Q by one copy a segment (bf16 operands, group a divisor of 128); else gathered
   int k_rows, v_rows;  // rows of a copy: K up to 64, V up to 128
   int all_cols;        // bf16: all 64-element columns in a copy (pages of a multiple of 64 tokens)
 };
@@ -207,7 +230,8 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
 
 template <int D, int kCache>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
-    chunk_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    chunk_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v,
                        const TileBoxes box, const ChunkParams p) {
   using L = TilesSmem<D, kCache>;
   constexpr bool kFp8 = L::kFp8;
@@ -229,25 +253,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   const uint32_t sOp = sbase + L::kOpOff;
   const uint32_t sRaw = sbase + L::kRawOff;
   const uint32_t bars = sbase + L::kBarOff;
-  const uint32_t bar_q_ready = bars;      // leader: Q written in both CTAs (one arrive per converter warp)
-  const uint32_t bar_q_empty = bars + 8;  // the segment's last QK^T has read Q (MMA commit, both CTAs)
-  // This CTA's row factors written, by segment parity (two: the converters may
-  // be a segment ahead of a softmax warp that has not waited yet).
-  auto bar_rows = [&](int s) { return bars + 16 + 8u * (s & 1); };
-  const uint32_t bar_o_free = bars + 32;  // leader: O of the segment read by every softmax warp of both CTAs
+  // By segment parity (the buffers of Q with two; what runs ahead could pass a
+  // single barrier by two phases, which its parity does not show):
+  // leader: Q written in both CTAs (one arrive per converter warp; a copy: the
+  // bytes of both);
+  auto bar_q_ready = [&](int sg) { return bars + 8u * (sg & 1); };
+  // the segment's last QK^T has read Q (MMA commit, both CTAs);
+  auto bar_q_empty = [&](int sg) { return bars + 16 + 8u * (sg & 1); };
+  // this CTA's row factors written (four of them: see kFactorBufs).
+  auto bar_rows = [&](int sg) { return bars + 32 + 8u * (sg & (L::kFactorBufs - 1)); };
+  const uint32_t bar_o_free = bars + 64;  // leader: O of the segment read by every softmax warp of both CTAs
   // Leader: scores of the buffer in registers (kTurns: its next QK^T may be issued).
-  auto bar_s_free = [&](int b) { return bars + 40 + 8u * b; };
-  auto bar_land_full = [&](int s) { return bars + 8u * (7 + s); };
-  auto bar_land_empty = [&](int s) { return bars + 8u * (7 + NL + s); };
-  auto bar_op_full = [&](int s) { return bars + 8u * (7 + NL + NR + s); };
-  auto bar_op_empty = [&](int s) { return bars + 8u * (7 + NL + NR + NS + s); };
-  constexpr int kB2 = 7 + NL + NR + 2 * NS;
+  auto bar_s_free = [&](int b) { return bars + 72 + 8u * b; };
+  // kTurns: the other warpgroup's part of a segment's sums, by segment parity.
+  auto bar_part = [&](int sg) { return bars + 88 + 8u * (sg & 1); };
+  auto bar_land_full = [&](int s) { return bars + 8u * (13 + s); };
+  auto bar_land_empty = [&](int s) { return bars + 8u * (13 + NL + s); };
+  auto bar_op_full = [&](int s) { return bars + 8u * (13 + NL + NR + s); };
+  auto bar_op_empty = [&](int s) { return bars + 8u * (13 + NL + NR + NS + s); };
+  constexpr int kB2 = 13 + NL + NR + 2 * NS;
   auto bar_s_full = [&](int b) { return bars + 8u * (kB2 + b); };
   auto bar_p_full = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
   auto bar_o = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
   const uint32_t bar_td = bars + 8u * (kB2 + 6);
   auto bar_ref = [&](int b) { return bars + 8u * (kB2 + 7 + b); };
   auto bar_scale = [&](int b) { return bars + 8u * (kB2 + 9 + b); };
+  auto bar_seg_full = [&](int sg) { return bars + 8u * (kB2 + 9 + NB + sg % kTileSegments); };
+  auto bar_seg_empty = [&](int sg) { return bars + 8u * (kB2 + 9 + NB + kTileSegments + sg % kTileSegments); };
+  TileSegment* segments = reinterpret_cast<TileSegment*>(smem + L::kSegOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
@@ -259,10 +292,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   const int lane = threadIdx.x & 31;
 
   if (warp == kProducerWarp && lane == 0) {
-    mbar_init(bar_q_ready, 2 * kTilesConvWarps);
-    mbar_init(bar_q_empty, 1);
-    mbar_init(bar_rows(0), kTilesConvWarps);
-    mbar_init(bar_rows(1), kTilesConvWarps);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_q_ready(b), box.q_copy ? 1 : 2 * kTilesConvWarps);
+      mbar_init(bar_q_empty(b), 1);
+    }
+    for (int b = 0; b < L::kFactorBufs; ++b) mbar_init(bar_rows(b), kTilesConvWarps);
     for (int s = 0; s < NL; ++s) mbar_init(bar_land_full(s), 1);
     for (int s = 0; s < NR; ++s) mbar_init(bar_land_empty(s), kTilesConvWarps);
     for (int s = 0; s < NS; ++s) {
@@ -278,7 +312,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       mbar_init(bar_ref(b), L::kTurns ? 128 : 256);
     }
     for (int b = 0; b < NB; ++b) mbar_init(bar_scale(b), kTilesConvWarps);
-    mbar_init(bar_o_free, 2 * 8);
+    mbar_init(bar_o_free, L::kTurns ? 2 * 4 : 2 * 8);
+    mbar_init(bar_part(0), 128);
+    mbar_init(bar_part(1), 128);
+    for (int b = 0; b < kTileSegments; ++b) {
+      mbar_init(bar_seg_full(b), 1);
+      mbar_init(bar_seg_empty(b), 8 + 1 + 1 + 1 + kTilesConvWarps);  // every warp that reads them
+    }
     mbar_init(bar_td, 1);
     *abort_flag = 0;
     plan.err = 0;
@@ -296,36 +336,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   grid_launch_dependents();  // the merge may wait on the SMs
   chunk_plan<true>(p, plan, p.tile_pairs, pair);
 
-  // Calls body(unit, kt0, kt1) for each part of this pair's range until
-  // it returns false; returns false if it did.
+  // Segment sg of this pair's range, for a whole warp; false after the last (or
+  // when the kernel gives up).
+  auto get_segment = [&](int sg, ChunkUnit& un, int& kt0, int& kt1) -> bool {
+    if (!__all_sync(0xffffffffu, mbar_wait(bar_seg_full(sg), (sg / kTileSegments) & 1u, abort_flag, err, kErrWaitQ)))
+      return false;
+    const TileSegment& s = segments[sg % kTileSegments];
+    un = s.un;
+    kt0 = s.kt0;
+    kt1 = s.kt1;
+    return kt1 > 0;
+  };
+  auto put_back = [&](int sg) {  // read by this warp
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_seg_empty(sg));
+  };
+  // Calls body(unit, kt0, kt1, segment) for each segment until it returns false;
+  // returns false if it did.
   auto for_each_segment = [&](auto&& body) -> bool {
-    ChunkWalk<true> walk;
-    walk.init(plan);
     ChunkUnit un;
     int kt0, kt1;
-    while (walk.next(p, err, un, kt0, kt1))
-      if (!body(un, kt0, kt1)) return false;
-    return true;
-  };
-  // The items of a segment in the order of their loads, conversions and MMAs:
-  // K of the first kAhead tiles, then (K of tile j + kAhead, V of tile j).
-  auto for_each_item = [&](int kt0, int kt1, auto&& body) -> bool {
-    for (int kt = kt0 - L::kAhead; kt < kt1; ++kt) {
-      if (kt + L::kAhead < kt1 && !body(false, kt + L::kAhead)) return false;
-      if (kt >= kt0 && !body(true, kt)) return false;
+    for (int sg = 0; get_segment(sg, un, kt0, kt1); ++sg) {
+      put_back(sg);
+      if (!body(un, kt0, kt1, sg)) return false;
     }
-    return true;
+    return *abort_flag == 0;
+  };
+  // Keys of tile kt that the sequence has (may be 0 when it has none at all).
+  auto tile_valid = [&](const ChunkUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
+  // The items of the range in the order of their loads, conversions and MMAs: K
+  // of a tile kAhead tiles before V of its own place (without kTurns, within a
+  // segment: Q has one buffer).  body(is_v, unit, tile, tiles before it, segment,
+  // segment's first tile, its last) until it returns false.
+  auto for_each_item = [&](auto&& body) -> bool {
+    if constexpr (!L::kTurns) {
+      uint32_t J = 0;
+      return for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int sg) -> bool {
+        if (!body(false, un, kt0, J, sg, true, kt0 + 1 == kt1)) return false;
+#pragma unroll 1
+        for (int kt = kt0; kt < kt1; ++kt, ++J) {
+          if (kt + 1 < kt1 && !body(false, un, kt + 1, J + 1, sg, false, kt + 2 == kt1)) return false;
+          if (!body(true, un, kt, J, sg, kt == kt0, false)) return false;
+        }
+        return true;
+      });
+    } else {
+      ChunkUnit k, v;
+      int k0, k1, v0, v1, kseg = 0, vseg = 0;
+      uint32_t kj = 0, vj = 0;
+      if (!get_segment(0, k, k0, k1)) return *abort_flag == 0;
+      put_back(0);
+      v = k;
+      v0 = k0;
+      v1 = k1;
+      int kt = k0;
+      bool more = true;
+      while (true) {
+        for (int vt = v0; vt < v1; ++vt, ++vj) {
+#pragma unroll 1
+          while (more && kj <= vj + L::kAhead) {
+            if (!body(false, k, kt, kj, kseg, kt == k0, kt + 1 == k1)) return false;
+            ++kj;
+            if (++kt == k1) {
+              more = get_segment(++kseg, k, k0, k1);
+              kt = k0;
+            }
+          }
+          if (!body(true, v, vt, vj, vseg, vt == v0, false)) return false;
+        }
+        if (!get_segment(++vseg, v, v0, v1)) return *abort_flag == 0;
+        put_back(vseg);
+      }
+    }
   };
   // V's 64-element columns in an operand stage: each of 128 rows, or (copied 64
   // rows at a time) all columns of keys 0-63, then of 64-127.
   const bool v_halves = !kFp8 && box.all_cols && box.v_rows == 64;
   const uint32_t v_col = v_halves ? L::kVBox / 2 : L::kVBox;
   const uint32_t v_half = v_halves ? (D / 128) * (L::kVBox / 2) - 64 * 128 : 0;  // beyond 64 rows
-  // Keys of tile kt that the sequence has (may be 0 when it has none at all).
-  auto tile_valid = [&](const ChunkUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
 
   if (warp >= kProducerWarp && warp < kTilesConvWarp0) {
-    setmaxnreg_dec<kTilesControlRegs>();
+    setmaxnreg_dec<L::kControlRegs>();
     // Both roles walk with the whole warp and issue from one elected lane: in
     // code that only one lane runs, every operand of an MMA or a copy takes its
     // way through a vector register (100 cycles an MMA; the tensor cores waited).
@@ -393,13 +484,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ++c;
         return true;
       };
-      const bool ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
-        return for_each_item(kt0, kt1, [&](bool is_v, int kt) { return issue(un, is_v, kt); });
+      const bool ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool, bool) {
+        return issue(un, is_v, kt);
       });
       if (!ok && elected)  // let this CTA's copies still in flight land before it exits
         for (uint32_t i = (c > (uint32_t)NL ? c - NL : 0); i < c; ++i)
           mbar_wait_teardown(bar_land_full(i % NL), (i / NL) & 1u);
     }
+    if (warp == kSegmentWarp) {
+      // ------------------------------------------------ walks the range --
+      ChunkWalk<true> walk;
+      walk.init(p, plan, err);
+      ChunkUnit un;
+      int kt0, kt1;
+      for (int sg = 0;; ++sg) {
+        const bool more = walk.next(p, err, un, kt0, kt1);
+        if (sg >= kTileSegments &&
+            !__all_sync(0xffffffffu, mbar_wait(bar_seg_empty(sg), ((sg / kTileSegments) & 1u) ^ 1u, abort_flag, err,
+                                               kErrWaitQ)))
+          break;
+        if (elected) {
+          TileSegment& s = segments[sg % kTileSegments];
+          s.un = un;
+          s.kt0 = kt0;
+          s.kt1 = more ? kt1 : 0;
+          mbar_arrive(bar_seg_full(sg));
+        }
+        if (!more) break;
+      }
+    }
+    if (warp == kQWarp) {
+      // ------------------------------------- Q, where a copy brings it --
+      // Rows token * group + head of a unit as boxes of {64 elements, group, 128
+      // / group tokens, two columns}; tokens past the sequence bring other
+      // rows, whose results nobody reads.  Both CTAs' bytes count on the leader.
+      uint32_t landed = 0;
+      const bool ok = for_each_segment([&](const ChunkUnit& un, int, int, int sg) -> bool {
+        if (!box.q_copy) return true;
+        if (sg >= L::kQBufs &&
+            !__all_sync(0xffffffffu, mbar_wait(bar_q_empty(sg - L::kQBufs), ((sg - L::kQBufs) >> 1) & 1u, abort_flag,
+                                               err, kErrWaitQ)))
+          return false;
+        if (elected) {
+          if (leader) mbar_arrive_expect_tx(bar_q_ready(sg), 2 * L::kQBytes);
+          const int token = un.q0 + un.row0 / p.group + static_cast<int>(rank) * (kTileM / p.group);
+          for (int b = 0; b < D / 64; b += 2)
+            tma_load_5d_pair(sQ + (L::kQBufs > 1 ? (sg & 1) * L::kQBytes : 0) + b * kBoxBytes, &tm_q, 0, 0, token, b,
+                             un.head, mapa_shared(bar_q_ready(sg), 0));
+        }
+        landed = sg + 1;
+        return true;
+      });
+      // After a failure: let the copies land.
+      if (!ok && leader && elected && landed > 0)
+        mbar_wait_teardown(bar_q_ready(landed - 1), ((landed - 1) >> 1) & 1u);
+    }
+    if (warp == kMmaWarp && !leader) for_each_segment([](const ChunkUnit&, int, int, int) { return true; });
     if (warp == kMmaWarp && leader) {
       // ------------------------------------------ MMA issuer (leader only) --
       constexpr uint32_t idesc_qk =
@@ -407,16 +547,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       constexpr uint32_t idesc_pv =
           kFp8 ? make_idesc_f16(kUnitRows, D, false, true) : make_idesc_bf16(kUnitRows, D, false, true);
       uint32_t c = 0;
-      uint32_t J = 0;  // tiles of all earlier segments
-      int segs = 0;
       auto wait = [&](uint32_t bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
       };
       // Descriptors of the first k step; the others differ in the address alone.
-      const uint64_t q_desc = make_sw128_desc(sQ, 16, 1024);
+      const uint64_t q_desc0 = make_sw128_desc(sQ, 16, 1024);
       const uint64_t k_desc = make_sw128_desc(sOp, 16, 1024);
       const uint64_t v_desc = make_sw128_desc(sOp, v_col, 1024);
-      auto qk = [&](uint32_t jg) {
+      auto qk = [&](uint32_t jg, int seg) {
+        const uint64_t q_desc = q_desc0 + (L::kQBufs > 1 ? (seg & 1) * (L::kQBytes >> 4) : 0);
         const uint32_t s_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
         const int st = c % NS;
         if (L::kTurns && jg >= 2 && !wait(bar_s_free(jg & 1), ((jg - 2) >> 1) & 1u, kErrWaitSFull)) return false;
@@ -459,19 +598,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ++c;
         return true;
       };
-      for_each_segment([&](const ChunkUnit&, int kt0, int kt1) -> bool {
-        const uint32_t n = static_cast<uint32_t>(kt1 - kt0);
-        if (!wait(bar_q_ready, segs & 1u, kErrWaitQ)) return false;
-        tc_fence_after();
-        const bool ok = for_each_item(0, static_cast<int>(n), [&](bool is_v, int j) {
-          if (is_v) return pv(J + j, j == 0, segs);
-          if (!qk(J + j)) return false;
-          if (j + 1 == static_cast<int>(n) && elected) umma_commit_pair(bar_q_empty, kChunkBothCtas);  // the segment's last
-          return true;
-        });
-        if (!ok) return false;
-        J += n;
-        ++segs;
+      for_each_item([&](bool is_v, const ChunkUnit&, int, uint32_t J, int seg, bool first, bool last) {
+        if (is_v) return pv(J, first, seg);
+        if (first) {
+          if (!wait(bar_q_ready(seg), (seg >> 1) & 1u, kErrWaitQ)) return false;
+          tc_fence_after();
+        }
+        if (!qk(J, seg)) return false;
+        if (last && elected) umma_commit_pair(bar_q_empty(seg), kChunkBothCtas);
         return true;
       });
       // Drain: completes when every MMA issued above has.
@@ -482,7 +616,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     }
     __syncwarp();
   } else if (warp >= kTilesConvWarp0) {
-    setmaxnreg_dec<kTilesConvRegs>();
+    setmaxnreg_dec<L::kConvRegs>();
     // ------------------------------- Q gather, e4m3 -> f16, V past the end --
     const int ct = threadIdx.x - kTilesConvWarp0 * 32;
     const int cw = warp - kTilesConvWarp0;
@@ -569,7 +703,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       ++c;
       return true;
     };
-    for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
+    auto gather_q = [&](const ChunkUnit& un) -> bool {
       // Q rows into the swizzled operand layout: a row over D / 8 lanes,
       // kFlight loads a lane in flight, the first of them before the wait for the
       // previous segment's QK^T to be done with the buffer.
@@ -589,7 +723,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
                 p.q + static_cast<long long>(un.head * p.group + row % p.group) * p.q_head +
                 static_cast<long long>(un.q0 + row / p.group) * p.q_row + 8 * ch);
         }
-        if (r0 == cw * 32 && segs > 0 && !wait_all(bar_q_empty, (segs - 1) & 1u, kErrWaitQ)) return false;
+        if (r0 == cw * 32 && segs >= L::kQBufs && !wait_all(bar_q_empty(segs - L::kQBufs), ((segs - L::kQBufs) >> 1) & 1u, kErrWaitQ))
+          return false;
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
           const int r = r0 + u * kSide + side;
@@ -606,25 +741,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             for (int o = D / 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int e = m == 0 ? 0 : max(static_cast<int>(m >> 23) - 127 - 14, -112);
             const float down = exp2_of_int(-e);
-            if (ch == 0) factors[(segs & 1) * kTileM + r] = p.scale_log2 * exp2_of_int(e);
+            if (ch == 0) factors[(segs & (L::kFactorBufs - 1)) * kTileM + r] = p.scale_log2 * exp2_of_int(e);
             x[u] = make_uint4(pack_f16x2(f[0] * down, f[1] * down), pack_f16x2(f[2] * down, f[3] * down),
                               pack_f16x2(f[4] * down, f[5] * down), pack_f16x2(f[6] * down, f[7] * down));
           }
-          sts128(sQ + (ch / 8) * kBoxBytes + r * 128 + (((ch % 8) ^ (r & 7)) << 4), x[u]);
+          sts128(sQ + (L::kQBufs > 1 ? (segs & 1) * L::kQBytes : 0) + (ch / 8) * kBoxBytes + r * 128 + (((ch % 8) ^ (r & 7)) << 4), x[u]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar_rows(segs));
-        mbar_arrive_remote(mapa_shared(bar_q_ready, 0));
+        mbar_arrive_remote(mapa_shared(bar_q_ready(segs), 0));
       }
       ++segs;
-      return for_each_item(kt0, kt1, [&](bool is_v, int kt) { return item(un, is_v, kt); });
+      return true;
+    };
+    for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool first, bool) {
+      if (!is_v && first && !box.q_copy && !gather_q(un)) return false;
+      return item(un, is_v, kt);
     });
     __syncwarp();
   } else {
-    setmaxnreg_inc<kTilesSoftmaxRegs>();
+    setmaxnreg_inc<L::kSoftmaxRegs>();
     // ---------------------------------------- softmax / correction / epilogue --
     constexpr int kOCols = D / 2;
     constexpr int kKeys = L::kTurns ? kTileN : kTileN / 2;  // a thread's keys of a tile
@@ -632,17 +771,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     const int row = threadIdx.x & (kTileM - 1);  // == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     // kTurns: refs[2][128], each row's reference after a tile, by the tile's
-    // parity; else the halves' maxima [tile parity][2][128].  At the end refs is
-    // each warpgroup's last reference and sums its l.
+    // parity, and sums[2][128] (m, l), one warpgroup's part of a segment for the
+    // other, by the segment's parity.  Else the halves' maxima [tile
+    // parity][2][128], and at the end refs, sums [2][128].
     float* refs = red;
     float* sums = red + 2 * kTileM;
     uint32_t J = 0;
-    int segs = 0;
     // The leader keeps the pair's record.
     ChunkRecord& rec = p.work.tile_rec[pair];
     const bool keeps = leader && threadIdx.x == 0;
     if (keeps) clear_record(rec);
-    const bool done = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1) -> bool {
+    const bool done = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int seg) -> bool {
       if (keeps) note_part(rec, un, kt0, kt1);
       bool ok = true;
       const int r = static_cast<int>(rank) * kTileM + row;  // row of the unit
@@ -651,11 +790,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int pos = un.kvlen - un.qlen + at / p.group;  // last key this row sees
       const uint32_t Jend = J + (kt1 - kt0);
       float rf = p.scale_log2;
-      if (kFp8) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(segs), (segs >> 1) & 1u, abort_flag, err, kErrWaitQ));
-        if (ok) rf = factors[(segs & 1) * kTileM + row];
+      // (A warpgroup without a tile here needs none, and does not wait.)
+      if (kFp8 && (!L::kTurns || J + ((J ^ wg) & 1u) < Jend)) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(seg), (seg / L::kFactorBufs) & 1u, abort_flag, err, kErrWaitQ));
+        if (ok) rf = factors[(seg & (L::kFactorBufs - 1)) * kTileM + row];
       }
-      ++segs;
       float m = -INFINITY;  // (this warpgroup's last) reference: log2 units, V's exponents included
       float l = 0.f;        // its keys' weights over 2^m
 
@@ -748,13 +887,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           ok = scores(jg, s, ev);
           if (!ok) break;
           const float tmax = row_max(s) * rf + ev;
-          float before = -INFINITY;
-          if (jg > J) {
+          // (A segment's first tile waits too, though it starts anew: the steps
+          // go in the tiles' order, or a barrier could get two phases ahead.)
+          if (jg > 0) {
             ok = __all_sync(0xffffffffu,
                             mbar_wait(bar_ref(wg ^ 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitRed));
             if (!ok) break;
-            before = refs[(wg ^ 1) * kTileM + row];
           }
+          const float before = jg > J ? refs[(wg ^ 1) * kTileM + row] : -INFINITY;
           const bool need = tmax > before + kRescaleThreshold;
           const float ref = need ? tmax : before;
           refs[wg * kTileM + row] = ref;
@@ -824,45 +964,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           release(jg);
         }
       }
-      if (ok) {
-        // The last product.  A warpgroup that did not do its tile has not seen
-        // the one before on that barrier complete, and its parity alone could
-        // not tell the two apart: that one first.
-        const uint32_t jl = Jend - 1;
-        if (jl >= 2) ok = mbar_wait(bar_o(jl & 1), ((jl >> 1) & 1u) ^ 1u, abort_flag, err, kErrWaitODone);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
-      }
-      refs[wg * kTileM + row] = m;  // (both read by the other warpgroup only below)
-      sums[wg * kTileM + row] = l;
-      ok = named_bar_and(1, kSoftmaxThreads, ok && (*abort_flag == 0));
-      if (!ok) return false;
+      const uint32_t jl = Jend - 1;  // the last tile
       J = Jend;
-      tc_fence_after();
-      // O carries the last reference, the larger of the two.
-      const float m_other = refs[(wg ^ 1) * kTileM + row], l_other = sums[(wg ^ 1) * kTileM + row];
-      const float top = fmaxf(m, m_other);
-      const float l_tot = (m == top ? l : l * ex2_approx(m - top)) +
-                          (m_other == top ? l_other : l_other * ex2_approx(m_other - top));
-      // Both read: the next segment may reuse the slots.
-      named_bar_sync(2, kSoftmaxThreads);
-      const float inv_l = l_tot == 0.f ? 0.f : 1.f / l_tot;  // no key seen: zeros
       const int slot = part_slot(un, kt0, kt1, pair);
       __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
-                           static_cast<long long>(un.q0 + at / p.group) * p.out_row + wg * kOCols;
+                           static_cast<long long>(un.q0 + at / p.group) * p.out_row;
       const long long pr = static_cast<long long>(slot) * kUnitRows + r;
-      if (slot >= 0 && live && wg == 0)
-        p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __log2f(l_tot);
+      // l over both warpgroups' keys at the last reference, `top`; no key seen:
+      // zeros.
+      auto finish = [&](float m_other, float l_other, float& top) {
+        top = fmaxf(m, m_other);
+        const float l_tot = (m == top ? l : l * ex2_approx(m - top)) +
+                            (m_other == top ? l_other : l_other * ex2_approx(m_other - top));
+        if (slot >= 0 && live && (L::kTurns || wg == 0))
+          p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __log2f(l_tot);
+        return l_tot == 0.f ? 0.f : 1.f / l_tot;
+      };
+      float top;
       if constexpr (L::kTurns) {
+        float2* part = reinterpret_cast<float2*>(sums) + (seg & 1) * kTileM + row;
+        if (!ok) return false;
+        if ((jl & 1u) != static_cast<uint32_t>(wg)) {  // the other one writes the output
+          *part = make_float2(m, l);
+          mbar_arrive(bar_part(seg));
+          return true;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_part(seg), (seg >> 1) & 1u, abort_flag, err, kErrWaitRed) &&
+                                         mbar_wait(bar_o(wg), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
+        if (!ok) return false;
+        tc_fence_after();
+        const float2 other = *part;
+        const float inv_l = finish(other.x, other.y, top);
         uint8_t* turn = smem + L::kOutOff + warp * 4096;
-        if (slot < 0)
-          store_rows<kOCols, true>(t_row + wg * kOCols, inv_l, live ? out : nullptr, turn, lane);
-        else
-          store_rows<kOCols, false>(t_row + wg * kOCols, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr,
-                                    turn, lane);
-      } else if (slot < 0) {
-        store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l, out, live);
+        if (slot < 0) store_rows<D, true>(t_row, inv_l, live ? out : nullptr, turn, lane);
+        else store_rows<D, false>(t_row, inv_l, live ? p.work.tile_o + pr * D : nullptr, turn, lane);
       } else {
-        store_o_partial<kOCols>(t_row + wg * kOCols, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
+        refs[wg * kTileM + row] = m;  // (the maxima there were read before the last product)
+        sums[wg * kTileM + row] = l;
+        ok = named_bar_and(1, kSoftmaxThreads, ok && (*abort_flag == 0));
+        if (!ok) return false;
+        tc_fence_after();
+        const float inv_l = finish(refs[(wg ^ 1) * kTileM + row], sums[(wg ^ 1) * kTileM + row], top);
+        // Both read: the next segment may reuse the slots.
+        named_bar_sync(2, kSoftmaxThreads);
+        if (slot < 0) store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l, out + wg * kOCols, live);
+        else store_o_partial<kOCols>(t_row + wg * kOCols, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
       }
       tc_fence_before();
       __syncwarp();

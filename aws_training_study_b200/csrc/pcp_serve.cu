@@ -226,6 +226,20 @@ int make_rows_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows, uint3
                 box, true);
 }
 
+// Q as {64 elements, query heads of a KV head, rows, 64-element columns, KV
+// heads}: a box is the 128 rows (row * group + head) of a CTA, two columns, each
+// in the 128-byte swizzle.
+int make_q_map(CUtensorMap* tm, const pcp::ChunkParams& p, int D) {
+  const uint64_t G = p.group, head = static_cast<uint64_t>(p.q_head) * 2, row = static_cast<uint64_t>(p.q_row) * 2;
+  // (The stride of an axis of one is 0 here; any multiple of 16 does.)
+  const cuuint64_t dims[5] = {64, G, static_cast<cuuint64_t>(p.batch.rows), static_cast<cuuint64_t>(D / 64),
+                              static_cast<cuuint64_t>(p.pool.heads)};
+  const cuuint64_t strides[4] = {std::max<uint64_t>(head, 16), std::max<uint64_t>(row, 16), 128,
+                                 std::max<uint64_t>(G * head, 16)};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(128 / G), 2, 1};
+  return encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16*>(p.q), dims, strides, box, true);
+}
+
 // Scale bytes [blocks][2][Hkv][bs] as {bs, Hkv, 2 * blocks}: boxes of box_rows
 // of K and of V of one head.
 int make_scale_map(CUtensorMap* tm, const pcp_pool_t& p, uint32_t box_rows) {
@@ -276,11 +290,15 @@ template <int D, int kCache>
 int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
   using L = pcp::TilesSmem<D, kCache>;
   // Copies of as many rows as a page's length and a tile (K: half a tile) share.
-  pcp::TileBoxes box{64, 128, 0};
+  pcp::TileBoxes box{0, 64, 128, 0};
   while (pool.block_size % box.k_rows) box.k_rows /= 2;
   while (pool.block_size % box.v_rows) box.v_rows /= 2;
   box.all_cols = !L::kFp8 && box.k_rows == 64;
-  CUtensorMap tk, tv;
+  CUtensorMap tq{}, tk, tv;
+  // (Heads or rows that are all the same one, stride 0, have no such map.)
+  box.q_copy = !L::kFp8 && 128 % p.group == 0 && (p.q_head > 0 || p.group * p.pool.heads == 1) &&
+               (p.q_row > 0 || p.batch.rows == 1);
+  if (box.q_copy) PCP_TRY(make_q_map(&tq, p, D));
   if (L::kFp8) {
     PCP_TRY(make_pool_map(&tk, pool, D, box.k_rows));
     PCP_TRY(make_pool_map(&tv, pool, D / 2, box.v_rows));
@@ -289,7 +307,7 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
     PCP_TRY(make_rows_map(&tv, pool, box.v_rows, box.all_cols ? D / 128 : 1, 1));
   }
   PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes, pcp::kTilesLaunchRegs)));
-  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tk, tv, box, p);
+  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tq, tk, tv, box, p);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
 }
