@@ -7,28 +7,23 @@
 // attn_kv.cuh a cluster of two CTAs shares every tcgen05 MMA (cta_group::2: each
 // CTA holds 128 query rows, half of each K tile's keys and half of each V tile's
 // columns), and scores and probabilities live in TMEM.  What differs:
-//   * D = 128: the two softmax warpgroups of a CTA take turns, one with the even
-//     key tiles and one with the odd ones, a thread a whole row of 128 keys.  Each
-//     has two tiles' time for one, its loads and maxima run under the other's
-//     exponentials, and all that passes between them is each row's reference
-//     maximum, which the other published half a turn ago.  The accumulator leaves
-//     TMEM columns to keep P apart from S, so that a score buffer is free, and the
-//     next QK^T but one issued, once its scores are in registers.  The turns go on
-//     from unit to unit: Q has two buffers, and while the warpgroup that did a
-//     unit's last tile writes its output, the other is at the next unit's first.
-//   * D = 256: no columns are left; P overwrites S, and a tile's QK^T waits for the
-//     product before last.  That chain (softmax, PV, QK^T and about 1300 cycles of
-//     hand-over in two tiles) is the limit, and the warpgroups split each tile's
-//     keys between them, which makes its softmax shortest.
+//   * The two softmax warpgroups of a CTA split each tile's keys between them.  (One
+//     with the even tiles and one with the odd ones, a thread a whole row, was
+//     slower: 400 to 358 us for four prompts of 2048, D = 128.)
+//   * D = 128: TMEM has room for two accumulators, and the converter warps write a
+//     finished one out while the softmax warps and the MMAs are at the next unit;
+//     Q has two buffers, so that the next unit's first QK^T is issued ahead of the
+//     last PV of the one before.
+//   * D = 256: one of each; the softmax warps write the output.
 //   * Units come from the plan (chunk_plan.cuh): any mix of sequences, each pair
 //     walking an equal range of the batch's steps.
 //   * K and V are read from pages of any multiple of 16 tokens, through the
 //     sequence's table, box by box.
 //   * Rows are (token, query head) pairs of a strided Q, gathered by the
 //     converter warps instead of TMA; each row sees keys up to its position.
-//   * bf16 caches land in operand layout straight from TMA; the converter warps
-//     only pass the tile on (and clear V rows past the sequence, which may hold
-//     anything: 0 * NaN would reach every row).
+//   * bf16 caches land in operand layout straight from TMA, both CTAs' bytes on
+//     the leader's barrier; the converter warps only clear V rows past the
+//     sequence (which may hold anything: 0 * NaN would reach every row).
 //   * An e4m3 cache that many query tiles read is expanded into a bf16 copy first
 //     (chunk_expand_kernel; exact, scales included), when the copy is of moderate
 //     size: reading it in place converts every key tile again for each 256 rows.
@@ -39,6 +34,9 @@
 
 #include <cuda.h>
 #include <cuda_bf16.h>
+
+#include <climits>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "attn_softmax.cuh"
@@ -57,7 +55,6 @@ constexpr int kSegmentWarp = 10, kQWarp = 11;
 constexpr int kTilesConvWarp0 = 12;
 constexpr int kTilesThreads = 512;
 constexpr int kTilesLaunchRegs = 128;
-constexpr int kTurnsP = 128;  // TMEM columns of P, D = 128: O 0-127, P 128-255, S 256-511
 constexpr uint16_t kChunkBothCtas = 3, kChunkLeader = 1;
 
 // A segment: the part [kt0, kt1) of a unit's key tiles; kt1 = 0 after the last.
@@ -77,39 +74,41 @@ struct TilesSmem {
   static constexpr int kQBytes = D * 2 * kTileM;
   static constexpr int kOpBytes = 128 * D;  // 16-bit K half [64, D] or V half [128, D/2], swizzled
   static constexpr int kRawBytes = 64 * D;  // e4m3 K half [64][D] or V half [128][D/2]
-  static constexpr bool kTurns = D == 128;  // the softmax warpgroups take turns
-  static constexpr int kSoftmaxRegs = kTurns ? 168 : 144, kControlRegs = kTurns ? 88 : 112, kConvRegs = kControlRegs;
+  static constexpr bool kTwo = D == 128;  // two accumulators and buffers of Q, output by the converter warps
+  static constexpr int kSoftmaxRegs = 144, kControlRegs = 112, kConvRegs = 112;
   static_assert(2 * kSoftmaxRegs + kControlRegs + kConvRegs <= 4 * kTilesLaunchRegs, "more than the launch's registers");
-  static constexpr int kAhead = kTurns ? 2 : 1;  // QK^T issued ahead of PV, in tiles
-  static constexpr int kQBufs = kTurns ? 2 : 1;
-  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 5) : (D == 256 ? 5 : 7);
+  static constexpr int kQBufs = kTwo ? 2 : 1;
+  static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 5) : (D == 256 ? 5 : 8);
   static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 5) : 0;
   static constexpr int kLandStages = kFp8 ? kRawStages : kOpStages;  // stages the TMA fills
   static constexpr int kKBox = 64 * 128;
   static constexpr int kVBox = 128 * 128;
   // A tile's scales are rewritten once its P has been consumed: among the items
-  // in their order, V of tile J is at most 2 J + kAhead + 1, K of tile J + k at
-  // least 2 (J + k) - kAhead, and an item is converted once the one kOpStages
-  // before it was consumed.
-  static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 2 * kAhead + 2) / 2 : 0;
-  static constexpr int kOutBytes = kTurns ? 8 * 4096 : 0;  // output rows on their way out, 4 KB a softmax warp
+  // in their order, V of tile J is at most 2 J + 2, K of tile J + k at least
+  // 2 (J + k) - 1, and an item is converted once the one kOpStages before it was
+  // consumed.
+  static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 4) / 2 : 0;
+  static constexpr int kOutBytes = kTwo ? kTilesConvWarps * 4096 : 0;  // output rows on their way out
   static constexpr int kOpOff = kQBufs * kQBytes;
   static constexpr int kRawOff = kOpOff + kOpStages * kOpBytes;
   static constexpr int kOutOff = kRawOff + kRawStages * kRawBytes;
   static constexpr int kScaleOff = kOutOff + kOutBytes;  // float k[128], v[128], int vmax[4]
   static constexpr int kScaleBuf = 2 * kTileN * 4 + 16;
-  // Row factors of a segment, float[128] each.  Q of a segment is written once
-  // QK^T of the one kQBufs before it is done, and QK^T of a tile once the scores
-  // two tiles back were read: so a softmax warpgroup may be three segments behind
-  // (of one tile each) with kTurns, one without.
-  static constexpr int kFactorBufs = kTurns ? 4 : 2;
+  // Row factors of a segment, float[128] each, and (kTwo) its rows' sums of either
+  // warpgroup and references.  Q of a segment is written once QK^T of the one
+  // kQBufs before it is done, and QK^T of a tile is issued after PV two tiles
+  // back: a softmax warpgroup may be three segments (of one tile each) behind Q
+  // with kTwo, one without.  The same PV, if it is a segment's first, waits for the
+  // output of the segment two before it: the softmax warps are at most three
+  // segments ahead of the output.
+  static constexpr int kSegBufs = kTwo ? 4 : 2;
   static constexpr int kFactorOff = kScaleOff + kScaleBufs * kScaleBuf;
-  static constexpr int kRedOff = kFactorOff + (kFp8 ? kFactorBufs * kTileM * 4 : 0);
-  static constexpr int kBarOff = kRedOff + (kTurns ? 6 : 4) * kTileM * 4;
-  // q_ready[2], q_empty[2], rows[4], o_free, s_free[2], part[2], land_full[NL], land_empty[NR], op_full[NS],
-  // op_empty[NS], s_full[2], p_full[2], o_done[2], teardown, ref[2], scale[NB],
-  // seg_full[], seg_empty[]
-  static constexpr int kNumBars = 13 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs + 2 * kTileSegments;
+  static constexpr int kRedOff = kFactorOff + (kFp8 ? kSegBufs * kTileM * 4 : 0);
+  static constexpr int kBarOff = kRedOff + (4 + (kTwo ? 3 * kSegBufs : 0)) * kTileM * 4;
+  // q_ready[2], q_empty[2], rows[4], o_free[2], sums[4], seg_o[2], land_full[NL],
+  // land_empty[NR], op_full[NS], op_empty[NS], s_full[2], p_full[2], o_done[2],
+  // teardown, ref[2], scale[NB], seg_full[], seg_empty[]
+  static constexpr int kNumBars = 16 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs + 2 * kTileSegments;
   static constexpr int kMiscOff = (kBarOff + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kSegOff = kMiscOff + 16;  // TileSegment[kTileSegments]
   static constexpr int kPlanOff = kSegOff + kTileSegments * sizeof(TileSegment);  // ChunkPlanShared
@@ -121,8 +120,7 @@ struct TilesSmem {
 // A warp's 32 rows (a lane each), O * inv_l of kCols TMEM columns from t_o, to
 // `dst` (NULL: not written), bf16 or fp32.  128 bytes of each row at a time turn
 // in 4 KB of shared memory, so that eight lanes store 128 bytes of one row (a
-// lane storing its own row touches 32 lines with every instruction: 3700 cycles
-// a unit).
+// lane storing its own row touches 32 lines with every instruction).
 template <int kCols, bool kBf16, typename T>
 __device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, uint8_t* turn, int lane) {
   constexpr int kStep = kBf16 ? 64 : 32;  // columns of 128 bytes
@@ -261,17 +259,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   // the segment's last QK^T has read Q (MMA commit, both CTAs);
   auto bar_q_empty = [&](int sg) { return bars + 16 + 8u * (sg & 1); };
   // this CTA's row factors written (four of them: see kFactorBufs).
-  auto bar_rows = [&](int sg) { return bars + 32 + 8u * (sg & (L::kFactorBufs - 1)); };
-  const uint32_t bar_o_free = bars + 64;  // leader: O of the segment read by every softmax warp of both CTAs
-  // Leader: scores of the buffer in registers (kTurns: its next QK^T may be issued).
-  auto bar_s_free = [&](int b) { return bars + 72 + 8u * b; };
-  // kTurns: the other warpgroup's part of a segment's sums, by segment parity.
-  auto bar_part = [&](int sg) { return bars + 88 + 8u * (sg & 1); };
-  auto bar_land_full = [&](int s) { return bars + 8u * (13 + s); };
-  auto bar_land_empty = [&](int s) { return bars + 8u * (13 + NL + s); };
-  auto bar_op_full = [&](int s) { return bars + 8u * (13 + NL + NR + s); };
-  auto bar_op_empty = [&](int s) { return bars + 8u * (13 + NL + NR + NS + s); };
-  constexpr int kB2 = 13 + NL + NR + 2 * NS;
+  auto bar_rows = [&](int sg) { return bars + 32 + 8u * (sg & (L::kSegBufs - 1)); };
+  // Leader: O of the segment read by every warp of both CTAs that writes it out (two
+  // of them with kTwo).
+  auto bar_o_free = [&](int sg) { return bars + 64 + 8u * (L::kTwo ? sg & 1 : 0); };
+  // kTwo: the segment's sums and references are in shared memory;
+  auto bar_sums = [&](int sg) { return bars + 80 + 8u * (sg & (L::kSegBufs - 1)); };
+  // its last PV is done (MMA commit, both CTAs).
+  auto bar_seg_o = [&](int sg) { return bars + 112 + 8u * (sg & 1); };
+  auto bar_land_full = [&](int s) { return bars + 8u * (16 + s); };
+  auto bar_land_empty = [&](int s) { return bars + 8u * (16 + NL + s); };
+  auto bar_op_full = [&](int s) { return bars + 8u * (16 + NL + NR + s); };
+  auto bar_op_empty = [&](int s) { return bars + 8u * (16 + NL + NR + NS + s); };
+  constexpr int kB2 = 16 + NL + NR + 2 * NS;
   auto bar_s_full = [&](int b) { return bars + 8u * (kB2 + b); };
   auto bar_p_full = [&](int b) { return bars + 8u * (kB2 + 2 + b); };
   auto bar_o = [&](int b) { return bars + 8u * (kB2 + 4 + b); };
@@ -296,25 +296,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       mbar_init(bar_q_ready(b), box.q_copy ? 1 : 2 * kTilesConvWarps);
       mbar_init(bar_q_empty(b), 1);
     }
-    for (int b = 0; b < L::kFactorBufs; ++b) mbar_init(bar_rows(b), kTilesConvWarps);
+    for (int b = 0; b < L::kSegBufs; ++b) {
+      mbar_init(bar_rows(b), kTilesConvWarps);
+      if (L::kTwo) mbar_init(bar_sums(b), 8);
+    }
     for (int s = 0; s < NL; ++s) mbar_init(bar_land_full(s), 1);
     for (int s = 0; s < NR; ++s) mbar_init(bar_land_empty(s), kTilesConvWarps);
     for (int s = 0; s < NS; ++s) {
-      mbar_init(bar_op_full(s), 2 * kTilesConvWarps);
+      // e4m3: every converter warp; bf16: the leader's producer twice, with the
+      // bytes of both CTAs, or (V cleared past the sequence) each CTA once.
+      mbar_init(bar_op_full(s), kFp8 ? 2 * kTilesConvWarps : 2);
       mbar_init(bar_op_empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_s_full(b), 1);
-      // One arrive per softmax warp that does the tile, of both CTAs.
-      mbar_init(bar_p_full(b), L::kTurns ? 2 * 4 : 2 * 8);
-      mbar_init(bar_s_free(b), 2 * 4);
+      mbar_init(bar_p_full(b), 2 * 8);  // one arrive per softmax warp of both CTAs
       mbar_init(bar_o(b), 1);
-      mbar_init(bar_ref(b), L::kTurns ? 128 : 256);
+      mbar_init(bar_ref(b), 256);
+      if (L::kTwo || b == 0) mbar_init(bar_o_free(b), L::kTwo ? 2 * kTilesConvWarps : 2 * 8);
+      mbar_init(bar_seg_o(b), 1);
     }
     for (int b = 0; b < NB; ++b) mbar_init(bar_scale(b), kTilesConvWarps);
-    mbar_init(bar_o_free, L::kTurns ? 2 * 4 : 2 * 8);
-    mbar_init(bar_part(0), 128);
-    mbar_init(bar_part(1), 128);
     for (int b = 0; b < kTileSegments; ++b) {
       mbar_init(bar_seg_full(b), 1);
       mbar_init(bar_seg_empty(b), 8 + 1 + 1 + 1 + kTilesConvWarps);  // every warp that reads them
@@ -364,19 +366,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   };
   // Keys of tile kt that the sequence has (may be 0 when it has none at all).
   auto tile_valid = [&](const ChunkUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
-  // The items of the range in the order of their loads, conversions and MMAs: K
-  // of a tile kAhead tiles before V of its own place (without kTurns, within a
-  // segment: Q has one buffer).  body(is_v, unit, tile, tiles before it, segment,
-  // segment's first tile, its last) until it returns false.
+  // The items of the range in the order of their loads, conversions and MMAs: K of
+  // a tile ahead of V of the tile before it (one buffer of Q: within a segment).
+  // body(is_v, unit, tile, tiles before it, segment, the segment's first tile, its
+  // last) until it returns false.
   auto for_each_item = [&](auto&& body) -> bool {
-    if constexpr (!L::kTurns) {
+    if constexpr (!L::kTwo) {
       uint32_t J = 0;
       return for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int sg) -> bool {
         if (!body(false, un, kt0, J, sg, true, kt0 + 1 == kt1)) return false;
 #pragma unroll 1
         for (int kt = kt0; kt < kt1; ++kt, ++J) {
           if (kt + 1 < kt1 && !body(false, un, kt + 1, J + 1, sg, false, kt + 2 == kt1)) return false;
-          if (!body(true, un, kt, J, sg, kt == kt0, false)) return false;
+          if (!body(true, un, kt, J, sg, kt == kt0, kt + 1 == kt1)) return false;
         }
         return true;
       });
@@ -394,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       while (true) {
         for (int vt = v0; vt < v1; ++vt, ++vj) {
 #pragma unroll 1
-          while (more && kj <= vj + L::kAhead) {
+          while (more && kj <= vj + 1) {
             if (!body(false, k, kt, kj, kseg, kt == k0, kt + 1 == k1)) return false;
             ++kj;
             if (++kt == k1) {
@@ -402,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
               kt = k0;
             }
           }
-          if (!body(true, v, vt, vj, vseg, vt == v0, false)) return false;
+          if (!body(true, v, vt, vj, vseg, vt == v0, vt + 1 == v1)) return false;
         }
         if (!get_segment(++vseg, v, v0, v1)) return *abort_flag == 0;
         put_back(vseg);
@@ -423,73 +425,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     const bool elected = elect_one();
     if (warp == kProducerWarp) {
       // ---------------------------------------------------- TMA producer --
-      uint32_t c = 0;
+      // This warp's instructions set the pace of short tiles (with two divisions, a
+      // table entry loaded and a modulus a copy, 1400 cycles an item): where it
+      // stands is carried on from item to item.
       if (elected) {
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
       }
-      int seq = -1, cached_lb = -1, cached_page = 0;
-      auto page_of = [&](const ChunkUnit& un, int lb) -> int {
-        if (un.seq == seq && lb == cached_lb) return cached_page;
-        int b = lb >= p.batch.table_width ? -1
-                : p.batch.tables          ? p.batch.tables[un.seq * p.batch.table_stride + lb]
-                                          : un.seq;  // the expanded copy
+      const int bs = p.pool.block_size;
+      // Where K and V (a tile behind) stand: a lane holds one of 32 entries of the
+      // sequence's table from `first`; row `at` of page `lb` is next.
+      struct Cursor {
+        int seq = -1, first = 0, page = 0, key = -1, lb = 0, at = 0;
+      } cur_k, cur_v;
+      auto page_of = [&](Cursor& w) -> int {
+        if (!p.batch.tables) return w.seq;  // the expanded copy
+        if (w.lb < w.first || w.lb >= w.first + 32) {
+          w.first = w.lb;
+          w.page = w.lb + lane < p.batch.table_width ? p.batch.tables[w.seq * p.batch.table_stride + w.lb + lane] : -1;
+        }
+        int b = __shfl_sync(0xffffffffu, w.page, w.lb - w.first);
         if (b < 0 || b >= p.pool.blocks) {  // reported; block 0 keeps the load in bounds
           if (elected) atomicCAS(err, 0, kErrBlockTable);
           b = 0;
         }
-        seq = un.seq;
-        cached_lb = lb;
-        return cached_page = b;
+        return b;
       };
       // Rows [key0, key0 + n) of K or V of one head; row 0 of `dst` is key0.
-      auto load_rows = [&](const ChunkUnit& un, bool is_v, int key0, int n, uint32_t dst, uint32_t full) {
+      // bf16: `full` is a cluster address.
+      auto load_rows = [&](auto v, Cursor& w, const ChunkUnit& un, int key0, int n, uint32_t dst, uint32_t full) {
+        constexpr bool is_v = decltype(v)::value;
         const int step = is_v ? box.v_rows : box.k_rows;
+        if (w.seq != un.seq || w.key != key0) {
+          if (w.seq != un.seq) w.first = INT_MIN;
+          w.seq = un.seq;
+          w.lb = key0 / bs;
+          w.at = key0 - w.lb * bs;
+        }
         for (int r = 0; r < n; r += step) {
-          const int key = key0 + r;
-          const int pg = page_of(un, key / p.pool.block_size), at = key % p.pool.block_size;
-          if (!elected) continue;
-          if (kFp8) {
-            if (is_v)
-              tma_load_5d(dst + r * (D / 2), &tm_v, static_cast<int>(rank) * (D / 2), at, un.head, 1, pg, full);
-            else
-              tma_load_5d(dst + r * D, &tm_k, 0, at, un.head, 0, pg, full);
-          } else if (box.all_cols) {  // {64 elements, rows, columns, head, 2 page + K/V}
-            if (is_v)
-              tma_load_5d(dst + r * D, &tm_v, 0, at, static_cast<int>(rank) * (D / 128), un.head, 2 * pg + 1, full);
-            else
-              tma_load_5d(dst, &tm_k, 0, at, 0, un.head, 2 * pg, full);
-          } else if (is_v) {
-            for (int b = 0; b < D / 128; ++b)
-              tma_load_5d(dst + b * L::kVBox + r * 128, &tm_v, 0, at, static_cast<int>(rank) * (D / 128) + b, un.head,
-                          2 * pg + 1, full);
-          } else {
-            for (int b = 0; b < D / 64; ++b)
-              tma_load_5d(dst + b * L::kKBox + r * 128, &tm_k, 0, at, b, un.head, 2 * pg, full);
+          const int pg = page_of(w);
+          if (elected) {
+            if (kFp8) {
+              if (is_v)
+                tma_load_5d(dst + r * (D / 2), &tm_v, static_cast<int>(rank) * (D / 2), w.at, un.head, 1, pg, full);
+              else
+                tma_load_5d(dst + r * D, &tm_k, 0, w.at, un.head, 0, pg, full);
+            } else if (box.all_cols) {  // {64 elements, rows, columns, head, 2 page + K/V}
+              if (is_v)
+                tma_load_5d_pair(dst + r * D, &tm_v, 0, w.at, static_cast<int>(rank) * (D / 128), un.head, 2 * pg + 1, full);
+              else
+                tma_load_5d_pair(dst, &tm_k, 0, w.at, 0, un.head, 2 * pg, full);
+            } else if (is_v) {
+              for (int b = 0; b < D / 128; ++b)
+                tma_load_5d_pair(dst + b * L::kVBox + r * 128, &tm_v, 0, w.at, static_cast<int>(rank) * (D / 128) + b,
+                                 un.head, 2 * pg + 1, full);
+            } else {
+              for (int b = 0; b < D / 64; ++b)
+                tma_load_5d_pair(dst + b * L::kKBox + r * 128, &tm_k, 0, w.at, b, un.head, 2 * pg, full);
+            }
+          }
+          w.at += step;  // a divisor of the page's rows
+          if (w.at == bs) {
+            w.at = 0;
+            ++w.lb;
           }
         }
+        w.key = -1;
+        if (n == (is_v ? 128 : 64)) {  // on to the next tile
+          w.key = key0 + kTileN;
+          if (!is_v)
+            for (w.at += 64; w.at >= bs; w.at -= bs) ++w.lb;
+        }
       };
-      auto issue = [&](const ChunkUnit& un, bool is_v, int kt) {
-        const int st = c % NL;
+      uint32_t c = 0, parity = 1;
+      int st = 0;
+      const uint32_t own_bars = kFp8 ? bars : mapa_shared(bars, rank), leader_bars = mapa_shared(bars, 0);
+      auto issue = [&](auto v, Cursor& w, const ChunkUnit& un, int kt) {
+        constexpr bool is_v = decltype(v)::value;
         const uint32_t empty = kFp8 ? bar_land_empty(st) : bar_op_empty(st);
-        if (!__all_sync(0xffffffffu, mbar_wait(empty, ((c / NL) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty)))
-          return false;
+        if (!__all_sync(0xffffffffu, mbar_wait(empty, parity, abort_flag, err, kErrWaitKvEmpty))) return false;
         const uint32_t dst = kFp8 ? sRaw + st * L::kRawBytes : sOp + st * L::kOpBytes;
-        const int off = is_v ? 0 : 64 * static_cast<int>(rank), most = is_v ? 128 : 64;
-        const int n = min(most, max(0, tile_valid(un, kt) - off));
-        const int step = is_v ? box.v_rows : box.k_rows;
-        const int rows = (n + step - 1) / step * step;
-        if (elected) mbar_arrive_expect_tx(bar_land_full(st), rows * (is_v ? D / 2 : D) * (kFp8 ? 1 : 2));
-        load_rows(un, is_v, kt * kTileN + off, n, dst, bar_land_full(st));
+        constexpr int row_bytes = (is_v ? D / 2 : D) * (kFp8 ? 1 : 2), most = is_v ? 128 : 64;
+        const int valid = tile_valid(un, kt);
+        const int off = is_v ? 0 : 64 * static_cast<int>(rank);
+        const int n = min(most, max(0, valid - off));
+        // Bytes of CTA rk's half, in whole copies (a power of two of rows).
+        auto bytes_of = [&](int rk) {
+          const int step = is_v ? box.v_rows : box.k_rows;
+          return ((min(most, max(0, valid - (is_v ? 0 : 64 * rk))) + step - 1) & -step) * row_bytes;
+        };
+        uint32_t full;
+        if (kFp8 || (is_v && valid < kTileN)) {  // to this CTA's converters
+          if (elected) mbar_arrive_expect_tx(bar_land_full(st), bytes_of(static_cast<int>(rank)));
+          full = own_bars + (bar_land_full(st) - bars);
+        } else {
+          if (leader && elected) {
+            mbar_arrive_expect_tx(bar_op_full(st), valid >= kTileN ? 2 * most * row_bytes : bytes_of(0) + bytes_of(1));
+            mbar_arrive(bar_op_full(st));
+          }
+          full = leader_bars + (bar_op_full(st) - bars);
+        }
+        load_rows(v, w, un, kt * kTileN + off, n, dst, full);
         ++c;
+        if (++st == NL) {
+          st = 0;
+          parity ^= 1u;
+        }
         return true;
       };
       const bool ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool, bool) {
-        return issue(un, is_v, kt);
+        return is_v ? issue(std::true_type(), cur_v, un, kt) : issue(std::false_type(), cur_k, un, kt);
       });
-      if (!ok && elected)  // let this CTA's copies still in flight land before it exits
+      // After a failure: let the copies still in flight land (bf16: those of both
+      // CTAs are counted on the leader).
+      if (!ok && elected && (kFp8 || leader))
         for (uint32_t i = (c > (uint32_t)NL ? c - NL : 0); i < c; ++i)
-          mbar_wait_teardown(bar_land_full(i % NL), (i / NL) & 1u);
+          mbar_wait_teardown(kFp8 ? bar_land_full(i % NL) : bar_op_full(i % NL), (i / NL) & 1u);
     }
     if (warp == kSegmentWarp) {
       // ------------------------------------------------ walks the range --
@@ -558,7 +609,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         const uint64_t q_desc = q_desc0 + (L::kQBufs > 1 ? (seg & 1) * (L::kQBytes >> 4) : 0);
         const uint32_t s_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
         const int st = c % NS;
-        if (L::kTurns && jg >= 2 && !wait(bar_s_free(jg & 1), ((jg - 2) >> 1) & 1u, kErrWaitSFull)) return false;
         if (!wait(bar_op_full(st), (c / NS) & 1u, kErrWaitKvFull)) return false;
         tc_fence_after();
         const uint64_t kd = k_desc + static_cast<uint32_t>(st) * (L::kOpBytes >> 4);
@@ -573,33 +623,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ++c;
         return true;
       };
-      auto pv = [&](uint32_t jg, bool first, int seg) {
-        // O of the previous segment has been read out.
-        if (first && seg > 0 && !wait(bar_o_free, (seg - 1) & 1u, kErrWaitODone)) return false;
+      auto pv = [&](uint32_t jg, bool first, bool last, int seg) {
+        // The output of the segment that had this accumulator has been read.
+        constexpr int kO = L::kTwo ? 2 : 1;
+        if (first && seg >= kO && !wait(bar_o_free(seg - kO), ((seg - kO) / kO) & 1u, kErrWaitODone)) return false;
         if (!wait(bar_p_full(jg & 1), (jg >> 1) & 1u, kErrWaitPFull)) return false;
         const int st = c % NS;
         if (!wait(bar_op_full(st), (c / NS) & 1u, kErrWaitKvFull)) return false;
         tc_fence_after();
-        const uint32_t p_tmem = tmem + (L::kTurns ? kTurnsP + (jg & 1) * (kTileN / 2) : kTmemS0 + (jg & 1) * kTileN);
+        const uint32_t p_tmem = tmem + kTmemS0 + (jg & 1) * kTileN;
+        const uint32_t o_tmem = tmem + (L::kTwo ? (seg & 1) * D : 0);
         const uint64_t vd = v_desc + static_cast<uint32_t>(st) * (L::kOpBytes >> 4);
         const uint64_t vd2 = vd + (v_half >> 4);
         if (elected) {
 #pragma unroll
           for (int kk = 0; kk < kTileN / 16; ++kk) {
-            // A = P (kTurns: its own TMEM columns; else over S, each warpgroup's
-            // in its own half), B = V half, MN-major: 64-dim chunks v_col apart,
-            // 8-key groups 1 KB apart.
-            umma_ts_pair(tmem, p_tmem + kk * 8 + (!L::kTurns && kk >= 4 ? 32 : 0), (kk >= 4 ? vd2 : vd) + kk * (2048 >> 4),
+            // A = P (over S, each warpgroup's in its own half), B = V half, MN-major:
+            // 64-dim chunks v_col apart, 8-key groups 1 KB apart.
+            umma_ts_pair(o_tmem, p_tmem + kk * 8 + (kk >= 4 ? 32 : 0), (kk >= 4 ? vd2 : vd) + kk * (2048 >> 4),
                          idesc_pv, (!first || kk > 0) ? 1u : 0u);
           }
           umma_commit_pair(bar_op_empty(st), kChunkBothCtas);
           umma_commit_pair(bar_o(jg & 1), kChunkBothCtas);
+          if (L::kTwo && last) umma_commit_pair(bar_seg_o(seg), kChunkBothCtas);
         }
         ++c;
         return true;
       };
       for_each_item([&](bool is_v, const ChunkUnit&, int, uint32_t J, int seg, bool first, bool last) {
-        if (is_v) return pv(J, first, seg);
+        if (is_v) return pv(J, first, last, seg);
         if (first) {
           if (!wait(bar_q_ready(seg), (seg >> 1) & 1u, kErrWaitQ)) return false;
           tc_fence_after();
@@ -617,7 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     __syncwarp();
   } else if (warp >= kTilesConvWarp0) {
     setmaxnreg_dec<L::kConvRegs>();
-    // ------------------------------- Q gather, e4m3 -> f16, V past the end --
+    // ----------- Q gather, e4m3 -> f16, V past the end; D = 128: the output --
     const int ct = threadIdx.x - kTilesConvWarp0 * 32;
     const int cw = warp - kTilesConvWarp0;
     const ConvGeo geo_k = conv_geo(ct, D / 64, L::kKBox);
@@ -688,17 +740,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           mbar_arrive(bar_land_empty(ls));
           mbar_arrive_remote(mapa_shared(bar_op_full(os), 0));
         }
-      } else {
-        if (!wait_all(bar_land_full(ls), (c / NL) & 1u, kErrWaitKvFull)) return false;
-        if (is_v && valid < kTileN) {
-          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t op = sOp + os * L::kOpBytes;
-          for (int i = max(0, valid) * 8 + ct; i < kTileN * 8; i += kTilesConvThreads)
-            for (int b = 0; b < D / 128; ++b) sts128(op + b * v_col + (i >= 64 * 8 ? v_half : 0) + i * 16, zero);
-          fence_proxy_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(mapa_shared(bar_op_full(os), 0));
       }
       ++c;
       return true;
@@ -708,7 +749,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       // kFlight loads a lane in flight, the first of them before the wait for the
       // previous segment's QK^T to be done with the buffer.
       constexpr int kSide = 256 / D;  // rows side by side in a warp
-      constexpr int kFlight = kFp8 ? 4 : 16;  // (the conversion unrolled 16 times costs the instruction cache more)
+      constexpr int kFlight = 4;
       const int side = lane / (D / 8), ch = lane % (D / 8);
 #pragma unroll 1
       for (int r0 = cw * 32; r0 < cw * 32 + 32; r0 += kFlight * kSide) {
@@ -741,7 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             for (int o = D / 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int e = m == 0 ? 0 : max(static_cast<int>(m >> 23) - 127 - 14, -112);
             const float down = exp2_of_int(-e);
-            if (ch == 0) factors[(segs & (L::kFactorBufs - 1)) * kTileM + r] = p.scale_log2 * exp2_of_int(e);
+            if (ch == 0) factors[(segs & (L::kSegBufs - 1)) * kTileM + r] = p.scale_log2 * exp2_of_int(e);
             x[u] = make_uint4(pack_f16x2(f[0] * down, f[1] * down), pack_f16x2(f[2] * down, f[3] * down),
                               pack_f16x2(f[4] * down, f[5] * down), pack_f16x2(f[6] * down, f[7] * down));
           }
@@ -757,25 +798,100 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       ++segs;
       return true;
     };
-    for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool first, bool) {
-      if (!is_v && first && !box.q_copy && !gather_q(un)) return false;
-      return item(un, is_v, kt);
-    });
+    // kTwo: the output of segment sg.  Called once all that its last PV waits for is
+    // on its way, Q and the first K of the next segment included.
+    const float* seg_sums = red + 4 * kTileM;  // [kSegBufs]{l of either warpgroup, m}[128]
+    auto write_out = [&](const ChunkUnit& un, int kt0, int kt1, int sg) -> bool {
+      if (!wait_all(bar_sums(sg), (sg / L::kSegBufs) & 1u, kErrWaitRed) ||
+          !wait_all(bar_seg_o(sg), (sg >> 1) & 1u, kErrWaitODone))
+        return false;
+      tc_fence_after();
+      const float* sums = seg_sums + (sg & (L::kSegBufs - 1)) * 3 * kTileM;
+      const float l = sums[ct] + sums[kTileM + ct], m = sums[2 * kTileM + ct];
+      const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+      const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
+      const bool live = r < un.rows;
+      const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
+      uint8_t* turn = smem + L::kOutOff + cw * 4096;
+      const int slot = part_slot(un, kt0, kt1, pair);
+      if (slot < 0) {
+        const int at = un.row0 + r;
+        __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
+                             static_cast<long long>(un.q0 + at / p.group) * p.out_row;
+        store_rows<D, true>(t_o, inv_l, live ? out : nullptr, turn, lane);
+      } else {
+        const long long pr = static_cast<long long>(slot) * kUnitRows + r;
+        if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
+        store_rows<D, false>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, turn, lane);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(mapa_shared(bar_o_free(sg), 0));
+      return true;
+    };
+    ChunkUnit last_un;
+    int last0 = 0, last1 = 0, last_seg = -1;
+    auto write_last = [&]() { return !L::kTwo || last_seg < 0 || write_out(last_un, last0, last1, last_seg); };
+    bool ok;
+    if constexpr (kFp8) {
+      ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int seg, bool first, bool last) {
+        if (!is_v && first && !gather_q(un)) return false;
+        if (!item(un, is_v, kt)) return false;
+        if (L::kTwo && is_v) {
+          if (first) {
+            if (!write_last()) return false;
+            last_un = un;
+            last0 = kt;
+            last_seg = seg;
+          }
+          if (last) last1 = kt + 1;
+        }
+        return true;
+      });
+    } else {
+      // The last tile of a sequence that ends inside it: V rows past its end,
+      // in the stage of that item (its place in the order of for_each_item).
+      const uint32_t tiles = static_cast<uint32_t>(plan.end - plan.x);
+      uint32_t J = 0, used = 0;  // bit st: parity of stage st's landings so far
+      ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int seg) -> bool {
+        if (!box.q_copy && !gather_q(un)) return false;
+        if (L::kTwo) {
+          if (!write_last()) return false;
+          last_un = un;
+          last0 = kt0;
+          last1 = kt1;
+          last_seg = seg;
+        }
+        J += kt1 - kt0;
+        const int valid = tile_valid(un, kt1 - 1);
+        if (valid >= kTileN) return true;
+        const uint32_t last = J - 1;
+        const uint32_t at = L::kTwo ? last + min(last + 2, tiles) : 2 * last + 1;
+        const int st = at % NS;
+        if (!wait_all(bar_land_full(st), (used >> st) & 1u, kErrWaitKvFull)) return false;
+        used ^= 1u << st;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t op = sOp + st * L::kOpBytes;
+        for (int i = max(0, valid) * 8 + ct; i < kTileN * 8; i += kTilesConvThreads)
+          for (int b = 0; b < D / 128; ++b) sts128(op + b * v_col + (i >= 64 * 8 ? v_half : 0) + i * 16, zero);
+        fence_proxy_async_smem();
+        named_bar_sync(3, kTilesConvThreads);
+        if (ct == 0) mbar_arrive_remote(mapa_shared(bar_op_full(st), 0));
+        return true;
+      });
+    }
+    if (ok) write_last();
     __syncwarp();
   } else {
     setmaxnreg_inc<L::kSoftmaxRegs>();
     // ---------------------------------------- softmax / correction / epilogue --
     constexpr int kOCols = D / 2;
-    constexpr int kKeys = L::kTurns ? kTileN : kTileN / 2;  // a thread's keys of a tile
+    constexpr int kKeys = kTileN / 2;  // a thread's keys of a tile
     const int wg = warp >> 2;
     const int row = threadIdx.x & (kTileM - 1);  // == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // kTurns: refs[2][128], each row's reference after a tile, by the tile's
-    // parity, and sums[2][128] (m, l), one warpgroup's part of a segment for the
-    // other, by the segment's parity.  Else the halves' maxima [tile
-    // parity][2][128], and at the end refs, sums [2][128].
-    float* refs = red;
-    float* sums = red + 2 * kTileM;
+    // red: the halves' maxima [tile parity][2][128].
+    float* sums = red;  // (one accumulator: a segment's sums, once its maxima were read)
     uint32_t J = 0;
     // The leader keeps the pair's record.
     ChunkRecord& rec = p.work.tile_rec[pair];
@@ -789,18 +905,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int at = un.row0 + (live ? r : un.rows - 1);
       const int pos = un.kvlen - un.qlen + at / p.group;  // last key this row sees
       const uint32_t Jend = J + (kt1 - kt0);
+      const uint32_t t_o = t_row + (L::kTwo ? (seg & 1) * D : 0) + wg * kOCols;
       float rf = p.scale_log2;
-      // (A warpgroup without a tile here needs none, and does not wait.)
-      if (kFp8 && (!L::kTurns || J + ((J ^ wg) & 1u) < Jend)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(seg), (seg / L::kFactorBufs) & 1u, abort_flag, err, kErrWaitQ));
-        if (ok) rf = factors[(seg & (L::kFactorBufs - 1)) * kTileM + row];
+      if (kFp8) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(seg), (seg / L::kSegBufs) & 1u, abort_flag, err, kErrWaitQ));
+        if (ok) rf = factors[(seg & (L::kSegBufs - 1)) * kTileM + row];
       }
-      float m = -INFINITY;  // (this warpgroup's last) reference: log2 units, V's exponents included
-      float l = 0.f;        // its keys' weights over 2^m
+      float m = -INFINITY;  // reference of both halves: log2 units, V's exponents included
+      float l = 0.f;        // this half's weights over 2^m
 
       // This thread's scores of tile jg: loaded, K's scales applied, keys past
       // the row's position at -inf.  `ev` gets the tile's largest V exponent.
-      const uint32_t first_key = L::kTurns ? 0 : wg * kKeys;
+      const uint32_t first_key = wg * kKeys;
       auto scores = [&](uint32_t jg, float (&s)[kKeys], float& ev) -> bool {
         if (!__all_sync(0xffffffffu, mbar_wait(bar_s_full(jg & 1), (jg >> 1) & 1u, abort_flag, err, kErrWaitSFull)))
           return false;
@@ -809,11 +925,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
         tmem_wait_ld();
-        if (L::kTurns) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(mapa_shared(bar_s_free(jg & 1), 0));
-        }
         ev = 0.f;
         if (kScaled) {
           if (!__all_sync(0xffffffffu, mbar_wait(bar_scale(jg % (NB ? NB : 1)), (jg / (NB ? NB : 1)) & 1u, abort_flag,
@@ -881,140 +992,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       // The reference moves when a tile's largest weight would pass 2^8 (and
       // from its start, as soon as a key is seen); O of the tiles before goes
       // over to the new one once their last product is in it.
-      if constexpr (L::kTurns) {
-        for (uint32_t jg = J + ((J ^ wg) & 1u); jg < Jend && ok; jg += 2) {
-          float s[kKeys], ev;
-          ok = scores(jg, s, ev);
-          if (!ok) break;
-          const float tmax = row_max(s) * rf + ev;
-          // (A segment's first tile waits too, though it starts anew: the steps
-          // go in the tiles' order, or a barrier could get two phases ahead.)
-          if (jg > 0) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait(bar_ref(wg ^ 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitRed));
-            if (!ok) break;
-          }
-          const float before = jg > J ? refs[(wg ^ 1) * kTileM + row] : -INFINITY;
-          const bool need = tmax > before + kRescaleThreshold;
-          const float ref = need ? tmax : before;
-          refs[wg * kTileM + row] = ref;
-          mbar_arrive(bar_ref(wg));
-          if (ref != m) {  // it moved since this warpgroup's last tile
-            l *= ex2_approx(m - ref);
-            m = ref;
-          }
-          // P's columns are free once the product before last is done.
-          if (jg >= 2) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar_o(wg), ((jg - 2) >> 1) & 1u, abort_flag, err, kErrWaitODone));
-            if (!ok) break;
-            tc_fence_after();
-          }
-          l += probs(jg, s, ref, t_row + kTurnsP + wg * (kTileN / 2));
-          if (jg > J && __any_sync(0xffffffffu, need)) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait(bar_o(wg ^ 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
-            if (!ok) break;
-            tc_fence_after();
-            rescale_o<D>(t_row, need ? ex2_approx(before - ref) : 1.f);
-          }
-          release(jg);
-        }
-      } else {
-        for (uint32_t jg = J; jg < Jend && ok; ++jg) {
-          const int b = jg & 1;
-          float s[kKeys], ev;
-          ok = scores(jg, s, ev);
-          if (!ok) break;
-          const float pmax = row_max(s);
-          red[(b * 2 + wg) * kTileM + row] = pmax;
-          mbar_arrive(bar_ref(b));
-          // Pass 0 (tiles after the first): speculative P with the current
-          // reference, before the other half's maximum is known.  Pass 1:
-          // exchange the half maxima; P is recomputed only when some row's
-          // moved past the threshold.
-          float tile_sum = 0.f;
-          float alpha = 1.f;
-          bool redo = false;
+      for (uint32_t jg = J; jg < Jend && ok; ++jg) {
+        const int b = jg & 1;
+        float s[kKeys], ev;
+        ok = scores(jg, s, ev);
+        if (!ok) break;
+        const float pmax = row_max(s);
+        red[(b * 2 + wg) * kTileM + row] = pmax;
+        mbar_arrive(bar_ref(b));
+        // Pass 0 (tiles after the first): speculative P with the current
+        // reference, before the other half's maximum is known.  Pass 1:
+        // exchange the half maxima; P is recomputed only when some row's
+        // moved past the threshold.
+        float tile_sum = 0.f;
+        float alpha = 1.f;
+        bool redo = false;
 #pragma unroll 1
-          for (int pass = jg > J ? 0 : 1; pass < 2; ++pass) {
-            if (pass == 1) {
-              ok = __all_sync(0xffffffffu, mbar_wait(bar_ref(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
-              if (!ok) break;
-              const float tmax = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]) * rf + ev;
-              const bool need = tmax > m + kRescaleThreshold;
-              redo = __any_sync(0xffffffffu, need) || jg == J;
-              if (need) {
-                alpha = ex2_approx(m - tmax);  // 0 from the start
-                m = tmax;
-                l *= alpha;
-              }
-              if (!redo) break;
-            }
-            tile_sum = probs(jg, s, m, t_row + kTmemS0 + b * kTileN + wg * kKeys);
-          }
-          if (!ok) break;
-          l += tile_sum;
-          if (jg > J && redo) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
+        for (int pass = jg > J ? 0 : 1; pass < 2; ++pass) {
+          if (pass == 1) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_ref(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
             if (!ok) break;
-            tc_fence_after();
-            rescale_o<kOCols>(t_row + wg * kOCols, alpha);
+            const float tmax = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]) * rf + ev;
+            const bool need = tmax > m + kRescaleThreshold;
+            redo = __any_sync(0xffffffffu, need) || jg == J;
+            if (need) {
+              alpha = ex2_approx(m - tmax);  // 0 from the start
+              m = tmax;
+              l *= alpha;
+            }
+            if (!redo) break;
           }
-          release(jg);
+          tile_sum = probs(jg, s, m, t_row + kTmemS0 + b * kTileN + wg * kKeys);
         }
+        if (!ok) break;
+        l += tile_sum;
+        if (jg > J && redo) {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
+          if (!ok) break;
+          tc_fence_after();
+          rescale_o<kOCols>(t_o, alpha);
+        }
+        release(jg);
       }
       const uint32_t jl = Jend - 1;  // the last tile
       J = Jend;
-      const int slot = part_slot(un, kt0, kt1, pair);
-      __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
-                           static_cast<long long>(un.q0 + at / p.group) * p.out_row;
-      const long long pr = static_cast<long long>(slot) * kUnitRows + r;
-      // l over both warpgroups' keys at the last reference, `top`; no key seen:
-      // zeros.
-      auto finish = [&](float m_other, float l_other, float& top) {
-        top = fmaxf(m, m_other);
-        const float l_tot = (m == top ? l : l * ex2_approx(m - top)) +
-                            (m_other == top ? l_other : l_other * ex2_approx(m_other - top));
-        if (slot >= 0 && live && (L::kTurns || wg == 0))
-          p.work.tile_lse[pr] = l_tot == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __log2f(l_tot);
-        return l_tot == 0.f ? 0.f : 1.f / l_tot;
-      };
-      float top;
-      if constexpr (L::kTurns) {
-        float2* part = reinterpret_cast<float2*>(sums) + (seg & 1) * kTileM + row;
+      if constexpr (L::kTwo) {
         if (!ok) return false;
-        if ((jl & 1u) != static_cast<uint32_t>(wg)) {  // the other one writes the output
-          *part = make_float2(m, l);
-          mbar_arrive(bar_part(seg));
-          return true;
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_part(seg), (seg >> 1) & 1u, abort_flag, err, kErrWaitRed) &&
-                                         mbar_wait(bar_o(wg), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
-        if (!ok) return false;
-        tc_fence_after();
-        const float2 other = *part;
-        const float inv_l = finish(other.x, other.y, top);
-        uint8_t* turn = smem + L::kOutOff + warp * 4096;
-        if (slot < 0) store_rows<D, true>(t_row, inv_l, live ? out : nullptr, turn, lane);
-        else store_rows<D, false>(t_row, inv_l, live ? p.work.tile_o + pr * D : nullptr, turn, lane);
+        float* part = red + 4 * kTileM + (seg & (L::kSegBufs - 1)) * 3 * kTileM;
+        part[wg * kTileM + row] = l;
+        if (wg == 0) part[2 * kTileM + row] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sums(seg));
+        return true;
       } else {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar_o(jl & 1), (jl >> 1) & 1u, abort_flag, err, kErrWaitODone));
-        refs[wg * kTileM + row] = m;  // (the maxima there were read before the last product)
         sums[wg * kTileM + row] = l;
         ok = named_bar_and(1, kSoftmaxThreads, ok && (*abort_flag == 0));
         if (!ok) return false;
         tc_fence_after();
-        const float inv_l = finish(refs[(wg ^ 1) * kTileM + row], sums[(wg ^ 1) * kTileM + row], top);
+        l += sums[(wg ^ 1) * kTileM + row];
         // Both read: the next segment may reuse the slots.
         named_bar_sync(2, kSoftmaxThreads);
-        if (slot < 0) store_o_bf16<kOCols>(t_row + wg * kOCols, inv_l, out + wg * kOCols, live);
-        else store_o_partial<kOCols>(t_row + wg * kOCols, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
+        const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+        const int slot = part_slot(un, kt0, kt1, pair);
+        if (slot < 0) {
+          __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
+                               static_cast<long long>(un.q0 + at / p.group) * p.out_row;
+          store_o_bf16<kOCols>(t_o, inv_l, out + wg * kOCols, live);
+        } else {
+          const long long pr = static_cast<long long>(slot) * kUnitRows + r;
+          if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
+          store_o_partial<kOCols>(t_o, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(bar_o_free(seg), 0));
+        return true;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(mapa_shared(bar_o_free, 0));
-      return true;
     });
     if (keeps && !done) clear_record(rec);  // after a failure nothing is merged
   }
