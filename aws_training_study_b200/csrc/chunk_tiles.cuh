@@ -49,9 +49,9 @@ enum : int { kCacheBf16 = 0, kCacheE4m3 = 1, kCacheScaled = 2 };
 
 constexpr int kTilesConvWarps = 4;
 constexpr int kTilesConvThreads = 32 * kTilesConvWarps;
-// Four warpgroups: softmax 0 and 1, K/V copies, MMA, segment and Q warps, converters;
-// they split the launch's 512 x 128 registers (TilesSmem).
-constexpr int kSegmentWarp = 10, kQWarp = 11;
+// Four warpgroups: softmax 0 and 1; K/V copies, MMA, segments and Q, K/V copies;
+// converters.  They split the launch's 512 x 128 registers (TilesSmem).
+constexpr int kSegmentWarp = 10, kProducerWarp2 = 11;
 constexpr int kTilesConvWarp0 = 12;
 constexpr int kTilesThreads = 512;
 constexpr int kTilesLaunchRegs = 128;
@@ -79,8 +79,13 @@ struct TilesSmem {
   static_assert(2 * kSoftmaxRegs + kControlRegs + kConvRegs <= 4 * kTilesLaunchRegs, "more than the launch's registers");
   static constexpr int kQBufs = kTwo ? 2 : 1;
   static constexpr int kOpStages = kFp8 ? (D == 256 ? 3 : 5) : (D == 256 ? 5 : 8);
-  static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 5) : 0;
+  static constexpr int kRawStages = kFp8 ? (D == 256 ? 3 : 6) : 0;
   static constexpr int kLandStages = kFp8 ? kRawStages : kOpStages;  // stages the TMA fills
+  // Warps that issue the copies.  Two: one the even items, one the odd (an item
+  // takes a warp some 1000 cycles, as long as half a tile's MMAs take with D = 128),
+  // and, with an even number of stages, each sees every filling of its own.
+  static constexpr int kProducers = kTwo ? 2 : 1;
+  static_assert(kLandStages % kProducers == 0, "a stage has one producer");
   static constexpr int kKBox = 64 * 128;
   static constexpr int kVBox = 128 * 128;
   // A tile's scales are rewritten once its P has been consumed: among the items
@@ -319,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     for (int b = 0; b < NB; ++b) mbar_init(bar_scale(b), kTilesConvWarps);
     for (int b = 0; b < kTileSegments; ++b) {
       mbar_init(bar_seg_full(b), 1);
-      mbar_init(bar_seg_empty(b), 8 + 1 + 1 + 1 + kTilesConvWarps);  // every warp that reads them
+      mbar_init(bar_seg_empty(b), 8 + L::kProducers + 1 + kTilesConvWarps);  // every warp that reads them
     }
     mbar_init(bar_td, 1);
     *abort_flag = 0;
@@ -423,11 +428,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     // code that only one lane runs, every operand of an MMA or a copy takes its
     // way through a vector register (100 cycles an MMA; the tensor cores waited).
     const bool elected = elect_one();
-    if (warp == kProducerWarp) {
-      // ---------------------------------------------------- TMA producer --
-      // This warp's instructions set the pace of short tiles (with two divisions, a
-      // table entry loaded and a modulus a copy, 1400 cycles an item): where it
+    if (warp == kProducerWarp || (L::kProducers == 2 && warp == kProducerWarp2)) {
+      // --------------------------------------------------- TMA producers --
+      // Their instructions set the pace of short tiles (with two divisions, a table
+      // entry loaded and a modulus a copy, 1400 cycles an item): where a cursor
       // stands is carried on from item to item.
+      const uint32_t mine = warp == kProducerWarp ? 0 : 1;
       if (elected) {
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
@@ -502,6 +508,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const uint32_t own_bars = kFp8 ? bars : mapa_shared(bars, rank), leader_bars = mapa_shared(bars, 0);
       auto issue = [&](auto v, Cursor& w, const ChunkUnit& un, int kt) {
         constexpr bool is_v = decltype(v)::value;
+        if (c % L::kProducers != mine) return true;
         const uint32_t empty = kFp8 ? bar_land_empty(st) : bar_op_empty(st);
         if (!__all_sync(0xffffffffu, mbar_wait(empty, parity, abort_flag, err, kErrWaitKvEmpty))) return false;
         const uint32_t dst = kFp8 ? sRaw + st * L::kRawBytes : sOp + st * L::kOpBytes;
@@ -526,34 +533,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           full = leader_bars + (bar_op_full(st) - bars);
         }
         load_rows(v, w, un, kt * kTileN + off, n, dst, full);
+        return true;
+      };
+      const bool ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool, bool) {
+        if (!(is_v ? issue(std::true_type(), cur_v, un, kt) : issue(std::false_type(), cur_k, un, kt))) return false;
         ++c;
         if (++st == NL) {
           st = 0;
           parity ^= 1u;
         }
         return true;
-      };
-      const bool ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool, bool) {
-        return is_v ? issue(std::true_type(), cur_v, un, kt) : issue(std::false_type(), cur_k, un, kt);
       });
       // After a failure: let the copies still in flight land (bf16: those of both
       // CTAs are counted on the leader).
       if (!ok && elected && (kFp8 || leader))
         for (uint32_t i = (c > (uint32_t)NL ? c - NL : 0); i < c; ++i)
-          mbar_wait_teardown(kFp8 ? bar_land_full(i % NL) : bar_op_full(i % NL), (i / NL) & 1u);
+          if (i % L::kProducers == mine) mbar_wait_teardown(kFp8 ? bar_land_full(i % NL) : bar_op_full(i % NL), (i / NL) & 1u);
     }
     if (warp == kSegmentWarp) {
-      // ------------------------------------------------ walks the range --
+      // ------------- walks the range; Q, where a copy brings it --
+      // Rows token * group + head of a unit as boxes of {64 elements, group, 128 /
+      // group tokens, two columns}; tokens past the sequence bring other rows,
+      // whose results nobody reads.  Both CTAs' bytes count on the leader.
       ChunkWalk<true> walk;
       walk.init(p, plan, err);
       ChunkUnit un;
-      int kt0, kt1;
-      for (int sg = 0;; ++sg) {
+      int kt0, kt1, sg = 0, landed = 0;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, kErrWaitQ));
+      };
+      for (;; ++sg) {
         const bool more = walk.next(p, err, un, kt0, kt1);
-        if (sg >= kTileSegments &&
-            !__all_sync(0xffffffffu, mbar_wait(bar_seg_empty(sg), ((sg / kTileSegments) & 1u) ^ 1u, abort_flag, err,
-                                               kErrWaitQ)))
-          break;
+        if (sg >= kTileSegments) ok = wait(bar_seg_empty(sg), ((sg / kTileSegments) & 1u) ^ 1u);
+        if (!ok) break;
         if (elected) {
           TileSegment& s = segments[sg % kTileSegments];
           s.un = un;
@@ -562,20 +575,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           mbar_arrive(bar_seg_full(sg));
         }
         if (!more) break;
-      }
-    }
-    if (warp == kQWarp) {
-      // ------------------------------------- Q, where a copy brings it --
-      // Rows token * group + head of a unit as boxes of {64 elements, group, 128
-      // / group tokens, two columns}; tokens past the sequence bring other
-      // rows, whose results nobody reads.  Both CTAs' bytes count on the leader.
-      uint32_t landed = 0;
-      const bool ok = for_each_segment([&](const ChunkUnit& un, int, int, int sg) -> bool {
-        if (!box.q_copy) return true;
-        if (sg >= L::kQBufs &&
-            !__all_sync(0xffffffffu, mbar_wait(bar_q_empty(sg - L::kQBufs), ((sg - L::kQBufs) >> 1) & 1u, abort_flag,
-                                               err, kErrWaitQ)))
-          return false;
+        if (!box.q_copy) continue;
+        if (sg >= L::kQBufs) ok = wait(bar_q_empty(sg - L::kQBufs), ((sg - L::kQBufs) >> 1) & 1u);
+        if (!ok) break;
         if (elected) {
           if (leader) mbar_arrive_expect_tx(bar_q_ready(sg), 2 * L::kQBytes);
           const int token = un.q0 + un.row0 / p.group + static_cast<int>(rank) * (kTileM / p.group);
@@ -584,11 +586,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
                              un.head, mapa_shared(bar_q_ready(sg), 0));
         }
         landed = sg + 1;
-        return true;
-      });
-      // After a failure: let the copies land.
-      if (!ok && leader && elected && landed > 0)
-        mbar_wait_teardown(bar_q_ready(landed - 1), ((landed - 1) >> 1) & 1u);
+      }
+      // Let the copies land, if nobody waits for them any more.
+      if ((!ok || *abort_flag) && leader && elected)
+        for (int i = max(0, landed - L::kQBufs); i < landed; ++i) mbar_wait_teardown(bar_q_ready(i), (i >> 1) & 1u);
     }
     if (warp == kMmaWarp && !leader) for_each_segment([](const ChunkUnit&, int, int, int) { return true; });
     if (warp == kMmaWarp && leader) {
