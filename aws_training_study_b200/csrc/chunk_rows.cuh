@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     // -------------------------------------------------------- producer --
     if (kFp8) setmaxnreg_dec<kRowsProducerRegs>();
     if (warp > L::kWarps) return;
+    // The whole warp walks and waits, one elected lane issues (chunk_tiles.cuh).
+    const bool elected = elect_one();
     bool ok = true;
     const bool scaled = kFp8 && p.pool.scales;
     const int bs = p.pool.block_size;
@@ -171,12 +173,10 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       for (int key = k0; key < k1; key += L::kStageKeys) {
         const int st = c % L::kStages;
         const int boxes = (min(L::kStageKeys, k1 - key) + box_rows - 1) >> box_shift;
-        if (lane == 0) {
-          ok = mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty);
-          if (ok) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (scaled ? 2 * box_rows : 0)));
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty));
         if (!ok) break;
+        if (elected) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (scaled ? 2 * box_rows : 0)));
         for (int b = 0; b < boxes; ++b, ++i) {
           if (i == 32) {
             i = 0;
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
             }
           }
           const int pg = 2 * __shfl_sync(0xffffffffu, page, i), at = __shfl_sync(0xffffffffu, row, i);
-          if (lane == 0) {
+          if (elected) {
             tma_load_5d(sbase + st * L::kStageBytes + b * box_bytes, &tm_kv, 0, at, 0, un.head, pg, bar_full(st));
             if (scaled)
               tma_load_3d(sScale + st * L::kScaleStage + b * scale_slot, &tm_scale, at, un.head, pg, bar_full(st));
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         ++c;
       }
     }
-    if (!ok && lane == 0)  // let the copies in flight land before the CTA ends
+    if (!ok && elected)  // let the copies in flight land before the CTA ends
       for (uint32_t i = c > L::kStages ? c - L::kStages : 0; i < c; ++i)
         mbar_wait_teardown(bar_full(i % L::kStages), (i / L::kStages) & 1u);
     return;
