@@ -70,6 +70,7 @@ struct ChunkParams {
   int max_chunk;
   float scale_log2;
   int small_ctas, tile_pairs;  // grids of the two kernels (0 pairs: not launched)
+  int small_y, tile_y;         // blocks that merge a unit of either kind
   int* status;
 };
 
@@ -100,9 +101,10 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-// CTAs (or pairs) that a list of `steps` is cut for: at least one step each.
-__host__ __device__ __forceinline__ long long chunk_ranges(long long steps, int grid) {
-  return steps < grid ? (steps > 1 ? steps : 1) : grid;
+// CTAs (or pairs) that a list of `steps` is cut for: at least one step each (at
+// least 2 or 4 took the same times, 16 to 256 tokens over 500 to 32768).
+__device__ __forceinline__ long long chunk_ranges(long long steps, int grid) {
+  return min(max(steps, 1LL), static_cast<long long>(grid));
 }
 
 // Steps of rows [row0, row0 + rows) of a sequence: tiles up to the last row's
@@ -456,13 +458,12 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
         make_uint2(pack_bf16x2(acc[k] * inv, acc[k + 1] * inv), pack_bf16x2(acc[k + 2] * inv, acc[k + 3] * inv));
 }
 
-constexpr int kCombineSmallY = kSmallRows / 2;  // 4 warps a row
-constexpr int kCombineTileY = kUnitRows / 8;    // a warp a row
+constexpr int kCombineSmallW = 4, kCombineTileW = 1;  // warps a row
 
 template <int D>
 __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
   grid_dependency_wait();
-  const int small_blocks = p.small_ctas * kCombineSmallY;
+  const int small_blocks = p.small_ctas * p.small_y;
   if (blockIdx.x == 0) {
     int err = 0;
     for (int i = threadIdx.x; i < p.small_ctas + 2 * p.tile_pairs; i += 256) {
@@ -479,12 +480,12 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
     }
   }
   if (blockIdx.x < small_blocks) {
-    combine_rows<D, 4>(p, p.work.small_rec, p.small_ctas, kSmallRows, p.work.small_o, p.work.small_lse,
-                       blockIdx.x / kCombineSmallY, blockIdx.x % kCombineSmallY);
+    combine_rows<D, kCombineSmallW>(p, p.work.small_rec, p.small_ctas, kSmallRows, p.work.small_o, p.work.small_lse,
+                       blockIdx.x / p.small_y, blockIdx.x % p.small_y);
   } else {
     const int b = blockIdx.x - small_blocks;
-    combine_rows<D, 1>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse, b / kCombineTileY,
-                       b % kCombineTileY);
+    combine_rows<D, kCombineTileW>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse,
+                                   b / p.tile_y, b % p.tile_y);
   }
 }
 

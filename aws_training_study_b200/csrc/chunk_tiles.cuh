@@ -93,11 +93,9 @@ struct TilesSmem {
   // 2 (J + k) - 1, and an item is converted once the one kOpStages before it was
   // consumed.
   static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 4) / 2 : 0;
-  static constexpr int kOutBytes = kTwo ? kTilesConvWarps * 4096 : 0;  // output rows on their way out
   static constexpr int kOpOff = kQBufs * kQBytes;
   static constexpr int kRawOff = kOpOff + kOpStages * kOpBytes;
-  static constexpr int kOutOff = kRawOff + kRawStages * kRawBytes;
-  static constexpr int kScaleOff = kOutOff + kOutBytes;  // float k[128], v[128], int vmax[4]
+  static constexpr int kScaleOff = kRawOff + kRawStages * kRawBytes;  // float k[128], v[128], int vmax[4]
   static constexpr int kScaleBuf = 2 * kTileN * 4 + 16;
   // Row factors of a segment, float[128] each, and (kTwo) its rows' sums of either
   // warpgroup and references.  Q of a segment is written once QK^T of the one
@@ -122,43 +120,78 @@ struct TilesSmem {
   static_assert(kRawOff % 1024 == 0 && kScaleOff % 16 == 0 && kSegOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
 };
 
-// A warp's 32 rows (a lane each), O * inv_l of kCols TMEM columns from t_o, to
-// `dst` (NULL: not written), bf16 or fp32.  128 bytes of each row at a time turn
-// in 4 KB of shared memory, so that eight lanes store 128 bytes of one row (a
-// lane storing its own row touches 32 lines with every instruction).
-template <int kCols, bool kBf16, typename T>
-__device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, uint8_t* turn, int lane) {
-  constexpr int kStep = kBf16 ? 64 : 32;  // columns of 128 bytes
-  const uint32_t base = smem_u32(turn);
-#pragma unroll 1
-  for (int c = 0; c < kCols; c += kStep) {
+// 16 rows (lanes l / 4 and l / 4 + 8) of 32 TMEM columns: o[4 i], o[4 i + 1] are
+// columns 8 i + 2 (l % 4), + 1 of the first row, o[4 i + 2], o[4 i + 3] of the second.
+__device__ __forceinline__ void tmem_ld16x32(uint32_t t, float (&o)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(t));
 #pragma unroll
-    for (int h = 0; h < kStep / 32; ++h) {
-      float o[32];
-      tmem_ld32(t_o + c + 32 * h, o);
+  for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(r[i]);
+}
+
+// A warp's 32 rows (a lane each), O * inv_l of kCols TMEM columns from t_o, to
+// `dst` (NULL: not written), bf16 or fp32.  Four lanes hold and store 64 bytes of
+// a row (a lane storing its own row touched 32 lines with every instruction: 11600
+// cycles a unit, D = 256).
+template <int kCols, typename T>
+__device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, int lane) {
+  constexpr bool kBf16 = sizeof(T) == 2;
+  const int q = lane & 3;
+  const bool odd = q & 1, high = q & 2;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {  // rows 16 h ..
+    float inv[2];
+    T* to[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 16 * h + 8 * e + lane / 4;
+      inv[e] = __shfl_sync(0xffffffffu, inv_l, r);
+      to[e] = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+    }
+#pragma unroll 2
+    for (int c = 0; c < kCols; c += 32) {
+      float o[16];
+      tmem_ld16x32(t_o + (static_cast<uint32_t>(16 * h) << 16) + c, o);
       tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] *= inv_l;
+      for (int e = 0; e < 2; ++e) {
+        if (kBf16) {
+          // Lane q gets the four words of columns 8 q ..: a 4 x 4 transposition.
+          uint32_t w[4];
 #pragma unroll
-      for (int q = 0; q < (kBf16 ? 4 : 8); ++q) {
-        const uint4 v = kBf16 ? make_uint4(pack_bf16x2(o[(8 * q) & 31], o[(8 * q + 1) & 31]),
-                                           pack_bf16x2(o[(8 * q + 2) & 31], o[(8 * q + 3) & 31]),
-                                           pack_bf16x2(o[(8 * q + 4) & 31], o[(8 * q + 5) & 31]),
-                                           pack_bf16x2(o[(8 * q + 6) & 31], o[(8 * q + 7) & 31]))
-                              : make_uint4(__float_as_uint(o[4 * q]), __float_as_uint(o[4 * q + 1]),
-                                           __float_as_uint(o[4 * q + 2]), __float_as_uint(o[4 * q + 3]));
-        sts128(base + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4), v);
+          for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(o[4 * i + 2 * e] * inv[e], o[4 * i + 2 * e + 1] * inv[e]);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const uint32_t x = __shfl_xor_sync(0xffffffffu, odd ? w[i] : w[i + 1], 1);
+            w[i] = odd ? x : w[i];
+            w[i + 1] = odd ? w[i + 1] : x;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = __shfl_xor_sync(0xffffffffu, high ? w[i] : w[i + 2], 2);
+            w[i] = high ? x : w[i];
+            w[i + 2] = high ? w[i + 2] : x;
+          }
+          if (to[e]) *reinterpret_cast<uint4*>(to[e] + c + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          // Even lanes get four columns of group i, odd ones of group i + 1.
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float a0 = o[4 * i + 2 * e] * inv[e], a1 = o[4 * i + 2 * e + 1] * inv[e];
+            const float b0 = o[4 * i + 4 + 2 * e] * inv[e], b1 = o[4 * i + 4 + 2 * e + 1] * inv[e];
+            const float x = __shfl_xor_sync(0xffffffffu, odd ? a0 : b0, 1);
+            const float y = __shfl_xor_sync(0xffffffffu, odd ? a1 : b1, 1);
+            if (to[e])
+              *reinterpret_cast<float4*>(to[e] + c + 8 * (i + (odd ? 1 : 0)) + 2 * (q & 2)) =
+                  odd ? make_float4(x, y, b0, b1) : make_float4(a0, a1, x, y);
+          }
+        }
       }
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + lane / 8;
-      const unsigned long long at = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r);
-      const uint4 v = lds128(base + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-      if (at) reinterpret_cast<uint4*>(at + c * sizeof(T))[lane & 7] = v;
-    }
-    __syncwarp();
   }
 }
 
@@ -173,12 +206,13 @@ struct TileBoxes {
 
 // The pages of sequences with tile units as bf16: sequence s is one block of
 // `copy`, [2][Hkv][copy_rows][D].  Bound by HBM (1 byte read, 2 written an
-// element); a thread block takes the rows of one head of K or V of a page at a
-// time.
+// element); a thread block takes 64 rows of one head of K or V at a time (pages
+// of a multiple of 64 tokens; else 16).
 struct ExpandParams {
   ChunkParams c;
   __nv_bfloat16* copy;
   int copy_rows;  // table_width * block_size, up to a multiple of 128
+  int item_rows;  // 64 or 16
 };
 
 template <int D>
@@ -186,25 +220,30 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
   constexpr int kPerRow = D / 16;
   const PoolView& pool = p.c.pool;
   const int per_page = 2 * pool.heads;
-  const long long items = static_cast<long long>(p.c.batch.seqs) * p.c.batch.table_width * per_page;
+  const int pieces = pool.block_size / p.item_rows;
+  const long long items = static_cast<long long>(p.c.batch.seqs) * p.c.batch.table_width * pieces * per_page;
   __shared__ int s_ignored;  // lengths the attention reports itself
   if (threadIdx.x == 0) s_ignored = 0;
   __syncthreads();
+  grid_launch_dependents();
   for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const long long page = it / per_page;
-    const int which = static_cast<int>(it - page * per_page);
-    const int s = static_cast<int>(page / p.c.batch.table_width), lb = static_cast<int>(page - static_cast<long long>(s) * p.c.batch.table_width);
+    const long long piece = it / per_page;
+    const int which = static_cast<int>(it - piece * per_page);
+    const long long page = piece / pieces;
+    const int row0 = static_cast<int>(piece - page * pieces) * p.item_rows;
+    const int s = static_cast<int>(page / p.c.batch.table_width);
+    const int lb = static_cast<int>(page - static_cast<long long>(s) * p.c.batch.table_width);
     const ChunkSeq q = chunk_seq<true>(p.c, s, &s_ignored);
-    const int n = min(pool.block_size, q.kvlen - lb * pool.block_size);
+    const int n = min(p.item_rows, q.kvlen - lb * pool.block_size - row0);
     if (q.tiles == 0 || n <= 0) continue;
     const int blk = p.c.batch.tables[s * p.c.batch.table_stride + lb];
     const bool found = blk >= 0 && blk < pool.blocks;
     if (!found && threadIdx.x == 0) atomicCAS(p.c.status, 0, kErrBlockTable);
-    const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size;
+    const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size + row0;
     const uint4* codes = reinterpret_cast<const uint4*>(pool.data + src * D);
     const uint8_t* scales = pool.scales ? pool.scales + src : nullptr;
     uint4* dst = reinterpret_cast<uint4*>(
-        p.copy + ((static_cast<long long>(s) * per_page + which) * p.copy_rows + static_cast<long long>(lb) * pool.block_size) * D);
+        p.copy + ((static_cast<long long>(s) * per_page + which) * p.copy_rows + static_cast<long long>(lb) * pool.block_size + row0) * D);
     for (int e0 = threadIdx.x; e0 < n * kPerRow; e0 += 4 * 256) {
       uint4 x[4];
       uint32_t sc[4];
@@ -229,6 +268,7 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
       }
     }
   }
+  grid_dependency_wait();  // the small units, as in chunk_tiles_kernel
 }
 
 template <int D, int kCache>
@@ -438,6 +478,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
       }
+      if (!p.batch.tables) grid_dependency_wait();  // the expanded copy is there
       const int bs = p.pool.block_size;
       // Where K and V (a tile behind) stand: a lane holds one of 32 entries of the
       // sequence's table from `first`; row `at` of page `lb` is next.
@@ -813,17 +854,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
       const bool live = r < un.rows;
       const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
-      uint8_t* turn = smem + L::kOutOff + cw * 4096;
       const int slot = part_slot(un, kt0, kt1, pair);
       if (slot < 0) {
         const int at = un.row0 + r;
         __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                              static_cast<long long>(un.q0 + at / p.group) * p.out_row;
-        store_rows<D, true>(t_o, inv_l, live ? out : nullptr, turn, lane);
+        store_rows<D>(t_o, inv_l, live ? out : nullptr, lane);
       } else {
         const long long pr = static_cast<long long>(slot) * kUnitRows + r;
         if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
-        store_rows<D, false>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, turn, lane);
+        store_rows<D>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -1060,11 +1100,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         if (slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                                static_cast<long long>(un.q0 + at / p.group) * p.out_row;
-          store_o_bf16<kOCols>(t_o, inv_l, out + wg * kOCols, live);
+          store_rows<kOCols>(t_o, inv_l, live ? out + wg * kOCols : nullptr, lane);
         } else {
           const long long pr = static_cast<long long>(slot) * kUnitRows + r;
           if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
-          store_o_partial<kOCols>(t_o, inv_l, p.work.tile_o + pr * D + wg * kOCols, live);
+          store_rows<kOCols>(t_o, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr, lane);
         }
         tc_fence_before();
         __syncwarp();
@@ -1080,6 +1120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
+  grid_dependency_wait();  // the small units: the merge waits for them through this kernel
   if (threadIdx.x == 0) p.work.tile_rec[blockIdx.x].err = *static_cast<volatile int*>(err);
   if (warp == kMmaWarp) {
     tc_fence_after();

@@ -125,9 +125,12 @@ struct ChunkLayout {
 };
 
 // An e4m3 cache is expanded for the tile units from kExpandRows rows a KV head
-// on (8 tiles), while the copy of all sequences' tables stays within
-// kExpandBytes.  EXPAND_FIGURES
-constexpr int64_t kExpandRows = 2048;
+// on (4 tiles), while the copy of all sequences' tables stays within
+// kExpandBytes.  In place against expanded, us: heads of 256 over 32768 tokens, 512
+// rows 101 / 101, 1024 126 / 118, 2048 183 / 153, 8192 517 / 378; over 131072, 512
+// 196 / 235, 1024 312 / 312, 2048 554 / 476, 8192 1795 / 1373; heads of 128 over
+// 32768, 512 198 / 169, 1024 345 / 238, 4096 1254 / 579.
+constexpr int64_t kExpandRows = 1024;
 constexpr int64_t kExpandBytes = int64_t(1) << 30;
 
 bool has_tiles(int32_t max_chunk, int32_t group) { return static_cast<int64_t>(max_chunk) * group > pcp::kSmallRows; }
@@ -271,6 +274,26 @@ int allow_smem(int bytes, int regs = 0) {
   return PCP_OK;
 }
 
+// A kernel whose blocks may be placed while the one before it ends; it waits for
+// that one itself where it needs its results, and at the latest at its own end, so
+// that whoever waits for it has waited for both.
+template <typename... Args>
+int launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+                  const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args...));
+  return PCP_OK;
+}
+
 template <int D, bool kFp8>
 int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
   using L = pcp::RowsSmem<D, kFp8>;
@@ -307,19 +330,20 @@ int launch_tiles(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t
     PCP_TRY(make_rows_map(&tv, pool, box.v_rows, box.all_cols ? D / 128 : 1, 1));
   }
   PCP_TRY((allow_smem<pcp::chunk_tiles_kernel<D, kCache>>(L::kBytes, pcp::kTilesLaunchRegs)));
-  pcp::chunk_tiles_kernel<D, kCache><<<2 * kPairs, pcp::kTilesThreads, L::kBytes, st>>>(tq, tk, tv, box, p);
-  CUDA_TRY(cudaGetLastError());
-  return PCP_OK;
+  return launch_behind(pcp::chunk_tiles_kernel<D, kCache>, 2 * kPairs, pcp::kTilesThreads, L::kBytes, st, tq, tk, tv,
+                       box, p);
 }
 
 // Tile units over the bf16 copy of their pages.
 template <int D>
 int launch_expanded(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, cudaStream_t st) {
   const int rows = copy_rows(pool.block_size, p.batch.table_width);
-  const pcp::ExpandParams e{p, static_cast<__nv_bfloat16*>(copy), rows};
-  const int64_t items = static_cast<int64_t>(p.batch.seqs) * p.batch.table_width * 2 * pool.num_kv_heads;
-  pcp::chunk_expand_kernel<D><<<static_cast<unsigned>(std::min<int64_t>(items, 8 * kCtas)), 256, 0, st>>>(e);
-  CUDA_TRY(cudaGetLastError());
+  const int item_rows = pool.block_size % 64 ? 16 : 64;
+  const pcp::ExpandParams e{p, static_cast<__nv_bfloat16*>(copy), rows, item_rows};
+  const int64_t items = static_cast<int64_t>(p.batch.seqs) * p.batch.table_width * 2 * pool.num_kv_heads *
+                        (pool.block_size / item_rows);
+  PCP_TRY(launch_behind(pcp::chunk_expand_kernel<D>, static_cast<unsigned>(std::min<int64_t>(items, 8 * kCtas)), 256, 0,
+                        st, e));
   // The copy as a cache of one page a sequence.
   pcp_pool_t dense = pool;
   dense.data = copy;
@@ -345,19 +369,7 @@ int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, 
     else if (pool.scales) PCP_TRY((launch_tiles<D, pcp::kCacheScaled>(pool, p, st)));
     else PCP_TRY((launch_tiles<D, pcp::kCacheE4m3>(pool, p, st)));
   }
-  // The merge's blocks may be placed while the kernel before it ends (it waits
-  // for that kernel itself).
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(p.small_ctas * pcp::kCombineSmallY + p.tile_pairs * pcp::kCombineTileY);
-  config.blockDim = dim3(256);
-  config.stream = st;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  CUDA_TRY(cudaLaunchKernelEx(&config, pcp::chunk_combine_kernel<D>, p));
-  return PCP_OK;
+  return launch_behind(pcp::chunk_combine_kernel<D>, p.small_ctas * p.small_y + p.tile_pairs * p.tile_y, 256, 0, st, p);
 }
 
 }  // namespace
@@ -482,6 +494,10 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
   p.small_ctas = kCtas;
   p.tile_pairs = has_tiles(max_chunk, group) ? kPairs : 0;
+  // Rows of the longest small and tile unit, over the rows a block merges.
+  const int64_t longest = std::min<int64_t>(max_chunk, batch->rows) * group;
+  p.small_y = static_cast<int>(ceil_div(std::min<int64_t>(longest, pcp::kSmallRows), 8 / pcp::kCombineSmallW));
+  p.tile_y = static_cast<int>(ceil_div(std::min<int64_t>(longest, pcp::kUnitRows), 8 / pcp::kCombineTileW));
   p.status = device_status;
   void* copy = w.expand ? ws + w.copy : nullptr;
   return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, copy, st) : launch_chunk<128>(*pool, p, copy, st);

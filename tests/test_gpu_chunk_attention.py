@@ -5,7 +5,7 @@ Tolerance, per element, with A = sum_j w_j |v_j| (w: the softmax's weights):
   * the output's rounding, half a step: 2^-8 |o|;
   * the weights' rounding before the second product: 2^-8 A in bf16 (bf16
     caches, and chunks of more than 32 rows a KV head in calls whose max_chunk
-    reaches 2048 rows, which read a bf16 copy of an e4m3 cache), 2^-11 A in f16
+    reaches 1024 rows, which read a bf16 copy of an e4m3 cache), 2^-11 A in f16
     (other e4m3 caches), and below f16's normal range half its least step, 2^-25,
     of weights whose largest is 1 or more: n 2^-25 max|v|;
   * the scores: fp32 sums over D / 16 tensor-core steps, each within 2^-22 of
@@ -105,7 +105,7 @@ class Case:
             o[h] = w @ v
             a = w @ v.abs()
             terms = (q[h].abs() @ k.abs().T * scale).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
-            expanded = max(self.new) * group >= 2048 and n * group > 32
+            expanded = max(self.new) * group >= 1024 and n * group > 32
             weights = 2.0 ** -8 if self.cache == "bf16" or expanded else 2.0 ** -11
             bound[h] = 2.0 ** -8 * o[h].abs() + weights * a + 2 * a * (cfg.head_dim / 16 * 2.0 ** -22 * terms + 2.0 ** -20)
             if self.cache != "bf16":
