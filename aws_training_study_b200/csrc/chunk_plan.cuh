@@ -114,6 +114,45 @@ __device__ __forceinline__ int unit_steps(int kvlen, int qlen, int last_row, int
   return max(1, (visible + kStepKeys - 1) / kStepKeys);
 }
 
+// Keys that every row from `row0` on sees (not positive: some row sees none).
+__device__ __forceinline__ int keys_all_see(int kvlen, int qlen, int row0, int group) {
+  return kvlen - qlen + row0 / group + 1;
+}
+
+// Non-finite values of V at a key that some rows of a unit see and others do
+// not: 0 * NaN would reach the others, so the kernels take zeros in their place,
+// note that they did, and the output is patched afterwards.  Of the elements d ..
+// d + 7 of V at `key`, those that are not finite (a bit each).
+template <int D>
+__device__ __noinline__ uint32_t nonfinite8(const ChunkParams& p, int seq, int head, int key, int d) {
+  const int bs = p.pool.block_size, lb = key / bs;
+  if (lb >= p.batch.table_width) return 0;
+  const int pg = p.batch.tables ? p.batch.tables[seq * p.batch.table_stride + lb] : seq;
+  if (pg < 0 || pg >= p.pool.blocks) return 0;
+  const long long at = (((pg * 2LL + 1) * p.pool.heads + head) * bs + key % bs) * D + d;
+  uint32_t bad = 0;
+  for (int i = 0; i < 8; ++i) {
+    const bool b = p.pool.bf16 ? (reinterpret_cast<const uint16_t*>(p.pool.data)[at + i] & 0x7F80) == 0x7F80
+                               : (p.pool.data[at + i] & 0x7F) == 0x7F;
+    bad |= (b ? 1u : 0u) << i;
+  }
+  return bad;
+}
+// The elements of a 32-bit word of two bf16 or four e4m3 codes that are not finite.
+template <bool kFp8>
+__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
+  return kFp8 ? __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu) : __vcmpeq2(w & 0x7F807F80u, 0x7F807F80u);
+}
+
+// Zeros in place of what is not finite; true if there was any.
+template <bool kFp8>
+__device__ __forceinline__ bool drop_nonfinite(uint4& x) {
+  const uint4 m = make_uint4(nonfinite_mask<kFp8>(x.x), nonfinite_mask<kFp8>(x.y), nonfinite_mask<kFp8>(x.z),
+                             nonfinite_mask<kFp8>(x.w));
+  x = make_uint4(x.x & ~m.x, x.y & ~m.y, x.z & ~m.z, x.w & ~m.w);
+  return (m.x | m.y | m.z | m.w) != 0;
+}
+
 // A sequence as a kernel sees it; `tiles` 0 unless it has units of that kind.
 struct ChunkSeq {
   int q0, qlen, kvlen;

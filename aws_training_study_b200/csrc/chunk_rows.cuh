@@ -107,7 +107,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
 template <int D, bool kFp8>
 __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     chunk_rows_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale,
-                      const int box_shift, const ChunkParams p) {
+                      const int box_shift, const __grid_constant__ ChunkParams p) {
   using L = RowsSmem<D, kFp8>;
   constexpr int kBoxElts = 128 / L::kElt;
   constexpr int kBoxSteps = kBoxElts / 16;  // MMA k steps of a box: 8 or 4
@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       mbar_init(bar_empty(s), L::kWarps);
     }
     *abort_flag = 0;
+    *reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4) = 0;
     plan.err = 0;
     fence_mbar_init();
   }
@@ -214,7 +215,9 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   const int part = warp % L::kTeam;          // this warp's 128 columns
   bool ok = true;
   if (threadIdx.x == 0) clear_record(rec);
-  while (walk.next(p, err, un, kt0, kt1)) {
+  // The number of the unit part if V had values taken for zeros (nonfinite8).
+  volatile int* patch = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  for (int unit = 1; walk.next(p, err, un, kt0, kt1); ++unit) {
     if (threadIdx.x == 0) note_part(rec, un, kt0, kt1);
     const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
     const bool two = un.rows > 16;  // two row tiles
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     const float f0 = row_factor[qt * 16 + gq], f1 = row_factor[qt * 16 + gq + 8];
     const int pos0 = row_pos[qt * 16 + gq], pos1 = row_pos[qt * 16 + gq + 8];
     // Keys that every live row of the tile sees: no comparison needed there.
-    const int all_see = un.kvlen - un.qlen + (un.row0 + qt * 16) / p.group + 1;
+    const int all_see = keys_all_see(un.kvlen, un.qlen, un.row0 + qt * 16, p.group);
     const bool scaled = kFp8 && p.pool.scales;
 
     float o[16][4];
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         const int left = k1 - key;  // keys of this group that are there
         const bool whole = left >= 16 && key + 16 <= all_see;
         float vs[4] = {1.f, 1.f, 1.f, 1.f};  // V scales of this lane's four keys
-        int ev = 127;                        // their largest exponent, biased
+        int ev = 127, ev1 = 127;             // their largest exponents, biased, of those that either row sees
         if (scaled) {
           const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
           ev = 0;
@@ -361,6 +364,18 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
             vs[2 * n] = __uint_as_float((vv & 0xFFu) << 23);
             vs[2 * n + 1] = __uint_as_float((vv >> 8) << 23);
             ev = max(ev, static_cast<int>(max(vv & 0xFFu, vv >> 8)));
+          }
+          ev1 = ev;
+          if (!whole) {
+            ev = ev1 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = key + 8 * (i / 2) + 2 * i4 + i % 2, e = static_cast<int>(__float_as_uint(vs[i]) >> 23);
+              if (at <= pos0) ev = max(ev, e);
+              if (at <= pos1) ev1 = max(ev1, e);
+            }
+#pragma unroll
+            for (int x = 1; x <= 2; x <<= 1) ev1 = max(ev1, __shfl_xor_sync(0xffffffffu, ev1, x));
           }
         }
         // Scores in log2 units, hidden keys at -inf.
@@ -387,7 +402,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         }
         if (scaled) {
           mx0 += static_cast<float>(ev - 127);
-          mx1 += static_cast<float>(ev - 127);
+          mx1 += static_cast<float>((whole ? ev : ev1) - 127);
         }
         // The reference moves when the largest weight would pass 2^8 (and
         // from its start); O and l follow.
@@ -437,6 +452,15 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
             if (2 * i4 + 8 >= left) v2 = zero;
             if (2 * i4 + 9 >= left) v3 = zero;
           }
+          if (!whole) {  // keys that some rows do not see: nothing that is not finite
+            const int look = all_see - key - 2 * i4;
+            bool found = false;
+            if (look <= 0) found |= drop_nonfinite<true>(v0);
+            if (look <= 1) found |= drop_nonfinite<true>(v1);
+            if (look <= 8) found |= drop_nonfinite<true>(v2);
+            if (look <= 9) found |= drop_nonfinite<true>(v3);
+            if (found) *patch = unit;
+          }
           const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
           const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
 #pragma unroll
@@ -454,6 +478,9 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         } else {
           const uint32_t z0 = (2 * i4 < left ? 0xFFFFu : 0u) | (2 * i4 + 1 < left ? 0xFFFF0000u : 0u);
           const uint32_t z1 = (2 * i4 + 8 < left ? 0xFFFFu : 0u) | (2 * i4 + 9 < left ? 0xFFFF0000u : 0u);
+          const int look = all_see - key - 2 * i4;
+          const uint32_t look0 = (look <= 0 ? 0xFFFFu : 0u) | (look <= 1 ? 0xFFFF0000u : 0u);
+          const uint32_t look1 = (look <= 8 ? 0xFFFFu : 0u) | (look <= 9 ? 0xFFFF0000u : 0u);
           const int vrow = lane & 15, vc = lane >> 4;
 #pragma unroll
           for (int b = 0; b < kWarpBoxes; ++b) {
@@ -462,6 +489,16 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
             for (int j = 0; j < 4; ++j) {
               uint32_t v[4];
               ldmatrix_x4_trans(vr + (((2 * j + vc) ^ (vrow & 7)) * 16), v);
+              if (!whole) {  // keys that some rows do not see: nothing that is not finite
+                uint32_t found = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t bad = nonfinite_mask<false>(v[i]) & ((i & 1) ? look1 : look0);
+                  v[i] &= ~bad;
+                  found |= bad & ((i & 1) ? z1 : z0);
+                }
+                if (found) *patch = unit;
+              }
               mma16816<false>(o[b * 8 + 2 * j], pa, v[0] & z0, v[1] & z1);
               mma16816<false>(o[b * 8 + 2 * j + 1], pa, v[2] & z0, v[3] & z1);
             }
@@ -563,6 +600,15 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no key seen: zeros
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] *= inv;
+      if (*patch == unit) {  // rare: see nonfinite8
+        const int first = keys_all_see(un.kvlen, un.qlen, un.row0 + 16 * t, p.group);
+        uint32_t bad = 0;
+        for (int key = max(first, k0); key < min(un.kvlen - un.qlen + (un.row0 + r) / p.group + 1, k1); ++key)
+          bad |= nonfinite8<D>(p, un.seq, un.head, key, d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((bad >> i) & 1u) f[i] = NAN;
+      }
       if (slot < 0) {
         const int row = un.row0 + r;
         Vec8<__nv_bfloat16>::store(p.out + static_cast<long long>(un.head * p.group + row % p.group) * p.out_head +

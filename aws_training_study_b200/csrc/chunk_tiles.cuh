@@ -57,11 +57,14 @@ constexpr int kTilesThreads = 512;
 constexpr int kTilesLaunchRegs = 128;
 constexpr uint16_t kChunkBothCtas = 3, kChunkLeader = 1;
 
+// A unit; keys from see_all on some rows do not see, from see_any on none does.
+struct TileUnit : ChunkUnit {
+  int see_all, see_any;
+};
 // A segment: the part [kt0, kt1) of a unit's key tiles; kt1 = 0 after the last.
 struct __align__(16) TileSegment {
-  ChunkUnit un;
+  TileUnit un;
   int kt0, kt1;
-  int pad[2];
 };
 // Segments on their way from the warp that walks the range to the others (each
 // walking by itself, the loads and divisions of a step took every role some 1500
@@ -113,7 +116,7 @@ struct TilesSmem {
   // teardown, ref[2], scale[NB], seg_full[], seg_empty[]
   static constexpr int kNumBars = 16 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs + 2 * kTileSegments;
   static constexpr int kMiscOff = (kBarOff + kNumBars * 8 + 15) / 16 * 16;
-  static constexpr int kSegOff = kMiscOff + 16;  // TileSegment[kTileSegments]
+  static constexpr int kSegOff = kMiscOff + 32;  // TileSegment[kTileSegments]
   static constexpr int kPlanOff = kSegOff + kTileSegments * sizeof(TileSegment);  // ChunkPlanShared
   static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
@@ -193,6 +196,7 @@ __device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, in
       }
     }
   }
+  __syncwarp();  // (the rows may be patched)
 }
 
 // How K and V tiles are copied.  A copy costs its issuer some 350 cycles
@@ -271,11 +275,27 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
   grid_dependency_wait();  // the small units, as in chunk_tiles_kernel
 }
 
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
+// NaN into the elements of an output row (of kCols columns from col0) whose column
+// of V has one among keys [key0, key1).  Rare, and slow.
+template <int D, int kCols, typename T>
+__device__ __noinline__ void patch_row(const ChunkParams& p, const ChunkUnit& un, int key0, int key1, T* dst, int col0) {
+  for (int d = 0; d < kCols; d += 8) {
+    uint32_t bad = 0;
+    for (int key = key0; key < key1; ++key) bad |= nonfinite8<D>(p, un.seq, un.head, key, col0 + d);
+    for (int i = 0; i < 8; ++i)
+      if ((bad >> i) & 1u) dst[d + i] = static_cast<T>(NAN);
+  }
+}
+
 template <int D, int kCache>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     chunk_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v,
-                       const TileBoxes box, const ChunkParams p) {
+                       const TileBoxes box, const __grid_constant__ ChunkParams p) {
   using L = TilesSmem<D, kCache>;
   constexpr bool kFp8 = L::kFp8;
   constexpr bool kScaled = kCache == kCacheScaled;
@@ -328,6 +348,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   TileSegment* segments = reinterpret_cast<TileSegment*>(smem + L::kSegOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  // By segment: its number + 1 if V had values that were taken for zeros
+  // (nonfinite8); set in both CTAs.  V of a segment is looked through after the
+  // item kOpStages before it was consumed, so at most three segments ahead of the
+  // output.
+  volatile int* patch = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 16);
+  auto set_patch = [&](int sg) {
+    for (uint32_t c = 0; c < 2; ++c)
+      st_cluster_u32(mapa_shared(sbase + L::kMiscOff + 16 + 4 * (sg & 3), c), sg + 1);
+  };
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   float* factors = reinterpret_cast<float*>(smem + L::kFactorOff);
 
@@ -349,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     for (int s = 0; s < NR; ++s) mbar_init(bar_land_empty(s), kTilesConvWarps);
     for (int s = 0; s < NS; ++s) {
       // e4m3: every converter warp; bf16: the leader's producer twice, with the
-      // bytes of both CTAs, or (V cleared past the sequence) each CTA once.
+      // bytes of both CTAs, or (V of edge tiles) each CTA once.
       mbar_init(bar_op_full(s), kFp8 ? 2 * kTilesConvWarps : 2);
       mbar_init(bar_op_empty(s), 1);
     }
@@ -368,6 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     }
     mbar_init(bar_td, 1);
     *abort_flag = 0;
+    for (int b = 0; b < 4; ++b) patch[b] = 0;
     plan.err = 0;
     fence_mbar_init();
   }
@@ -385,7 +415,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 
   // Segment sg of this pair's range, for a whole warp; false after the last (or
   // when the kernel gives up).
-  auto get_segment = [&](int sg, ChunkUnit& un, int& kt0, int& kt1) -> bool {
+  auto get_segment = [&](int sg, TileUnit& un, int& kt0, int& kt1) -> bool {
     if (!__all_sync(0xffffffffu, mbar_wait(bar_seg_full(sg), (sg / kTileSegments) & 1u, abort_flag, err, kErrWaitQ)))
       return false;
     const TileSegment& s = segments[sg % kTileSegments];
@@ -401,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   // Calls body(unit, kt0, kt1, segment) for each segment until it returns false;
   // returns false if it did.
   auto for_each_segment = [&](auto&& body) -> bool {
-    ChunkUnit un;
+    TileUnit un;
     int kt0, kt1;
     for (int sg = 0; get_segment(sg, un, kt0, kt1); ++sg) {
       put_back(sg);
@@ -409,8 +439,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     }
     return *abort_flag == 0;
   };
+  // V of tile kt passes through the converter warps (bf16): rows to be cleared, or
+  // to be looked through.
+  auto edge = [&](const TileUnit& un, int kt) { return (kt + 1) * kTileN > un.see_all; };
   // Keys of tile kt that the sequence has (may be 0 when it has none at all).
-  auto tile_valid = [&](const ChunkUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
+  auto tile_valid = [&](const TileUnit& un, int kt) { return min(kTileN, un.kvlen - kt * kTileN); };
   // The items of the range in the order of their loads, conversions and MMAs: K of
   // a tile ahead of V of the tile before it (one buffer of Q: within a segment).
   // body(is_v, unit, tile, tiles before it, segment, the segment's first tile, its
@@ -418,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   auto for_each_item = [&](auto&& body) -> bool {
     if constexpr (!L::kTwo) {
       uint32_t J = 0;
-      return for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int sg) -> bool {
+      return for_each_segment([&](const TileUnit& un, int kt0, int kt1, int sg) -> bool {
         if (!body(false, un, kt0, J, sg, true, kt0 + 1 == kt1)) return false;
 #pragma unroll 1
         for (int kt = kt0; kt < kt1; ++kt, ++J) {
@@ -428,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         return true;
       });
     } else {
-      ChunkUnit k, v;
+      TileUnit k, v;
       int k0, k1, v0, v1, kseg = 0, vseg = 0;
       uint32_t kj = 0, vj = 0;
       if (!get_segment(0, k, k0, k1)) return *abort_flag == 0;
@@ -500,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       };
       // Rows [key0, key0 + n) of K or V of one head; row 0 of `dst` is key0.
       // bf16: `full` is a cluster address.
-      auto load_rows = [&](auto v, Cursor& w, const ChunkUnit& un, int key0, int n, uint32_t dst, uint32_t full) {
+      auto load_rows = [&](auto v, Cursor& w, const TileUnit& un, int key0, int n, uint32_t dst, uint32_t full) {
         constexpr bool is_v = decltype(v)::value;
         const int step = is_v ? box.v_rows : box.k_rows;
         if (w.seq != un.seq || w.key != key0) {
@@ -547,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       uint32_t c = 0, parity = 1;
       int st = 0;
       const uint32_t own_bars = kFp8 ? bars : mapa_shared(bars, rank), leader_bars = mapa_shared(bars, 0);
-      auto issue = [&](auto v, Cursor& w, const ChunkUnit& un, int kt) {
+      auto issue = [&](auto v, Cursor& w, const TileUnit& un, int kt) {
         constexpr bool is_v = decltype(v)::value;
         if (c % L::kProducers != mine) return true;
         const uint32_t empty = kFp8 ? bar_land_empty(st) : bar_op_empty(st);
@@ -563,7 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           return ((min(most, max(0, valid - (is_v ? 0 : 64 * rk))) + step - 1) & -step) * row_bytes;
         };
         uint32_t full;
-        if (kFp8 || (is_v && valid < kTileN)) {  // to this CTA's converters
+        if (kFp8 || (is_v && edge(un, kt))) {  // to this CTA's converters
           if (elected) mbar_arrive_expect_tx(bar_land_full(st), bytes_of(static_cast<int>(rank)));
           full = own_bars + (bar_land_full(st) - bars);
         } else {
@@ -576,7 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         load_rows(v, w, un, kt * kTileN + off, n, dst, full);
         return true;
       };
-      const bool ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int, bool, bool) {
+      const bool ok = for_each_item([&](bool is_v, const TileUnit& un, int kt, uint32_t, int, bool, bool) {
         if (!(is_v ? issue(std::true_type(), cur_v, un, kt) : issue(std::false_type(), cur_k, un, kt))) return false;
         ++c;
         if (++st == NL) {
@@ -598,7 +631,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       // whose results nobody reads.  Both CTAs' bytes count on the leader.
       ChunkWalk<true> walk;
       walk.init(p, plan, err);
-      ChunkUnit un;
+      TileUnit un;
       int kt0, kt1, sg = 0, landed = 0;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -606,6 +639,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       };
       for (;; ++sg) {
         const bool more = walk.next(p, err, un, kt0, kt1);
+        if (more) {
+          un.see_all = keys_all_see(un.kvlen, un.qlen, un.row0, p.group);
+          un.see_any = keys_all_see(un.kvlen, un.qlen, un.row0 + un.rows - 1, p.group);
+        }
         if (sg >= kTileSegments) ok = wait(bar_seg_empty(sg), ((sg / kTileSegments) & 1u) ^ 1u);
         if (!ok) break;
         if (elected) {
@@ -632,7 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       if ((!ok || *abort_flag) && leader && elected)
         for (int i = max(0, landed - L::kQBufs); i < landed; ++i) mbar_wait_teardown(bar_q_ready(i), (i >> 1) & 1u);
     }
-    if (warp == kMmaWarp && !leader) for_each_segment([](const ChunkUnit&, int, int, int) { return true; });
+    if (warp == kMmaWarp && !leader) for_each_segment([](const TileUnit&, int, int, int) { return true; });
     if (warp == kMmaWarp && leader) {
       // ------------------------------------------ MMA issuer (leader only) --
       constexpr uint32_t idesc_qk =
@@ -692,7 +729,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ++c;
         return true;
       };
-      for_each_item([&](bool is_v, const ChunkUnit&, int, uint32_t J, int seg, bool first, bool last) {
+      for_each_item([&](bool is_v, const TileUnit&, int, uint32_t J, int seg, bool first, bool last) {
         if (is_v) return pv(J, first, last, seg);
         if (first) {
           if (!wait(bar_q_ready(seg), (seg >> 1) & 1u, kErrWaitQ)) return false;
@@ -721,7 +758,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
     };
-    auto item = [&](const ChunkUnit& un, bool is_v, int kt) -> bool {
+    auto item = [&](const TileUnit& un, bool is_v, int kt, int seg) -> bool {
       const int ls = c % NL, os = c % NS;
       const int valid = tile_valid(un, kt);
       if (kFp8) {
@@ -758,7 +795,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         // As attn_kv.cuh: D/32 16-byte chunks a thread, four in flight; rows
         // past the sequence are zeros.
         const ConvGeo& g = is_v ? geo_v : geo_k;
-        const int vrows = is_v ? valid : valid - 64 * static_cast<int>(rank);
+        const int vrows = is_v ? min(valid, un.see_any - kt * kTileN) : valid - 64 * static_cast<int>(rank);
+        const int look = is_v ? un.see_all - kt * kTileN : kTileN;  // rows to look through
+        bool found = false;
         const int row_step = is_v ? 64 / (D / 64) : 32 / (D / 64);
         const uint32_t op_step = row_step * 128;
 #pragma unroll 1
@@ -767,6 +806,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 #pragma unroll
           for (int m = 0; m < 4; ++m)
             x[m] = g.row + (m0 + m) * row_step < vrows ? lds128(raw + g.raw + (m0 + m) * 2048) : zero;
+          if (look < kTileN) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+              if (g.row + (m0 + m) * row_step >= look) found |= drop_nonfinite<true>(x[m]);
+          }
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             uint4 lo, hi;
@@ -776,6 +820,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             sts128(o + g.hi, hi);
           }
         }
+        if (found) set_patch(seg);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -786,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       ++c;
       return true;
     };
-    auto gather_q = [&](const ChunkUnit& un) -> bool {
+    auto gather_q = [&](const TileUnit& un) -> bool {
       // Q rows into the swizzled operand layout: a row over D / 8 lanes,
       // kFlight loads a lane in flight, the first of them before the wait for the
       // previous segment's QK^T to be done with the buffer.
@@ -843,7 +888,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     // kTwo: the output of segment sg.  Called once all that its last PV waits for is
     // on its way, Q and the first K of the next segment included.
     const float* seg_sums = red + 4 * kTileM;  // [kSegBufs]{l of either warpgroup, m}[128]
-    auto write_out = [&](const ChunkUnit& un, int kt0, int kt1, int sg) -> bool {
+    auto write_out = [&](const TileUnit& un, int kt0, int kt1, int sg) -> bool {
       if (!wait_all(bar_sums(sg), (sg / L::kSegBufs) & 1u, kErrWaitRed) ||
           !wait_all(bar_seg_o(sg), (sg >> 1) & 1u, kErrWaitODone))
         return false;
@@ -854,30 +899,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
       const bool live = r < un.rows;
       const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
+      const bool patched = patch[sg & 3] == sg + 1;
+      const int key0 = max(un.see_all, kt0 * kTileN), key1 = min(un.see_all + (un.row0 % p.group + r) / p.group, kt1 * kTileN);
       const int slot = part_slot(un, kt0, kt1, pair);
       if (slot < 0) {
         const int at = un.row0 + r;
         __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                              static_cast<long long>(un.q0 + at / p.group) * p.out_row;
         store_rows<D>(t_o, inv_l, live ? out : nullptr, lane);
+        if (patched && live) patch_row<D, D>(p, un, key0, key1, out, 0);
       } else {
         const long long pr = static_cast<long long>(slot) * kUnitRows + r;
         if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
         store_rows<D>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, lane);
+        if (patched && live) patch_row<D, D>(p, un, key0, key1, p.work.tile_o + pr * D, 0);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(mapa_shared(bar_o_free(sg), 0));
       return true;
     };
-    ChunkUnit last_un;
+    TileUnit last_un;
     int last0 = 0, last1 = 0, last_seg = -1;
     auto write_last = [&]() { return !L::kTwo || last_seg < 0 || write_out(last_un, last0, last1, last_seg); };
     bool ok;
     if constexpr (kFp8) {
-      ok = for_each_item([&](bool is_v, const ChunkUnit& un, int kt, uint32_t, int seg, bool first, bool last) {
+      ok = for_each_item([&](bool is_v, const TileUnit& un, int kt, uint32_t, int seg, bool first, bool last) {
         if (!is_v && first && !gather_q(un)) return false;
-        if (!item(un, is_v, kt)) return false;
+        if (!item(un, is_v, kt, seg)) return false;
         if (L::kTwo && is_v) {
           if (first) {
             if (!write_last()) return false;
@@ -890,11 +939,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         return true;
       });
     } else {
-      // The last tile of a sequence that ends inside it: V rows past its end,
-      // in the stage of that item (its place in the order of for_each_item).
+      // V of edge tiles: rows that no row of the unit sees become zeros (those
+      // past the sequence's end may hold anything), values that are not finite
+      // in rows that only some see too.  An item's stage follows from its place
+      // in the order of for_each_item.
       const uint32_t tiles = static_cast<uint32_t>(plan.end - plan.x);
       uint32_t J = 0, used = 0;  // bit st: parity of stage st's landings so far
-      ok = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int seg) -> bool {
+      ok = for_each_segment([&](const TileUnit& un, int kt0, int kt1, int seg) -> bool {
         if (!box.q_copy && !gather_q(un)) return false;
         if (L::kTwo) {
           if (!write_last()) return false;
@@ -903,21 +954,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           last1 = kt1;
           last_seg = seg;
         }
+        for (int kt = max(kt0, max(0, un.see_all) / kTileN); kt < kt1; ++kt) {
+          const uint32_t j = kt - kt0;
+          const uint32_t at = L::kTwo ? J + j + min(J + j + 2, tiles) : 2 * (J + j) + (kt + 1 < kt1 ? 2 : 1);
+          const int st = at % NS;
+          if (!wait_all(bar_land_full(st), (used >> st) & 1u, kErrWaitKvFull)) return false;
+          used ^= 1u << st;
+          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t op = sOp + st * L::kOpBytes;
+          bool found = false;
+          for (int i = max(0, un.see_all - kt * kTileN) * 8 + ct; i < kTileN * 8; i += kTilesConvThreads) {
+            const bool seen = kt * kTileN + i / 8 < un.see_any;
+            for (int b = 0; b < D / 128; ++b) {
+              const uint32_t a = op + b * v_col + (i >= 64 * 8 ? v_half : 0) + i * 16;
+              uint4 x = seen ? lds128(a) : zero;
+              if (seen) {
+                if (!drop_nonfinite<false>(x)) continue;
+                found = true;
+              }
+              sts128(a, x);
+            }
+          }
+          if (found) set_patch(seg);
+          fence_proxy_async_smem();
+          named_bar_sync(3, kTilesConvThreads);
+          if (ct == 0) mbar_arrive_remote(mapa_shared(bar_op_full(st), 0));
+        }
         J += kt1 - kt0;
-        const int valid = tile_valid(un, kt1 - 1);
-        if (valid >= kTileN) return true;
-        const uint32_t last = J - 1;
-        const uint32_t at = L::kTwo ? last + min(last + 2, tiles) : 2 * last + 1;
-        const int st = at % NS;
-        if (!wait_all(bar_land_full(st), (used >> st) & 1u, kErrWaitKvFull)) return false;
-        used ^= 1u << st;
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t op = sOp + st * L::kOpBytes;
-        for (int i = max(0, valid) * 8 + ct; i < kTileN * 8; i += kTilesConvThreads)
-          for (int b = 0; b < D / 128; ++b) sts128(op + b * v_col + (i >= 64 * 8 ? v_half : 0) + i * 16, zero);
-        fence_proxy_async_smem();
-        named_bar_sync(3, kTilesConvThreads);
-        if (ct == 0) mbar_arrive_remote(mapa_shared(bar_op_full(st), 0));
         return true;
       });
     }
@@ -938,7 +1001,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     ChunkRecord& rec = p.work.tile_rec[pair];
     const bool keeps = leader && threadIdx.x == 0;
     if (keeps) clear_record(rec);
-    const bool done = for_each_segment([&](const ChunkUnit& un, int kt0, int kt1, int seg) -> bool {
+    const bool done = for_each_segment([&](const TileUnit& un, int kt0, int kt1, int seg) -> bool {
       if (keeps) note_part(rec, un, kt0, kt1);
       bool ok = true;
       const int r = static_cast<int>(rank) * kTileM + row;  // row of the unit
@@ -974,6 +1037,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
           const int4 vm = *reinterpret_cast<const int4*>(sf + 2 * kTileN);
           ev = static_cast<float>(max(max(vm.x, vm.y), max(vm.z, vm.w)) - 127);
+          const int seen = pos + 1 - (kt0 + static_cast<int>(jg - J)) * kTileN;
+          if (seen < kTileN) {  // of the keys that this row sees alone
+            float top = 0.f;
+            const float4* vs = reinterpret_cast<const float4*>(sf + kTileN);
+#pragma unroll 4
+            for (int i = 0; i < kTileN; i += 4) {
+              const float4 v4 = vs[i / 4];
+              top = fmaxf(top, fmaxf(fmaxf(i < seen ? v4.x : 0.f, i + 1 < seen ? v4.y : 0.f),
+                                     fmaxf(i + 2 < seen ? v4.z : 0.f, i + 3 < seen ? v4.w : 0.f)));
+            }
+            ev = static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127);
+          }
           const float4* ks = reinterpret_cast<const float4*>(sf + first_key);
 #pragma unroll
           for (int i = 0; i < kKeys / 4; ++i) {
@@ -1097,14 +1172,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         named_bar_sync(2, kSoftmaxThreads);
         const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
         const int slot = part_slot(un, kt0, kt1, pair);
+        const bool patched = patch[seg & 3] == seg + 1;
+        const int key0 = max(un.see_all, kt0 * kTileN), key1 = min(pos + 1, kt1 * kTileN);
         if (slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                                static_cast<long long>(un.q0 + at / p.group) * p.out_row;
           store_rows<kOCols>(t_o, inv_l, live ? out + wg * kOCols : nullptr, lane);
+          if (patched && live) patch_row<D, kOCols>(p, un, key0, key1, out + wg * kOCols, wg * kOCols);
         } else {
           const long long pr = static_cast<long long>(slot) * kUnitRows + r;
           if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
-          store_rows<kOCols>(t_o, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr, lane);
+          float* part = p.work.tile_o + pr * D + wg * kOCols;
+          store_rows<kOCols>(t_o, inv_l, live ? part : nullptr, lane);
+          if (patched && live) patch_row<D, kOCols>(p, un, key0, key1, part, wg * kOCols);
         }
         tc_fence_before();
         __syncwarp();

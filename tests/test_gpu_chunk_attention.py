@@ -234,6 +234,43 @@ def test_a_nan_key_spoils_only_rows_that_see_it(new, cache):
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new,kv,heads,dim", [(2, 40, (8, 2), 128), (9, 9, (2, 2), 256), (32, 100, (2, 2), 128), (3, 300, (16, 2), 256),
+                                              (40, 200, (16, 2), 128), (70, 70, (8, 8), 256), (300, 300, (4, 4), 128),
+                                              (300, 1000, (16, 2), 256), (300, 1000, (32, 4), 128)])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(new, kv, heads, dim, cache):
+    """V of one new token has one (bf16: infinite) element that is not finite; V of another is NaN altogether."""
+    case = Case([new, 1], [kv, 50], heads, dim, 64, cache, seed=18)
+    clean = case.run()
+    group = heads[0] // heads[1]
+    one, all_ = kv - new + new // 2, kv - 1  # positions
+    page = case.pool.view(torch.uint8).view(-1, 2, heads[1], 64, dim * case.pool.element_size())
+    at = page[int(case.tables[0, one // 64]), 1, 0, one % 64]
+    if cache == "bf16":
+        at.view(torch.bfloat16)[37] = -torch.inf
+    else:
+        at[37] = 0x7F
+    page[int(case.tables[0, all_ // 64]), 1, 1 % heads[1], all_ % 64] = 0xFF
+    got = case.run()
+    spoilt = torch.zeros_like(got, dtype=torch.bool)
+    spoilt[:group, new // 2:new, 37] = True
+    spoilt[(1 % heads[1]) * group:(1 % heads[1] + 1) * group, new - 1] = True
+    assert torch.equal(~got.isfinite(), spoilt)
+    assert torch.equal(got[~spoilt], clean[~spoilt])
+
+
+@pytest.mark.parametrize("new,heads,dim", [(2, (8, 2), 128), (7, (8, 2), 256), (40, (16, 2), 256), (60, (16, 4), 128)])
+def test_a_large_value_that_a_row_does_not_see_costs_it_nothing(new, heads, dim):
+    """The last token's V is 2^100 times the others': the rows before it keep their accuracy."""
+    case = Case([new], [200], heads, dim, 64, "scaled", seed=19)
+    clean = case.run()
+    sc = case.scales.view(torch.uint8).view(-1, 2, heads[1], 64)
+    sc[int(case.tables[0, 199 // 64]), 1, :, 199 % 64] += 100
+    got = case.run()
+    assert torch.equal(got[:, :new - 1], clean[:, :new - 1])
+    assert (got[:, new - 1].float().abs().amax(-1) > 2.0 ** 60).all()
+
+
 def test_strides_streams_and_views():
     """Contiguous [heads, rows, D], [rows, heads, D] seen transposed, a view of
     wider rows; on a side stream; tables as a view of wider ones."""
