@@ -47,6 +47,7 @@ struct ChunkRecord {
   int last_cut;
   int first_state;  // 0: no partial, 1: does not end its unit, 2: ends it
   int err;          // the CTA's (pair's) device error
+  int patch;        // tile units: V had values that were taken for zeros (nonfinite8)
 };
 
 struct ChunkWork {
@@ -119,25 +120,6 @@ __device__ __forceinline__ int keys_all_see(int kvlen, int qlen, int row0, int g
   return kvlen - qlen + row0 / group + 1;
 }
 
-// Non-finite values of V at a key that some rows of a unit see and others do
-// not: 0 * NaN would reach the others, so the kernels take zeros in their place,
-// note that they did, and the output is patched afterwards.  Of the elements d ..
-// d + 7 of V at `key`, those that are not finite (a bit each).
-template <int D>
-__device__ __noinline__ uint32_t nonfinite8(const ChunkParams& p, int seq, int head, int key, int d) {
-  const int bs = p.pool.block_size, lb = key / bs;
-  if (lb >= p.batch.table_width) return 0;
-  const int pg = p.batch.tables ? p.batch.tables[seq * p.batch.table_stride + lb] : seq;
-  if (pg < 0 || pg >= p.pool.blocks) return 0;
-  const long long at = (((pg * 2LL + 1) * p.pool.heads + head) * bs + key % bs) * D + d;
-  uint32_t bad = 0;
-  for (int i = 0; i < 8; ++i) {
-    const bool b = p.pool.bf16 ? (reinterpret_cast<const uint16_t*>(p.pool.data)[at + i] & 0x7F80) == 0x7F80
-                               : (p.pool.data[at + i] & 0x7F) == 0x7F;
-    bad |= (b ? 1u : 0u) << i;
-  }
-  return bad;
-}
 // The elements of a 32-bit word of two bf16 or four e4m3 codes that are not finite.
 template <bool kFp8>
 __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
@@ -151,6 +133,34 @@ __device__ __forceinline__ bool drop_nonfinite(uint4& x) {
                              nonfinite_mask<kFp8>(x.w));
   x = make_uint4(x.x & ~m.x, x.y & ~m.y, x.z & ~m.z, x.w & ~m.w);
   return (m.x | m.y | m.z | m.w) != 0;
+}
+
+// Non-finite values of V at a key that some rows of a unit see and others do
+// not: 0 * NaN would reach the others, so the kernels take zeros in their place,
+// note that they did, and the output is patched afterwards.  Of the elements d ..
+// d + 7 of V at `key`, those that are not finite (a bit each).
+template <int D>
+__device__ __forceinline__ uint32_t nonfinite8(const ChunkParams& p, int seq, int head, int key, int d) {
+  const int bs = p.pool.block_size, lb = key / bs;
+  if (lb >= p.batch.table_width) return 0;
+  const int pg = p.batch.tables ? p.batch.tables[seq * p.batch.table_stride + lb] : seq;
+  if (pg < 0 || pg >= p.pool.blocks) return 0;
+  const long long at = (((pg * 2LL + 1) * p.pool.heads + head) * bs + key % bs) * D + d;
+  uint32_t bad = 0;
+  if (p.pool.bf16) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p.pool.data + 2 * at);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = nonfinite_mask<false>(w[i]);
+      bad |= ((m & 1u) | ((m >> 16) & 1u) << 1) << (2 * i);
+    }
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(p.pool.data + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad |= ((nonfinite_mask<true>(i < 4 ? x.x : x.y) >> (8 * (i & 3))) & 1u) << i;
+  }
+  return bad;
 }
 
 // A sequence as a kernel sees it; `tiles` 0 unless it has units of that kind.
@@ -422,7 +432,7 @@ __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddep
 // unit that range g left unfinished, if any (kW warps a row, each every kW-th
 // part: few rows of many parts, as a long cache leaves them, or many of few).
 // Block (0, 0) also writes the call's status.
-template <int D, int kW>
+template <int D, int kW, bool kTile>
 __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRecord* rec, int grid, int unit_rows,
                                              const float* part_o, const float* part_lse, int g, int y) {
   constexpr int kPer = D / 32;
@@ -489,6 +499,19 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
   if (!live) return;
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   const int row = unit.row0 + r;
+  if (kTile) {
+    bool patch = false;
+    for (int i = lane; i < 2 * parts; i += 32) patch |= rec[2 * g + i].patch != 0;
+    if (__any_sync(0xffffffffu, patch)) {
+      uint32_t bad = 0;
+      const int pos = unit.kvlen - unit.qlen + row / p.group;
+      for (int key = max(0, keys_all_see(unit.kvlen, unit.qlen, unit.row0, p.group)); key <= pos; ++key)
+        bad |= nonfinite8<D>(p, unit.seq, unit.head, key, lane * kPer & ~7) >> (lane * kPer & 7);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if ((bad >> k) & 1u) acc[k] = NAN;
+    }
+  }
   __nv_bfloat16* dst = p.out + static_cast<long long>(unit.head * p.group + row % p.group) * p.out_head +
                        static_cast<long long>(unit.q0 + row / p.group) * p.out_row + lane * kPer;
 #pragma unroll
@@ -498,6 +521,43 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
 }
 
 constexpr int kCombineSmallW = 4, kCombineTileW = 1;  // warps a row
+
+// The whole units of tile range g, if it took any values of V for zeros: NaN into
+// the output of the rows that see them, in their columns.  A warp a unit, eight
+// columns a lane.
+template <int D>
+__device__ __forceinline__ void patch_range(const ChunkParams& p, int g) {
+  if (!p.work.tile_rec[2 * g].patch && !p.work.tile_rec[2 * g + 1].patch) return;
+  __shared__ ChunkPlanShared sh;
+  if (threadIdx.x == 0) sh.err = 0;  // (reported already)
+  __syncthreads();
+  chunk_plan<true>(p, sh, p.tile_pairs, g);
+  ChunkWalk<true> walk;
+  walk.init(p, sh, &sh.err);
+  ChunkUnit u;
+  int kt0, kt1;
+  for (int n = 0; walk.next(p, &sh.err, u, kt0, kt1); ++n) {
+    if (n % 8 != threadIdx.x / 32 || part_slot(u, kt0, kt1, g) >= 0) continue;  // (a cut one: combine_rows)
+    const int before = u.kvlen - u.qlen;
+    for (int d = 8 * (threadIdx.x & 31); d < D; d += 256) {
+      uint32_t bad = 0;
+      const int end = before + (u.row0 + u.rows - 1) / p.group;
+      for (int key = max(0, keys_all_see(u.kvlen, u.qlen, u.row0, p.group)); key <= end; ++key) {
+        bad |= nonfinite8<D>(p, u.seq, u.head, key, d);
+        if (bad == 0) continue;
+        const int token = key - before;
+        for (int h = 0; h < p.group; ++h) {
+          const int row = token * p.group + h;
+          if (row < u.row0 || row >= u.row0 + u.rows) continue;
+          __nv_bfloat16* dst = p.out + static_cast<long long>(u.head * p.group + h) * p.out_head +
+                               static_cast<long long>(u.q0 + token) * p.out_row + d;
+          for (int i = 0; i < 8; ++i)
+            if ((bad >> i) & 1u) dst[i] = __float2bfloat16(NAN);
+        }
+      }
+    }
+  }
+}
 
 template <int D>
 __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
@@ -519,11 +579,15 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
     }
   }
   if (blockIdx.x < small_blocks) {
-    combine_rows<D, kCombineSmallW>(p, p.work.small_rec, p.small_ctas, kSmallRows, p.work.small_o, p.work.small_lse,
+    combine_rows<D, kCombineSmallW, false>(p, p.work.small_rec, p.small_ctas, kSmallRows, p.work.small_o, p.work.small_lse,
                        blockIdx.x / p.small_y, blockIdx.x % p.small_y);
   } else {
     const int b = blockIdx.x - small_blocks;
-    combine_rows<D, kCombineTileW>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse,
+    if (b >= p.tile_pairs * p.tile_y) {
+      patch_range<D>(p, b - p.tile_pairs * p.tile_y);
+      return;
+    }
+    combine_rows<D, kCombineTileW, true>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse,
                                    b / p.tile_y, b % p.tile_y);
   }
 }

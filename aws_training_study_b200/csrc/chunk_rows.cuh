@@ -7,10 +7,11 @@
 // (the tile kernel reads 2.4 TB/s on such a unit); here a warp's mma.sync tile is
 // 16 rows, which one token's group of heads fills, and warps split the KEYS:
 //   * A producer warp streams 32 KB stages (K and V of one head) through a ring of
-//     four with TMA.  A copy costs its issuer some 350 cycles whatever its size,
-//     and the SM's share of HBM is 8 KB in that time: so one copy brings all of a
-//     stage's rows that share a page (16 to 128: pages of any multiple of 16
-//     tokens), K and V together, 128-byte columns swizzled for the MMAs.
+//     four with TMA.  A copy and what surrounds it cost its issuer some 300 cycles
+//     whatever its size, and the SM's share of HBM is 7 KB in that time: so one
+//     copy brings all of a stage's rows that share a page (16 to 128: pages of any
+//     multiple of 16 tokens), K and V together, 128-byte columns swizzled for the
+//     MMAs.
 //   * Teams of D / 128 warps take 16 keys each in turn: a team scores its keys
 //     against all rows and adds P V into its own accumulators, with its own running
 //     maximum, so teams exchange nothing until the unit ends.  Within a team of
@@ -38,6 +39,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "chunk_plan.cuh"
 
@@ -107,7 +110,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
 template <int D, bool kFp8>
 __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     chunk_rows_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale,
-                      const int box_shift, const __grid_constant__ ChunkParams p) {
+                      const int box_shift, const ChunkParams p) {
   using L = RowsSmem<D, kFp8>;
   constexpr int kBoxElts = 128 / L::kElt;
   constexpr int kBoxSteps = kBoxElts / 16;  // MMA k steps of a box: 8 or 4
@@ -342,168 +345,174 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
           swap ^= 1;
         }
         const int left = k1 - key;  // keys of this group that are there
-        const bool whole = left >= 16 && key + 16 <= all_see;
-        float vs[4] = {1.f, 1.f, 1.f, 1.f};  // V scales of this lane's four keys
-        int ev = 127, ev1 = 127;             // their largest exponents, biased, of those that either row sees
-        if (scaled) {
-          const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
-          ev = 0;
+        // The softmax and P V; `all`: every row sees all 16 keys, as all but the
+        // last of a decode step's.
+        auto finish = [&](auto all) {
+          constexpr bool whole = decltype(all)::value;
+          float vs[4] = {1.f, 1.f, 1.f, 1.f};  // V scales of this lane's four keys
+          int ev = 127, ev1 = 127;             // their largest exponents, biased, of those that either row sees
+          if (scaled) {
+            const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
+            ev = 0;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t kb = *reinterpret_cast<const uint16_t*>(sc + 8 * n);
+              uint32_t vv = *reinterpret_cast<const uint16_t*>(sc + box_rows + 8 * n);
+              if (!whole) {  // keys that are not there: any byte
+                if (8 * n + 2 * i4 >= left) vv &= 0xFF00u;
+                if (8 * n + 2 * i4 + 1 >= left) vv &= 0x00FFu;
+              }
+              const float ka = __uint_as_float((kb & 0xFFu) << 23), kc = __uint_as_float((kb >> 8) << 23);
+              s[n][0] *= ka;
+              s[n][1] *= kc;
+              s[n][2] *= ka;
+              s[n][3] *= kc;
+              vs[2 * n] = __uint_as_float((vv & 0xFFu) << 23);
+              vs[2 * n + 1] = __uint_as_float((vv >> 8) << 23);
+              ev = max(ev, static_cast<int>(max(vv & 0xFFu, vv >> 8)));
+            }
+            ev1 = ev;
+            if (!whole) {
+              ev = ev1 = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int at = key + 8 * (i / 2) + 2 * i4 + i % 2, e = static_cast<int>(__float_as_uint(vs[i]) >> 23);
+                if (at <= pos0) ev = max(ev, e);
+                if (at <= pos1) ev1 = max(ev1, e);
+              }
+#pragma unroll
+              for (int x = 1; x <= 2; x <<= 1) ev1 = max(ev1, __shfl_xor_sync(0xffffffffu, ev1, x));
+            }
+          }
+          // Scores in log2 units, hidden keys at -inf.
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              s[n][j] *= f0;
+              s[n][j + 2] *= f1;
+              if (!whole) {
+                const int kk = 8 * n + 2 * i4 + j;
+                if (kk >= left || key + kk > pos0) s[n][j] = -INFINITY;
+                if (kk >= left || key + kk > pos1) s[n][j + 2] = -INFINITY;
+              }
+              mx0 = fmaxf(mx0, s[n][j]);
+              mx1 = fmaxf(mx1, s[n][j + 2]);
+            }
+#pragma unroll
+          for (int x = 1; x <= 2; x <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+            if (scaled) ev = max(ev, __shfl_xor_sync(0xffffffffu, ev, x));
+          }
+          if (scaled) {
+            mx0 += static_cast<float>(ev - 127);
+            mx1 += static_cast<float>((whole ? ev : ev1) - 127);
+          }
+          // The reference moves when the largest weight would pass 2^8 (and
+          // from its start); O and l follow.
+          const bool up0 = mx0 > m0 + kRescaleThreshold, up1 = mx1 > m1 + kRescaleThreshold;
+          if (__any_sync(0xffffffffu, up0 || up1)) {
+            float a0 = 1.f, a1 = 1.f;
+            if (up0) a0 = ex2_approx(m0 - mx0), m0 = mx0;
+            if (up1) a1 = ex2_approx(m1 - mx1), m1 = mx1;
+            l0 *= a0;
+            l1 *= a1;
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+              o[t][0] *= a0;
+              o[t][1] *= a0;
+              o[t][2] *= a1;
+              o[t][3] *= a1;
+            }
+          }
+          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+          uint32_t pk[4];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const uint32_t kb = *reinterpret_cast<const uint16_t*>(sc + 8 * n);
-            uint32_t vv = *reinterpret_cast<const uint16_t*>(sc + box_rows + 8 * n);
-            if (!whole) {  // keys that are not there: any byte
-              if (8 * n + 2 * i4 >= left) vv &= 0xFF00u;
-              if (8 * n + 2 * i4 + 1 >= left) vv &= 0x00FFu;
+            float pa = ex2_approx(s[n][0] - r0), pb = ex2_approx(s[n][1] - r0);
+            float pc = ex2_approx(s[n][2] - r1), pd = ex2_approx(s[n][3] - r1);
+            l0 += pa + pb;
+            l1 += pc + pd;
+            if (scaled) {
+              pa *= vs[2 * n];
+              pb *= vs[2 * n + 1];
+              pc *= vs[2 * n];
+              pd *= vs[2 * n + 1];
             }
-            const float ka = __uint_as_float((kb & 0xFFu) << 23), kc = __uint_as_float((kb >> 8) << 23);
-            s[n][0] *= ka;
-            s[n][1] *= kc;
-            s[n][2] *= ka;
-            s[n][3] *= kc;
-            vs[2 * n] = __uint_as_float((vv & 0xFFu) << 23);
-            vs[2 * n + 1] = __uint_as_float((vv >> 8) << 23);
-            ev = max(ev, static_cast<int>(max(vv & 0xFFu, vv >> 8)));
+            pk[2 * n] = kFp8 ? pack_f16x2(pa, pb) : pack_bf16x2(pa, pb);
+            pk[2 * n + 1] = kFp8 ? pack_f16x2(pc, pd) : pack_bf16x2(pc, pd);
           }
-          ev1 = ev;
-          if (!whole) {
-            ev = ev1 = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int at = key + 8 * (i / 2) + 2 * i4 + i % 2, e = static_cast<int>(__float_as_uint(vs[i]) >> 23);
-              if (at <= pos0) ev = max(ev, e);
-              if (at <= pos1) ev1 = max(ev1, e);
+          const uint4 pa = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          // O += P V; rows of keys that are not there may hold anything: zeros.
+          if (kFp8) {
+            const uint32_t vr = base + kV + 2 * i4 * 128;
+            const uint32_t ce = (gq ^ (2 * i4)) * 16, co = (gq ^ (2 * i4 + 1)) * 16;
+            uint4 v0 = lds128(vr + ce), v1 = lds128(vr + 128 + co);
+            uint4 v2 = lds128(vr + 1024 + ce), v3 = lds128(vr + 1024 + 128 + co);
+            if (!whole && left < 16) {
+              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+              if (2 * i4 >= left) v0 = zero;
+              if (2 * i4 + 1 >= left) v1 = zero;
+              if (2 * i4 + 8 >= left) v2 = zero;
+              if (2 * i4 + 9 >= left) v3 = zero;
             }
-#pragma unroll
-            for (int x = 1; x <= 2; x <<= 1) ev1 = max(ev1, __shfl_xor_sync(0xffffffffu, ev1, x));
-          }
-        }
-        // Scores in log2 units, hidden keys at -inf.
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            s[n][j] *= f0;
-            s[n][j + 2] *= f1;
-            if (!whole) {
-              const int kk = 8 * n + 2 * i4 + j;
-              if (kk >= left || key + kk > pos0) s[n][j] = -INFINITY;
-              if (kk >= left || key + kk > pos1) s[n][j + 2] = -INFINITY;
+            if (!whole) {  // keys that some rows do not see: nothing that is not finite
+              const int look = all_see - key - 2 * i4;
+              bool found = false;
+              if (look <= 0) found |= drop_nonfinite<true>(v0);
+              if (look <= 1) found |= drop_nonfinite<true>(v1);
+              if (look <= 8) found |= drop_nonfinite<true>(v2);
+              if (look <= 9) found |= drop_nonfinite<true>(v3);
+              if (found) *patch = unit;
             }
-            mx0 = fmaxf(mx0, s[n][j]);
-            mx1 = fmaxf(mx1, s[n][j + 2]);
-          }
-#pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
-          if (scaled) ev = max(ev, __shfl_xor_sync(0xffffffffu, ev, x));
-        }
-        if (scaled) {
-          mx0 += static_cast<float>(ev - 127);
-          mx1 += static_cast<float>((whole ? ev : ev1) - 127);
-        }
-        // The reference moves when the largest weight would pass 2^8 (and
-        // from its start); O and l follow.
-        const bool up0 = mx0 > m0 + kRescaleThreshold, up1 = mx1 > m1 + kRescaleThreshold;
-        if (__any_sync(0xffffffffu, up0 || up1)) {
-          float a0 = 1.f, a1 = 1.f;
-          if (up0) a0 = ex2_approx(m0 - mx0), m0 = mx0;
-          if (up1) a1 = ex2_approx(m1 - mx1), m1 = mx1;
-          l0 *= a0;
-          l1 *= a1;
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            o[t][0] *= a0;
-            o[t][1] *= a0;
-            o[t][2] *= a1;
-            o[t][3] *= a1;
-          }
-        }
-        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-        uint32_t pk[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float pa = ex2_approx(s[n][0] - r0), pb = ex2_approx(s[n][1] - r0);
-          float pc = ex2_approx(s[n][2] - r1), pd = ex2_approx(s[n][3] - r1);
-          l0 += pa + pb;
-          l1 += pc + pd;
-          if (scaled) {
-            pa *= vs[2 * n];
-            pb *= vs[2 * n + 1];
-            pc *= vs[2 * n];
-            pd *= vs[2 * n + 1];
-          }
-          pk[2 * n] = kFp8 ? pack_f16x2(pa, pb) : pack_bf16x2(pa, pb);
-          pk[2 * n + 1] = kFp8 ? pack_f16x2(pc, pd) : pack_bf16x2(pc, pd);
-        }
-        const uint4 pa = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        // O += P V; rows of keys that are not there may hold anything: zeros.
-        if (kFp8) {
-          const uint32_t vr = base + kV + 2 * i4 * 128;
-          const uint32_t ce = (gq ^ (2 * i4)) * 16, co = (gq ^ (2 * i4 + 1)) * 16;
-          uint4 v0 = lds128(vr + ce), v1 = lds128(vr + 128 + co);
-          uint4 v2 = lds128(vr + 1024 + ce), v3 = lds128(vr + 1024 + 128 + co);
-          if (left < 16) {
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-            if (2 * i4 >= left) v0 = zero;
-            if (2 * i4 + 1 >= left) v1 = zero;
-            if (2 * i4 + 8 >= left) v2 = zero;
-            if (2 * i4 + 9 >= left) v3 = zero;
-          }
-          if (!whole) {  // keys that some rows do not see: nothing that is not finite
-            const int look = all_see - key - 2 * i4;
-            bool found = false;
-            if (look <= 0) found |= drop_nonfinite<true>(v0);
-            if (look <= 1) found |= drop_nonfinite<true>(v1);
-            if (look <= 8) found |= drop_nonfinite<true>(v2);
-            if (look <= 9) found |= drop_nonfinite<true>(v3);
-            if (found) *patch = unit;
-          }
-          const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
-          const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t a0, a1, b0, b1;
-            e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x5140), a0, a1);
-            e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x5140), b0, b1);
-            mma16816<true>(o[4 * j], pa, a0, b0);
-            mma16816<true>(o[4 * j + 1], pa, a1, b1);
-            e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x7362), a0, a1);
-            e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x7362), b0, b1);
-            mma16816<true>(o[4 * j + 2], pa, a0, b0);
-            mma16816<true>(o[4 * j + 3], pa, a1, b1);
-          }
-        } else {
-          const uint32_t z0 = (2 * i4 < left ? 0xFFFFu : 0u) | (2 * i4 + 1 < left ? 0xFFFF0000u : 0u);
-          const uint32_t z1 = (2 * i4 + 8 < left ? 0xFFFFu : 0u) | (2 * i4 + 9 < left ? 0xFFFF0000u : 0u);
-          const int look = all_see - key - 2 * i4;
-          const uint32_t look0 = (look <= 0 ? 0xFFFFu : 0u) | (look <= 1 ? 0xFFFF0000u : 0u);
-          const uint32_t look1 = (look <= 8 ? 0xFFFFu : 0u) | (look <= 9 ? 0xFFFF0000u : 0u);
-          const int vrow = lane & 15, vc = lane >> 4;
-#pragma unroll
-          for (int b = 0; b < kWarpBoxes; ++b) {
-            const uint32_t vr = base + kV + b * col + vrow * 128;
+            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+            const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint32_t v[4];
-              ldmatrix_x4_trans(vr + (((2 * j + vc) ^ (vrow & 7)) * 16), v);
-              if (!whole) {  // keys that some rows do not see: nothing that is not finite
-                uint32_t found = 0;
+              uint32_t a0, a1, b0, b1;
+              e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x5140), a0, a1);
+              e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x5140), b0, b1);
+              mma16816<true>(o[4 * j], pa, a0, b0);
+              mma16816<true>(o[4 * j + 1], pa, a1, b1);
+              e4m3x4_to_f16x4(__byte_perm(w0[j], w1[j], 0x7362), a0, a1);
+              e4m3x4_to_f16x4(__byte_perm(w2[j], w3[j], 0x7362), b0, b1);
+              mma16816<true>(o[4 * j + 2], pa, a0, b0);
+              mma16816<true>(o[4 * j + 3], pa, a1, b1);
+            }
+          } else {
+            const uint32_t z0 = (whole || 2 * i4 < left ? 0xFFFFu : 0u) | (whole || 2 * i4 + 1 < left ? 0xFFFF0000u : 0u);
+            const uint32_t z1 = (whole || 2 * i4 + 8 < left ? 0xFFFFu : 0u) | (whole || 2 * i4 + 9 < left ? 0xFFFF0000u : 0u);
+            const int look = all_see - key - 2 * i4;
+            const uint32_t look0 = (look <= 0 ? 0xFFFFu : 0u) | (look <= 1 ? 0xFFFF0000u : 0u);
+            const uint32_t look1 = (look <= 8 ? 0xFFFFu : 0u) | (look <= 9 ? 0xFFFF0000u : 0u);
+            const int vrow = lane & 15, vc = lane >> 4;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint32_t bad = nonfinite_mask<false>(v[i]) & ((i & 1) ? look1 : look0);
-                  v[i] &= ~bad;
-                  found |= bad & ((i & 1) ? z1 : z0);
+            for (int b = 0; b < kWarpBoxes; ++b) {
+              const uint32_t vr = base + kV + b * col + vrow * 128;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint32_t v[4];
+                ldmatrix_x4_trans(vr + (((2 * j + vc) ^ (vrow & 7)) * 16), v);
+                if (!whole) {  // keys that some rows do not see: nothing that is not finite
+                  uint32_t found = 0;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const uint32_t bad = nonfinite_mask<false>(v[i]) & ((i & 1) ? look1 : look0);
+                    v[i] &= ~bad;
+                    found |= bad & ((i & 1) ? z1 : z0);
+                  }
+                  if (found) *patch = unit;
                 }
-                if (found) *patch = unit;
+                mma16816<false>(o[b * 8 + 2 * j], pa, v[0] & z0, v[1] & z1);
+                mma16816<false>(o[b * 8 + 2 * j + 1], pa, v[2] & z0, v[3] & z1);
               }
-              mma16816<false>(o[b * 8 + 2 * j], pa, v[0] & z0, v[1] & z1);
-              mma16816<false>(o[b * 8 + 2 * j + 1], pa, v[2] & z0, v[3] & z1);
             }
           }
-        }
+        };
+        if (left >= 16 && key + 16 <= all_see) finish(std::true_type());
+        else finish(std::false_type());
       }
       next -= L::kStageKeys;
       __syncwarp();

@@ -1,6 +1,10 @@
 // Attention of longer chunks over a paged cache: tiles of 256 query rows on
 // the tensor cores.
 //
+// 512 tokens over 131072 (32 / 2 heads of 256, e4m3 expanded): 1.59 ms, 1.39
+// PFLOP/s, what a long GEMM sustains here; four prompts of 2048 (64 / 8 heads of
+// 128, bf16): 285 us, 0.70 PFLOP/s of the causal half, the softmax its limit (per
+// tile 1050 cycles of exponentials in some 2200).
 // Bound by the MMAs (4 * 256 * 128 * D flops per 128-key tile of a unit against
 // 2 * 128 * D cache elements), with the softmax next: 128 x 128 exponentials a
 // CTA and tile take the MUFU 1024 cycles, the MMAs 1024 (D = 128) or 2048.  As in
@@ -9,7 +13,7 @@
 // columns), and scores and probabilities live in TMEM.  What differs:
 //   * The two softmax warpgroups of a CTA split each tile's keys between them.  (One
 //     with the even tiles and one with the odd ones, a thread a whole row, was
-//     slower: 400 to 358 us for four prompts of 2048, D = 128.)
+//     slower: 400 us for the four prompts where this, otherwise alike, took 358.)
 //   * D = 128: TMEM has room for two accumulators, and the converter warps write a
 //     finished one out while the softmax warps and the MMAs are at the next unit;
 //     Q has two buffers, so that the next unit's first QK^T is issued ahead of the
@@ -19,11 +23,13 @@
 //     walking an equal range of the batch's steps.
 //   * K and V are read from pages of any multiple of 16 tokens, through the
 //     sequence's table, box by box.
-//   * Rows are (token, query head) pairs of a strided Q, gathered by the
-//     converter warps instead of TMA; each row sees keys up to its position.
+//   * Rows are (token, query head) pairs of a strided Q: boxes of {group, tokens}
+//     by TMA (bf16 operands, group a divisor of 128), else gathered by the
+//     converter warps; each row sees keys up to its position.
 //   * bf16 caches land in operand layout straight from TMA, both CTAs' bytes on
-//     the leader's barrier; the converter warps only clear V rows past the
-//     sequence (which may hold anything: 0 * NaN would reach every row).
+//     the leader's barrier; the converter warps only see V of a unit's last tiles,
+//     where they clear the rows that no row sees (they may hold anything: 0 * NaN
+//     would reach every row) and values that are not finite (nonfinite8).
 //   * An e4m3 cache that many query tiles read is expanded into a bf16 copy first
 //     (chunk_expand_kernel; exact, scales included), when the copy is of moderate
 //     size: reading it in place converts every key tile again for each 256 rows.
@@ -116,7 +122,7 @@ struct TilesSmem {
   // teardown, ref[2], scale[NB], seg_full[], seg_empty[]
   static constexpr int kNumBars = 16 + kLandStages + kRawStages + 2 * kOpStages + 9 + kScaleBufs + 2 * kTileSegments;
   static constexpr int kMiscOff = (kBarOff + kNumBars * 8 + 15) / 16 * 16;
-  static constexpr int kSegOff = kMiscOff + 32;  // TileSegment[kTileSegments]
+  static constexpr int kSegOff = kMiscOff + 16;  // TileSegment[kTileSegments]
   static constexpr int kPlanOff = kSegOff + kTileSegments * sizeof(TileSegment);  // ChunkPlanShared
   static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
   static_assert(kBytes <= 232448, "exceeds the 227 KB of shared memory per CTA");
@@ -196,10 +202,9 @@ __device__ __forceinline__ void store_rows(uint32_t t_o, float inv_l, T* dst, in
       }
     }
   }
-  __syncwarp();  // (the rows may be patched)
 }
 
-// How K and V tiles are copied.  A copy costs its issuer some 350 cycles
+// How K and V tiles are copied.  A copy costs its issuer 170 cycles and more,
 // whatever its size (eight a tile held the kernel at 2900 cycles a tile, D = 256),
 // so one brings as many rows, and as many 64-element columns, as the pages allow.
 struct TileBoxes {
@@ -275,27 +280,11 @@ __global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p)
   grid_dependency_wait();  // the small units, as in chunk_tiles_kernel
 }
 
-__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
-}
-
-// NaN into the elements of an output row (of kCols columns from col0) whose column
-// of V has one among keys [key0, key1).  Rare, and slow.
-template <int D, int kCols, typename T>
-__device__ __noinline__ void patch_row(const ChunkParams& p, const ChunkUnit& un, int key0, int key1, T* dst, int col0) {
-  for (int d = 0; d < kCols; d += 8) {
-    uint32_t bad = 0;
-    for (int key = key0; key < key1; ++key) bad |= nonfinite8<D>(p, un.seq, un.head, key, col0 + d);
-    for (int i = 0; i < 8; ++i)
-      if ((bad >> i) & 1u) dst[d + i] = static_cast<T>(NAN);
-  }
-}
-
 template <int D, int kCache>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     chunk_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v,
-                       const TileBoxes box, const __grid_constant__ ChunkParams p) {
+                       const TileBoxes box, const ChunkParams p) {
   using L = TilesSmem<D, kCache>;
   constexpr bool kFp8 = L::kFp8;
   constexpr bool kScaled = kCache == kCacheScaled;
@@ -306,6 +295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   if (sbase & 1023u) {  // identical in both CTAs: neither starts
     if (threadIdx.x == 0) {
       p.work.tile_rec[blockIdx.x].err = kErrSmemAlign;
+      p.work.tile_rec[blockIdx.x].patch = 0;
       clear_record(p.work.tile_rec[blockIdx.x >> 1]);
     }
     return;
@@ -348,15 +338,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   TileSegment* segments = reinterpret_cast<TileSegment*>(smem + L::kSegOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
-  // By segment: its number + 1 if V had values that were taken for zeros
-  // (nonfinite8); set in both CTAs.  V of a segment is looked through after the
-  // item kOpStages before it was consumed, so at most three segments ahead of the
-  // output.
-  volatile int* patch = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 16);
-  auto set_patch = [&](int sg) {
-    for (uint32_t c = 0; c < 2; ++c)
-      st_cluster_u32(mapa_shared(sbase + L::kMiscOff + 16 + 4 * (sg & 3), c), sg + 1);
-  };
+  // V had values that were taken for zeros (nonfinite8).
+  volatile int* patch = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 8);
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   float* factors = reinterpret_cast<float*>(smem + L::kFactorOff);
 
@@ -397,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     }
     mbar_init(bar_td, 1);
     *abort_flag = 0;
-    for (int b = 0; b < 4; ++b) patch[b] = 0;
+    *patch = 0;
     plan.err = 0;
     fence_mbar_init();
   }
@@ -758,7 +741,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
     };
-    auto item = [&](const TileUnit& un, bool is_v, int kt, int seg) -> bool {
+    auto item = [&](const TileUnit& un, bool is_v, int kt) -> bool {
       const int ls = c % NL, os = c % NS;
       const int valid = tile_valid(un, kt);
       if (kFp8) {
@@ -820,7 +803,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             sts128(o + g.hi, hi);
           }
         }
-        if (found) set_patch(seg);
+        if (found) *patch = 1;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -899,20 +882,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
       const bool live = r < un.rows;
       const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
-      const bool patched = patch[sg & 3] == sg + 1;
-      const int key0 = max(un.see_all, kt0 * kTileN), key1 = min(un.see_all + (un.row0 % p.group + r) / p.group, kt1 * kTileN);
       const int slot = part_slot(un, kt0, kt1, pair);
       if (slot < 0) {
         const int at = un.row0 + r;
         __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                              static_cast<long long>(un.q0 + at / p.group) * p.out_row;
         store_rows<D>(t_o, inv_l, live ? out : nullptr, lane);
-        if (patched && live) patch_row<D, D>(p, un, key0, key1, out, 0);
       } else {
         const long long pr = static_cast<long long>(slot) * kUnitRows + r;
         if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
         store_rows<D>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, lane);
-        if (patched && live) patch_row<D, D>(p, un, key0, key1, p.work.tile_o + pr * D, 0);
       }
       tc_fence_before();
       __syncwarp();
@@ -926,7 +905,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     if constexpr (kFp8) {
       ok = for_each_item([&](bool is_v, const TileUnit& un, int kt, uint32_t, int seg, bool first, bool last) {
         if (!is_v && first && !gather_q(un)) return false;
-        if (!item(un, is_v, kt, seg)) return false;
+        if (!item(un, is_v, kt)) return false;
         if (L::kTwo && is_v) {
           if (first) {
             if (!write_last()) return false;
@@ -975,7 +954,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
               sts128(a, x);
             }
           }
-          if (found) set_patch(seg);
+          if (found) *patch = 1;
           fence_proxy_async_smem();
           named_bar_sync(3, kTilesConvThreads);
           if (ct == 0) mbar_arrive_remote(mapa_shared(bar_op_full(st), 0));
@@ -1172,19 +1151,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         named_bar_sync(2, kSoftmaxThreads);
         const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
         const int slot = part_slot(un, kt0, kt1, pair);
-        const bool patched = patch[seg & 3] == seg + 1;
-        const int key0 = max(un.see_all, kt0 * kTileN), key1 = min(pos + 1, kt1 * kTileN);
         if (slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
                                static_cast<long long>(un.q0 + at / p.group) * p.out_row;
           store_rows<kOCols>(t_o, inv_l, live ? out + wg * kOCols : nullptr, lane);
-          if (patched && live) patch_row<D, kOCols>(p, un, key0, key1, out + wg * kOCols, wg * kOCols);
         } else {
           const long long pr = static_cast<long long>(slot) * kUnitRows + r;
           if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
-          float* part = p.work.tile_o + pr * D + wg * kOCols;
-          store_rows<kOCols>(t_o, inv_l, live ? part : nullptr, lane);
-          if (patched && live) patch_row<D, kOCols>(p, un, key0, key1, part, wg * kOCols);
+          store_rows<kOCols>(t_o, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr, lane);
         }
         tc_fence_before();
         __syncwarp();
@@ -1201,7 +1175,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   tc_fence_before();
   cluster_sync_all();
   grid_dependency_wait();  // the small units: the merge waits for them through this kernel
-  if (threadIdx.x == 0) p.work.tile_rec[blockIdx.x].err = *static_cast<volatile int*>(err);
+  if (threadIdx.x == 0) {
+    p.work.tile_rec[blockIdx.x].err = *static_cast<volatile int*>(err);
+    p.work.tile_rec[blockIdx.x].patch = *patch;
+  }
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, kTmemCols);

@@ -369,7 +369,7 @@ int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, 
     else if (pool.scales) PCP_TRY((launch_tiles<D, pcp::kCacheScaled>(pool, p, st)));
     else PCP_TRY((launch_tiles<D, pcp::kCacheE4m3>(pool, p, st)));
   }
-  return launch_behind(pcp::chunk_combine_kernel<D>, p.small_ctas * p.small_y + p.tile_pairs * p.tile_y, 256, 0, st, p);
+  return launch_behind(pcp::chunk_combine_kernel<D>, p.small_ctas * p.small_y + p.tile_pairs * (p.tile_y + 1), 256, 0, st, p);
 }
 
 }  // namespace
