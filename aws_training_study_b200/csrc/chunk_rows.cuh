@@ -377,6 +377,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int at = key + 8 * (i / 2) + 2 * i4 + i % 2, e = static_cast<int>(__float_as_uint(vs[i]) >> 23);
+                vs[i] = fminf(vs[i], __uint_as_float(254u << 23));  // (255, no scale: finite where not seen)
                 if (at <= pos0) ev = max(ev, e);
                 if (at <= pos1) ev1 = max(ev1, e);
               }

@@ -756,7 +756,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
                                 (static_cast<long long>(pg) * 2 * p.pool.heads + un.head) * p.pool.block_size +
                                 key - lb * p.pool.block_size;
             kb = sc[0];
-            vb = sc[static_cast<long long>(p.pool.heads) * p.pool.block_size];
+            // (255, no scale: finite, for rows that do not see the key.)
+            vb = min(sc[static_cast<long long>(p.pool.heads) * p.pool.block_size], uint8_t(254));
           }
           float* sf = reinterpret_cast<float*>(smem + L::kScaleOff + (J % (NB ? NB : 1)) * L::kScaleBuf);
           // (The buffer is free: see kScaleBufs; the item's op stage is waited

@@ -350,7 +350,7 @@ __device__ __forceinline__ int sequence_of(const BatchView& b, int row) {
 __device__ __forceinline__ void e4m3x16_to_bf16(const uint4& codes, uint32_t b, uint4* out) {
   uint4 h[2];
   e4m3x16_to_f16(codes, h[0], h[1]);
-  const float s = __uint_as_float(b << 23);
+  const float s = __uint_as_float(min(b, 254u) << 23);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t hw[4] = {h[i].x, h[i].y, h[i].z, h[i].w};

@@ -23,6 +23,8 @@ import torch
 
 from .. import _capi
 from .config import PCPAttentionConfig
+from .layout import global_positions_for_rank
+from .rotary import Rotary, qk_norm_rope
 
 SUPPORTED_HEAD_DIMS = (128, 256)
 
@@ -182,6 +184,7 @@ class HistoryAttention:
                 raise ValueError(f"kv_path must be one of {sorted(_capi.KV_PATHS)}, got {kv_path!r}")
             _capi.check(lib.pcp_set_kv_path(self._handle, _capi.KV_PATHS[kv_path]))
         self.kv_path = kv_path or "default"
+        self._striped: torch.Tensor | None = None
 
     # -- calls -------------------------------------------------------------
     def _check_inputs(self, q: torch.Tensor, packed_kv: torch.Tensor) -> None:
@@ -197,6 +200,16 @@ class HistoryAttention:
                 raise ValueError(f"{name} is on {t.device}, expected {self.device}")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
+
+    def _positions(self, first: int) -> torch.Tensor:
+        """Global positions of this rank's current tokens, the first of all at ``first``."""
+        if self._striped is None:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("this rank's positions are not on the device yet: call once before the capture")
+            cfg = self.config
+            self._striped = global_positions_for_rank(cfg.current_len, self.rank, cfg.pcp_size,
+                                                      cfg.interleave_size).to(self.device)
+        return self._striped + first
 
     def _valid(self, valid_len) -> ctypes.Array:
         if valid_len is None:
@@ -278,20 +291,37 @@ class HistoryAttention:
         return out
 
     def prefill(self, q: torch.Tensor, packed_kv: torch.Tensor, k_cur: torch.Tensor, v_cur: torch.Tensor,
-                valid_len=None, out: torch.Tensor | None = None,
-                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+                valid_len=None, out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None,
+                rotary: Rotary | None = None, q_weight: torch.Tensor | None = None,
+                k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                first_position: int | None = None) -> torch.Tensor:
         """History attention plus causal attention over the current (prefill)
         tokens of every rank, merged by log-sum-exp.  ``k_cur``/``v_cur`` are
         this rank's current tokens' K/V shard ``[Hkv, Qloc, D]`` bf16, striped
         like ``q`` (``shard_query`` layout); a query sees every history key and
-        the current keys at global positions up to its own."""
+        the current keys at global positions up to its own.
+
+        With ``rotary``, ``q`` and ``k_cur`` are as projected: they are normed
+        (``q_weight``, ``k_weight``, ``eps``) and rotated by this rank's global
+        positions first (``qk_norm_rope``, into tensors of the call's own).  The
+        current tokens start at ``first_position``, by default behind the
+        history's ``sum(valid_len)`` tokens.  The first such call of a handle
+        copies its positions to the device, so it comes before any capture."""
         self._check_inputs(q, packed_kv)
         _check_current(self.config, k_cur, v_cur, False, self.device)
+        if rotary is None and not (q_weight is None and k_weight is None and first_position is None):
+            raise ValueError("q_weight, k_weight and first_position need rotary (of rotary_dim 0 for norms alone)")
         if out is None:
             out = torch.empty_like(q)
         elif tuple(out.shape) != tuple(q.shape) or out.dtype != torch.bfloat16 or not out.is_contiguous():
             raise ValueError("out must be a contiguous bf16 tensor shaped like q")
         vals = self._valid(valid_len)
+        if rotary is not None:
+            if rotary.head_dim != self.config.head_dim:
+                raise ValueError(f"rotary of heads of {rotary.head_dim}, expected {self.config.head_dim}")
+            first = sum(vals) if first_position is None else int(first_position)
+            with torch.cuda.device(self.device), torch.cuda.stream(stream):
+                q, k_cur = qk_norm_rope(q, k_cur, self._positions(first), rotary, q_weight, k_weight, eps)
         with torch.cuda.device(self.device):
             _capi.check(
                 _capi.lib().pcp_forward_prefill(

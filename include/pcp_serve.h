@@ -85,7 +85,7 @@ int pcp_qk_norm_rope(int32_t dtype, int32_t rows, int32_t head_dim, int32_t rota
 /* A paged cache: blocks of [2][num_kv_heads][block_size][head_dim] e4m3fn or
  * bf16, K then V.  scales (e4m3 only; NULL: unit scale): one byte b per token,
  * head and K/V, [blocks][2][num_kv_heads][block_size]; the row's values are
- * code * 2^(b - 127). */
+ * code * 2^(b - 127), b up to 254. */
 typedef struct pcp_pool {
   void* data;
   uint8_t* scales;
@@ -130,6 +130,10 @@ int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_h
  * KV head h serving query heads h * G .. h * G + G - 1.  Single tokens, chunks
  * of a prompt and whole prompts may be mixed in a batch.  Rows that see nothing
  * (positions below 0) are zeros; rows of no sequence are left as they were.
+ * What a row does not see (later tokens, pages past the length) costs it
+ * nothing, whatever it holds: infinities and NaN there too.  An element of V that is
+ * not finite makes its column of the rows that see it not finite (NaN for those of
+ * the new tokens themselves).
  *   - max_chunk bounds every sequence's rows (HOST value; it picks which
  *     kernels are launched).  Lengths and tables are read on the device.
  *   - q, out: bf16 [num_q_heads][rows][head_dim] at any 16-byte aligned stride.

@@ -259,6 +259,14 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(new, kv, heads
     assert torch.equal(got[~spoilt], clean[~spoilt])
 
 
+@pytest.mark.parametrize("new,heads,dim", [(2, (8, 2), 128), (40, (16, 2), 256), (600, (16, 4), 128)])
+def test_a_byte_that_is_no_scale_reaches_only_rows_that_see_it(new, heads, dim):
+    case = Case([new], [700], heads, dim, 64, "scaled", seed=20)
+    clean = case.run()
+    case.scales.view(torch.uint8).view(-1, 2, heads[1], 64)[int(case.tables[0, 699 // 64]), :, :, 699 % 64] = 255
+    assert torch.equal(case.run()[:, :new - 1], clean[:, :new - 1])
+
+
 @pytest.mark.parametrize("new,heads,dim", [(2, (8, 2), 128), (7, (8, 2), 256), (40, (16, 2), 256), (60, (16, 4), 128)])
 def test_a_large_value_that_a_row_does_not_see_costs_it_nothing(new, heads, dim):
     """The last token's V is 2^100 times the others': the rows before it keep their accuracy."""

@@ -15,6 +15,7 @@ import math
 import pytest
 import torch
 
+from aws_training_study_b200.pcp_attention import PCPAttentionConfig
 from aws_training_study_b200.pcp_attention.rotary import Rotary, qk_norm_rope, rotary_frequencies
 
 pytestmark = pytest.mark.gpu
@@ -151,3 +152,38 @@ def test_refusals():
             qk_norm_rope(args.pop("q"), args.pop("k"), args.pop("pos"), rotary, **args)
     empty = qk_norm_rope(q[:, :0], q[:1, :0], pos[:0], rotary)
     assert empty[0].shape == (2, 0, 128) and empty[1].shape == (1, 0, 128)
+
+
+def test_prefill_prepares_its_queries_and_keys():
+    """HistoryAttention.prefill with a rotation: the same as preparing q and k
+    first, at the positions behind the history or where told; on a side stream."""
+    from aws_training_study_b200.pcp_attention.cuda_backend import HistoryAttention
+
+    from parity import make_case, make_current, packed_shards
+
+    cfg = PCPAttentionConfig(1, 1024, 4096, 4096, 512, 64, 16, 2, 128)
+    _, _, _, q_shards, k_shards, v_shards = make_case(cfg, seed=31)
+    _, _, kc_shards, vc_shards = make_current(cfg, seed=31)
+    q, kv = q_shards[0].cuda(), packed_shards(cfg, k_shards, v_shards)[0].cuda()
+    k, v = kc_shards[0].cuda(), vc_shards[0].cuda()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wq, wk = (torch.rand(128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    rotary = Rotary(128, 64)
+    attn = HistoryAttention(cfg, rank=0, device=0)
+    keep = q.clone(), k.clone()
+    for first, args in ((4096, {}), (7, {"first_position": 7}), (3000, {"valid_len": [3000]})):
+        pos = torch.arange(first, first + 1024, device="cuda")
+        qn, kn = qk_norm_rope(q, k, pos, rotary, wq, wk, 1e-5)
+        want = attn.prefill(qn, kv, kn, v, valid_len=args.get("valid_len"))
+        assert torch.equal(attn.prefill(q, kv, k, v, rotary=rotary, q_weight=wq, k_weight=wk, eps=1e-5, **args), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out = attn.prefill(q, kv, k, v, rotary=rotary, q_weight=wq, k_weight=wk, eps=1e-5, valid_len=[3000], stream=side)
+    side.synchronize()
+    assert torch.equal(out, want) and torch.equal(q, keep[0]) and torch.equal(k, keep[1])
+    with pytest.raises(ValueError, match="rotary"):
+        attn.prefill(q, kv, k, v, q_weight=wq)
+    with pytest.raises(ValueError, match="heads of 256"):
+        attn.prefill(q, kv, k, v, rotary=Rotary(256))
+    attn.status()
+    attn.close()

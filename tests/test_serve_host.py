@@ -94,3 +94,65 @@ def test_batches_hold_whole_sequences():
     pool = torch.zeros(2, 2 * 2 * 64 * 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="pcp_size"):
         paged._pool_struct(cfg, pool, None)
+
+
+def test_chunk_attention_refusals():
+    lib = _capi.lib()
+
+    def call(pool=None, batch=None, q=None, out=None, max_chunk=4, scale=0.1, ws=256, nbytes=1 << 40, status=16):
+        pool = {"data": 16, "scales": 16, "blocks": 4, "num_kv_heads": 2, "head_dim": 128, "block_size": 64,
+                "kv_dtype": 0, **(pool or {})}
+        batch = {"offsets": 16, "kv_len": 16, "block_tables": 16, "table_stride": 4, "table_width": 4, "num_seqs": 1,
+                 "rows": 4, **(batch or {})}
+        return lib.pcp_chunk_attention(ctypes.byref(_capi.PcpPool(**pool)), ctypes.byref(_capi.PcpBatch(**batch)),
+                                       q or _heads(heads=4), out or _heads(heads=4), max_chunk, scale, ws, nbytes,
+                                       status, None)
+
+    nan, inf = float("nan"), float("inf")
+    for args in (dict(pool={"head_dim": 64}), dict(pool={"block_size": 24}), dict(pool={"kv_dtype": 2}),
+                 dict(pool={"kv_dtype": 1}), dict(pool={"data": 0}), dict(pool={"scales": 8}),
+                 dict(pool={"num_kv_heads": 3}), dict(batch={"rows": -1}), dict(batch={"num_seqs": -1}),
+                 dict(batch={"kv_len": 0}), dict(batch={"block_tables": 0}), dict(q=_heads(heads=3)),
+                 dict(q=_heads(heads=4, row=4)), dict(q=_heads(heads=4, data=8)), dict(out=_heads(heads=4, data=0)),
+                 dict(out=_heads(heads=2)), dict(max_chunk=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=nan),
+                 dict(scale=inf), dict(ws=0), dict(ws=128), dict(nbytes=1000), dict(status=0)):
+        assert call(**args) in (1, 2), args
+        assert lib.pcp_last_error()
+    assert call(batch={"rows": 0}) == 0 and call(batch={"num_seqs": 0}) == 0  # nothing to do
+
+
+def test_chunk_attention_workspace():
+    """Small while every chunk is small; a bf16 copy of the cache from 1024 rows a KV head on, up to 1 GiB of it."""
+    lib = _capi.lib()
+
+    def need(q_heads=8, seqs=2, rows=4096, width=16, max_chunk=1, **pool):
+        pool = _capi.PcpPool(**{"data": 16, "scales": 16, "blocks": 4, "num_kv_heads": 2, "head_dim": 128,
+                                "block_size": 64, "kv_dtype": 0, **pool})
+        nbytes = ctypes.c_size_t()
+        rc = lib.pcp_chunk_attention_workspace_size(ctypes.byref(pool), q_heads, seqs, rows, width, max_chunk,
+                                                    ctypes.byref(nbytes))
+        return nbytes.value if rc == 0 else -rc
+
+    copy = 2 * 2 * 128 * 2 * 2 * 1024  # K and V of 2 heads, bf16, 2 sequences of 16 pages of 64
+    assert need() == need(max_chunk=8) < need(max_chunk=9) == need(max_chunk=255) == need(max_chunk=256) - copy
+    assert need(max_chunk=256, kv_dtype=1, scales=0) == need(max_chunk=255)
+    assert need(max_chunk=256, width=1 << 20) == need(max_chunk=255) == need(max_chunk=256, width=0)
+    assert need(q_heads=3) == need(max_chunk=0) == need(rows=-1) == -1
+    assert need(rows=2 ** 30, q_heads=64) in (-1, -2)
+
+
+@pytest.mark.parametrize("P", [1, 4])
+def test_prefill_positions(P):
+    """The current tokens' global positions of every rank, from the first on, each once."""
+    from aws_training_study_b200.pcp_attention.cuda_backend import HistoryAttention
+
+    got = []
+    for rank in range(P):
+        attn = HistoryAttention.__new__(HistoryAttention)
+        attn.config, attn.rank, attn.device = PCPAttentionConfig(P, 512, 1024, 1024, 64, 32, 4, 2, 128), rank, torch.device("cpu")
+        attn._striped, attn._handle = None, None
+        first = attn._positions(1000)
+        assert first.dtype == torch.int64 and first[0] == 1000 + 32 * rank
+        assert torch.equal(attn._positions(0), first - 1000)
+        got.append(first)
+    assert torch.equal(torch.cat(got).sort().values, torch.arange(1000, 1512))
