@@ -225,56 +225,64 @@ struct ExpandParams {
 };
 
 template <int D>
-__global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p) {
+__device__ __forceinline__ void expand_item(const ExpandParams& p, int s, int kvlen, long long item) {
   constexpr int kPerRow = D / 16;
   const PoolView& pool = p.c.pool;
   const int per_page = 2 * pool.heads;
-  const int pieces = pool.block_size / p.item_rows;
-  const long long items = static_cast<long long>(p.c.batch.seqs) * p.c.batch.table_width * pieces * per_page;
+  const int piece = static_cast<int>(item / per_page), which = static_cast<int>(item - static_cast<long long>(piece) * per_page);
+  const int key0 = piece * p.item_rows, lb = key0 / pool.block_size, row0 = key0 - lb * pool.block_size;
+  const int n = min(p.item_rows, kvlen - key0);
+  const int blk = p.c.batch.tables[s * p.c.batch.table_stride + lb];
+  const bool found = blk >= 0 && blk < pool.blocks;
+  if (!found && threadIdx.x == 0) atomicCAS(p.c.status, 0, kErrBlockTable);
+  const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size + row0;
+  const uint4* codes = reinterpret_cast<const uint4*>(pool.data + src * D);
+  const uint8_t* scales = pool.scales ? pool.scales + src : nullptr;
+  uint4* dst = reinterpret_cast<uint4*>(p.copy + ((static_cast<long long>(s) * per_page + which) * p.copy_rows + key0) * D);
+  for (int e0 = threadIdx.x; e0 < n * kPerRow; e0 += 4 * 256) {
+    uint4 x[4];
+    uint32_t sc[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * 256;
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      sc[u] = 127;
+      if (found && e < n * kPerRow) {
+        x[u] = codes[e];
+        if (scales) sc[u] = scales[e / kPerRow];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * 256;
+      if (e >= n * kPerRow) break;
+      uint4 o[2];
+      e4m3x16_to_bf16(x[u], sc[u], o);
+      dst[2 * e] = o[0];
+      dst[2 * e + 1] = o[1];
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(256) chunk_expand_kernel(const ExpandParams p) {
+  const int per_page = 2 * p.c.pool.heads, lane = threadIdx.x & 31;
   __shared__ int s_ignored;  // lengths the attention reports itself
   if (threadIdx.x == 0) s_ignored = 0;
   __syncthreads();
   grid_launch_dependents();
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const long long piece = it / per_page;
-    const int which = static_cast<int>(it - piece * per_page);
-    const long long page = piece / pieces;
-    const int row0 = static_cast<int>(piece - page * pieces) * p.item_rows;
-    const int s = static_cast<int>(page / p.c.batch.table_width);
-    const int lb = static_cast<int>(page - static_cast<long long>(s) * p.c.batch.table_width);
-    const ChunkSeq q = chunk_seq<true>(p.c, s, &s_ignored);
-    const int n = min(p.item_rows, q.kvlen - lb * pool.block_size - row0);
-    if (q.tiles == 0 || n <= 0) continue;
-    const int blk = p.c.batch.tables[s * p.c.batch.table_stride + lb];
-    const bool found = blk >= 0 && blk < pool.blocks;
-    if (!found && threadIdx.x == 0) atomicCAS(p.c.status, 0, kErrBlockTable);
-    const long long src = (static_cast<long long>(found ? blk : 0) * per_page + which) * pool.block_size + row0;
-    const uint4* codes = reinterpret_cast<const uint4*>(pool.data + src * D);
-    const uint8_t* scales = pool.scales ? pool.scales + src : nullptr;
-    uint4* dst = reinterpret_cast<uint4*>(
-        p.copy + ((static_cast<long long>(s) * per_page + which) * p.copy_rows + static_cast<long long>(lb) * pool.block_size + row0) * D);
-    for (int e0 = threadIdx.x; e0 < n * kPerRow; e0 += 4 * 256) {
-      uint4 x[4];
-      uint32_t sc[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = e0 + u * 256;
-        x[u] = make_uint4(0u, 0u, 0u, 0u);
-        sc[u] = 127;
-        if (found && e < n * kPerRow) {
-          x[u] = codes[e];
-          if (scales) sc[u] = scales[e / kPerRow];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = e0 + u * 256;
-        if (e >= n * kPerRow) break;
-        uint4 o[2];
-        e4m3x16_to_bf16(x[u], sc[u], o);
-        dst[2 * e] = o[0];
-        dst[2 * e + 1] = o[1];
-      }
+  // Items of the sequences with tile units alone, dealt out over the blocks (a
+  // table may be far wider than the sequences are long).
+  long long next = blockIdx.x;  // this block's next item, from the sequence's first
+  for (int s0 = 0; s0 < p.c.batch.seqs; s0 += 32) {
+    ChunkSeq mine{};
+    if (s0 + lane < p.c.batch.seqs) mine = chunk_seq<true>(p.c, s0 + lane, &s_ignored);
+    for (uint32_t with = __ballot_sync(0xffffffffu, mine.tiles > 0); with; with &= with - 1) {
+      const int s = s0 + __ffs(with) - 1;
+      const int kvlen = __shfl_sync(0xffffffffu, mine.kvlen, s - s0);
+      const long long items = static_cast<long long>((kvlen + p.item_rows - 1) / p.item_rows) * per_page;
+      for (; next < items; next += gridDim.x) expand_item<D>(p, s, kvlen, next);
+      next -= items;
     }
   }
   grid_dependency_wait();  // the small units, as in chunk_tiles_kernel

@@ -221,6 +221,30 @@ def test_rows_that_see_nothing():
 
 
 @pytest.mark.parametrize("cache", CACHES)
+def test_long_chunks_that_mostly_see_nothing(cache):
+    case = Case([600, 300], [100, 0], (16, 2), 128, 16, cache, seed=21)
+    out = case.run(out=torch.full_like(case.q, 7.0))
+    assert (out[:, :500] == 0).all() and (out[:, 600:] == 0).all()
+    want, bound = case.expected(0)
+    assert ((out[:, 500:600].double() - want[:, 500:]).abs() <= bound[:, 500:]).all()
+
+
+@pytest.mark.parametrize("heads,dim,bs", [((16, 2), 256, 64), ((8, 1), 128, 48)])
+def test_chunks_among_many_decodes_with_wide_tables(heads, dim, bs):
+    """70 sequences, two of them with chunks, tables far wider than the
+    sequences are long, whose unused entries lead outside the pool."""
+    new = [1] * 70
+    kv = [10 + 37 * b % 900 for b in range(70)]
+    new[33], new[69] = 140, 133
+    kv[33], kv[69] = 500, 133
+    case = Case(new, kv, heads, dim, bs, "scaled", seed=22)
+    wide = torch.full((70, case.tables.shape[1] + 60), -1, dtype=torch.int32, device=DEV)
+    for b, t in enumerate(kv):
+        wide[b, :-(-t // bs)] = case.tables[b, :-(-t // bs)]
+    case.check(case.run(block_tables=wide))
+
+
+@pytest.mark.parametrize("cache", CACHES)
 @pytest.mark.parametrize("new", [1, 50])
 def test_a_nan_key_spoils_only_rows_that_see_it(new, cache):
     case = Case([new, new], [400, 300], (16, 2), 128, 64, cache, seed=13)
