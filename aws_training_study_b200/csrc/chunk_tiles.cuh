@@ -1061,18 +1061,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       auto probs = [&](uint32_t jg, const float (&s)[kKeys], float ref, uint32_t t_p) -> float {
         const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
         const float neg = ref == -INFINITY ? 0.f : -ref;
-        float sum0 = 0.f, sum1 = 0.f;
+        const f32x2 rf2 = pcp::pair(rf, rf), neg2 = pcp::pair(neg, neg);
+        f32x2 sum = pcp::pair(0.f, 0.f);
 #pragma unroll
         for (int c2 = 0; c2 < kKeys / 32; ++c2) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float q0 = ex2_approx(fmaf(s[c2 * 32 + 2 * i], rf, neg));
-            float q1 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 1], rf, neg));
-            float q2 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 2], rf, neg));
-            float q3 = ex2_approx(fmaf(s[c2 * 32 + 2 * i + 3], rf, neg));
-            sum0 += q0 + q2;
-            sum1 += q1 + q3;
+            float q0, q1, q2, q3;
+            split(fma2(pcp::pair(s[c2 * 32 + 2 * i], s[c2 * 32 + 2 * i + 1]), rf2, neg2), q0, q1);
+            split(fma2(pcp::pair(s[c2 * 32 + 2 * i + 2], s[c2 * 32 + 2 * i + 3]), rf2, neg2), q2, q3);
+            q0 = ex2_approx(q0);
+            q1 = ex2_approx(q1);
+            q2 = ex2_approx(q2);
+            q3 = ex2_approx(q3);
+            sum = add2(sum, add2(pcp::pair(q0, q1), pcp::pair(q2, q3)));
             if (kScaled) {
               const float4 v4 = *reinterpret_cast<const float4*>(sf + kTileN + first_key + c2 * 32 + 2 * i);
               q0 *= v4.x;
@@ -1086,6 +1089,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           tmem_st16(t_p + c2 * 16, pk);
         }
         tmem_wait_st();
+        float sum0, sum1;
+        split(sum, sum0, sum1);
         return sum0 + sum1;
       };
       auto release = [&](uint32_t jg) {  // tile jg's P is in place
