@@ -268,7 +268,7 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     """Causal attention of a batch of sequences' new tokens over their paged
     caches, which hold those tokens too (``cache_append`` first): the query at
     position p sees positions 0 .. p of its sequence.  ``q`` ``[Hq, rows, D]``
-    bf16 (heads and rows at any 16-byte aligned stride; so may ``out``);
+    bf16 (heads and rows at any 16-byte aligned stride; so may ``out``, and be ``q`` itself);
     single tokens, chunks and whole prompts may be mixed.  ``max_chunk`` (default
     ``rows``) bounds the rows of every sequence; 1 for a decode step saves the
     launches that longer chunks would need.  ``softmax_scale`` defaults to

@@ -95,6 +95,33 @@ def test_append_and_read_back_scaled(new, kv, D, heads, bs):
     assert (out[0][:, n:] == 7).all() and (out[1][:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("kv_dtype", [torch.float8_e4m3fn, torch.bfloat16], ids=["e4m3", "bf16"])
+def test_pages_and_rows_far_into_memory(kv_dtype):
+    """Pages beyond 2^32 bytes (and elements) of the pool, heads 2^31 elements
+    apart: what goes in comes back out, and the pages are a small pool's."""
+    cfg = _config(2, 256, 512)
+    offsets, kv_len, tables = _batch([70, 1], [1000, 300], 512, 5)
+    extra = (1 << 32) // (2 * 2 * 512 * 256) + 1
+    small = make_pool(cfg, 5, kv_dtype, DEV)
+    pool = torch.empty(5 + extra, small.shape[1], dtype=kv_dtype, device=DEV)
+    pool.view(torch.uint8)[extra:] = 0
+    e4m3 = kv_dtype == torch.float8_e4m3fn
+    small_scales, scales = (make_scales(cfg, n, DEV) if e4m3 else None for n in (5, 5 + extra))
+    gap = 1 << 31
+    far = torch.empty(2 * gap, dtype=torch.bfloat16, device=DEV)
+    k, v, k_out, v_out = (far.as_strided((2, 71, 256), (gap, 256, 1), n * gap // 4) for n in range(4))
+    g = torch.Generator(device=DEV).manual_seed(6)
+    for x in (k, v):
+        x.copy_(torch.randn(2, 71, 256, generator=g, device=DEV))
+    cache_append(cfg, k.contiguous(), v.contiguous(), offsets, kv_len, tables, small, scales=small_scales)
+    cache_append(cfg, k, v, offsets, kv_len, tables + extra, pool, scales=scales)
+    assert torch.equal(pool[extra:].view(torch.uint8), small.view(torch.uint8))
+    assert not e4m3 or torch.equal(scales[extra:], small_scales)
+    want = cache_read(cfg, offsets, kv_len, tables, small, rows=71, scales=small_scales)
+    cache_read(cfg, offsets, kv_len, tables + extra, pool, scales=scales, k_out=k_out, v_out=v_out)
+    assert torch.equal(k_out, want[0]) and torch.equal(v_out, want[1])
+
+
 def test_every_bf16_pattern():
     """All 65536 patterns against one large element: every rounding, ties
     included; infinities and NaN become NaN and spare their row."""

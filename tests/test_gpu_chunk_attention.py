@@ -320,6 +320,35 @@ def test_strides_streams_and_views():
     assert torch.equal(case.run(q=case.q.contiguous()), want)
 
 
+def test_output_over_the_queries():
+    for new, kv, cache in (([1, 3, 0, 90], [700, 40, 5, 91], "scaled"), ([400, 1], [1000, 30], "bf16")):
+        case = Case(new, kv, (16, 2), 128, 64, cache, seed=23)
+        want = case.run()
+        q = case.q.clone()
+        assert case.run(q=q, out=q) is q
+        assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "scaled"])
+@pytest.mark.parametrize("new,kv", [([1, 2], [900, 1500]), ([100, 1], [1500, 900])])
+def test_pages_and_rows_far_into_memory(new, kv, cache):
+    """Pages beyond 2^32 bytes (and elements) of the pool, heads of q and out
+    2^31 elements apart: the same as a small pool, bit for bit."""
+    case = Case(new, kv, (2, 2), 256, 512, cache, seed=24)
+    want = case.run()
+    small, scales = case.pool, case.scales
+    extra = (1 << 32) // (2 * 2 * 512 * 256) + 1
+    case.pool = torch.empty(small.shape[0] + extra, small.shape[1], dtype=small.dtype, device=DEV)
+    case.pool.view(torch.uint8)[extra:] = small.view(torch.uint8)
+    if scales is not None:
+        case.scales = torch.cat((torch.full((extra, scales.shape[1]), 255, dtype=torch.uint8, device=DEV), scales))
+    rows, gap = case.q.shape[1], 1 << 31
+    far = torch.empty(2 * gap + gap // 2, dtype=torch.bfloat16, device=DEV)
+    out = far.as_strided((2, rows, 256), (gap, 256, 1), gap // 2)
+    case.q = far.as_strided((2, rows, 256), (gap, 256, 1)).copy_(case.q)
+    assert torch.equal(case.run(block_tables=case.tables + extra, out=out), want)
+
+
 def test_two_captured_graphs_and_new_lengths():
     """Graphs with workspaces of their own, replayed at once on two streams,
     with lengths, tables and queries that changed since the capture."""

@@ -108,6 +108,18 @@ def test_strides_in_place_and_streams():
     assert all(torch.equal(out[i], out[0]) for i in range(4))
 
 
+def test_heads_far_apart_in_memory():
+    gap = 1 << 31
+    far = torch.empty(3 * gap, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = far.as_strided((2, 9, 128), (gap, 128, 1)).copy_(torch.randn(2, 9, 128, generator=g, device="cuda"))
+    out = far.as_strided((2, 9, 128), (gap, 128, 1), gap // 2)
+    positions = torch.arange(9, device="cuda") + (1 << 40)
+    want, _ = qk_norm_rope(q.contiguous(), None, positions, Rotary(128))
+    qk_norm_rope(q, None, positions, Rotary(128), q_out=out)
+    assert torch.equal(out, want)
+
+
 def test_captured_and_replayed():
     rotary = Rotary(256, 64)
     q = torch.randn(32, 5, 256, device=DEV).to(torch.bfloat16)
