@@ -234,6 +234,12 @@ __device__ __forceinline__ long long warp_scan(long long v) {  // inclusive
   return v;
 }
 
+// a / b of numbers that are not negative; the short way where 32 bits hold them.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 // The whole block (at most 16 warps): finds range g of `grid` in the list of
 // units, in the order sequence, KV head, unit.  Warps sum runs of sequences;
 // the one whose run holds the range's first step looks it up.  A batch whose
@@ -253,33 +259,37 @@ __device__ __forceinline__ void chunk_plan(const ChunkParams& p, ChunkPlanShared
     return warp_sum(n);
   };
   bool bad = false;
-  for (int s = s0 + lane; s < s1; s += 32) {
+  auto check = [&](int s) {
     const int o0 = p.batch.offsets[s], o1 = p.batch.offsets[s + 1];
     bad |= o0 < 0 || o1 < o0 || o1 > p.batch.rows;
-  }
-  bad = __syncthreads_or(bad);
+  };
   long long sum = 0;
-  if (!bad) {
-    if (kTile) {
-      for (int s = s0; s < s1; ++s) sum += steps_of(s);
-    } else {
-      for (int s = s0 + lane; s < s1; s += 32) sum += steps_of(s);
-      sum = warp_sum(sum);
+  if (kTile) {
+    for (int s = s0; s < s1; ++s) {
+      check(s);
+      sum += steps_of(s);
     }
-  } else if (threadIdx.x == 0) {
-    atomicCAS(&sh.err, 0, kErrSequence);
+  } else {
+    for (int s = s0 + lane; s < s1; s += 32) {
+      check(s);
+      sum += steps_of(s);
+    }
+    sum = warp_sum(sum);
   }
   if (lane == 0) sh.sums[warp] = sum;
-  __syncthreads();
+  bad = __syncthreads_or(bad);
+  if (bad && threadIdx.x == 0) atomicCAS(&sh.err, 0, kErrSequence);
   long long before = 0, total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += sh.sums[w];
-    total += sh.sums[w];
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const long long n = w < warps && !bad ? sh.sums[w] : 0;
+    if (w < warp) before += n;
+    total += n;
   }
   const int heads = p.pool.heads;
   const long long steps = total * heads, ranges = chunk_ranges(steps, grid);
   const bool none = total == 0 || g >= ranges;
-  const long long x = none ? 0 : steps * g / ranges, end = none ? 0 : steps * (g + 1) / ranges;
+  const long long x = none ? 0 : quotient(steps * g, ranges), end = none ? 0 : quotient(steps * (g + 1), ranges);
   if (threadIdx.x == 0) {
     sh.x = x;
     sh.end = end;
@@ -309,8 +319,8 @@ __device__ __forceinline__ void chunk_plan(const ChunkParams& p, ChunkPlanShared
       }
     }
     const long long rest = x - at * heads;
-    const int head = static_cast<int>(rest / in_seq);
-    long long kt = rest % in_seq;
+    const int head = static_cast<int>(quotient(rest, in_seq));
+    long long kt = rest - head * in_seq;
     int unit = 0;
     if (kTile) {
       const ChunkSeq q = chunk_seq<kTile>(p, seq, &sh.err);

@@ -76,7 +76,8 @@ struct RowsSmem {
   // buffers' space before the merge.
   static constexpr int kRowOff = kBufOff + kBufs * kBufBytes;  // float score factor[32], int position[32]
   static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;  // float m, l: [team][16]
-  static constexpr int kBarOff = kMlOff + 2 * kTeams * 16 * 4;  // full, empty
+  static constexpr int kInvOff = kMlOff + 2 * kTeams * 16 * 4;  // float 1 / sum of the weights [32]
+  static constexpr int kBarOff = kInvOff + kSmallRows * 4;  // full, empty
   static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
   static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
   static constexpr int kBytes = kPlanOff + sizeof(ChunkPlanShared);
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   int* row_pos = reinterpret_cast<int*>(smem + L::kRowOff) + kSmallRows;
   float* s_m = reinterpret_cast<float*>(smem + L::kMlOff);
   float* s_l = s_m + L::kTeams * 16;
+  float* s_inv = reinterpret_cast<float*>(smem + L::kInvOff);
   auto bar_full = [&](int s) { return sbase + L::kBarOff + 8u * s; };
   auto bar_empty = [&](int s) { return sbase + L::kBarOff + 8u * (L::kStages + s); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff);
@@ -148,6 +150,10 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     *reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4) = 0;
     plan.err = 0;
     fence_mbar_init();
+  }
+  if (warp == L::kWarps && lane == 0) {
+    tma_prefetch_desc(&tm_kv);
+    if (kFp8 && p.pool.scales) tma_prefetch_desc(&tm_scale);
   }
   grid_launch_dependents();  // the merge may wait on the SMs
   __syncthreads();
@@ -584,22 +590,29 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         }
       }
     };
+    // Each row's sum over its teams (the rounds' barriers pass it on).
+    const int slot = part_slot(un, kt0, kt1, blockIdx.x);
+    if (threadIdx.x < (two ? 32 : 16)) {
+      const int r = threadIdx.x, t0 = r / 16 * teams;
+      float M = -INFINITY, lsum = 0.f;
+      for (int w = t0; w < t0 + teams; ++w) M = fmaxf(M, s_m[w * 16 + r % 16]);
+      for (int w = t0; w < t0 + teams; ++w) {
+        const float mw = s_m[w * 16 + r % 16];
+        // Without a maximum the sum is 0, or NaN where every score was NaN.
+        lsum += mw == -INFINITY ? s_l[w * 16 + r % 16] : s_l[w * 16 + r % 16] * ex2_approx(mw - M);
+      }
+      s_inv[r] = lsum == 0.f ? 0.f : 1.f / lsum;  // no key seen: zeros
+      if (slot >= 0 && r < un.rows)
+        p.work.small_lse[static_cast<long long>(slot) * kSmallRows + r] = lsum == 0.f ? -INFINITY : M + __log2f(lsum);
+    }
     for (int round = (teams - 1) / bufs; round >= 0; --round) {
       if (turn / bufs == round) exchange(turn + bufs < teams);
       named_bar_sync(1, kConsumers);
     }
     // Every thread eight elements of a row: sum the buffers, divide, write.
-    const int slot = part_slot(un, kt0, kt1, blockIdx.x);
     for (int x = threadIdx.x; x < un.rows * (D / 8); x += kConsumers) {
       const int r = x / (D / 8), d = (x % (D / 8)) * 8;
       const int t = r / 16;
-      float M = -INFINITY, lsum = 0.f;
-      for (int w = t * teams; w < (t + 1) * teams; ++w) M = fmaxf(M, s_m[w * 16 + r % 16]);
-      for (int w = t * teams; w < (t + 1) * teams; ++w) {
-        const float mw = s_m[w * 16 + r % 16];
-        // Without a maximum the sum is 0, or NaN where every score was NaN.
-        lsum += mw == -INFINITY ? s_l[w * 16 + r % 16] : s_l[w * 16 + r % 16] * ex2_approx(mw - M);
-      }
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       const float* src = reinterpret_cast<const float*>(smem + L::kBufOff) + (r % 16) * L::kRowFloats + d + 4 * (d / 32);
       for (int k = 0; k < bufs; ++k) {
@@ -607,7 +620,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         const float4 u = at[0], v = at[1];
         f[0] += u.x, f[1] += u.y, f[2] += u.z, f[3] += u.w, f[4] += v.x, f[5] += v.y, f[6] += v.z, f[7] += v.w;
       }
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no key seen: zeros
+      const float inv = s_inv[r];
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] *= inv;
       if (*patch == unit) {  // rare: see nonfinite8
@@ -627,7 +640,6 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
       } else {
         const long long at = static_cast<long long>(slot) * kSmallRows + r;
         Vec8<float>::store(p.work.small_o + at * D + d, f);
-        if (d == 0) p.work.small_lse[at] = lsum == 0.f ? -INFINITY : M + __log2f(lsum);
       }
     }
   }
