@@ -279,17 +279,15 @@ __device__ __forceinline__ void chunk_plan(const ChunkParams& p, ChunkPlanShared
   if (lane == 0) sh.sums[warp] = sum;
   bad = __syncthreads_or(bad);
   if (bad && threadIdx.x == 0) atomicCAS(&sh.err, 0, kErrSequence);
-  long long before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    const long long n = w < warps && !bad ? sh.sums[w] : 0;
-    if (w < warp) before += n;
-    total += n;
-  }
+  const long long of_lane = lane < warps && !bad ? sh.sums[lane] : 0;
+  const long long before = warp_sum(lane < warp ? of_lane : 0), total = warp_sum(of_lane);
   const int heads = p.pool.heads;
   const long long steps = total * heads, ranges = chunk_ranges(steps, grid);
   const bool none = total == 0 || g >= ranges;
-  const long long x = none ? 0 : quotient(steps * g, ranges), end = none ? 0 : quotient(steps * (g + 1), ranges);
+  // The first `more` ranges have a step more than the others.
+  const long long each = quotient(steps, ranges), more = steps - each * ranges;
+  const long long x = none ? 0 : g * each + min(static_cast<long long>(g), more);
+  const long long end = none ? 0 : x + each + (g < more ? 1 : 0);
   if (threadIdx.x == 0) {
     sh.x = x;
     sh.end = end;
