@@ -294,10 +294,10 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     int next = 16 * turn;  // this team's next keys, from the stage's first
     for (int key0 = k0; key0 < k1; key0 += L::kStageKeys, ++c) {
       const int st = c % L::kStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_full(st), (c / L::kStages) & 1u, abort_flag, err, kErrWaitKvFull));
-      // (The warps of a team of two go on together or not at all.)
-      if (L::kTeam > 1) ok = named_bar_and(2 + team, 32 * L::kTeam, ok);
-      if (!ok) break;
+      // (After a failed wait a warp goes on, over whatever the stages hold, so that its
+      // team's barriers are met; nothing of it is merged.)
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_full(st), (c / L::kStages) & 1u, abort_flag, err, kErrWaitKvFull)))
+        ok = false;
       const int here = min(L::kStageKeys, k1 - key0);
       for (; next < here; next += 16 * teams) {
         const int key = key0 + next;
