@@ -7,7 +7,7 @@
 // (the tile kernel reads 2.4 TB/s on such a unit); here a warp's mma.sync tile is
 // 16 rows, which one token's group of heads fills, and warps split the KEYS:
 //   * A producer warp streams 32 KB stages (K and V of one head) through a ring of
-//     four with TMA.  A copy and what surrounds it cost its issuer some 300 cycles
+//     four or five with TMA.  A copy and what surrounds it cost its issuer some 300 cycles
 //     whatever its size, and the SM's share of HBM is 7 KB in that time: so one
 //     copy brings all of a stage's rows that share a page (16 to 128: pages of any
 //     multiple of 16 tokens), K and V together, 128-byte columns swizzled for the
@@ -19,10 +19,15 @@
 //     are summed through shared memory, and half the output.  128 columns are
 //     what lets 12 such warps live on an SM (64 accumulators a thread): one
 //     warp with all 256 columns at two warps a scheduler spilled, and read 2.0
-//     TB/s where this reads the figures below.  17 to 32 rows are two row
-//     tiles, each with half the teams, on the same stages.
+//     TB/s where this reads 3.9.  17 to 32 rows are two row tiles, each with half
+//     the teams, on the same stages.
 //   * The teams' (m, l, O) are merged through shared memory when the unit's part
 //     ends, into bf16 rows or an fp32 partial.
+// 64 sequences of 4096 (bf16, 32 / 8 heads of 128): 5.6 TB/s, 86 % of a copy's rate.
+// 16 of 32768 (e4m3 with scales, 32 / 2 heads of 256): 3.9 TB/s, bound by issue and
+// latency (half of the issue slots; conversions and MMAs are half the instructions).
+// Multiplying a visit's scores under the softmax of the one before held the stages
+// longer and was slower (87 to 100 us, bf16 129 to 153).
 //
 // e4m3 codes become f16 in registers (exact) on their way into the MMA.  No
 // ldmatrix: the order of an MMA's k index is free as long as both operands
@@ -59,7 +64,7 @@ struct RowsSmem {
   static constexpr int kBoxes = D * kElt / 128;             // 128-byte columns of a row
   static constexpr int kStageBytes = 32768;
   static constexpr int kStageKeys = kStageBytes / (256 * kBoxes);  // 32 to 128
-  static constexpr int kStages = 4;
+  static constexpr int kStages = kFp8 ? 4 : 5;  // bf16, which HBM bounds: 5 127.5 us, 4 128.4
   // Scale bytes of a stage: a copy's K rows, then its V rows, at 128-byte slots.
   static constexpr int kScaleStage = kFp8 ? kStageKeys / 16 * 128 : 0;
   // O exchange: 16 rows of D floats, 4 floats of padding every 32, rows 16

@@ -1,10 +1,11 @@
 // Attention of longer chunks over a paged cache: tiles of 256 query rows on
 // the tensor cores.
 //
-// 512 tokens over 131072 (32 / 2 heads of 256, e4m3 expanded): 1.59 ms, 1.39
+// 512 tokens over 131072 (32 / 2 heads of 256, e4m3 expanded): 1.55 ms, 1.42
 // PFLOP/s, what a long GEMM sustains here; four prompts of 2048 (64 / 8 heads of
-// 128, bf16): 285 us, 0.70 PFLOP/s of the causal half, the softmax its limit (per
-// tile 1050 cycles of exponentials in some 2200).
+// 128, bf16): 280 us, 0.72 PFLOP/s of the causal half, the softmax its limit (per
+// tile 1050 cycles of exponentials in some 2200; a quarter of them as polynomials
+// on the FMA pipe made it 305 us).
 // Bound by the MMAs (4 * 256 * 128 * D flops per 128-key tile of a unit against
 // 2 * 128 * D cache elements), with the softmax next: 128 x 128 exponentials a
 // CTA and tile take the MUFU 1024 cycles, the MMAs 1024 (D = 128) or 2048.  As in
