@@ -221,11 +221,12 @@ def cache_append(config: PCPAttentionConfig, k_src: torch.Tensor, v_src: torch.T
     and raises."""
     ps = _pool_struct(config, pool, scales)
     rows = k_src.shape[1] if k_src.dim() == 3 else -1
-    for name, t in (("k_src", k_src), ("v_src", v_src)):
-        _check_rows(name, t, (config.num_kv_heads, rows, config.head_dim), torch.bfloat16, pool.device)
-    batch = _batch_struct(offsets, kv_len, block_tables, rows, pool.device)
-    st = _Status(status, pool.device, stream)
-    _launch(pool.device, stream, _capi.lib().pcp_cache_append, ps, batch, _heads(k_src), _heads(v_src), st.ptr)
+    device, shape = pool.device, (config.num_kv_heads, rows, config.head_dim)
+    hk = _check_rows("k_src", k_src, shape, torch.bfloat16, device)
+    hv = _check_rows("v_src", v_src, shape, torch.bfloat16, device)
+    batch = _batch_struct(offsets, kv_len, block_tables, rows, device)
+    st = _Status(status, device, stream)
+    _launch(device, stream, _capi.lib().pcp_cache_append, ps, batch, hk, hv, st.ptr)
     st.finish(stream)
 
 
@@ -245,18 +246,19 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
         if k_out is None:
             raise ValueError("cache_read needs rows, or k_out and v_out")
         rows = k_out.shape[1] if k_out.dim() == 3 else -1
-    shape = (config.num_kv_heads, int(rows), config.head_dim)
-    outs = []
+    device, shape = pool.device, (config.num_kv_heads, int(rows), config.head_dim)
+    outs, structs = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:
-            t = torch.empty(shape, dtype=torch.bfloat16, device=pool.device)
+            t = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            structs.append(_heads(t))
         else:
-            _check_rows(name, t, shape, torch.bfloat16, pool.device)
+            structs.append(_check_rows(name, t, shape, torch.bfloat16, device))
             _check_writable(name, t)
         outs.append(t)
-    batch = _batch_struct(offsets, kv_len, block_tables, int(rows), pool.device)
-    st = _Status(status, pool.device, stream)
-    _launch(pool.device, stream, _capi.lib().pcp_cache_read, ps, batch, _heads(outs[0]), _heads(outs[1]), st.ptr)
+    batch = _batch_struct(offsets, kv_len, block_tables, int(rows), device)
+    st = _Status(status, device, stream)
+    _launch(device, stream, _capi.lib().pcp_cache_read, ps, batch, *structs, st.ptr)
     st.finish(stream)
     return outs[0], outs[1]
 
@@ -278,13 +280,13 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     ps = _pool_struct(config, pool, scales)
     rows = q.shape[1] if q.dim() == 3 else -1
     shape = (config.num_q_heads, rows, config.head_dim)
-    _check_rows("q", q, shape, torch.bfloat16, pool.device)
+    device = pool.device
+    hq = _check_rows("q", q, shape, torch.bfloat16, device)
     if out is None:
         out = torch.empty_like(q)
-    else:
-        _check_rows("out", out, shape, torch.bfloat16, pool.device)
+    ho = _check_rows("out", out, shape, torch.bfloat16, device)
     _check_writable("out", out)
-    batch = _batch_struct(offsets, kv_len, block_tables, rows, pool.device)
+    batch = _batch_struct(offsets, kv_len, block_tables, rows, device)
     max_chunk = max(1, rows) if max_chunk is None else int(max_chunk)
     if max_chunk <= 0:
         raise ValueError(f"max_chunk must be positive, got {max_chunk}")
@@ -293,9 +295,9 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     nbytes = ctypes.c_size_t()
     _capi.check(lib.pcp_chunk_attention_workspace_size(ps, config.num_q_heads, batch.num_seqs, rows,
                                                        batch.table_width, max_chunk, ctypes.byref(nbytes)))
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=pool.device)
-    st = _Status(status, pool.device, stream)
-    _launch(pool.device, stream, lib.pcp_chunk_attention, ps, batch, _heads(q), _heads(out), max_chunk, scale,
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    st = _Status(status, device, stream)
+    _launch(device, stream, lib.pcp_chunk_attention, ps, batch, hq, ho, max_chunk, scale,
             ws.data_ptr(), nbytes.value, st.ptr)
     if stream is not None:
         ws.record_stream(stream)

@@ -121,17 +121,21 @@ def _heads(t: torch.Tensor | None) -> _capi.PcpHeads:
     return _capi.PcpHeads(t.data_ptr(), head if heads > 1 else 0, row if rows > 1 else 0, heads, 0)
 
 
-def _check_rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
+def _check_rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> _capi.PcpHeads:
     """A packed tensor ``[heads, rows, head_dim]`` whose rows are contiguous
-    and 16-byte aligned; the heads and rows may lie at any stride."""
+    and 16-byte aligned; the heads and rows may lie at any stride.  Returns it
+    as the C ABI takes it."""
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"expected {name} {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     head, row, one = t.stride()
-    unit = 16 // t.element_size()
-    if t.numel() and (one != 1 or t.data_ptr() % 16 or (head % unit and shape[0] > 1) or (row % unit and shape[1] > 1)):
+    heads, rows, _ = shape
+    head, row = head if heads > 1 else 0, row if rows > 1 else 0  # an axis of one has no step to check
+    data, unit = t.data_ptr(), 4 if dtype == torch.float32 else 8
+    if heads and rows and (one != 1 or data % 16 or head % unit or row % unit):
         raise ValueError(f"{name} needs contiguous, 16-byte aligned rows, got strides {t.stride()}")
+    return _capi.PcpHeads(data, head, row, heads, 0)
 
 
 def _check_writable(name: str, t: torch.Tensor) -> None:
@@ -173,11 +177,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if q.dtype not in _DTYPES:
         raise ValueError(f"dtype {q.dtype} is not supported (bfloat16, float16 or float32)")
     rows, D, dev = q.shape[1], rotary.head_dim, q.device
-    _check_rows("q", q, (q.shape[0], rows, D), q.dtype, dev)
+    hq, hk = _check_rows("q", q, (q.shape[0], rows, D), q.dtype, dev), _heads(None)
     if k is not None:
         if k.dim() != 3:
             raise ValueError("k must be [heads, rows, head_dim]")
-        _check_rows("k", k, (k.shape[0], rows, D), q.dtype, dev)
+        hk = _check_rows("k", k, (k.shape[0], rows, D), q.dtype, dev)
     elif k_out is not None or k_weight is not None:
         raise ValueError("k_out or k_weight without k")
     if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (rows,) or \
@@ -187,16 +191,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or w.device != dev or
                               not w.is_contiguous() or w.data_ptr() % 16):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned [{D}] {q.dtype} tensor on {dev}")
-    outs = []
-    for name, x, o in (("q_out", q, q_out), ("k_out", k, k_out)):
+    outs, structs = [], []
+    for name, x, o, h in (("q_out", q, q_out, hq), ("k_out", k, k_out, hk)):
         if o is None:
             o = None if x is None else torch.empty_like(x)
+            h = _heads(o)
         elif o is not x:
-            _check_rows(name, o, tuple(x.shape), q.dtype, dev)
+            h = _check_rows(name, o, tuple(x.shape), q.dtype, dev)
             _check_writable(name, o)
         outs.append(o)
+        structs.append(h)
     _launch(dev, stream, _capi.lib().pcp_qk_norm_rope, _DTYPES[q.dtype], rows, D, rotary.rotary_dim,
-            _LAYOUTS[rotary.layout], _heads(q), _heads(k), _heads(outs[0]), _heads(outs[1]), positions.data_ptr(),
+            _LAYOUTS[rotary.layout], hq, hk, *structs, positions.data_ptr(),
             int(positions.dtype == torch.int64), rotary.turns(dev).data_ptr(), rotary.magnitude,
             0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps)
     return outs[0], outs[1]
