@@ -153,29 +153,38 @@ def history_attention_paged_single(q: torch.Tensor, pool: torch.Tensor, block_ta
 
 
 def _pool_struct(config: PCPAttentionConfig, pool: torch.Tensor, scales: torch.Tensor | None) -> _capi.PcpPool:
+    heads, block, dim, dtype = config.num_kv_heads, config.block_size, config.head_dim, pool.dtype
     if config.pcp_size != 1:
         raise ValueError(f"a batch holds whole sequences: pcp_size must be 1, got {config.pcp_size}")
-    if config.block_size % 16:
-        raise ValueError(f"block_size must be a multiple of 16, got {config.block_size}")
-    code = _kv_code(pool.dtype)
-    _check_pool(config, pool, pool.dtype)
-    if scales is not None:
-        shape = (pool.shape[0], 2 * config.num_kv_heads * config.block_size)
-        if code != _capi.PCP_KV_E4M3:
-            raise ValueError("scales need an e4m3 pool")
-        if scales.shape != shape or scales.dtype != torch.uint8 or scales.device != pool.device or \
-                not scales.is_contiguous() or scales.data_ptr() % 16:
-            raise ValueError(f"scales must be a contiguous, 16-byte aligned uint8 {shape} tensor on {pool.device}")
-    return _capi.PcpPool(pool.data_ptr(), 0 if scales is None else scales.data_ptr(), pool.shape[0],
-                         config.num_kv_heads, config.head_dim, config.block_size, code)
+    if block % 16:
+        raise ValueError(f"block_size must be a multiple of 16, got {block}")
+    code = _kv_code(dtype)
+    _check_pool(config, pool, dtype)
+    blocks = pool.shape[0]
+    if scales is None:
+        return _capi.PcpPool(pool.data_ptr(), 0, blocks, heads, dim, block, code)
+    data = scales.data_ptr()
+    if code != _capi.PCP_KV_E4M3:
+        raise ValueError("scales need an e4m3 pool")
+    if scales.shape != (blocks, 2 * heads * block) or scales.dtype != torch.uint8 or scales.device != pool.device or \
+            data % 16 or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous, 16-byte aligned uint8 {(blocks, 2 * heads * block)} tensor on "
+                         f"{pool.device}")
+    return _capi.PcpPool(pool.data_ptr(), data, blocks, heads, dim, block, code)
 
 
 def _batch_struct(offsets: torch.Tensor, kv_len: torch.Tensor, block_tables: torch.Tensor, rows: int,
                   device: torch.device) -> _capi.PcpBatch:
-    for name, t, dims in (("offsets", offsets, 1), ("kv_len", kv_len, 1), ("block_tables", block_tables, 2)):
-        if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.stride(-1) != 1 and t.numel()):
-            raise ValueError(f"{name} must be an int32 tensor of {dims} dimensions with contiguous rows on {device}")
-    seqs, (tables, width) = kv_len.shape[0], block_tables.shape
+    int32, shape = torch.int32, block_tables.shape
+    if offsets.dtype != int32 or kv_len.dtype != int32 or block_tables.dtype != int32 or offsets.dim() != 1 or \
+            kv_len.dim() != 1 or len(shape) != 2 or offsets.device != device or kv_len.device != device or \
+            block_tables.device != device or not offsets.is_contiguous() or not kv_len.is_contiguous() or \
+            (block_tables.stride(1) != 1 and block_tables.numel()):
+        given = ", ".join(f"{name} {tuple(t.shape)} {t.dtype} on {t.device}" for name, t in
+                          (("offsets", offsets), ("kv_len", kv_len), ("block_tables", block_tables)))
+        raise ValueError("offsets, kv_len and block_tables must be int32 tensors of 1, 1 and 2 dimensions with "
+                         f"contiguous rows on {device}, got {given}")
+    seqs, (tables, width) = kv_len.shape[0], shape
     if offsets.shape[0] != seqs + 1 or tables != seqs:
         raise ValueError(f"{seqs} sequences need {seqs + 1} offsets and {seqs} block tables, got {offsets.shape[0]} "
                          f"and {tables}")
