@@ -436,15 +436,16 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Merges the parts of cut units: O = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i -
-// M); rows that saw no key are zeros.  Block (g, y) takes 8 / kW rows of the
-// unit that range g left unfinished, if any (kW warps a row, each every kW-th
-// part: few rows of many parts, as a long cache leaves them, or many of few).
-// Block (0, 0) also writes the call's status.
+// M); rows that saw no key are zeros.  Block (g, y) takes the rows [8 / kW y, ...)
+// of the unit that range g left unfinished, if any: kW warps a row, each every
+// kW-th part (few rows of many parts, as a long cache leaves them, or many of few).
+// For tile units one: four gained 4 us with 37 parts a unit and lost 4 to 6 with 4
+// to 8; four rows a warp, their loads side by side, lost up to 30.
 template <int D, int kW, bool kTile>
 __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRecord* rec, int grid, int unit_rows,
                                              const float* part_o, const float* part_lse, int g, int y) {
   constexpr int kPer = D / 32;
-  __shared__ float s_acc[8][D];
+  __shared__ float s_acc[kW > 1 ? 8 : 1][D];
   __shared__ float s_w[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (!rec[g].last_cut) return;
@@ -462,33 +463,34 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
     }
     parts += 32;
   }
-  const bool live = r < unit.rows;
+  // (Warps behind the unit's last row go along with it and write nothing.)
+  auto row_of = [&](int i) {
+    return static_cast<long long>(i == 0 ? 2 * g + 1 : 2 * (g + i)) * unit_rows + min(r, unit.rows - 1);
+  };
   float m = -INFINITY, acc[kPer], wsum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  if (live) {
-    auto row_of = [&](int i) { return static_cast<long long>(i == 0 ? 2 * g + 1 : 2 * (g + i)) * unit_rows + r; };
-    for (int b = 0; b < parts; b += 32) m = fmaxf(m, b + lane < parts ? part_lse[row_of(b + lane)] : -INFINITY);
+  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+  for (int b = lane; b < parts; b += 32) m = fmaxf(m, part_lse[row_of(b)]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.f : m;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (m == -INFINITY) m = 0.f;
 #pragma unroll 4
-    for (int i = warp % kW; i < parts; i += kW) {
-      const long long row = row_of(i);
-      const float lse = part_lse[row];
-      // A part whose row saw nothing weighs nothing, whatever its O holds; a
-      // NaN (a NaN score somewhere) passes on.
-      const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - ref);
-      wsum += w;
-      const float* src = part_o + row * D + lane * kPer;
+  for (int i = warp % kW; i < parts; i += kW) {
+    const long long row = row_of(i);
+    const float lse = part_lse[row];
+    float4 v[kPer / 4];
 #pragma unroll
-      for (int k = 0; k < kPer; k += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + k);
-        acc[k] = w == 0.f ? acc[k] : fmaf(w, v.x, acc[k]);
-        acc[k + 1] = w == 0.f ? acc[k + 1] : fmaf(w, v.y, acc[k + 1]);
-        acc[k + 2] = w == 0.f ? acc[k + 2] : fmaf(w, v.z, acc[k + 2]);
-        acc[k + 3] = w == 0.f ? acc[k + 3] : fmaf(w, v.w, acc[k + 3]);
-      }
+    for (int c = 0; c < kPer / 4; ++c) v[c] = reinterpret_cast<const float4*>(part_o + row * D + lane * kPer)[c];
+    // A part whose row saw nothing weighs nothing, whatever its O holds; a NaN (a
+    // NaN score somewhere) passes on.
+    const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - m);
+    wsum += w;
+#pragma unroll
+    for (int c = 0; c < kPer / 4; ++c) {
+      acc[4 * c] = w == 0.f ? acc[4 * c] : fmaf(w, v[c].x, acc[4 * c]);
+      acc[4 * c + 1] = w == 0.f ? acc[4 * c + 1] : fmaf(w, v[c].y, acc[4 * c + 1]);
+      acc[4 * c + 2] = w == 0.f ? acc[4 * c + 2] : fmaf(w, v[c].z, acc[4 * c + 2]);
+      acc[4 * c + 3] = w == 0.f ? acc[4 * c + 3] : fmaf(w, v[c].w, acc[4 * c + 3]);
     }
   }
   if (kW > 1) {
@@ -504,7 +506,7 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
       for (int k = 0; k < kPer; ++k) acc[k] += s_acc[warp + w][lane * kPer + k];
     }
   }
-  if (!live) return;
+  if (r >= unit.rows) return;
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   const int row = unit.row0 + r;
   if (kTile) {
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
       return;
     }
     combine_rows<D, kCombineTileW, true>(p, p.work.tile_rec, p.tile_pairs, kUnitRows, p.work.tile_o, p.work.tile_lse,
-                                   b / p.tile_y, b % p.tile_y);
+                                         b / p.tile_y, b % p.tile_y);
   }
 }
 
