@@ -293,8 +293,10 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     hq = _check_rows("q", q, shape, torch.bfloat16, device)
     if out is None:
         out = torch.empty_like(q)
-    ho = _check_rows("out", out, shape, torch.bfloat16, device)
-    _check_writable("out", out)
+        ho = _heads(out)
+    else:
+        ho = _check_rows("out", out, shape, torch.bfloat16, device)
+        _check_writable("out", out)
     batch = _batch_struct(offsets, kv_len, block_tables, rows, device)
     max_chunk = max(1, rows) if max_chunk is None else int(max_chunk)
     if max_chunk <= 0:
