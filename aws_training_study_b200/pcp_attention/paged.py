@@ -34,7 +34,7 @@ import torch
 from .. import _capi
 from .config import PCPAttentionConfig
 from .cuda_backend import _cuda_stream_ptr, _kv_code, make_dims, payload_elements
-from .rotary import _check_rows, _check_writable, _heads, _launch
+from .rotary import _allocate, _check_rows, _check_writable, _heads, _launch
 
 
 def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -259,7 +259,8 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
     outs, structs = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:
-            t = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            t = torch.empty(shape, dtype=torch.bfloat16, device=device) if stream is None else \
+                _allocate(stream, torch.empty, shape, dtype=torch.bfloat16, device=device)
             structs.append(_heads(t))
         else:
             structs.append(_check_rows(name, t, shape, torch.bfloat16, device))
@@ -292,7 +293,7 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     device = pool.device
     hq = _check_rows("q", q, shape, torch.bfloat16, device)
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q) if stream is None else _allocate(stream, torch.empty_like, q)
         ho = _heads(out)
     else:
         ho = _check_rows("out", out, shape, torch.bfloat16, device)
@@ -306,11 +307,10 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     nbytes = ctypes.c_size_t()
     _capi.check(lib.pcp_chunk_attention_workspace_size(ps, config.num_q_heads, batch.num_seqs, rows,
                                                        batch.table_width, max_chunk, ctypes.byref(nbytes)))
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if stream is None else \
+        _allocate(stream, torch.empty, nbytes.value, dtype=torch.uint8, device=device)
     st = _Status(status, device, stream)
     _launch(device, stream, lib.pcp_chunk_attention, ps, batch, hq, ho, max_chunk, scale,
             ws.data_ptr(), nbytes.value, st.ptr)
-    if stream is not None:
-        ws.record_stream(stream)
     st.finish(stream)
     return out

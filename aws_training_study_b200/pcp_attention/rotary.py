@@ -149,6 +149,14 @@ def _check_writable(name: str, t: torch.Tensor) -> None:
             reach += stride * (n - 1)
 
 
+def _allocate(stream: torch.cuda.Stream, make, *args, **kwargs) -> torch.Tensor:
+    """``make(...)`` with memory of ``stream``, for a call that was given one: a
+    block that the current stream freed may still be in use by work it has yet to
+    run."""
+    with torch.cuda.stream(stream):
+        return make(*args, **kwargs)
+
+
 def _launch(device: torch.device, stream: torch.cuda.Stream | None, entry, *args) -> None:
     """``entry(*args, stream)`` on ``device`` and ``stream`` (default: the
     current one of the device); raises its error.  The device and stream are
@@ -194,7 +202,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     outs, structs = [], []
     for name, x, o, h in (("q_out", q, q_out, hq), ("k_out", k, k_out, hk)):
         if o is None:
-            o = None if x is None else torch.empty_like(x)
+            if x is not None:
+                o = torch.empty_like(x) if stream is None else _allocate(stream, torch.empty_like, x)
             h = _heads(o)
         elif o is not x:
             h = _check_rows(name, o, tuple(x.shape), q.dtype, dev)

@@ -320,6 +320,33 @@ def test_strides_streams_and_views():
     assert torch.equal(case.run(q=case.q.contiguous()), want)
 
 
+def test_memory_of_a_call_on_a_side_stream_is_that_streams(monkeypatch):
+    """What a call allocates may not be memory that work still to run on the
+    current stream uses (a freed block goes back to its own stream alone)."""
+    from aws_training_study_b200.pcp_attention import paged
+
+    seen = []
+    launch = paged._launch
+    monkeypatch.setattr(paged, "_launch", lambda *args: (seen.append(args), launch(*args)))
+    case = Case([1, 50], [300, 200], (8, 2), 128, 64, "scaled", seed=25)
+    side, status = torch.cuda.Stream(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    want = case.run(status=status).clone()
+    busy = [case.run(status=status).data_ptr(), seen[-1][-3]]  # output and workspace, both free again
+    out = case.run(status=status, stream=side)
+    assert out.data_ptr() not in busy and seen[-1][-3] not in busy
+    side.synchronize()
+    assert torch.equal(out, want)
+    args = (case.cfg, case.offsets, case.kv_len, case.tables, case.pool, 51, case.scales)
+    busy = [t.data_ptr() for t in paged.cache_read(*args, status=status)]
+    got = paged.cache_read(*args, status=status, stream=side)
+    assert not {t.data_ptr() for t in got} & set(busy)
+    busy = qk_norm_rope(case.q, None, torch.arange(51, device=DEV), Rotary(128))[0].data_ptr()
+    side.wait_stream(torch.cuda.current_stream())
+    assert qk_norm_rope(case.q, None, torch.arange(51, device=DEV), Rotary(128), stream=side)[0].data_ptr() != busy
+    side.synchronize()
+
+
 def test_output_over_the_queries():
     for new, kv, cache in (([1, 3, 0, 90], [700, 40, 5, 91], "scaled"), ([400, 1], [1000, 30], "bf16")):
         case = Case(new, kv, (16, 2), 128, 64, cache, seed=23)
