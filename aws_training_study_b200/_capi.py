@@ -156,6 +156,7 @@ SIGNATURES = {
         _c.c_int, [_PPOOL, _I32, _I32, _I32, _I32, _I32, _c.POINTER(_c.c_size_t)]),
     "pcp_chunk_attention": (
         _c.c_int, [_PPOOL, _PBATCH, _PHEADS, _PHEADS, _I32, _c.c_float, _P, _c.c_size_t, _P, _P]),
+    "pcp_chunk_cut_parts": (_c.c_int, [_c.POINTER(_I32), _c.POINTER(_I32), _I32, _I32, _c.POINTER(_I32)]),
 }
 
 _lock = threading.Lock()

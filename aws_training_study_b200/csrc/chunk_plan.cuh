@@ -46,13 +46,14 @@ struct ChunkRecord {
   ChunkUnit last;   // the unfinished unit, when `last_cut`
   int last_cut;
   int first_state;  // 0: no partial, 1: does not end its unit, 2: ends it
-  int err;          // the CTA's (pair's) device error
+  int err;          // the CTA's device error
+  int failed;       // a wait of the CTA ran out: what it left may be unwritten
   int patch;        // tile units: V had values that were taken for zeros (nonfinite8)
 };
 
 struct ChunkWork {
   ChunkRecord* small_rec;  // [small CTAs]
-  ChunkRecord* tile_rec;   // [2 pairs] (error of each CTA; the rest by pair)
+  ChunkRecord* tile_rec;   // [2 pairs] (err, failed and patch of each CTA; the rest by pair)
   float* small_o;          // [2 small CTAs][kSmallRows][D] partials, normalised
   float* small_lse;        // [2 small CTAs][kSmallRows], log2
   float* tile_o;           // [2 pairs][kUnitRows][D]
@@ -435,6 +436,27 @@ __device__ __forceinline__ void note_part(ChunkRecord& r, const ChunkUnit& u, in
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Parts of the unit that range g of `grid` leaves unfinished: that range's, then the
+// first parts of the ranges behind it up to the one that ends the unit.  0 if it
+// cannot be merged: a range among them failed, or left no part of it.
+// masks(b, stop, end): bits of the ranges b .. b + 31 whose first part is not one that
+// goes on (or that failed, or do not exist), and of those whose part ends its unit.
+template <typename Masks>
+__host__ __device__ __forceinline__ int cut_parts(int g, int grid, bool failed, Masks masks) {
+  if (failed) return 0;
+  for (int b = g + 1; b < grid; b += 32) {
+    uint32_t stop, end;
+    masks(b, stop, end);
+    if (stop == 0) continue;
+    const uint32_t first = stop & (0u - stop);
+    if ((end & first) == 0) return 0;
+    int parts = b - g;  // g .. b - 1
+    for (uint32_t i = first; i != 0; i >>= 1) ++parts;
+    return parts;
+  }
+  return 0;
+}
+
 // Merges the parts of cut units: O = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i -
 // M); rows that saw no key are zeros.  Block (g, y) takes the rows [8 / kW y, ...)
 // of the unit that range g left unfinished, if any: kW warps a row, each every
@@ -452,17 +474,16 @@ __device__ __forceinline__ void combine_rows(const ChunkParams& p, const ChunkRe
   const ChunkUnit unit = rec[g].last;
   const int r = y * (8 / kW) + warp / kW;
   if (y * (8 / kW) >= unit.rows) return;
-  // Parts: slot 2 g + 1, then the first parts of the ranges behind it, up to
-  // the one that ends the unit.
-  int parts = 1;
-  for (int b = g + 1; b < grid; b += 32) {
-    const uint32_t ends = __ballot_sync(0xffffffffu, b + lane < grid && rec[b + lane].first_state == 2);
-    if (ends) {
-      parts += __ffs(ends);
-      break;
-    }
-    parts += 32;
-  }
+  // Slot 2 g + 1, then the first parts of the ranges behind it.
+  auto failed_range = [&](int i) { return (kTile ? p.work.tile_rec[2 * i].failed | p.work.tile_rec[2 * i + 1].failed
+                                                 : p.work.small_rec[i].failed) != 0; };
+  const int parts = cut_parts(g, grid, failed_range(g), [&](int b, uint32_t& stop, uint32_t& end) {
+    const bool there = b + lane < grid && !failed_range(b + lane);
+    const int state = there ? rec[b + lane].first_state : 0;
+    stop = __ballot_sync(0xffffffffu, state != 1);
+    end = __ballot_sync(0xffffffffu, state == 2);
+  });
+  if (parts == 0) return;
   // (Warps behind the unit's last row go along with it and write nothing.)
   auto row_of = [&](int i) {
     return static_cast<long long>(i == 0 ? 2 * g + 1 : 2 * (g + i)) * unit_rows + min(r, unit.rows - 1);

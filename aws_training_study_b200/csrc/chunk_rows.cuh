@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     if (threadIdx.x == 0) {
       clear_record(rec);
       rec.err = kErrSmemAlign;
+      rec.failed = 1;
     }
     return;
   }
@@ -649,8 +650,8 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     }
   }
   if (threadIdx.x == 0) {
-    // After a failure nothing is merged: the partials may be unwritten.
-    if (!ok) clear_record(rec);
+    // After a failure nothing of the range is merged: its partials may be unwritten.
+    rec.failed = !ok || *abort_flag;
     rec.err = *static_cast<volatile int*>(err);
   }
 }

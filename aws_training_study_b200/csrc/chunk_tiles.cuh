@@ -304,9 +304,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   if (sbase & 1023u) {  // identical in both CTAs: neither starts
     if (threadIdx.x == 0) {
       p.work.tile_rec[blockIdx.x].err = kErrSmemAlign;
+      p.work.tile_rec[blockIdx.x].failed = 1;
       p.work.tile_rec[blockIdx.x].patch = 0;
       clear_record(p.work.tile_rec[blockIdx.x >> 1]);
     }
+    grid_dependency_wait();
     return;
   }
   const uint32_t rank = cluster_ctarank();
@@ -990,7 +992,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     ChunkRecord& rec = p.work.tile_rec[pair];
     const bool keeps = leader && threadIdx.x == 0;
     if (keeps) clear_record(rec);
-    const bool done = for_each_segment([&](const TileUnit& un, int kt0, int kt1, int seg) -> bool {
+    for_each_segment([&](const TileUnit& un, int kt0, int kt1, int seg) -> bool {
       if (keeps) note_part(rec, un, kt0, kt1);
       bool ok = true;
       const int r = static_cast<int>(rank) * kTileM + row;  // row of the unit
@@ -1181,7 +1183,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         return true;
       }
     });
-    if (keeps && !done) clear_record(rec);  // after a failure nothing is merged
   }
 
   // Both CTAs: the leader's MMAs (which read the peer's smem and TMEM) are
@@ -1192,6 +1193,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   grid_dependency_wait();  // the small units: the merge waits for them through this kernel
   if (threadIdx.x == 0) {
     p.work.tile_rec[blockIdx.x].err = *static_cast<volatile int*>(err);
+    p.work.tile_rec[blockIdx.x].failed = *abort_flag;  // (nothing of the range is merged then)
     p.work.tile_rec[blockIdx.x].patch = *patch;
   }
   if (warp == kMmaWarp) {

@@ -503,4 +503,18 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, copy, st) : launch_chunk<128>(*pool, p, copy, st);
 }
 
+int pcp_chunk_cut_parts(const int32_t* states, const int32_t* failed, int32_t ranges, int32_t range, int32_t* parts) {
+  if (!states || !failed || !parts || ranges <= 0 || range < 0 || range >= ranges)
+    return fail(PCP_ERR_INVALID_ARGUMENT, "bad arguments");
+  *parts = pcp::cut_parts(range, ranges, failed[range] != 0, [&](int b, uint32_t& stop, uint32_t& end) {
+    stop = end = 0;
+    for (int i = 0; i < 32; ++i) {
+      const int state = b + i < ranges && !failed[b + i] ? states[b + i] : 0;
+      stop |= static_cast<uint32_t>(state != 1) << i;
+      end |= static_cast<uint32_t>(state == 2) << i;
+    }
+  });
+  return PCP_OK;
+}
+
 }  // extern "C"

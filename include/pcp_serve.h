@@ -146,6 +146,14 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
                         int32_t max_chunk, float softmax_scale, void* workspace, size_t workspace_bytes,
                         int32_t* device_status, void* stream);
 
+/* Host-side view of the merge of a unit that work ranges share (the same code
+ * the kernel runs), for tests and tools: the parts of the unit that range
+ * `range` of `ranges` leaves unfinished.  states (HOST [ranges]): a range's first
+ * part is 0 none (of a unit begun before it), 1 one that goes on behind it, 2 the
+ * unit's last; failed (HOST [ranges]): not 0 where a wait ran out.  *parts is 0 when
+ * the unit is not merged: a part of it is missing or may be unwritten. */
+int pcp_chunk_cut_parts(const int32_t* states, const int32_t* failed, int32_t ranges, int32_t range, int32_t* parts);
+
 #ifdef __cplusplus
 }
 #endif
