@@ -28,6 +28,8 @@
 
 namespace pcp {
 
+enum : int { kCacheBf16 = 0, kCacheE4m3 = 1, kCacheScaled = 2 };
+
 constexpr int kSmallRows = 32;
 constexpr int kUnitRows = 256;  // rows of a tile unit: a CTA pair's
 constexpr int kStepKeys = 128;
@@ -79,6 +81,9 @@ struct ChunkParams {
 __device__ __forceinline__ float exp2_of_int(int e) {  // 2^e, 0 below the normal range
   return __uint_as_float(static_cast<uint32_t>(min(max(e + 127, 0), 254)) << 23);
 }
+
+// A scale byte's exponent, b - 127: b as the low bits of 1.5 * 2^23.
+__device__ __forceinline__ float exponent_of_scale(uint32_t b) { return __uint_as_float(0x4B400000u | b) - 12583039.f; }
 
 // 5-D tiled TMA load into THIS CTA's shared memory whose bytes count on
 // `cluster_bar`, an mbarrier of either CTA of the pair.  Local-GPU memory; no

@@ -34,10 +34,14 @@
 // agree, so a lane takes 16 consecutive bytes of a K row as four k steps (Q's
 // fragments are laid out to match), and of a V row as 16 output columns (pairs
 // of keys are zipped with byte permutes).  All accesses hit distinct banks.
-// Scales: K's 2^e multiplies its key's score, V's 2^e its key's weight p.  The
-// softmax's reference m is kept above (score + V exponent) instead of the score
-// alone, so that p 2^e stays in f16's range whatever the exponents; m cancels
-// between O and l as ever.  f16's 11 bits for p 2^e are three more than bf16's.
+// Scales: K's 2^e multiplies its key's score, V's 2^e its key's weight, as part of
+// the exponent: 2^(s + e - m), where m follows the largest s + e, key by key, that
+// the row sees.  So the weights that enter f16 are at most 2^8, the largest contribution
+// is 1 or more whatever the exponents, and a large V whose key weighs nothing takes
+// nothing from the others (a reference of the largest s and the largest e, of
+// different keys, did); m cancels between O and l as ever.  f16's 11 bits are three
+// more than bf16's; contributions below 2^-24 of the largest are lost.  The second
+// exponential in place of a product costs 1 % of a decode step (16 of 32768: 84.1 to 85.0 us).
 // Q is brought to f16 by a power of two of its row.
 #pragma once
 
@@ -113,10 +117,11 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "memory");
 }
 
-template <int D, bool kFp8>
-__global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
+template <int D, int kCache>
+__global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1)
     chunk_rows_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale,
                       const int box_shift, const ChunkParams p) {
+  constexpr bool kFp8 = kCache != kCacheBf16, kScaled = kCache == kCacheScaled;
   using L = RowsSmem<D, kFp8>;
   constexpr int kBoxElts = 128 / L::kElt;
   constexpr int kBoxSteps = kBoxElts / 16;  // MMA k steps of a box: 8 or 4
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
   }
   if (warp == L::kWarps && lane == 0) {
     tma_prefetch_desc(&tm_kv);
-    if (kFp8 && p.pool.scales) tma_prefetch_desc(&tm_scale);
+    if (kScaled) tma_prefetch_desc(&tm_scale);
   }
   grid_launch_dependents();  // the merge may wait on the SMs
   __syncthreads();
@@ -179,7 +184,6 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     // The whole warp walks and waits, one elected lane issues (chunk_tiles.cuh).
     const bool elected = elect_one();
     bool ok = true;
-    const bool scaled = kFp8 && p.pool.scales;
     const int bs = p.pool.block_size;
     while (ok && walk.next(p, err, un, kt0, kt1)) {
       const int k0 = kt0 * kStepKeys, k1 = min(kt1 * kStepKeys, un.kvlen);
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         ok = __all_sync(0xffffffffu,
                         mbar_wait(bar_empty(st), ((c / L::kStages) & 1u) ^ 1u, abort_flag, err, kErrWaitKvEmpty));
         if (!ok) break;
-        if (elected) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (scaled ? 2 * box_rows : 0)));
+        if (elected) mbar_arrive_expect_tx(bar_full(st), boxes * (box_bytes + (kScaled ? 2 * box_rows : 0)));
         for (int b = 0; b < boxes; ++b, ++i) {
           if (i == 32) {
             i = 0;
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
           const int pg = 2 * __shfl_sync(0xffffffffu, page, i), at = __shfl_sync(0xffffffffu, row, i);
           if (elected) {
             tma_load_5d(sbase + st * L::kStageBytes + b * box_bytes, &tm_kv, 0, at, 0, un.head, pg, bar_full(st));
-            if (scaled)
+            if (kScaled)
               tma_load_3d(sScale + st * L::kScaleStage + b * scale_slot, &tm_scale, at, un.head, pg, bar_full(st));
           }
         }
@@ -289,7 +293,6 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
     const int pos0 = row_pos[qt * 16 + gq], pos1 = row_pos[qt * 16 + gq + 8];
     // Keys that every live row of the tile sees: no comparison needed there.
     const int all_see = keys_all_see(un.kvlen, un.qlen, un.row0 + qt * 16, p.group);
-    const bool scaled = kFp8 && p.pool.scales;
 
     float o[16][4];
 #pragma unroll
@@ -361,67 +364,42 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
         // last of a decode step's.
         auto finish = [&](auto all) {
           constexpr bool whole = decltype(all)::value;
-          float vs[4] = {1.f, 1.f, 1.f, 1.f};  // V scales of this lane's four keys
-          int ev = 127, ev1 = 127;             // their largest exponents, biased, of those that either row sees
-          if (scaled) {
-            const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
-            ev = 0;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t kb = *reinterpret_cast<const uint16_t*>(sc + 8 * n);
-              uint32_t vv = *reinterpret_cast<const uint16_t*>(sc + box_rows + 8 * n);
-              if (!whole) {  // keys that are not there: any byte
-                if (8 * n + 2 * i4 >= left) vv &= 0xFF00u;
-                if (8 * n + 2 * i4 + 1 >= left) vv &= 0x00FFu;
-              }
-              const float ka = __uint_as_float((kb & 0xFFu) << 23), kc = __uint_as_float((kb >> 8) << 23);
-              s[n][0] *= ka;
-              s[n][1] *= kc;
-              s[n][2] *= ka;
-              s[n][3] *= kc;
-              vs[2 * n] = __uint_as_float((vv & 0xFFu) << 23);
-              vs[2 * n + 1] = __uint_as_float((vv >> 8) << 23);
-              ev = max(ev, static_cast<int>(max(vv & 0xFFu, vv >> 8)));
-            }
-            ev1 = ev;
-            if (!whole) {
-              ev = ev1 = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = key + 8 * (i / 2) + 2 * i4 + i % 2, e = static_cast<int>(__float_as_uint(vs[i]) >> 23);
-                vs[i] = fminf(vs[i], __uint_as_float(254u << 23));  // (255, no scale: finite where not seen)
-                if (at <= pos0) ev = max(ev, e);
-                if (at <= pos1) ev1 = max(ev1, e);
-              }
-#pragma unroll
-              for (int x = 1; x <= 2; x <<= 1) ev1 = max(ev1, __shfl_xor_sync(0xffffffffu, ev1, x));
-            }
-          }
-          // Scores in log2 units, hidden keys at -inf.
+          // Scores in log2 units, hidden keys at -inf (their scale bytes may be any);
+          // the V exponents of this lane's four keys.
+          float ev[4] = {0.f, 0.f, 0.f, 0.f};
           float mx0 = -INFINITY, mx1 = -INFINITY;
+          const uint8_t* sc = smem + L::kScaleOff + st * L::kScaleStage + box * scale_slot + in_box + 2 * i4;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2; ++n) {
+            uint32_t kb = 0;
+            if (kScaled) {
+              kb = *reinterpret_cast<const uint16_t*>(sc + 8 * n);
+              const uint32_t vb = *reinterpret_cast<const uint16_t*>(sc + box_rows + 8 * n);
+              ev[2 * n] = exponent_of_scale(vb & 0xFFu);
+              ev[2 * n + 1] = exponent_of_scale(vb >> 8);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               s[n][j] *= f0;
               s[n][j + 2] *= f1;
+              if (kScaled) {
+                const float k2 = __uint_as_float((j ? kb >> 8 : kb & 0xFFu) << 23);
+                s[n][j] *= k2;
+                s[n][j + 2] *= k2;
+              }
               if (!whole) {
                 const int kk = 8 * n + 2 * i4 + j;
                 if (kk >= left || key + kk > pos0) s[n][j] = -INFINITY;
                 if (kk >= left || key + kk > pos1) s[n][j + 2] = -INFINITY;
               }
-              mx0 = fmaxf(mx0, s[n][j]);
-              mx1 = fmaxf(mx1, s[n][j + 2]);
+              mx0 = fmaxf(mx0, kScaled ? s[n][j] + ev[2 * n + j] : s[n][j]);
+              mx1 = fmaxf(mx1, kScaled ? s[n][j + 2] + ev[2 * n + j] : s[n][j + 2]);
             }
+          }
 #pragma unroll
           for (int x = 1; x <= 2; x <<= 1) {
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
-            if (scaled) ev = max(ev, __shfl_xor_sync(0xffffffffu, ev, x));
-          }
-          if (scaled) {
-            mx0 += static_cast<float>(ev - 127);
-            mx1 += static_cast<float>((whole ? ev : ev1) - 127);
           }
           // The reference moves when the largest weight would pass 2^8 (and
           // from its start); O and l follow.
@@ -448,11 +426,9 @@ __global__ void __launch_bounds__(RowsSmem<D, kFp8>::kThreads, 1)
             float pc = ex2_approx(s[n][2] - r1), pd = ex2_approx(s[n][3] - r1);
             l0 += pa + pb;
             l1 += pc + pd;
-            if (scaled) {
-              pa *= vs[2 * n];
-              pb *= vs[2 * n + 1];
-              pc *= vs[2 * n];
-              pd *= vs[2 * n + 1];
+            if (kScaled) {
+              pa = ex2_approx(s[n][0] + ev[2 * n] - r0), pb = ex2_approx(s[n][1] + ev[2 * n + 1] - r0);
+              pc = ex2_approx(s[n][2] + ev[2 * n] - r1), pd = ex2_approx(s[n][3] + ev[2 * n + 1] - r1);
             }
             pk[2 * n] = kFp8 ? pack_f16x2(pa, pb) : pack_bf16x2(pa, pb);
             pk[2 * n + 1] = kFp8 ? pack_f16x2(pc, pd) : pack_bf16x2(pc, pd);

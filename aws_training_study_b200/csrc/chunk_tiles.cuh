@@ -34,9 +34,9 @@
 //   * An e4m3 cache that many query tiles read is expanded into a bf16 copy first
 //     (chunk_expand_kernel; exact, scales included), when the copy is of moderate
 //     size: reading it in place converts every key tile again for each 256 rows.
-//   * Scaled e4m3 caches: K's 2^e multiplies the scores of its key, V's 2^e the
-//     weights, and the softmax reference is kept above score + V exponent, as in
-//     chunk_rows.cuh.
+//   * Scaled e4m3 caches: K's 2^e multiplies the scores of its key, V's e is added to
+//     the exponent of its weight, and the softmax reference follows the largest
+//     score + V exponent, key by key, as in chunk_rows.cuh.
 #pragma once
 
 #include <cuda.h>
@@ -51,8 +51,6 @@
 #include "conv_geo.cuh"
 
 namespace pcp {
-
-enum : int { kCacheBf16 = 0, kCacheE4m3 = 1, kCacheScaled = 2 };
 
 constexpr int kTilesConvWarps = 4;
 constexpr int kTilesConvThreads = 32 * kTilesConvWarps;
@@ -105,8 +103,8 @@ struct TilesSmem {
   static constexpr int kScaleBufs = kCache == kCacheScaled ? (kOpStages + 4) / 2 : 0;
   static constexpr int kOpOff = kQBufs * kQBytes;
   static constexpr int kRawOff = kOpOff + kOpStages * kOpBytes;
-  static constexpr int kScaleOff = kRawOff + kRawStages * kRawBytes;  // float k[128], v[128], int vmax[4]
-  static constexpr int kScaleBuf = 2 * kTileN * 4 + 16;
+  static constexpr int kScaleOff = kRawOff + kRawStages * kRawBytes;  // float k[128] (2^e), v[128] (e)
+  static constexpr int kScaleBuf = 2 * kTileN * 4;
   // Row factors of a segment, float[128] each, and (kTwo) its rows' sums of either
   // warpgroup and references.  Q of a segment is written once QK^T of the one
   // kQBufs before it is done, and QK^T of a tile is issued after PV two tiles
@@ -758,7 +756,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       if (kFp8) {
         if (kScaled && !is_v) {  // this tile's scales: a key a thread
           const int key = kt * kTileN + ct;
-          uint32_t kb = 127, vb = 0;
+          uint32_t kb = 127, vb = 127;
           if (ct < valid) {
             const int lb = key / p.pool.block_size;
             int pg = lb < p.batch.table_width ? p.batch.tables[un.seq * p.batch.table_stride + lb] : 0;
@@ -767,17 +765,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
                                 (static_cast<long long>(pg) * 2 * p.pool.heads + un.head) * p.pool.block_size +
                                 key - lb * p.pool.block_size;
             kb = sc[0];
-            // (255, no scale: finite, for rows that do not see the key.)
-            vb = min(sc[static_cast<long long>(p.pool.heads) * p.pool.block_size], uint8_t(254));
+            vb = sc[static_cast<long long>(p.pool.heads) * p.pool.block_size];
           }
           float* sf = reinterpret_cast<float*>(smem + L::kScaleOff + (J % (NB ? NB : 1)) * L::kScaleBuf);
           // (The buffer is free: see kScaleBufs; the item's op stage is waited
           // for below, so wait for it here first.)
           if (!wait_all(bar_op_empty(os), ((c / NS) & 1u) ^ 1u, kErrWaitKvEmpty)) return false;
           sf[ct] = __uint_as_float(kb << 23);
-          sf[kTileN + ct] = __uint_as_float(vb << 23);
-          const uint32_t vm = __reduce_max_sync(0xffffffffu, vb);
-          if (lane == 0) reinterpret_cast<int*>(sf + 2 * kTileN)[cw] = static_cast<int>(vm);
+          sf[kTileN + ct] = exponent_of_scale(vb);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_scale(J % (NB ? NB : 1)));
         }
@@ -1006,13 +1001,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(bar_rows(seg), (seg / L::kSegBufs) & 1u, abort_flag, err, kErrWaitQ));
         if (ok) rf = factors[(seg & (L::kSegBufs - 1)) * kTileM + row];
       }
-      float m = -INFINITY;  // reference of both halves: log2 units, V's exponents included
+      float m = -INFINITY;  // reference of both halves, log2 units (kScaled: V's exponents included)
       float l = 0.f;        // this half's weights over 2^m
 
-      // This thread's scores of tile jg: loaded, K's scales applied, keys past
-      // the row's position at -inf.  `ev` gets the tile's largest V exponent.
+      // This thread's scores of tile jg: loaded, keys past the row's position at
+      // -inf; kScaled: in log2 units (the row's factor first: it is below 1 for queries up
+      // to 2^17, so that large K scales do not overflow), else without the row's factor.
       const uint32_t first_key = wg * kKeys;
-      auto scores = [&](uint32_t jg, float (&s)[kKeys], float& ev) -> bool {
+      auto scores = [&](uint32_t jg, float (&s)[kKeys]) -> bool {
         if (!__all_sync(0xffffffffu, mbar_wait(bar_s_full(jg & 1), (jg >> 1) & 1u, abort_flag, err, kErrWaitSFull)))
           return false;
         tc_fence_after();
@@ -1020,34 +1016,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
         tmem_wait_ld();
-        ev = 0.f;
         if (kScaled) {
           if (!__all_sync(0xffffffffu, mbar_wait(bar_scale(jg % (NB ? NB : 1)), (jg / (NB ? NB : 1)) & 1u, abort_flag,
                                                  err, kErrWaitKvFull)))
             return false;
           const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
-          const int4 vm = *reinterpret_cast<const int4*>(sf + 2 * kTileN);
-          ev = static_cast<float>(max(max(vm.x, vm.y), max(vm.z, vm.w)) - 127);
-          const int seen = pos + 1 - (kt0 + static_cast<int>(jg - J)) * kTileN;
-          if (seen < kTileN) {  // of the keys that this row sees alone
-            float top = 0.f;
-            const float4* vs = reinterpret_cast<const float4*>(sf + kTileN);
-#pragma unroll 4
-            for (int i = 0; i < kTileN; i += 4) {
-              const float4 v4 = vs[i / 4];
-              top = fmaxf(top, fmaxf(fmaxf(i < seen ? v4.x : 0.f, i + 1 < seen ? v4.y : 0.f),
-                                     fmaxf(i + 2 < seen ? v4.z : 0.f, i + 3 < seen ? v4.w : 0.f)));
-            }
-            ev = static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127);
-          }
           const float4* ks = reinterpret_cast<const float4*>(sf + first_key);
+          const f32x2 rf2 = pcp::pair(rf, rf);
 #pragma unroll
           for (int i = 0; i < kKeys / 4; ++i) {
             const float4 k4 = ks[i];
-            s[4 * i] *= k4.x;
-            s[4 * i + 1] *= k4.y;
-            s[4 * i + 2] *= k4.z;
-            s[4 * i + 3] *= k4.w;
+            split(mul2(mul2(pcp::pair(s[4 * i], s[4 * i + 1]), rf2), pcp::pair(k4.x, k4.y)), s[4 * i], s[4 * i + 1]);
+            split(mul2(mul2(pcp::pair(s[4 * i + 2], s[4 * i + 3]), rf2), pcp::pair(k4.z, k4.w)), s[4 * i + 2],
+                  s[4 * i + 3]);
           }
         }
         const int visible = pos + 1 - (kt0 + static_cast<int>(jg - J)) * kTileN - static_cast<int>(first_key);
@@ -1058,9 +1039,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         }
         return true;
       };
-      // P = 2^(s rf - ref), times V's scales, into TMEM columns [t_p, t_p + kKeys
-      // / 2); returns the sum of 2^(s rf - ref).  A row that has seen nothing yet
-      // has only -inf scores.
+      // The largest score + V exponent of this thread's keys of tile jg (kScaled).
+      auto top = [&](uint32_t jg, const float (&s)[kKeys]) -> float {
+        const float4* ve = reinterpret_cast<const float4*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf) +
+                           (kTileN + first_key) / 4;
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kKeys / 4; ++i) {
+          const float4 e = ve[i];
+          mx0 = fmaxf(mx0, fmaxf(s[4 * i] + e.x, s[4 * i + 1] + e.y));
+          mx1 = fmaxf(mx1, fmaxf(s[4 * i + 2] + e.z, s[4 * i + 3] + e.w));
+        }
+        return fmaxf(mx0, mx1);
+      };
+      // P = 2^(s rf - ref), kScaled 2^(s + V's exponent - ref), into TMEM columns
+      // [t_p, t_p + kKeys / 2); returns the sum of the weights without V's exponents.
+      // A row that has seen nothing yet has only -inf scores.
       auto probs = [&](uint32_t jg, const float (&s)[kKeys], float ref, uint32_t t_p) -> float {
         const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
         const float neg = ref == -INFINITY ? 0.f : -ref;
@@ -1072,19 +1066,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             float q0, q1, q2, q3;
-            split(fma2(pcp::pair(s[c2 * 32 + 2 * i], s[c2 * 32 + 2 * i + 1]), rf2, neg2), q0, q1);
-            split(fma2(pcp::pair(s[c2 * 32 + 2 * i + 2], s[c2 * 32 + 2 * i + 3]), rf2, neg2), q2, q3);
+            const f32x2 s0 = pcp::pair(s[c2 * 32 + 2 * i], s[c2 * 32 + 2 * i + 1]);
+            const f32x2 s1 = pcp::pair(s[c2 * 32 + 2 * i + 2], s[c2 * 32 + 2 * i + 3]);
+            split(kScaled ? add2(s0, neg2) : fma2(s0, rf2, neg2), q0, q1);
+            split(kScaled ? add2(s1, neg2) : fma2(s1, rf2, neg2), q2, q3);
             q0 = ex2_approx(q0);
             q1 = ex2_approx(q1);
             q2 = ex2_approx(q2);
             q3 = ex2_approx(q3);
             sum = add2(sum, add2(pcp::pair(q0, q1), pcp::pair(q2, q3)));
             if (kScaled) {
-              const float4 v4 = *reinterpret_cast<const float4*>(sf + kTileN + first_key + c2 * 32 + 2 * i);
-              q0 *= v4.x;
-              q1 *= v4.y;
-              q2 *= v4.z;
-              q3 *= v4.w;
+              const float4 e = *reinterpret_cast<const float4*>(sf + kTileN + first_key + c2 * 32 + 2 * i);
+              split(add2(add2(s0, pcp::pair(e.x, e.y)), neg2), q0, q1);
+              split(add2(add2(s1, pcp::pair(e.z, e.w)), neg2), q2, q3);
+              q0 = ex2_approx(q0);
+              q1 = ex2_approx(q1);
+              q2 = ex2_approx(q2);
+              q3 = ex2_approx(q3);
             }
             pk[i] = kFp8 ? pack_f16x2(q0, q1) : pack_bf16x2(q0, q1);
             pk[i + 1] = kFp8 ? pack_f16x2(q2, q3) : pack_bf16x2(q2, q3);
@@ -1106,10 +1104,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       // over to the new one once their last product is in it.
       for (uint32_t jg = J; jg < Jend && ok; ++jg) {
         const int b = jg & 1;
-        float s[kKeys], ev;
-        ok = scores(jg, s, ev);
+        float s[kKeys];
+        ok = scores(jg, s);
         if (!ok) break;
-        const float pmax = row_max(s);
+        const float pmax = kScaled ? top(jg, s) : row_max(s);
         red[(b * 2 + wg) * kTileM + row] = pmax;
         mbar_arrive(bar_ref(b));
         // Pass 0 (tiles after the first): speculative P with the current
@@ -1124,7 +1122,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           if (pass == 1) {
             ok = __all_sync(0xffffffffu, mbar_wait(bar_ref(b), (jg >> 1) & 1u, abort_flag, err, kErrWaitRed));
             if (!ok) break;
-            const float tmax = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]) * rf + ev;
+            const float both = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]);
+            const float tmax = kScaled ? both : both * rf;
             const bool need = tmax > m + kRescaleThreshold;
             redo = __any_sync(0xffffffffu, need) || jg == J;
             if (need) {

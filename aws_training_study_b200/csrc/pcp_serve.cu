@@ -294,17 +294,18 @@ int launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threads, size
   return PCP_OK;
 }
 
-template <int D, bool kFp8>
+template <int D, int kCache>
 int launch_rows(const pcp_pool_t& pool, const pcp::ChunkParams& p, cudaStream_t st) {
+  constexpr bool kFp8 = kCache != pcp::kCacheBf16;
   using L = pcp::RowsSmem<D, kFp8>;
   // Rows of a copy: as many as a page's length and a stage share.
   int shift = 4;
   while ((2 << shift) <= L::kStageKeys && pool.block_size % (2 << shift) == 0) ++shift;
   CUtensorMap tm, ts{};
   PCP_TRY(make_rows_map(&tm, pool, 1 << shift, L::kBoxes, 2));
-  if (pool.scales) PCP_TRY(make_scale_map(&ts, pool, 1 << shift));
-  PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kFp8>>(L::kBytes, kFp8 ? pcp::kRowsLaunchRegs : 0)));
-  pcp::chunk_rows_kernel<D, kFp8><<<kCtas, L::kThreads, L::kBytes, st>>>(tm, ts, shift, p);
+  if (kCache == pcp::kCacheScaled) PCP_TRY(make_scale_map(&ts, pool, 1 << shift));
+  PCP_TRY((allow_smem<pcp::chunk_rows_kernel<D, kCache>>(L::kBytes, kFp8 ? pcp::kRowsLaunchRegs : 0)));
+  pcp::chunk_rows_kernel<D, kCache><<<kCtas, L::kThreads, L::kBytes, st>>>(tm, ts, shift, p);
   CUDA_TRY(cudaGetLastError());
   return PCP_OK;
 }
@@ -361,8 +362,9 @@ int launch_expanded(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* cop
 template <int D>
 int launch_chunk(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* copy, cudaStream_t st) {
   const bool bf16 = pool.kv_dtype == PCP_KV_BF16;
-  if (bf16) PCP_TRY((launch_rows<D, false>(pool, p, st)));
-  else PCP_TRY((launch_rows<D, true>(pool, p, st)));
+  if (bf16) PCP_TRY((launch_rows<D, pcp::kCacheBf16>(pool, p, st)));
+  else if (pool.scales) PCP_TRY((launch_rows<D, pcp::kCacheScaled>(pool, p, st)));
+  else PCP_TRY((launch_rows<D, pcp::kCacheE4m3>(pool, p, st)));
   if (p.tile_pairs) {
     if (copy) PCP_TRY(launch_expanded<D>(pool, p, copy, st));
     else if (bf16) PCP_TRY((launch_tiles<D, pcp::kCacheBf16>(pool, p, st)));

@@ -1,0 +1,138 @@
+"""Attention over a paged cache whose scales, scores and maxima go to their ends
+(needs a B200), against the definition in 64 bits.
+
+Tolerance, per element, with A = sum_j w_j |v_j| (w: the softmax's weights):
+  * the output's rounding, half a step: 2^-8 |o|;
+  * the weights' rounding before the second product: 2^-8 A in bf16 (bf16
+    caches and bf16 copies of e4m3 ones), 2^-11 A in f16 (e4m3 caches read in
+    place), where the scale is part of the weight: the largest w_j 2^e_j of a row
+    is 1 or more in f16, and half of f16's least step, 2^-25, is what the others may
+    lose: 2^-25 max_j (w_j 2^e_j) sum_j |code_j| over the keys that the row sees;
+  * the scores: fp32 sums over D / 16 tensor-core steps, each within 2^-22 of
+    the terms' magnitudes; the sum of score and exponent (below 2^7 here, so half
+    a step is 2^-18) and the products with its factors; ex2 within 2^-22:
+    (D / 16 * 2^-22 * max_j scale * sum_d |q_d k_jd| + 2^-17) * 2 A."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_chunk_attention import DEV, Case
+
+pytestmark = pytest.mark.gpu
+
+# Where a batch of `new` tokens over `kv` is computed, with eight query heads a KV head.
+PATHS = [("rows", [1], [200]), ("rows", [4, 1], [700, 5000]), ("tiles", [60], [333]), ("tiles", [40, 5, 90], [900, 60, 91]),
+         ("copy", [130], [200]), ("copy", [150, 1], [1100, 300])]
+
+
+def two_to(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+class Rows(Case):
+    """A batch whose cached rows are set one by one; `wide` puts a table behind
+    it that holds too many tokens for a copy."""
+
+    def __init__(self, new, kv, D=128, cache="scaled", seed=0, heads=(16, 2), bs=64, wide=False):
+        super().__init__(new, kv, heads, D, bs, cache, seed=seed)
+        self.bs, self.wide = bs, wide
+        if wide:
+            tables = torch.full((len(kv), (1 << 30) // (4 * heads[1] * D * bs * len(kv)) + 1), -1, dtype=torch.int32,
+                                device=DEV)
+            tables[:, : self.tables.shape[1]] = self.tables
+            self.tables = tables
+        self.e = [torch.zeros(2, heads[1], t, dtype=torch.long, device=DEV) for t in kv]
+        for b in range(len(kv)):
+            self.put(b)
+
+    def _at(self, b):
+        pos = torch.arange(self.kv[b], device=DEV)
+        return self.tables[b, pos // self.bs].long(), pos % self.bs
+
+    def put(self, b, k=None, v=None, ke=None, ve=None):
+        """Rows of sequence b as values over 2^e ([Hkv, t, D], [Hkv, t]); None: as they are."""
+        cfg, (page, slot) = self.cfg, self._at(b)
+        shape = (-1, 2, cfg.num_kv_heads, self.bs)
+        rows = self.pool.view(*shape, cfg.head_dim)
+        for which, (x, e) in enumerate(((k, ke), (v, ve))):
+            if x is not None:
+                rows.view(torch.uint8 if rows.element_size() == 1 else rows.dtype)[page, which, :, slot] = (
+                    x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8) if rows.element_size() == 1
+                    else x.to(torch.bfloat16)).transpose(0, 1)
+            if e is not None:
+                self.scales.view(shape)[page, which, :, slot] = (e + 127).to(torch.uint8).T
+        self.load(b)
+
+    def load(self, b):
+        """What the pages hold, in 64 bits."""
+        cfg, (page, slot) = self.cfg, self._at(b)
+        shape = (-1, 2, cfg.num_kv_heads, self.bs)
+        codes = self.pool.view(*shape, cfg.head_dim)
+        codes = codes.view(torch.uint8)[page, :, :, slot].view(codes.dtype) if codes.element_size() == 1 else \
+            codes[page, :, :, slot]
+        x = codes.double().permute(1, 2, 0, 3)
+        if self.scales is not None:
+            self.e[b] = self.scales.view(shape)[page, :, :, slot].long().permute(1, 2, 0) - 127
+        x = x * two_to(self.e[b])[..., None]
+        self.k[b], self.v[b] = x[0], x[1]
+
+    def codes(self, b, which):
+        return (self.k if which == 0 else self.v)[b] * two_to(-self.e[b][which])[..., None]
+
+    def expected(self, b, scale=None):
+        cfg, n, t = self.cfg, self.new[b], self.kv[b]
+        scale = cfg.softmax_scale if scale is None else scale
+        q = self.q[:, int(self.offsets[b]):int(self.offsets[b]) + n].double()
+        group = cfg.num_q_heads // cfg.num_kv_heads
+        o, bound = torch.zeros_like(q), torch.zeros_like(q)
+        hidden = torch.arange(t, device=DEV) > torch.arange(t - n, t, device=DEV)[:, None]
+        copied = self.cache != "bf16" and max(self.new) * group >= 1024 and n * group > 32 and not self.wide
+        for h in range(cfg.num_q_heads):
+            k, v = self.k[b][h // group], self.v[b][h // group]
+            s = (q[h] @ k.T * scale).masked_fill(hidden, -math.inf)
+            w = torch.softmax(s, -1)
+            o[h] = w @ v
+            a = w @ v.abs()
+            terms = (q[h].abs() @ k.abs().T * scale).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+            weights = 2.0 ** -8 if self.cache == "bf16" or copied else 2.0 ** -11
+            bound[h] = 2.0 ** -8 * o[h].abs() + weights * a + 2 * a * (cfg.head_dim / 16 * 2.0 ** -22 * terms + 2.0 ** -17)
+            if self.cache != "bf16" and not copied:
+                e = self.e[b][1, h // group]
+                top = (w * two_to(e)).amax(-1, keepdim=True)
+                bound[h] += 2.0 ** -25 * top * ((~hidden).double() @ self.codes(b, 1)[h // group].abs())
+        return o, bound
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("power", [12, 26, 40])
+@pytest.mark.parametrize("path,new,kv", PATHS)
+def test_a_large_value_of_no_weight_costs_nothing(path, new, kv, power, D):
+    """Visible keys whose score is 60 log2 units below the others' and whose V is
+    2^power times theirs: less than half a step of the output, and no more than
+    that for the others' weights."""
+    case = Rows(new, kv, D, seed=power)
+    u = torch.where(torch.rand(D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) < 0.5, -1.0, 1.0)
+    case.q = (case.q * 0.25 + u).to(torch.bfloat16)
+    low = 60 * math.log(2) * math.sqrt(D) / D
+    for b, t in enumerate(kv):
+        at = torch.arange(min(5, t - new[b]), t - new[b] + 1, 97, device=DEV)
+        k, e = case.codes(b, 0), case.e[b].clone()
+        k -= (k @ u.double())[..., None] / D * u.double()  # nothing along u but in those keys
+        e[0], e[1] = 0, torch.randint(-3, 1, e[1].shape, device=DEV)
+        k[:, at] = -u.double() * low
+        e[1][:, at] = power
+        case.put(b, k=k, ke=e[0], ve=e[1])
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "scaled"])
+@pytest.mark.parametrize("heads,D", [((16, 2), 128), ((32, 2), 256), ((20, 4), 128)])
+@pytest.mark.parametrize("new,kv", [([300], [1500]), ([130, 1, 400, 7], [130, 900, 3001, 64])])
+def test_long_chunks_without_room_for_a_copy(new, kv, heads, D, cache):
+    """Units of many tiles over an e4m3 cache read in place."""
+    case = Rows(new, kv, D, cache, seed=6, heads=heads, wide=True)
+    case.check(case.run())
