@@ -85,6 +85,14 @@ __device__ __forceinline__ float exp2_of_int(int e) {  // 2^e, 0 below the norma
 // A scale byte's exponent, b - 127: b as the low bits of 1.5 * 2^23.
 __device__ __forceinline__ float exponent_of_scale(uint32_t b) { return __uint_as_float(0x4B400000u | b) - 12583039.f; }
 
+// What O, weights of 2^(s + e - m), is to be multiplied with when the sum of the
+// weights alone, 2^(s - ref), is l: 2^(m - ref) / l.  In two halves: it is in fp32's
+// range, 2^(m - ref) need not be.
+__device__ __forceinline__ float output_factor(float m, float ref, float l) {
+  const float h = ex2_approx(0.5f * (m - ref));
+  return h / l * h;
+}
+
 // 5-D tiled TMA load into THIS CTA's shared memory whose bytes count on
 // `cluster_bar`, an mbarrier of either CTA of the pair.  Local-GPU memory; no
 // multicast.

@@ -39,9 +39,13 @@
 // the row sees.  So the weights that enter f16 are at most 2^8, the largest contribution
 // is 1 or more whatever the exponents, and a large V whose key weighs nothing takes
 // nothing from the others (a reference of the largest s and the largest e, of
-// different keys, did); m cancels between O and l as ever.  f16's 11 bits are three
-// more than bf16's; contributions below 2^-24 of the largest are lost.  The second
-// exponential in place of a product costs 1 % of a decode step (16 of 32768: 84.1 to 85.0 us).
+// different keys, did).  f16's 11 bits are three more than bf16's; contributions
+// below 2^-24 of the largest are lost.  The sum of the weights, 2^(s - ref), has a
+// reference of its own, a score that the row has seen (within 2^16 of the largest): under
+// m it would sit at 2^-e, and an e of 120 flushed all but the largest weights, one of
+// -100 left the sum little of fp32's range.  O's factor at the end is 2^(m - ref) / l.
+// (One reference of largest score and largest exponent for both took 84.1 us for the
+// 16 of 32768, a key's own sum 85.0, two references 86.4.)
 // Q is brought to f16 by a power of two of its row.
 #pragma once
 
@@ -84,8 +88,8 @@ struct RowsSmem {
   // The halves of a team's scores, [2 slots][warp][2][lane][4] floats, use the
   // buffers' space before the merge.
   static constexpr int kRowOff = kBufOff + kBufs * kBufBytes;  // float score factor[32], int position[32]
-  static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;  // float m, l: [team][16]
-  static constexpr int kInvOff = kMlOff + 2 * kTeams * 16 * 4;  // float 1 / sum of the weights [32]
+  static constexpr int kMlOff = kRowOff + 2 * kSmallRows * 4;  // float m, l, l's reference: [team][16]
+  static constexpr int kInvOff = kMlOff + 3 * kTeams * 16 * 4;  // float factor of O [32]
   static constexpr int kBarOff = kInvOff + kSmallRows * 4;  // full, empty
   static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
   static constexpr int kPlanOff = kMiscOff + 16;  // ChunkPlanShared
@@ -142,6 +146,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
   int* row_pos = reinterpret_cast<int*>(smem + L::kRowOff) + kSmallRows;
   float* s_m = reinterpret_cast<float*>(smem + L::kMlOff);
   float* s_l = s_m + L::kTeams * 16;
+  float* s_ref = kScaled ? s_l + L::kTeams * 16 : s_m;
   float* s_inv = reinterpret_cast<float*>(smem + L::kInvOff);
   auto bar_full = [&](int s) { return sbase + L::kBarOff + 8u * s; };
   auto bar_empty = [&](int s) { return sbase + L::kBarOff + 8u * (L::kStages + s); };
@@ -298,6 +303,7 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
 #pragma unroll
     for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float ref0 = -INFINITY, ref1 = -INFINITY;  // kScaled: l's reference
 
     uint32_t swap = 0;     // which of the two score exchange slots
     int next = 16 * turn;  // this team's next keys, from the stage's first
@@ -401,6 +407,17 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
           }
+          auto of_row = [](float x) {  // the largest of a row's four lanes
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          };
+          // kScaled: l's references up to the scores seen here, of the rows that ask for it.
+          auto raise_refs = [&](bool row0, bool row1) {
+            const float g0 = of_row(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
+            const float g1 = of_row(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])));
+            if (row0 && g0 > ref0) l0 *= ex2_approx(ref0 - g0), ref0 = g0;
+            if (row1 && g1 > ref1) l1 *= ex2_approx(ref1 - g1), ref1 = g1;
+          };
           // The reference moves when the largest weight would pass 2^8 (and
           // from its start); O and l follow.
           const bool up0 = mx0 > m0 + kRescaleThreshold, up1 = mx1 > m1 + kRescaleThreshold;
@@ -408,8 +425,12 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
             float a0 = 1.f, a1 = 1.f;
             if (up0) a0 = ex2_approx(m0 - mx0), m0 = mx0;
             if (up1) a1 = ex2_approx(m1 - mx1), m1 = mx1;
-            l0 *= a0;
-            l1 *= a1;
+            if (kScaled) {
+              raise_refs(up0, up1);
+            } else {
+              l0 *= a0;
+              l1 *= a1;
+            }
 #pragma unroll
             for (int t = 0; t < 16; ++t) {
               o[t][0] *= a0;
@@ -418,17 +439,33 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
               o[t][3] *= a1;
             }
           }
+          if (kScaled) {
+            float sum0, sum1;
+            auto weigh = [&]() {
+              const float q0 = ref0 == -INFINITY ? 0.f : ref0, q1 = ref1 == -INFINITY ? 0.f : ref1;
+              sum0 = (ex2_approx(s[0][0] - q0) + ex2_approx(s[0][1] - q0)) + (ex2_approx(s[1][0] - q0) + ex2_approx(s[1][1] - q0));
+              sum1 = (ex2_approx(s[0][2] - q1) + ex2_approx(s[0][3] - q1)) + (ex2_approx(s[1][2] - q1) + ex2_approx(s[1][3] - q1));
+            };
+            weigh();
+            if (__any_sync(0xffffffffu, fmaxf(sum0, sum1) > 65536.f)) {
+              raise_refs(of_row(sum0) > 65536.f, of_row(sum1) > 65536.f);
+              weigh();
+            }
+            l0 += sum0;
+            l1 += sum1;
+          }
           const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
           uint32_t pk[4];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            float pa = ex2_approx(s[n][0] - r0), pb = ex2_approx(s[n][1] - r0);
-            float pc = ex2_approx(s[n][2] - r1), pd = ex2_approx(s[n][3] - r1);
-            l0 += pa + pb;
-            l1 += pc + pd;
-            if (kScaled) {
-              pa = ex2_approx(s[n][0] + ev[2 * n] - r0), pb = ex2_approx(s[n][1] + ev[2 * n + 1] - r0);
-              pc = ex2_approx(s[n][2] + ev[2 * n] - r1), pd = ex2_approx(s[n][3] + ev[2 * n + 1] - r1);
+            const float ea = kScaled ? ev[2 * n] : 0.f, eb = kScaled ? ev[2 * n + 1] : 0.f;
+            const float pa = ex2_approx(kScaled ? s[n][0] + ea - r0 : s[n][0] - r0);
+            const float pb = ex2_approx(kScaled ? s[n][1] + eb - r0 : s[n][1] - r0);
+            const float pc = ex2_approx(kScaled ? s[n][2] + ea - r1 : s[n][2] - r1);
+            const float pd = ex2_approx(kScaled ? s[n][3] + eb - r1 : s[n][3] - r1);
+            if (!kScaled) {
+              l0 += pa + pb;
+              l1 += pc + pd;
             }
             pk[2 * n] = kFp8 ? pack_f16x2(pa, pb) : pack_bf16x2(pa, pb);
             pk[2 * n + 1] = kFp8 ? pack_f16x2(pc, pd) : pack_bf16x2(pc, pd);
@@ -514,11 +551,15 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
       l0 += __shfl_xor_sync(0xffffffffu, l0, x);
       l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
-    if (i4 == 0 && part == 0) {  // a team's warps hold the same m and l
+    if (i4 == 0 && part == 0) {  // a team's warps hold the same
       s_m[team * 16 + gq] = m0;
       s_m[team * 16 + gq + 8] = m1;
       s_l[team * 16 + gq] = l0;
       s_l[team * 16 + gq + 8] = l1;
+      if (kScaled) {
+        s_ref[team * 16 + gq] = ref0;
+        s_ref[team * 16 + gq + 8] = ref1;
+      }
     }
     if (!(ok = named_bar_and(1, kConsumers, ok && *abort_flag == 0))) break;
     float M0 = -INFINITY, M1 = -INFINITY;
@@ -576,16 +617,19 @@ __global__ void __launch_bounds__(RowsSmem<D, kCache != kCacheBf16>::kThreads, 1
     const int slot = part_slot(un, kt0, kt1, blockIdx.x);
     if (threadIdx.x < (two ? 32 : 16)) {
       const int r = threadIdx.x, t0 = r / 16 * teams;
-      float M = -INFINITY, lsum = 0.f;
-      for (int w = t0; w < t0 + teams; ++w) M = fmaxf(M, s_m[w * 16 + r % 16]);
+      float M = -INFINITY, ref = -INFINITY, lsum = 0.f;
       for (int w = t0; w < t0 + teams; ++w) {
-        const float mw = s_m[w * 16 + r % 16];
-        // Without a maximum the sum is 0, or NaN where every score was NaN.
-        lsum += mw == -INFINITY ? s_l[w * 16 + r % 16] : s_l[w * 16 + r % 16] * ex2_approx(mw - M);
+        M = fmaxf(M, s_m[w * 16 + r % 16]);
+        ref = fmaxf(ref, s_ref[w * 16 + r % 16]);
       }
-      s_inv[r] = lsum == 0.f ? 0.f : 1.f / lsum;  // no key seen: zeros
+      for (int w = t0; w < t0 + teams; ++w) {
+        const float rw = s_ref[w * 16 + r % 16];
+        // Without a maximum the sum is 0, or NaN where every score was NaN.
+        lsum += rw == -INFINITY ? s_l[w * 16 + r % 16] : s_l[w * 16 + r % 16] * ex2_approx(rw - ref);
+      }
+      s_inv[r] = lsum == 0.f ? 0.f : kScaled ? output_factor(M, ref, lsum) : 1.f / lsum;  // no key seen: zeros
       if (slot >= 0 && r < un.rows)
-        p.work.small_lse[static_cast<long long>(slot) * kSmallRows + r] = lsum == 0.f ? -INFINITY : M + __log2f(lsum);
+        p.work.small_lse[static_cast<long long>(slot) * kSmallRows + r] = lsum == 0.f ? -INFINITY : ref + __log2f(lsum);
     }
     for (int round = (teams - 1) / bufs; round >= 0; --round) {
       if (turn / bufs == round) exchange(turn + bufs < teams);

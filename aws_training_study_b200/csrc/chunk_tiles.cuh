@@ -115,7 +115,10 @@ struct TilesSmem {
   static constexpr int kSegBufs = kTwo ? 4 : 2;
   static constexpr int kFactorOff = kScaleOff + kScaleBufs * kScaleBuf;
   static constexpr int kRedOff = kFactorOff + (kFp8 ? kSegBufs * kTileM * 4 : 0);
-  static constexpr int kBarOff = kRedOff + (4 + (kTwo ? 3 * kSegBufs : 0)) * kTileM * 4;
+  // The halves' maxima [tile parity][2][128]: scores, or (scaled) score + exponent, then scores.
+  static constexpr int kMaxima = kCache == kCacheScaled ? 8 : 4;
+  static constexpr int kSums = kCache == kCacheScaled ? 4 : 3;  // of a segment, kTwo
+  static constexpr int kBarOff = kRedOff + (kMaxima + (kTwo ? kSums * kSegBufs : 0)) * kTileM * 4;
   // q_ready[2], q_empty[2], rows[4], o_free[2], sums[4], seg_o[2], land_full[NL],
   // land_empty[NR], op_full[NS], op_empty[NS], s_full[2], p_full[2], o_done[2],
   // teardown, ref[2], scale[NB], seg_full[], seg_empty[]
@@ -877,15 +880,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     };
     // kTwo: the output of segment sg.  Called once all that its last PV waits for is
     // on its way, Q and the first K of the next segment included.
-    const float* seg_sums = red + 4 * kTileM;  // [kSegBufs]{l of either warpgroup, m}[128]
+    const float* seg_sums = red + L::kMaxima * kTileM;  // [kSegBufs]{l of either warpgroup, its reference, (scaled) m}[128]
     auto write_out = [&](const TileUnit& un, int kt0, int kt1, int sg) -> bool {
       if (!wait_all(bar_sums(sg), (sg / L::kSegBufs) & 1u, kErrWaitRed) ||
           !wait_all(bar_seg_o(sg), (sg >> 1) & 1u, kErrWaitODone))
         return false;
       tc_fence_after();
-      const float* sums = seg_sums + (sg & (L::kSegBufs - 1)) * 3 * kTileM;
-      const float l = sums[ct] + sums[kTileM + ct], m = sums[2 * kTileM + ct];
-      const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+      const float* sums = seg_sums + (sg & (L::kSegBufs - 1)) * L::kSums * kTileM;
+      const float l = sums[ct] + sums[kTileM + ct], ref = sums[2 * kTileM + ct];
+      // No key seen: zeros.
+      const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(sums[(L::kSums - 1) * kTileM + ct], ref, l) : 1.f / l;
       const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
       const bool live = r < un.rows;
       const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
@@ -897,7 +901,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         store_rows<D>(t_o, inv_l, live ? out : nullptr, lane);
       } else {
         const long long pr = static_cast<long long>(slot) * kUnitRows + r;
-        if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
+        if (live) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : ref + __log2f(l);
         store_rows<D>(t_o, inv_l, live ? p.work.tile_o + pr * D : nullptr, lane);
       }
       tc_fence_before();
@@ -980,7 +984,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
     const int wg = warp >> 2;
     const int row = threadIdx.x & (kTileM - 1);  // == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // red: the halves' maxima [tile parity][2][128].
     float* sums = red;  // (one accumulator: a segment's sums, once its maxima were read)
     uint32_t J = 0;
     // The leader keeps the pair's record.
@@ -1002,7 +1005,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         if (ok) rf = factors[(seg & (L::kSegBufs - 1)) * kTileM + row];
       }
       float m = -INFINITY;  // reference of both halves, log2 units (kScaled: V's exponents included)
-      float l = 0.f;        // this half's weights over 2^m
+      float ref = -INFINITY;  // kScaled: l's own reference (chunk_rows.cuh), scores alone
+      float l = 0.f;          // this half's weights, over 2^m or 2^ref
 
       // This thread's scores of tile jg: loaded, keys past the row's position at
       // -inf; kScaled: in log2 units (the row's factor first: it is below 1 for queries up
@@ -1052,13 +1056,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         }
         return fmaxf(mx0, mx1);
       };
-      // P = 2^(s rf - ref), kScaled 2^(s + V's exponent - ref), into TMEM columns
-      // [t_p, t_p + kKeys / 2); returns the sum of the weights without V's exponents.
+      // P = 2^(s rf - m), kScaled 2^(s + V's exponent - m), into TMEM columns
+      // [t_p, t_p + kKeys / 2); returns the sum of P, kScaled of 2^(s - ref).
       // A row that has seen nothing yet has only -inf scores.
-      auto probs = [&](uint32_t jg, const float (&s)[kKeys], float ref, uint32_t t_p) -> float {
+      auto probs = [&](uint32_t jg, const float (&s)[kKeys], uint32_t t_p) -> float {
         const float* sf = reinterpret_cast<const float*>(smem + L::kScaleOff + (jg % (NB ? NB : 1)) * L::kScaleBuf);
-        const float neg = ref == -INFINITY ? 0.f : -ref;
-        const f32x2 rf2 = pcp::pair(rf, rf), neg2 = pcp::pair(neg, neg);
+        const float neg = m == -INFINITY ? 0.f : -m, neg_ref = ref == -INFINITY ? 0.f : -ref;
+        const f32x2 rf2 = pcp::pair(rf, rf), neg2 = pcp::pair(neg, neg), neg_ref2 = pcp::pair(neg_ref, neg_ref);
         f32x2 sum = pcp::pair(0.f, 0.f);
 #pragma unroll
         for (int c2 = 0; c2 < kKeys / 32; ++c2) {
@@ -1068,8 +1072,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             float q0, q1, q2, q3;
             const f32x2 s0 = pcp::pair(s[c2 * 32 + 2 * i], s[c2 * 32 + 2 * i + 1]);
             const f32x2 s1 = pcp::pair(s[c2 * 32 + 2 * i + 2], s[c2 * 32 + 2 * i + 3]);
-            split(kScaled ? add2(s0, neg2) : fma2(s0, rf2, neg2), q0, q1);
-            split(kScaled ? add2(s1, neg2) : fma2(s1, rf2, neg2), q2, q3);
+            split(kScaled ? add2(s0, neg_ref2) : fma2(s0, rf2, neg2), q0, q1);
+            split(kScaled ? add2(s1, neg_ref2) : fma2(s1, rf2, neg2), q2, q3);
             q0 = ex2_approx(q0);
             q1 = ex2_approx(q1);
             q2 = ex2_approx(q2);
@@ -1108,7 +1112,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         ok = scores(jg, s);
         if (!ok) break;
         const float pmax = kScaled ? top(jg, s) : row_max(s);
+        const float smax = kScaled ? row_max(s) : pmax;
         red[(b * 2 + wg) * kTileM + row] = pmax;
+        if (kScaled) red[(4 + b * 2 + wg) * kTileM + row] = smax;
         mbar_arrive(bar_ref(b));
         // Pass 0 (tiles after the first): speculative P with the current
         // reference, before the other half's maximum is known.  Pass 1:
@@ -1116,7 +1122,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         // moved past the threshold.
         float tile_sum = 0.f;
         float alpha = 1.f;
-        bool redo = false;
+        bool moved = false;
 #pragma unroll 1
         for (int pass = jg > J ? 0 : 1; pass < 2; ++pass) {
           if (pass == 1) {
@@ -1125,19 +1131,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
             const float both = fmaxf(pmax, red[(b * 2 + (wg ^ 1)) * kTileM + row]);
             const float tmax = kScaled ? both : both * rf;
             const bool need = tmax > m + kRescaleThreshold;
-            redo = __any_sync(0xffffffffu, need) || jg == J;
+            moved = __any_sync(0xffffffffu, need);
+            bool redo = moved || jg == J;
             if (need) {
               alpha = ex2_approx(m - tmax);  // 0 from the start
               m = tmax;
-              l *= alpha;
+              if (!kScaled) l *= alpha;
+            }
+            if (kScaled) {
+              const float most = fmaxf(smax, red[(4 + b * 2 + (wg ^ 1)) * kTileM + row]);
+              const bool raise = most > ref + kRescaleThreshold;
+              redo |= __any_sync(0xffffffffu, raise);
+              if (raise) {
+                l *= ex2_approx(ref - most);
+                ref = most;
+              }
             }
             if (!redo) break;
           }
-          tile_sum = probs(jg, s, m, t_row + kTmemS0 + b * kTileN + wg * kKeys);
+          tile_sum = probs(jg, s, t_row + kTmemS0 + b * kTileN + wg * kKeys);
         }
         if (!ok) break;
         l += tile_sum;
-        if (jg > J && redo) {
+        if (jg > J && moved) {
           ok = __all_sync(0xffffffffu,
                           mbar_wait(bar_o((jg - 1) & 1), ((jg - 1) >> 1) & 1u, abort_flag, err, kErrWaitODone));
           if (!ok) break;
@@ -1150,9 +1166,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       J = Jend;
       if constexpr (L::kTwo) {
         if (!ok) return false;
-        float* part = red + 4 * kTileM + (seg & (L::kSegBufs - 1)) * 3 * kTileM;
+        float* part = red + (L::kMaxima + (seg & (L::kSegBufs - 1)) * L::kSums) * kTileM;
         part[wg * kTileM + row] = l;
-        if (wg == 0) part[2 * kTileM + row] = m;
+        if (wg == 0) part[2 * kTileM + row] = kScaled ? ref : m;
+        if (wg == 0 && kScaled) part[3 * kTileM + row] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_sums(seg));
         return true;
@@ -1165,7 +1182,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         l += sums[(wg ^ 1) * kTileM + row];
         // Both read: the next segment may reuse the slots.
         named_bar_sync(2, kSoftmaxThreads);
-        const float inv_l = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+        const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(m, ref, l) : 1.f / l;  // no key seen: zeros
         const int slot = part_slot(un, kt0, kt1, pair);
         if (slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +
@@ -1173,7 +1190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
           store_rows<kOCols>(t_o, inv_l, live ? out + wg * kOCols : nullptr, lane);
         } else {
           const long long pr = static_cast<long long>(slot) * kUnitRows + r;
-          if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : m + __log2f(l);
+          if (live && wg == 0) p.work.tile_lse[pr] = l == 0.f ? -INFINITY : (kScaled ? ref : m) + __log2f(l);
           store_rows<kOCols>(t_o, inv_l, live ? p.work.tile_o + pr * D + wg * kOCols : nullptr, lane);
         }
         tc_fence_before();

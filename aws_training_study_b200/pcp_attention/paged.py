@@ -48,7 +48,7 @@ def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtyp
 def make_scales(config: PCPAttentionConfig, pool_blocks: int,
                 device: int | torch.device | str = "cuda") -> torch.Tensor:
     """Scale bytes of an e4m3 pool, ``[pool_blocks, 2 * Hkv * bs]`` uint8: a
-    byte b stands for ``2 ** (b - 127)``; all at unit scale."""
+    byte b, 27 to 247, stands for ``2 ** (b - 127)``; all at unit scale."""
     if pool_blocks <= 0:
         raise ValueError("pool_blocks must be positive")
     shape = (pool_blocks, 2 * config.num_kv_heads * config.block_size)

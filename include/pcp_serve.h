@@ -85,7 +85,8 @@ int pcp_qk_norm_rope(int32_t dtype, int32_t rows, int32_t head_dim, int32_t rota
 /* A paged cache: blocks of [2][num_kv_heads][block_size][head_dim] e4m3fn or
  * bf16, K then V.  scales (e4m3 only; NULL: unit scale): one byte b per token,
  * head and K/V, [blocks][2][num_kv_heads][block_size]; the row's values are
- * code * 2^(b - 127), b up to 254. */
+ * code * 2^(b - 127), b from 27 to 247, as pcp_cache_append writes them (what other
+ * bytes of tokens that are read give is not specified). */
 typedef struct pcp_pool {
   void* data;
   uint8_t* scales;

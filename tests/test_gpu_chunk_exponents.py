@@ -8,10 +8,12 @@ Tolerance, per element, with A = sum_j w_j |v_j| (w: the softmax's weights):
     place), where the scale is part of the weight: the largest w_j 2^e_j of a row
     is 1 or more in f16, and half of f16's least step, 2^-25, is what the others may
     lose: 2^-25 max_j (w_j 2^e_j) sum_j |code_j| over the keys that the row sees;
+  * the ends of the number formats: half of bf16's least step, 2^-134, and one least
+    step of fp32 for each product with 16 keys, 2^-149: below (1 + t / 8) 2^-134;
   * the scores: fp32 sums over D / 16 tensor-core steps, each within 2^-22 of
-    the terms' magnitudes; the sum of score and exponent (below 2^7 here, so half
-    a step is 2^-18) and the products with its factors; ex2 within 2^-22:
-    (D / 16 * 2^-22 * max_j scale * sum_d |q_d k_jd| + 2^-17) * 2 A."""
+    the terms' magnitudes; the sum of score and exponent (below 2^9 here, so half
+    a step is 2^-16) and the products with its factors; ex2 within 2^-22:
+    (D / 16 * 2^-22 * max_j scale * sum_d |q_d k_jd| + 2^-15) * 2 A."""
 
 from __future__ import annotations
 
@@ -99,7 +101,8 @@ class Rows(Case):
             a = w @ v.abs()
             terms = (q[h].abs() @ k.abs().T * scale).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
             weights = 2.0 ** -8 if self.cache == "bf16" or copied else 2.0 ** -11
-            bound[h] = 2.0 ** -8 * o[h].abs() + weights * a + 2 * a * (cfg.head_dim / 16 * 2.0 ** -22 * terms + 2.0 ** -17)
+            bound[h] = 2.0 ** -8 * o[h].abs() + weights * a + 2 * a * (cfg.head_dim / 16 * 2.0 ** -22 * terms + 2.0 ** -15)
+            bound[h] += (1 + t / 8) * 2.0 ** -134
             if self.cache != "bf16" and not copied:
                 e = self.e[b][1, h // group]
                 top = (w * two_to(e)).amax(-1, keepdim=True)
@@ -127,6 +130,21 @@ def test_a_large_value_of_no_weight_costs_nothing(path, new, kv, power, D):
         e[1][:, at] = power
         case.put(b, k=k, ke=e[0], ve=e[1])
     case.check(case.run())
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("exponents", [(120,), (-100,), (-100, 120), (-100, -60, 0, 60, 120)])
+@pytest.mark.parametrize("path,new,kv", PATHS[:4])
+def test_exponents_that_an_append_may_write(path, new, kv, exponents, D):
+    """V's scales at the ends of what is written (bytes 27 and 247), alone and
+    mixed, under weights that fall off over many powers of two."""
+    case = Rows(new, kv, D, seed=len(exponents))
+    g = torch.Generator(device=DEV).manual_seed(2)
+    for b in range(len(kv)):
+        pick = torch.randint(len(exponents), case.e[b][1].shape, device=DEV, generator=g)
+        case.put(b, ke=torch.full_like(case.e[b][0], 1), ve=torch.tensor(exponents, device=DEV)[pick])
+    case.check(case.run())
+    case.check(case.run(softmax_scale=0.5), scale=0.5)
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "scaled"])
