@@ -73,6 +73,7 @@ struct ChunkParams {
   long long capacity;  // tokens a sequence's table holds
   int max_chunk;
   float scale_log2;
+  float v_factor;  // what V of a bf16 cache is to be multiplied with (kCopyShift)
   int small_ctas, tile_pairs;  // grids of the two kernels (0 pairs: not launched)
   int small_y, tile_y;         // blocks that merge a unit of either kind
   int* status;

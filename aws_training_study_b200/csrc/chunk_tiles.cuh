@@ -215,6 +215,13 @@ struct TileBoxes {
   int all_cols;        // bf16: all 64-element columns in a copy (pages of a multiple of 64 tokens)
 };
 
+// Values of a scaled cache are copied times 2^-kCopyShift, scores and output are
+// multiplied back: 448 * 2^120 is beyond bf16 (a value of 2^128, which an append may
+// write, became infinity and, where it passed the converter warps, vanished), and the
+// sums of weights up to 2^8 need room in fp32 too.  The least code, 2^-9, at the least
+// exponent, -100, is still a normal bf16 number.
+constexpr int kCopyShift = 16;
+
 // The pages of sequences with tile units as bf16: sequence s is one block of
 // `copy`, [2][Hkv][copy_rows][D].  Bound by HBM (1 byte read, 2 written an
 // element); a thread block takes 64 rows of one head of K or V at a time (pages
@@ -259,7 +266,7 @@ __device__ __forceinline__ void expand_item(const ExpandParams& p, int s, int kv
       const int e = e0 + u * 256;
       if (e >= n * kPerRow) break;
       uint4 o[2];
-      e4m3x16_to_bf16(x[u], sc[u], o);
+      e4m3x16_to_bf16(x[u], scales ? __uint_as_float((min(max(sc[u], kCopyShift + 1u), 254u) - kCopyShift) << 23) : 1.f, o);
       dst[2 * e] = o[0];
       dst[2 * e + 1] = o[1];
     }
@@ -298,6 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   using L = TilesSmem<D, kCache>;
   constexpr bool kFp8 = L::kFp8;
   constexpr bool kScaled = kCache == kCacheScaled;
+  const float v_factor = kFp8 ? 1.f : p.v_factor;
   constexpr int NS = L::kOpStages, NL = L::kLandStages, NR = L::kRawStages, NB = L::kScaleBufs;
 
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -889,7 +897,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
       const float* sums = seg_sums + (sg & (L::kSegBufs - 1)) * L::kSums * kTileM;
       const float l = sums[ct] + sums[kTileM + ct], ref = sums[2 * kTileM + ct];
       // No key seen: zeros.
-      const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(sums[(L::kSums - 1) * kTileM + ct], ref, l) : 1.f / l;
+      const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(sums[(L::kSums - 1) * kTileM + ct], ref, l)
+                                                  : v_factor / l;
       const int r = static_cast<int>(rank) * kTileM + ct;  // row of the unit
       const bool live = r < un.rows;
       const uint32_t t_o = tmem + (static_cast<uint32_t>(cw * 32) << 16) + (sg & 1) * D;
@@ -1182,7 +1191,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
         l += sums[(wg ^ 1) * kTileM + row];
         // Both read: the next segment may reuse the slots.
         named_bar_sync(2, kSoftmaxThreads);
-        const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(m, ref, l) : 1.f / l;  // no key seen: zeros
+        const float inv_l = l == 0.f ? 0.f : kScaled ? output_factor(m, ref, l) : v_factor / l;  // no key seen: zeros
         const int slot = part_slot(un, kt0, kt1, pair);
         if (slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<long long>(un.head * p.group + at % p.group) * p.out_head +

@@ -354,6 +354,10 @@ int launch_expanded(const pcp_pool_t& pool, const pcp::ChunkParams& p, void* cop
   dense.kv_dtype = PCP_KV_BF16;
   pcp::ChunkParams d = p;
   d.pool = pool_view(dense);
+  if (pool.scales) {
+    d.scale_log2 = std::ldexp(p.scale_log2, pcp::kCopyShift);
+    d.v_factor = std::ldexp(1.f, pcp::kCopyShift);
+  }
   d.batch.tables = nullptr;
   d.batch.table_width = 1;
   return launch_tiles<D, pcp::kCacheBf16>(dense, d, st);
@@ -494,6 +498,7 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.capacity = static_cast<int64_t>(batch->table_width) * pool->block_size;
   p.max_chunk = max_chunk;
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
+  p.v_factor = 1.f;
   p.small_ctas = kCtas;
   p.tile_pairs = has_tiles(max_chunk, group) ? kPairs : 0;
   // Rows of the longest small and tile unit, over the rows a block merges.
@@ -501,7 +506,9 @@ int pcp_chunk_attention(const pcp_pool_t* pool, const pcp_batch_t* batch, const 
   p.small_y = static_cast<int>(ceil_div(std::min<int64_t>(longest, pcp::kSmallRows), 8 / pcp::kCombineSmallW));
   p.tile_y = static_cast<int>(ceil_div(std::min<int64_t>(longest, pcp::kUnitRows), 8 / pcp::kCombineTileW));
   p.status = device_status;
-  void* copy = w.expand ? ws + w.copy : nullptr;
+  // (A scale that the copy's power of two would take out of fp32: in place.)
+  const bool fits = !pool->scales || !std::isinf(std::ldexp(p.scale_log2, pcp::kCopyShift));
+  void* copy = w.expand && fits ? ws + w.copy : nullptr;
   return pool->head_dim == 256 ? launch_chunk<256>(*pool, p, copy, st) : launch_chunk<128>(*pool, p, copy, st);
 }
 

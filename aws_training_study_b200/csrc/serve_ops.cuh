@@ -351,11 +351,10 @@ __device__ __forceinline__ int sequence_of(const BatchView& b, int row) {
   return b.offsets[lo] <= row && row < b.offsets[lo + 1] ? lo : -1;
 }
 
-// 16 codes times 2^(b - 127) as bf16: four significant bits, so exact.
-__device__ __forceinline__ void e4m3x16_to_bf16(const uint4& codes, uint32_t b, uint4* out) {
+// 16 codes times a power of two as bf16: four significant bits, so exact.
+__device__ __forceinline__ void e4m3x16_to_bf16(const uint4& codes, float s, uint4* out) {
   uint4 h[2];
   e4m3x16_to_f16(codes, h[0], h[1]);
-  const float s = __uint_as_float(min(b, 254u) << 23);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t hw[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
@@ -537,7 +536,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheRowsParams p
       for (int u = 0; u < kRowsInFlight; ++u) {
         if (c[u].blk != -2 && c[u].blk < 0) continue;  // -2: the token cannot be found, zeros
         uint4 o[2] = {x[u][0], x[u][1]};
-        if (!pool.bf16) e4m3x16_to_bf16(x[u][0], sc[u], o);
+        if (!pool.bf16) e4m3x16_to_bf16(x[u][0], __uint_as_float(min(sc[u], 254u) << 23), o);
         uint4* dst = reinterpret_cast<uint4*>(const_cast<__nv_bfloat16*>(packed_row(p, t0 + c[u].tok, c[u].which)) + 16 * l);
         dst[0] = o[0];
         dst[1] = o[1];

@@ -113,8 +113,8 @@ typedef struct pcp_batch {
  * number with max|x| <= 448 * 2^e (0 for a row of zeros, held to -100 .. 120)
  * over the row's finite elements, and b = e + 127: products by powers of two
  * lose nothing, and what is read back is exact in bf16 (but for values that
- * round up to 2^128, which read as infinity).  Non-finite elements become NaN
- * codes.  Without scales, as pcp_cache_write.  Two rows that map to
+ * round up to 2^128, which read as infinity; attention takes them as 2^128).
+ * Non-finite elements become NaN codes.  Without scales, as pcp_cache_write.  Two rows that map to
  * one slot race. */
 int pcp_cache_append(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_heads_t* k, const pcp_heads_t* v,
                      int32_t* device_status, void* stream);
@@ -135,6 +135,12 @@ int pcp_cache_read(const pcp_pool_t* pool, const pcp_batch_t* batch, const pcp_h
  * nothing, whatever it holds: infinities and NaN there too.  An element of V that is
  * not finite makes its column of the rows that see it not finite (NaN for those of
  * the new tokens themselves).
+ * Scores, sums and accumulators are fp32.  Weights are rounded before they meet V: to
+ * bf16 over bf16 caches, and over e4m3 caches that chunks read through a bf16 copy
+ * (max_chunk * G >= 1024, where the workspace has room for it); to f16 over other e4m3
+ * caches, a key's scale included, where contributions of keys below 2^-24 of the
+ * row's largest are lost.  Weights up to 2^8 times V are summed before the division:
+ * V of a bf16 cache beyond some 2^100 may overflow there.
  *   - max_chunk bounds every sequence's rows (HOST value; it picks which
  *     kernels are launched).  Lengths and tables are read on the device.
  *   - q, out: bf16 [num_q_heads][rows][head_dim] at any 16-byte aligned stride.

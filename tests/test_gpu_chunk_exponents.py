@@ -9,7 +9,8 @@ Tolerance, per element, with A = sum_j w_j |v_j| (w: the softmax's weights):
     is 1 or more in f16, and half of f16's least step, 2^-25, is what the others may
     lose: 2^-25 max_j (w_j 2^e_j) sum_j |code_j| over the keys that the row sees;
   * the ends of the number formats: half of bf16's least step, 2^-134, and one least
-    step of fp32 for each product with 16 keys, 2^-149: below (1 + t / 8) 2^-134;
+    step of fp32 for each product with 16 keys, 2^-149 (2^16 times that in a copy,
+    which holds 2^-16 of the values): (1 + t / 8) 2^-134;
   * the scores: fp32 sums over D / 16 tensor-core steps, each within 2^-22 of
     the terms' magnitudes; the sum of score and exponent (below 2^9 here, so half
     a step is 2^-16) and the products with its factors; ex2 within 2^-22:
@@ -22,6 +23,7 @@ import math
 import pytest
 import torch
 
+from aws_training_study_b200.pcp_attention.paged import cache_append
 from test_gpu_chunk_attention import DEV, Case
 
 pytestmark = pytest.mark.gpu
@@ -134,7 +136,7 @@ def test_a_large_value_of_no_weight_costs_nothing(path, new, kv, power, D):
 
 @pytest.mark.parametrize("D", [128, 256])
 @pytest.mark.parametrize("exponents", [(120,), (-100,), (-100, 120), (-100, -60, 0, 60, 120)])
-@pytest.mark.parametrize("path,new,kv", PATHS[:4])
+@pytest.mark.parametrize("path,new,kv", PATHS)
 def test_exponents_that_an_append_may_write(path, new, kv, exponents, D):
     """V's scales at the ends of what is written (bytes 27 and 247), alone and
     mixed, under weights that fall off over many powers of two."""
@@ -145,6 +147,34 @@ def test_exponents_that_an_append_may_write(path, new, kv, exponents, D):
         case.put(b, ke=torch.full_like(case.e[b][0], 1), ve=torch.tensor(exponents, device=DEV)[pick])
     case.check(case.run())
     case.check(case.run(softmax_scale=0.5), scale=0.5)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("where", ["seen by all", "seen by some"])
+@pytest.mark.parametrize("path,new,kv", PATHS)
+def test_values_that_round_up_to_2_128(path, new, kv, where, D):
+    """An appended element of 255 * 2^120 is stored as 256 * 2^120: finite in the
+    cache, too large for bf16.  The rows that see it get its weight times 2^128."""
+    case = Rows(new, kv, D, seed=4)
+    b = 0
+    pos = 7 if where == "seen by all" else kv[b] - new[b] + new[b] // 2
+    v = torch.zeros(2, 1, D, dtype=torch.bfloat16, device=DEV)
+    v[:, :, 37] = 255 * 2.0 ** 120
+    k = torch.zeros_like(v)  # of score 0, as every key's is about
+    offsets = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    cache_append(case.cfg, k, v, offsets, torch.tensor([pos + 1], dtype=torch.int32, device=DEV), case.tables[b:b + 1],
+                 case.pool, scales=case.scales)
+    case.load(b)
+    assert float(case.v[b][0, pos, 37]) == 2.0 ** 128
+    out = case.run()
+    want, bound = case.expected(b)
+    got = out[:, :new[b]].double()
+    most = float(torch.finfo(torch.bfloat16).max)
+    fits = want.abs() + bound < most  # (bf16 has nothing for the rest)
+    assert int(fits.sum()) > 0.99 * fits.numel() and (got[fits].isfinite()).all()
+    bad = fits & ~((got - want).abs() <= bound)
+    assert not bad.any(), f"{int(bad.sum())} beyond the bound"
+    assert (got[:, :, 37].abs() > 2.0 ** 100).sum() == (want[:, :, 37].abs() > 2.0 ** 100).sum() > 0
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "scaled"])
