@@ -178,7 +178,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     (or None) by ``positions`` ``[rows]`` (int32 or int64).  bf16, fp16 or
     fp32, weights of the same type; heads and rows at any 16-byte aligned
     stride, so ``[rows, heads, head_dim]`` projections are passed transposed.
-    ``q_out``/``k_out`` may be ``q``/``k`` themselves.  Returns both outputs
+    ``q_out``/``k_out`` may be ``q``/``k`` themselves (no row of which may then lie
+    on another).  Returns both outputs
     (new ones have the inputs' layout)."""
     if not q.is_cuda or q.dim() != 3:
         raise ValueError("q must be a CUDA tensor [heads, rows, head_dim]")
@@ -205,8 +206,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             if x is not None:
                 o = torch.empty_like(x) if stream is None else _allocate(stream, torch.empty_like, x)
             h = _heads(o)
-        elif o is not x:
-            h = _check_rows(name, o, tuple(x.shape), q.dtype, dev)
+        else:
+            if o is not x:
+                h = _check_rows(name, o, tuple(x.shape), q.dtype, dev)
             _check_writable(name, o)
         outs.append(o)
         structs.append(h)

@@ -11,7 +11,7 @@ import torch
 
 from aws_training_study_b200 import _capi
 from aws_training_study_b200.pcp_attention import PCPAttentionConfig
-from aws_training_study_b200.pcp_attention import paged
+from aws_training_study_b200.pcp_attention import paged, rotary
 from aws_training_study_b200.pcp_attention.rotary import Rotary, qk_norm_rope, rotary_frequencies
 
 
@@ -66,6 +66,28 @@ def test_qk_norm_rope_refusals():
     assert call(rows=0) == 0
     with pytest.raises(ValueError, match="CUDA"):
         qk_norm_rope(torch.zeros(1, 1, 128), None, torch.zeros(1, dtype=torch.int64), Rotary(128))
+
+
+def test_an_output_in_place_may_not_overlap_itself(monkeypatch):
+    """Broadcast heads or rows are inputs like any other, but not outputs: the
+    kernel would norm and rotate the same memory several times."""
+    launched = []
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(rotary, "_launch", lambda *args: launched.append(args))
+    plain, positions, turn = torch.zeros(4, 5, 128), torch.zeros(5, dtype=torch.int64), Rotary(128)
+    wide = [torch.zeros(1, 5, 128).expand(4, 5, 128), torch.zeros(4, 1, 128).expand(4, 5, 128),
+            torch.zeros(4 * 5 * 128).as_strided((4, 5, 128), (64, 512, 1))]
+    for x in wide:
+        with pytest.raises(ValueError, match="q_out overlaps"):
+            qk_norm_rope(x, None, positions, turn, q_out=x)
+        with pytest.raises(ValueError, match="k_out overlaps"):
+            qk_norm_rope(plain, x, positions, turn, k_out=x)
+    assert not launched
+    for x in [plain, *wide]:
+        out, _ = qk_norm_rope(x, None, positions, turn)
+        assert out.shape == x.shape and launched.pop()
+    assert qk_norm_rope(plain, plain, positions, turn, q_out=plain)[0] is plain and launched
 
 
 @pytest.mark.parametrize("entry", ["pcp_cache_append", "pcp_cache_read"])
