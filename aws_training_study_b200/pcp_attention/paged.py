@@ -34,7 +34,7 @@ import torch
 from .. import _capi
 from .config import PCPAttentionConfig
 from .cuda_backend import _cuda_stream_ptr, _kv_code, make_dims, payload_elements
-from .rotary import _allocate, _check_rows, _check_writable, _heads, _launch
+from .rotary import _allocate, _capturing, _check_rows, _check_writable, _heads, _launch
 
 
 def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -200,7 +200,7 @@ class _Status:
     def __init__(self, status: torch.Tensor | None, device: torch.device, stream: torch.cuda.Stream | None):
         self.own = status is None
         if self.own:
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(stream):
                 raise ValueError("a captured call needs a status tensor: its result cannot be read while recording")
             with torch.cuda.stream(stream):
                 status = torch.zeros(1, dtype=torch.int32, device=device)

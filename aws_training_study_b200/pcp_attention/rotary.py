@@ -77,6 +77,16 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
     return out, 0.1 * math.log(factor) + 1.0
 
 
+def _capturing(stream: torch.cuda.Stream | None) -> bool:
+    """Whether the current stream is being captured, or the one a call was given."""
+    if torch.cuda.is_current_stream_capturing():
+        return True
+    if stream is None:
+        return False
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class Rotary:
     """The rotation of the first ``rotary_dim`` (default all) elements of heads
     of ``head_dim``: ``layout`` ``"half"`` pairs i with i + rotary_dim / 2,
@@ -101,12 +111,12 @@ class Rotary:
         self._turns_host = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64)
         self._turns: dict[torch.device, torch.Tensor] = {}
 
-    def turns(self, device: torch.device) -> torch.Tensor:
+    def turns(self, device: torch.device, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The pairs' turns on ``device`` (copied there once; before any graph
-        capture that uses them)."""
+        capture that uses them, on the current stream or ``stream``)."""
         t = self._turns.get(device)
         if t is None:
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(stream):
                 raise RuntimeError("the rotation's table is not on this device yet: call once before the capture")
             t = self._turns[device] = self._turns_host.to(device)
         return t
@@ -214,6 +224,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         structs.append(h)
     _launch(dev, stream, _capi.lib().pcp_qk_norm_rope, _DTYPES[q.dtype], rows, D, rotary.rotary_dim,
             _LAYOUTS[rotary.layout], hq, hk, *structs, positions.data_ptr(),
-            int(positions.dtype == torch.int64), rotary.turns(dev).data_ptr(), rotary.magnitude,
+            int(positions.dtype == torch.int64), rotary.turns(dev, stream).data_ptr(), rotary.magnitude,
             0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps)
     return outs[0], outs[1]

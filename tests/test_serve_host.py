@@ -3,6 +3,7 @@ rotation, and the C ABI's refusals, which come before any device work."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -88,6 +89,36 @@ def test_an_output_in_place_may_not_overlap_itself(monkeypatch):
         out, _ = qk_norm_rope(x, None, positions, turn)
         assert out.shape == x.shape and launched.pop()
     assert qk_norm_rope(plain, plain, positions, turn, q_out=plain)[0] is plain and launched
+
+
+def test_a_capture_of_the_given_stream_is_seen(monkeypatch):
+    """What a call cannot do while its stream is captured is refused, whether
+    that stream is the current one or the one it was given."""
+    current = [None]
+
+    @contextlib.contextmanager
+    def stream(s):
+        before, current[0] = current[0], s
+        yield
+        current[0] = before
+
+    capturing = {None: False, "idle": False, "captured": True}
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[current[0]])
+    cpu, table = torch.device("cpu"), Rotary(128)
+    with pytest.raises(ValueError, match="captured"):
+        paged._Status(None, cpu, "captured")
+    with pytest.raises(RuntimeError, match="before the capture"):
+        table.turns(cpu, "captured")
+    paged._Status(torch.zeros(1, dtype=torch.int32), cpu, "captured")
+    assert paged._Status(None, cpu, "idle").own and paged._Status(None, cpu, None).own
+    with stream("captured"):
+        for given in (None, "idle"):
+            with pytest.raises(ValueError, match="captured"):
+                paged._Status(None, cpu, given)
+            with pytest.raises(RuntimeError, match="before the capture"):
+                table.turns(cpu, given)
+    assert table.turns(cpu, "idle") is table.turns(cpu, "captured")
 
 
 @pytest.mark.parametrize("entry", ["pcp_cache_append", "pcp_cache_read"])
