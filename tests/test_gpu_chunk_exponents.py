@@ -24,7 +24,7 @@ import pytest
 import torch
 
 from aws_training_study_b200.pcp_attention.paged import cache_append
-from test_gpu_chunk_attention import DEV, Case
+from test_gpu_chunk_attention import CACHES, DEV, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -175,6 +175,36 @@ def test_values_that_round_up_to_2_128(path, new, kv, where, D):
     bad = fits & ~((got - want).abs() <= bound)
     assert not bad.any(), f"{int(bad.sum())} beyond the bound"
     assert (got[:, :, 37].abs() > 2.0 ** 100).sum() == (want[:, :, 37].abs() > 2.0 ** 100).sum() > 0
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("power", [110, -100])
+@pytest.mark.parametrize("path,new,kv", PATHS)
+def test_keys_of_any_size(path, new, kv, power, D):
+    """K far from unit size, with queries that bring the scores back."""
+    case = Rows(new, kv, D, seed=3)
+    for b in range(len(kv)):
+        case.put(b, ke=case.e[b][0].clamp(-4, 1) + power)
+    case.q = (case.q.float() * 2.0 ** -power).to(torch.bfloat16)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("heads,D", [((16, 2), 128), ((16, 2), 256), ((7, 7), 128)])
+@pytest.mark.parametrize("new,kv,wide", [([1], [4000], False), ([2, 1], [1500, 9000], False), ([60], [1500], False),
+                                         ([150, 33], [2100, 700], False), ([150, 33], [2100, 700], True)])
+def test_maxima_that_grow_with_every_tile(new, kv, wide, heads, D, cache):
+    """Scores that grow by 12 log2 units with every 128 keys for half of the
+    queries, and stay for the others: O goes over to a new reference tile by tile."""
+    case = Rows(new, kv, D, cache, seed=5, heads=heads, wide=wide)
+    u = torch.where(torch.rand(D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) < 0.5, -1.0, 1.0)
+    grows = torch.arange(case.q.shape[1], device=DEV)[None, :, None] + torch.arange(heads[0], device=DEV)[:, None, None]
+    case.q = (case.q * 0.25 + u * (grows % 2)).to(torch.bfloat16)
+    for b, t in enumerate(kv):
+        x = torch.randn(heads[1], t, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(b)).double()
+        x += (torch.arange(t, device=DEV) // 128)[:, None] * (12 * math.log(2) / math.sqrt(D)) * u.double()
+        case.put(b, k=x, ke=torch.zeros_like(case.e[b][0]) if cache == "scaled" else None)
+    case.check(case.run())
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "scaled"])
