@@ -34,7 +34,7 @@ import torch
 from .. import _capi
 from .config import PCPAttentionConfig
 from .cuda_backend import _cuda_stream_ptr, _kv_code, make_dims, payload_elements
-from .rotary import _allocate, _capturing, _check_rows, _check_writable, _heads, _launch
+from .rotary import _allocate, _capturing, _check_apart, _check_rows, _check_writable, _heads, _launch
 
 
 def make_pool(config: PCPAttentionConfig, pool_blocks: int, kv_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -256,6 +256,7 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
             raise ValueError("cache_read needs rows, or k_out and v_out")
         rows = k_out.shape[1] if k_out.dim() == 3 else -1
     device, shape = pool.device, (config.num_kv_heads, int(rows), config.head_dim)
+    _check_apart("k_out", k_out, "v_out", v_out)
     outs, structs = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:

@@ -159,6 +159,12 @@ def _check_writable(name: str, t: torch.Tensor) -> None:
             reach += stride * (n - 1)
 
 
+def _check_apart(name: str, t: torch.Tensor | None, other: str, o: torch.Tensor | None) -> None:
+    """An output may not be another tensor of the call over again."""
+    if t is not None and o is not None and t.numel() and o.numel() and t.data_ptr() == o.data_ptr():
+        raise ValueError(f"{name} and {other} are the same memory")
+
+
 def _allocate(stream: torch.cuda.Stream, make, *args, **kwargs) -> torch.Tensor:
     """``make(...)`` with memory of ``stream``, for a call that was given one: a
     block that the current stream freed may still be in use by work it has yet to
@@ -210,6 +216,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or w.device != dev or
                               not w.is_contiguous() or w.data_ptr() % 16):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned [{D}] {q.dtype} tensor on {dev}")
+    if q_out is not None or k_out is not None:
+        _check_apart("q_out", q_out, "k_out", k_out)
+        _check_apart("q_out", q_out, "k", k)
+        _check_apart("k_out", k_out, "q", q)
     outs, structs = [], []
     for name, x, o, h in (("q_out", q, q_out, hq), ("k_out", k, k_out, hk)):
         if o is None:

@@ -88,7 +88,28 @@ def test_an_output_in_place_may_not_overlap_itself(monkeypatch):
     for x in [plain, *wide]:
         out, _ = qk_norm_rope(x, None, positions, turn)
         assert out.shape == x.shape and launched.pop()
-    assert qk_norm_rope(plain, plain, positions, turn, q_out=plain)[0] is plain and launched
+    assert qk_norm_rope(plain, plain.clone(), positions, turn, q_out=plain)[0] is plain and launched
+
+
+def test_two_outputs_may_not_be_the_same_memory(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    launched = []
+    for module in (rotary, paged):
+        monkeypatch.setattr(module, "_launch", lambda *args: launched.append(args))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    x, y, positions, turn = torch.zeros(2, 5, 128), torch.zeros(2, 5, 128), torch.zeros(5, dtype=torch.int64), Rotary(128)
+    for args in (dict(q_out=x, k_out=x), dict(q_out=y), dict(k_out=x), dict(q_out=torch.zeros(4, 5, 128)[2:], k_out=x)):
+        with pytest.raises(ValueError, match="the same memory"):
+            qk_norm_rope(x, y, positions, turn, **args)
+    qk_norm_rope(x, y, positions, turn, q_out=x, k_out=y)
+    cfg = PCPAttentionConfig(1, 64, 1024, 1024, 64, 16, 4, 2, 128)
+    pool, ints = torch.zeros(2, 2 * 2 * 64 * 128, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    both = torch.zeros(2, 5, 2, 128, dtype=torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32)
+    read = lambda k, v: paged.cache_read(cfg, ints, ints[:1], ints[None], pool, k_out=k, v_out=v, status=status)
+    with pytest.raises(ValueError, match="the same memory"):
+        read(both[:, :, 0], both[:, :, 0])
+    assert len(launched) == 1 and read(both[:, :, 0], both[:, :, 1]) and len(launched) == 2
 
 
 def test_a_capture_of_the_given_stream_is_seen(monkeypatch):
