@@ -256,7 +256,6 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
             raise ValueError("cache_read needs rows, or k_out and v_out")
         rows = k_out.shape[1] if k_out.dim() == 3 else -1
     device, shape = pool.device, (config.num_kv_heads, int(rows), config.head_dim)
-    _check_apart("k_out", k_out, "v_out", v_out)
     outs, structs = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:
@@ -267,6 +266,7 @@ def cache_read(config: PCPAttentionConfig, offsets: torch.Tensor, kv_len: torch.
             structs.append(_check_rows(name, t, shape, torch.bfloat16, device))
             _check_writable(name, t)
         outs.append(t)
+    _check_apart("k_out", outs[0], "v_out", outs[1])
     batch = _batch_struct(offsets, kv_len, block_tables, int(rows), device)
     st = _Status(status, device, stream)
     _launch(device, stream, _capi.lib().pcp_cache_read, ps, batch, *structs, st.ptr)
