@@ -24,7 +24,7 @@
 //   * The teams' (m, l, O) are merged through shared memory when the unit's part
 //     ends, into bf16 rows or an fp32 partial.
 // 64 sequences of 4096 (bf16, 32 / 8 heads of 128): 5.6 TB/s, 86 % of a copy's rate.
-// 16 of 32768 (e4m3 with scales, 32 / 2 heads of 256): 3.9 TB/s, bound by issue and
+// 16 of 32768 (e4m3 with scales, 32 / 2 heads of 256): 3.8 TB/s, bound by issue and
 // latency (half of the issue slots; conversions and MMAs are half the instructions).
 // Multiplying a visit's scores under the softmax of the one before held the stages
 // longer and was slower (87 to 100 us, bf16 129 to 153).

@@ -32,8 +32,11 @@
 //     where they clear the rows that no row sees (they may hold anything: 0 * NaN
 //     would reach every row) and values that are not finite (nonfinite8).
 //   * An e4m3 cache that many query tiles read is expanded into a bf16 copy first
-//     (chunk_expand_kernel; exact, scales included), when the copy is of moderate
-//     size: reading it in place converts every key tile again for each 256 rows.
+//     (chunk_expand_kernel; exact, scales included but for a common power of two),
+//     when the copy is of moderate size: reading it in place converts every key tile
+//     again for each 256 rows.  The weights are rounded to bf16 then, within
+//     2^-8 where in place it is 2^-11: an MMA's operands share a type, and f16 does not
+//     reach the scaled values.
 //   * Scaled e4m3 caches: K's 2^e multiplies the scores of its key, V's e is added to
 //     the exponent of its weight, and the softmax reference follows the largest
 //     score + V exponent, key by key, as in chunk_rows.cuh.
@@ -333,7 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTilesThreads, 1)
   auto bar_q_ready = [&](int sg) { return bars + 8u * (sg & 1); };
   // the segment's last QK^T has read Q (MMA commit, both CTAs);
   auto bar_q_empty = [&](int sg) { return bars + 16 + 8u * (sg & 1); };
-  // this CTA's row factors written (four of them: see kFactorBufs).
+  // this CTA's row factors written (kSegBufs of them).
   auto bar_rows = [&](int sg) { return bars + 32 + 8u * (sg & (L::kSegBufs - 1)); };
   // Leader: O of the segment read by every warp of both CTAs that writes it out (two
   // of them with kTwo).

@@ -125,11 +125,16 @@ struct ChunkLayout {
 };
 
 // An e4m3 cache is expanded for the tile units from kExpandRows rows a KV head
-// on (4 tiles), while the copy of all sequences' tables stays within
-// kExpandBytes.  In place against expanded, us: heads of 256 over 32768 tokens, 512
-// rows 101 / 101, 1024 126 / 118, 2048 183 / 153, 8192 517 / 378; over 131072, 512
-// 196 / 235, 1024 312 / 312, 2048 554 / 476, 8192 1795 / 1373; heads of 128 over
-// 32768, 512 198 / 169, 1024 345 / 238, 4096 1254 / 579.
+// on (4 tiles), while the copy of all sequences' tables stays within kExpandBytes.
+// In place / expanded, us, of a cache with scales: heads of 256 over 32768 tokens, 512
+// rows 92 / 81, 1024 122 / 99, 2048 188 / 135, 8192 588 / 360; over 131072, 512 226 /
+// 236, 1024 345 / 298, 2048 662 / 481, 8192 2230 / 1365; heads of 128 over 32768, 512
+// 271 / 150, 1024 388 / 194, 4096 1342 / 528.  At unit scale (no scales to apply in
+// place): heads of 256 over 32768, 512 74 / 81, 1024 91 / 97, 2048 128 / 131, 8192 362
+// / 360; over 131072, 512 167 / 222, 1024 223 / 300, 2048 422 / 497, 8192 1521 / 1485;
+// heads of 128 over 32768, 512 132 / 147, 1024 186 / 191, 4096 588 / 517: there the
+// copy pays from some 8192 rows (heads of 256) or 4096 (128) only, and costs up to a
+// third between.
 constexpr int64_t kExpandRows = 1024;
 constexpr int64_t kExpandBytes = int64_t(1) << 30;
 

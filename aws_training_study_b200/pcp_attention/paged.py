@@ -22,7 +22,9 @@ the last of the ``kv_len[b]`` tokens it then has; position p lives in row
 ``p % block_size`` of pool block ``block_tables[b, p // block_size]``.  An e4m3
 pool may carry ``scales`` (``make_scales``): a power of two for each token, head
 and K or V, so that rows of any size keep e4m3's relative precision and what is
-read back is exact in bf16.
+read back is exact in bf16.  Such a pool is for these three calls alone: a pool does
+not know its scales, and the other entries here, which stripe one sequence over ranks,
+read its codes at unit scale.
 """
 
 from __future__ import annotations
@@ -285,7 +287,10 @@ def chunk_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Ten
     single tokens, chunks and whole prompts may be mixed.  ``max_chunk`` (default
     ``rows``) bounds the rows of every sequence; 1 for a decode step saves the
     launches that longer chunks would need.  ``softmax_scale`` defaults to
-    ``config.softmax_scale``.  Rows that see nothing are zeros; rows of no
+    ``config.softmax_scale``.  Weights are rounded to bf16 over a bf16 pool, and over an
+    e4m3 one where ``max_chunk`` times the query heads of a KV head reaches 1024 (it is read
+    through a bf16 copy then, while all tables' tokens need no more than 1 GiB of it), else to
+    f16.  The call's workspace, that copy included, is allocated for it.  Rows that see nothing are zeros; rows of no
     sequence are left as they were.  ``status`` as in ``cache_append`` (112 also
     for a sequence of more than ``max_chunk`` rows, which is not written)."""
     ps = _pool_struct(config, pool, scales)

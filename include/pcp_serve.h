@@ -30,7 +30,8 @@
  *        as 0), more rows than max_chunk (the sequence's rows are not
  *        written), offsets that decrease or leave the rows (nothing is
  *        written);
- *   1xx  a wait in the attention kernel that ran out (see pcp_attn.h).
+ *   1xx  a wait in the attention kernel that ran out (see pcp_attn.h): rows that
+ *        the failed part of the work shares with others are not written.
  */
 #ifndef PCP_SERVE_H
 #define PCP_SERVE_H
